@@ -30,7 +30,7 @@ extern "C" {
 /* dtype codes used by the `*_dtype` parameters */
 #define XKB_BF16 0
 #define XKB_F32 1
-#define XKB_F16 2 /* accepted for router logits only */
+#define XKB_F16 2 /* accepted for logits (router, head) only */
 
 /* kernel-path selectors for the `path` parameters */
 #define XKB_PATH_AUTO 0  /* tensor-core kernel when the shape allows, else SIMT */
@@ -134,6 +134,101 @@ int xkb_topk_softmax(const void* gating_output, int dtype, float* topk_weights,
 int xkb_moe_sum_reduce(const void* y, int y_dtype, const void* w, int w_dtype,
                        void* out, int out_dtype, int64_t M, int top_k,
                        int64_t H, float routed_scaling_factor, void* stream);
+
+/* ------------------------------------------------------------------------
+ * moe_sum_reduce_backward: the gradients of moe_sum_reduce,
+ *   grad_y[m,k,:] = rsf * (w[m,k] or 1) * grad_out[m,:]
+ *   grad_w[m,k]   = rsf * sum_h grad_out[m,h] * y[m,k,h]
+ * No reference counterpart (its pure-torch form is differentiated by torch).
+ * grad_out [M, H], y [M, top_k, H] and grad_y of one dtype (XKB_BF16 or
+ * XKB_F32), w NULL or [M, top_k] (w_dtype), grad_w of w_dtype.  grad_y and
+ * grad_w may each be NULL (not wanted); y is read for grad_w only.  fp32 sums in
+ * a fixed order.  One launch, no workspace.
+ * ---------------------------------------------------------------------- */
+int xkb_moe_sum_reduce_backward(const void* grad_out, int dtype, const void* y,
+                                const void* w, int w_dtype, void* grad_y,
+                                void* grad_w, int64_t M, int top_k, int64_t H,
+                                float routed_scaling_factor, void* stream);
+
+/* ------------------------------------------------------------------------
+ * moe_balance_loss: per-expert counts and balance loss of a routing,
+ *   loss = E * sum_e counts[e] / (top_k * T) * mean_probs[e],
+ * counts[e] = slots of topk_ids that chose e, mean_probs[e] = mean over the
+ * tokens of softmax(gating)[e], over the T tokens that count.  1 for an even
+ * routing.  No reference counterpart.
+ * gating_output [M, E] (as for topk_softmax, E <= 1024), topk_ids [M, top_k];
+ * ids outside [0, E) are dropped slots and not counted.  token_mask NULL or [M]
+ * bytes: tokens with 0 count for nothing.  A row whose logits are all -inf has no
+ * probabilities (adds 0); NaN and +inf make mean_probs and loss NaN.  Outputs:
+ * loss [1] fp32, counts [E] int32, mean_probs [E] fp32, tokens [1] int32 (T).
+ * T = 0: loss 0.  M * top_k < 2^31.  Two launches; the same bits in every run.
+ * ---------------------------------------------------------------------- */
+int64_t xkb_moe_balance_loss_workspace_bytes(int64_t M, int E);
+int xkb_moe_balance_loss(const void* gating_output, int dtype,
+                         const int32_t* topk_ids, const uint8_t* token_mask,
+                         float* loss, int32_t* counts, float* mean_probs,
+                         int32_t* tokens, int64_t M, int E, int top_k,
+                         void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* ------------------------------------------------------------------------
+ * moe_router_backward: the gradient of the gating logits, from the routing
+ * weights of topk_softmax and / or from moe_balance_loss,
+ *   grad = p * (dp - sum_e p dp),   p = softmax(gating) in fp32.
+ * grad_weights NULL or [M, top_k] fp32, renormalize as in topk_softmax; ids
+ * outside [0, E) are dropped slots, an expert named twice takes both.
+ * counts NULL or [E]: adds the gradient of loss_scale * grad_loss * loss
+ * (grad_loss NULL: 1), with counts and tokens (NULL: M) as moe_balance_loss left
+ * them, or summed over the ranks of a data-parallel job; token_mask as there.
+ * A row that neither brings a gradient to is 0 whatever its logits.
+ * grad_gating [M, E] of gating's dtype.  One launch, no workspace.
+ * ---------------------------------------------------------------------- */
+int xkb_moe_router_backward(const void* gating_output, int dtype,
+                            const int32_t* topk_ids, const float* grad_weights,
+                            int renormalize, const int32_t* counts,
+                            const int32_t* tokens, const float* grad_loss,
+                            float loss_scale, const uint8_t* token_mask,
+                            void* grad_gating, int64_t M, int E, int top_k,
+                            void* stream);
+
+/* ------------------------------------------------------------------------
+ * token_logprobs: for each row of logits [M, V] (bf16 / fp32 / fp16, row stride
+ * ld elements) the log-probability of the given token, the entropy (nats), the
+ * statistics m = max x and l = ln sum exp(x - m) (stats [M, 2]; m + l is the
+ * log-sum-exp), and the top_k likeliest tokens with their log-probabilities,
+ * descending, ties by ascending id (NaN above all, -0 equal to 0).
+ * No reference counterpart.
+ * token_ids [M] int32, or int64 with ids64 = 1.  A negative id is padding:
+ * log-probability 0; an id >= V gives NaN.  A row without a live logit (all -inf)
+ * has log-probabilities -inf and entropy 0; a row with a NaN or +inf is NaN.
+ * top_logprobs, top_ids [M, top_k]; top_k <= min(V, 64), 0: none.
+ * M < 2^28.  One launch, no workspace; the same bits in every run.
+ * ---------------------------------------------------------------------- */
+int xkb_token_logprobs(const void* logits, int dtype, int64_t ld,
+                       const void* token_ids, int ids64, float* logprobs,
+                       float* entropy, float* stats, float* top_logprobs,
+                       int32_t* top_ids, int64_t M, int64_t V, int top_k,
+                       void* stream);
+
+/* ------------------------------------------------------------------------
+ * token_logprobs_backward: the gradient of the logits,
+ *   grad = -p (G + grad_entropy (ln p + entropy)) + what a column was given,
+ * G = grad_logprobs + sum_j grad_top_logprobs, p from stats.  Each of the three
+ * gradients may be NULL; a negative token id has none, an id >= V makes the row
+ * NaN; the same holds for top_ids.  A row without a live logit: p = 0.
+ * grad_logits [M, V] of logits' dtype, row stride ld_grad; every row has to start
+ * at the same place within 16 bytes as the row of logits (XKB_ERR_ARG).
+ * Not in place.  One launch, no workspace.
+ * ---------------------------------------------------------------------- */
+int xkb_token_logprobs_backward(const void* logits, int dtype, int64_t ld,
+                                const void* token_ids, int ids64,
+                                const float* stats, const float* entropy,
+                                const float* grad_logprobs,
+                                const float* grad_entropy,
+                                const int32_t* top_ids,
+                                const float* grad_top_logprobs, int top_k,
+                                void* grad_logits, int64_t ld_grad, int64_t M,
+                                int64_t V, void* stream);
 
 /* The token tile (positions of a token block) that a fused call picks on the
  * tensor cores, from its number of slots; no GPU is needed to ask.  INT4: 16,

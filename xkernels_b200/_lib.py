@@ -48,6 +48,31 @@ SIGNATURES = {
         c_int,
         [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int64, c_float, c_void_p],
     ),
+    "xkb_moe_sum_reduce_backward": (
+        c_int,
+        [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int, c_int64, c_float, c_void_p],
+    ),
+    "xkb_moe_balance_loss_workspace_bytes": (c_int64, [c_int64, c_int]),
+    "xkb_moe_balance_loss": (
+        c_int,
+        [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p,
+         c_int64, c_void_p],
+    ),
+    "xkb_moe_router_backward": (
+        c_int,
+        [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
+         c_int64, c_int, c_int, c_void_p],
+    ),
+    "xkb_token_logprobs": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+         c_int64, c_int, c_void_p],
+    ),
+    "xkb_token_logprobs_backward": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p],
+    ),
     "xkb_fused_moe_int4_w4a16_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
     "xkb_fused_moe_int4_w4a16": (
         c_int,

@@ -1,4 +1,4 @@
-"""Host side of the four ops: argument checks, output allocation, one C-ABI call.
+"""Host side of the ops: argument checks, output allocation, one C-ABI call.
 
 The callables keep the parameter names of the reference backends because the
 reference's ``verify`` harness calls a card as ``fn(**inputs)``
@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import functools
+from typing import NamedTuple
 
 import torch
 
@@ -302,6 +303,266 @@ def moe_sum_reduce(y, w=None, routed_scaling_factor=1.0):
                                    _DT[y.dtype], M, top_k, H, float(routed_scaling_factor),
                                    _stream(dev)),
             "xkb_moe_sum_reduce")
+    return out
+
+
+def _typed(name, what, t, shape, dtype):
+    """``t`` as a contiguous tensor of ``dtype``, after a look at its shape."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: {what} must be {list(shape)}, got {list(t.shape)}")
+    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
+
+
+def _mask(name, token_mask, M):
+    if token_mask is None:
+        return None
+    if token_mask.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"{name}: token_mask must be bool or uint8, got {token_mask.dtype}")
+    if tuple(token_mask.shape) != (M,):
+        raise ValueError(f"{name}: token_mask must be [{M}], got {list(token_mask.shape)}")
+    return token_mask.contiguous()
+
+
+def _gating(name, gating_output, topk_ids):
+    if gating_output.dim() != 2:
+        raise ValueError(f"{name}: gating_output must be [M, E]")
+    if gating_output.dtype not in _LOGIT_DT:
+        raise TypeError(f"{name}: logits must be bf16, fp16 or fp32, got {gating_output.dtype}")
+    M, E = gating_output.shape
+    if E < 1:
+        raise ValueError(f"{name}: no experts")
+    if topk_ids is not None:
+        if topk_ids.dim() != 2 or topk_ids.shape[0] != M:
+            raise ValueError(f"{name}: topk_ids must be [{M}, top_k], got {list(topk_ids.shape)}")
+        if topk_ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: topk_ids must be int32 or int64, got {topk_ids.dtype}")
+        topk_ids = topk_ids.to(torch.int32).contiguous()
+    return gating_output.contiguous(), topk_ids, M, E
+
+
+def moe_sum_reduce_backward(grad_out, y, w=None, routed_scaling_factor=1.0, need_grad_y=True, need_grad_w=True):
+    """The gradients of :func:`moe_sum_reduce`: ``(grad_y, grad_w)``, of ``y``'s and ``w``'s shape and dtype.
+
+    ``grad_y[m,k] = f * w[m,k] * grad_out[m]`` and ``grad_w[m,k] = f * sum_h grad_out[m,h] * y[m,k,h]``, sums in fp32 in a fixed
+    order.  What is not wanted, and ``grad_w`` without ``w``, is None.  No reference counterpart: the reference's
+    pure-torch form is differentiated by torch.
+    """
+    lib = _lib.load()
+    dev = _require_cuda("moe_sum_reduce_backward", grad_out, y, w)
+    if y.dim() != 3:
+        raise ValueError("y must be [M, top_k, H]")
+    if y.dtype not in _DT:
+        raise TypeError(f"moe_sum_reduce_backward: unsupported y dtype {y.dtype}")
+    M, top_k, H = y.shape
+    grad_out = _typed("moe_sum_reduce_backward", "grad_out", grad_out, (M, H), y.dtype)
+    need_grad_w = need_grad_w and w is not None
+    w_as = None
+    if w is not None:
+        w_as = _typed("moe_sum_reduce_backward", "w", w, (M, top_k), w.dtype if w.dtype in _DT else torch.float32)
+    if need_grad_w:
+        y = y.contiguous()
+    with _on(dev):
+        grad_y = torch.empty((M, top_k, H), dtype=y.dtype, device=dev) if need_grad_y else None
+        grad_w = torch.empty((M, top_k), dtype=w_as.dtype, device=dev) if need_grad_w else None
+        _lib.check(
+            lib.xkb_moe_sum_reduce_backward(
+                _ptr(grad_out), _DT[y.dtype], _ptr(y) if need_grad_w else 0, _ptr(w_as),
+                _lib.XKB_F32 if w_as is None else _DT[w_as.dtype], _ptr(grad_y), _ptr(grad_w), M, top_k, H,
+                float(routed_scaling_factor), _stream(dev)),
+            "xkb_moe_sum_reduce_backward")
+    if grad_w is not None and grad_w.dtype != w.dtype:
+        grad_w = grad_w.to(w.dtype)
+    return grad_y, grad_w
+
+
+class BalanceLoss(NamedTuple):
+    """What :func:`moe_balance_loss` returns."""
+
+    loss: torch.Tensor         # [] fp32
+    counts: torch.Tensor       # [E] int32: slots per expert
+    mean_probs: torch.Tensor   # [E] fp32: mean router probability per expert
+    tokens: torch.Tensor       # [] int32: tokens that count
+
+
+def moe_balance_loss(gating_output, topk_ids, token_mask=None):
+    """Balance loss and per-expert counts of a routing: ``E * sum_e counts[e] / (top_k * T) * mean_probs[e]``, which is 1
+    for an even one.
+
+    ``gating_output`` ``[M, E]`` logits as for :func:`topk_softmax`, ``topk_ids`` ``[M, top_k]`` its choice (ids outside
+    ``[0, E)`` are dropped slots: not counted), ``token_mask`` ``[M]`` bool: padding tokens (False) count for nothing; ``T`` is the
+    number of the others.  Without one (``T = 0``) the loss is 0.  A row of logits that are all -inf adds nothing to ``mean_probs``.
+    The same bits in every run.  The gradient: :func:`moe_router_backward`; in a data-parallel job ``counts`` and ``tokens`` may be
+    summed over the ranks before it, which makes it the gradient of the whole batch's loss.  No reference counterpart.
+    """
+    lib = _lib.load()
+    dev = _require_cuda("moe_balance_loss", gating_output, topk_ids, token_mask)
+    if topk_ids is None:
+        raise TypeError("moe_balance_loss: topk_ids is missing")
+    g, ids, M, E = _gating("moe_balance_loss", gating_output, topk_ids)
+    mask = _mask("moe_balance_loss", token_mask, M)
+    with _on(dev):
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty((E,), dtype=torch.int32, device=dev)
+        mean = torch.empty((E,), dtype=torch.float32, device=dev)
+        tokens = torch.empty((), dtype=torch.int32, device=dev)
+        ws_bytes = max(_bytes("xkb_moe_balance_loss_workspace_bytes", M, E), 0)   # of this call alone: calls may overlap
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+        _lib.check(
+            lib.xkb_moe_balance_loss(_ptr(g), _LOGIT_DT[g.dtype], _ptr(ids), _ptr(mask), _ptr(loss), _ptr(counts),
+                                     _ptr(mean), _ptr(tokens), M, E, ids.shape[1], _ptr(ws), ws_bytes, _stream(dev)),
+            "xkb_moe_balance_loss")
+    return BalanceLoss(loss, counts, mean, tokens)
+
+
+def moe_router_backward(gating_output, topk_ids, grad_weights=None, renormalize=True, counts=None, tokens=None,
+                        grad_loss=None, token_mask=None):
+    """The gradient of the gating logits, ``[M, E]`` of their dtype, in one pass.
+
+    From the routing weights: ``grad_weights`` ``[M, top_k]``, the gradient of :func:`topk_softmax`'s weights for
+    ``topk_ids`` (``renormalize`` as there).  From :func:`moe_balance_loss`: ``counts`` and ``tokens`` (None: M) as it returned them,
+    ``grad_loss`` the loss's gradient (a number or a one-element CUDA tensor; None: 1), ``token_mask`` as there.  Either may be
+    left out.  Ids outside ``[0, E)`` are dropped slots.  A row that neither brings a gradient to is 0, whatever its
+    logits.  No reference counterpart: the reference's pure-torch router is differentiated by torch.
+    """
+    lib = _lib.load()
+    name = "moe_router_backward"
+    on_device = grad_loss if isinstance(grad_loss, torch.Tensor) else None
+    dev = _require_cuda(name, gating_output, topk_ids, grad_weights, counts, tokens, on_device, token_mask)
+    if grad_weights is None and counts is None:
+        raise ValueError(f"{name}: neither grad_weights nor counts")
+    if counts is None and (grad_loss is not None or tokens is not None):
+        raise ValueError(f"{name}: grad_loss and tokens belong to counts")
+    if topk_ids is None:
+        raise TypeError(f"{name}: topk_ids is missing")
+    g, ids, M, E = _gating(name, gating_output, topk_ids)
+    top_k = ids.shape[1]
+    mask = _mask(name, token_mask, M)
+    gw = None if grad_weights is None else _typed(name, "grad_weights", grad_weights, (M, top_k), torch.float32)
+    scale = 1.0
+    if counts is not None:
+        counts = _typed(name, "counts", counts, (E,), torch.int32)
+        if tokens is not None:
+            tokens = _typed(name, "tokens", tokens.reshape(-1), (1,), torch.int32)
+        if on_device is not None:
+            on_device = _typed(name, "grad_loss", on_device.reshape(-1), (1,), torch.float32)
+        elif grad_loss is not None:
+            scale = float(grad_loss)
+    with _on(dev):
+        out = torch.empty((M, E), dtype=g.dtype, device=dev)
+        _lib.check(
+            lib.xkb_moe_router_backward(_ptr(g), _LOGIT_DT[g.dtype], _ptr(ids), _ptr(gw), 1 if renormalize else 0,
+                                        _ptr(counts), _ptr(tokens), _ptr(on_device), scale, _ptr(mask), _ptr(out), M, E,
+                                        top_k, _stream(dev)),
+            "xkb_moe_router_backward")
+    return out
+
+
+# ---------------------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` returns."""
+
+    logprobs: torch.Tensor       # [M] fp32
+    entropy: torch.Tensor        # [M] fp32, nats
+    stats: torch.Tensor          # [M, 2] fp32: row maximum m, ln sum exp(x - m)
+    top_logprobs: torch.Tensor   # [M, top_k] fp32, descending
+    top_ids: torch.Tensor        # [M, top_k] int32
+
+
+def _head(name, logits, token_ids):
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"{name}: logits must be [M, V]")
+    if logits.dtype not in _LOGIT_DT:
+        raise TypeError(f"{name}: logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    M, V = logits.shape
+    if token_ids is not None:
+        if token_ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: token_ids must be int32 or int64, got {token_ids.dtype}")
+        if tuple(token_ids.shape) != (M,):
+            raise ValueError(f"{name}: token_ids must be [{M}], got {list(token_ids.shape)}")
+        token_ids = token_ids.contiguous()
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    return logits, token_ids, M, V
+
+
+def token_logprobs(logits, token_ids, top_k=0):
+    """Log-probabilities of given tokens, entropy, and the ``top_k`` likeliest tokens of every row of a head's logits.
+
+    ``logits`` ``[M, V]`` bf16, fp16 or fp32; rows may lie apart (a slice of a padded head is read in place).  ``token_ids``
+    ``[M]`` int32 or int64; a negative id is padding and has log-probability 0, an id of V or more gives NaN.  ``top_k`` up to
+    ``min(V, 64)``; alternatives come in descending probability, ties by ascending id as in :func:`topk_softmax`.  A row whose
+    logits are all -inf has log-probabilities -inf and entropy 0, a row with a NaN or a +inf is NaN.  The same bits in every
+    run.  The gradient: :func:`token_logprobs_backward`.  No reference counterpart.
+    """
+    lib = _lib.load()
+    name = "token_logprobs"
+    dev = _require_cuda(name, logits, token_ids)
+    if token_ids is None:
+        raise TypeError(f"{name}: token_ids is missing")
+    logits, ids, M, V = _head(name, logits, token_ids)
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(V, 64):
+        raise ValueError(f"{name}: top_k must satisfy 0 <= top_k <= min(V, 64) (got top_k={top_k}, V={V})")
+    with _on(dev):
+        lp = torch.empty((M,), dtype=torch.float32, device=dev)
+        entropy = torch.empty((M,), dtype=torch.float32, device=dev)
+        stats = torch.empty((M, 2), dtype=torch.float32, device=dev)
+        top_lp = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+        top_ids = torch.empty((M, top_k), dtype=torch.int32, device=dev)
+        _lib.check(
+            lib.xkb_token_logprobs(_ptr(logits), _LOGIT_DT[logits.dtype], logits.stride(0), _ptr(ids),
+                                   1 if ids.dtype == torch.int64 else 0, _ptr(lp), _ptr(entropy), _ptr(stats),
+                                   _ptr(top_lp), _ptr(top_ids), M, V, top_k, _stream(dev)),
+            "xkb_token_logprobs")
+    return TokenLogprobs(lp, entropy, stats, top_lp, top_ids)
+
+
+def token_logprobs_backward(logits, token_ids, stats, entropy=None, grad_logprobs=None, grad_entropy=None, top_ids=None,
+                            grad_top_logprobs=None):
+    """The gradient of a head's logits, ``[M, V]`` of their dtype, from those of :func:`token_logprobs`'s outputs.
+
+    ``stats``, ``entropy`` (for ``grad_entropy``) and ``top_ids`` (for ``grad_top_logprobs``) are what the forward call returned.
+    Gradients that are left out count as 0; one at least is needed.  Padding tokens (negative ids) have no gradient.  The
+    result is contiguous, or, where the logits' rows do not start on 16 bytes, a view of rows that start like theirs.
+    """
+    lib = _lib.load()
+    name = "token_logprobs_backward"
+    dev = _require_cuda(name, logits, token_ids, stats, entropy, grad_logprobs, grad_entropy, top_ids, grad_top_logprobs)
+    if grad_logprobs is None and grad_entropy is None and grad_top_logprobs is None:
+        raise ValueError(f"{name}: no gradient is given")
+    if (grad_logprobs is not None and token_ids is None) or (grad_entropy is not None and entropy is None) or \
+            (grad_top_logprobs is not None and top_ids is None):
+        raise ValueError(f"{name}: grad_logprobs needs token_ids, grad_entropy needs entropy, grad_top_logprobs needs top_ids")
+    logits, ids, M, V = _head(name, logits, token_ids)
+    stats = _typed(name, "stats", stats, (M, 2), torch.float32)
+    if grad_logprobs is not None:
+        grad_logprobs = _typed(name, "grad_logprobs", grad_logprobs, (M,), torch.float32)
+    if grad_entropy is not None:
+        grad_entropy = _typed(name, "grad_entropy", grad_entropy, (M,), torch.float32)
+        entropy = _typed(name, "entropy", entropy, (M,), torch.float32)
+    top_k = 0
+    if grad_top_logprobs is not None:
+        top_k = int(top_ids.shape[-1])
+        top_ids = _typed(name, "top_ids", top_ids, (M, top_k), torch.int32)
+        grad_top_logprobs = _typed(name, "grad_top_logprobs", grad_top_logprobs, (M, top_k), torch.float32)
+        if top_k > 64:
+            raise ValueError(f"{name}: at most 64 alternatives (got {top_k})")
+    # rows of the gradient start where rows of the logits do within 16 bytes, so that both go in 16-byte pieces
+    es = logits.element_size()
+    ld, shift = logits.stride(0), logits.data_ptr() % 16 // es
+    ld_grad = V if M <= 1 else V + (ld - V) % (16 // es)
+    with _on(dev):
+        if ld_grad == V and shift == 0:
+            out = torch.empty((M, V), dtype=logits.dtype, device=dev)
+        else:
+            out = torch.empty((M * ld_grad + shift,), dtype=logits.dtype, device=dev).as_strided((M, V), (ld_grad, 1), shift)
+        _lib.check(
+            lib.xkb_token_logprobs_backward(
+                _ptr(logits), _LOGIT_DT[logits.dtype], ld, _ptr(ids), 1 if ids is not None and ids.dtype == torch.int64 else 0,
+                _ptr(stats), _ptr(entropy) if grad_entropy is not None else 0, _ptr(grad_logprobs), _ptr(grad_entropy),
+                _ptr(top_ids) if top_k else 0, _ptr(grad_top_logprobs) if top_k else 0, top_k, _ptr(out), ld_grad, M, V,
+                _stream(dev)),
+            "xkb_token_logprobs_backward")
     return out
 
 

@@ -159,6 +159,7 @@ class PythonCalls:
         return None
 
     topk_softmax = moe_align_block_size = moe_sum_reduce = _not_served
+    token_logprobs = token_logprobs_backward = moe_balance_loss = moe_router_backward = moe_sum_reduce_backward = _not_served
 
 
 def load_calls():
@@ -175,7 +176,9 @@ def load_calls():
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_torch_calls", loader))
     loader.exec_module(module)
     module.bind(*(ctypes.cast(fn, c_void_p).value for fn in (
-        lib.xkb_topk_softmax, lib.xkb_moe_align_block_size, lib.xkb_moe_align_workspace_bytes, lib.xkb_moe_sum_reduce)))
+        lib.xkb_topk_softmax, lib.xkb_moe_align_block_size, lib.xkb_moe_align_workspace_bytes, lib.xkb_moe_sum_reduce,
+        lib.xkb_token_logprobs, lib.xkb_token_logprobs_backward, lib.xkb_moe_balance_loss,
+        lib.xkb_moe_balance_loss_workspace_bytes, lib.xkb_moe_router_backward, lib.xkb_moe_sum_reduce_backward)))
     _calls = module
     return module
 

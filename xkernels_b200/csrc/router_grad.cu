@@ -5,8 +5,16 @@
 //   q_j = g_j for weights that are probabilities; (g_j - sum_i g_i w_i) / s for weights w_j = p_j / s, s = sum_j p_j
 //
 // A warp holds a row of up to 1024 experts in registers, in pieces of P neighbours (16 bytes where the row allows it).
-// Loss: warps take rows in turn and keep the sum of every expert's probability in registers; a block adds its warps up and
-// leaves one row of partial sums, which a second kernel adds in a fixed order: the result is the same in every run.
+//
+// Loss: warps take rows in turn and keep the sum of every expert's probability in registers.  A block adds its warps up, a
+// cluster of eight its blocks through distributed shared memory, and where there are several clusters a second kernel, which is already
+// resident by then, adds theirs.  Floats are added in a fixed order, only counts by atomics: the same bits in every run.
+//
+// Gradient: bound by instructions, so nothing goes through shared memory.  sum_e p dp splits into sum_e p_e a_e and the slots' part,
+// which is sum_j p_j g_j for raw weights and nothing for renormalised ones (they do not change along p); the row is written
+// with the first part alone, and the lanes that hold a slot put the chosen experts' gradients in afterwards, from logits
+// that they loaded themselves.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -14,8 +22,11 @@
 namespace xkb {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kMaxExperts = 1024;
-constexpr int kWarps = 8;
+constexpr int kWarps = 8;          // of a block of the gradient kernel
+constexpr float kLog2e = 1.44269504088896340736f;
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
@@ -32,12 +43,14 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 __device__ __forceinline__ float warp_max_nan(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v) : "f"(w));
-  }
-  return v;
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float exp_of(float x) {   // e^x to 2^-22 and the rounding of x log2(e); subnormal results are 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * kLog2e));
+  return r;
 }
 
 // A row in registers: the lane's t-th value belongs to expert (t / P * 32 + lane) * P + t % P.
@@ -68,23 +81,23 @@ struct Row {
       if ((c * 32 + lane) * P < E) reinterpret_cast<Piece*>(row)[c * 32 + lane] = q;
     }
   }
-  // logits -> probabilities; a row without a live logit has none: 0 everywhere.  NaN and +inf make the row NaN.
-  static __device__ __forceinline__ void softmax(float (&x)[PER_LANE]) {
+  // logits -> e^(x - max); their maximum (0 for a row without a live logit) and 1 / sum (0 for such a row).  NaN and +inf make
+  // the row NaN.
+  static __device__ __forceinline__ void exponentials(float (&x)[PER_LANE], float& max, float& inv) {
     float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < PER_LANE; ++t) asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(x[t]));
     mx = warp_max_nan(mx);
     const bool dead = mx == -INFINITY;
+    max = dead ? 0.f : mx;
     float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < PER_LANE; ++t) {
-      x[t] = expf(x[t] - (dead ? 0.f : mx));
+      x[t] = exp_of(x[t] - max);
       sum += x[t];
     }
     sum = warp_add(sum);
-    const float inv = dead ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) x[t] *= inv;
+    inv = dead ? 0.f : 1.f / sum;
   }
 };
 
@@ -93,65 +106,133 @@ struct LossArgs {
   const void* gating;
   const int32_t* ids;
   const uint8_t* mask;
-  float* part_p;        // [blocks, E]
-  int32_t* part_c;      // [blocks, E]
-  int32_t* part_t;      // [blocks]
+  float* part_p;        // [parts, E]: of every cluster, where there are several
+  int32_t* part_c;      // [parts, E]
+  int32_t* part_t;      // [parts]
   float* loss;
   int32_t* counts;
   float* mean;
   int32_t* tokens;
   int64_t M;
-  int E, k, blocks;
+  int E, k, parts;
 };
 
+constexpr int kLossWarps = 16;
+constexpr int kCluster = 8;
+
+__device__ __forceinline__ void write_loss(const LossArgs& a, double sum, int T) {
+  *a.loss = T > 0 && a.k > 0 ? (float)(sum * a.E / ((double)a.k * T)) : 0.f;
+  *a.tokens = T;
+}
+
 template <typename T, int PER_LANE, int P>
-__global__ void __launch_bounds__(32 * kWarps)
-balance_partial_kernel(LossArgs a) {
+__global__ void __launch_bounds__(32 * kLossWarps)
+balance_kernel(LossArgs a) {
   using R = Row<T, PER_LANE, P>;
-  __shared__ float s_sum[32 * PER_LANE];
-  __shared__ int s_count[32 * PER_LANE];
+  constexpr int kPlaces = 32 * PER_LANE;
+  __shared__ float s_sum[kLossWarps / 2][kPlaces];
+  __shared__ int s_count[kPlaces];
   __shared__ int s_tokens;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e < 32 * PER_LANE; e += 32 * kWarps) s_count[e] = 0;
-  if (threadIdx.x == 0) s_tokens = 0;
+  __shared__ double s_term;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster.block_rank();
+  chain_trigger();   // the joining kernel may become resident
+  for (int e = threadIdx.x; e < kPlaces; e += 32 * kLossWarps) s_count[e] = 0;
+  if (threadIdx.x == 0) {
+    s_tokens = 0;
+    s_term = 0.0;
+  }
   __syncthreads();
   float acc[PER_LANE];
 #pragma unroll
   for (int t = 0; t < PER_LANE; ++t) acc[t] = 0.f;
   int mine = 0;
-  for (int64_t m = (int64_t)blockIdx.x * kWarps + warp; m < a.M; m += (int64_t)a.blocks * kWarps) {
+  const int64_t step = (int64_t)gridDim.x * kLossWarps;
+#pragma unroll 2
+  for (int64_t m = (int64_t)blockIdx.x * kLossWarps + warp; m < a.M; m += step) {
     if (a.mask != nullptr && a.mask[m] == 0) continue;
     ++mine;
-    float x[PER_LANE];
+    float x[PER_LANE], max, inv;
     R::load(static_cast<const T*>(a.gating) + m * a.E, a.E, lane, x);
     for (int j = lane; j < a.k; j += 32) {
       const int e = a.ids[m * a.k + j];
       if (e >= 0 && e < a.E) atomicAdd(&s_count[e], 1);
     }
-    R::softmax(x);
+    R::exponentials(x, max, inv);
 #pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) acc[t] += x[t];
+    for (int t = 0; t < PER_LANE; ++t) acc[t] = fmaf(x[t], inv, acc[t]);
   }
-  if (lane == 0) atomicAdd(&s_tokens, mine);
-  // one warp after the other, so that the order is fixed
-  for (int w = 0; w < kWarps; ++w) {
-    if (warp == w) {
+  if (lane == 0 && mine != 0) atomicAdd(&s_tokens, mine);
+  // the upper half of the warps hands its sums to the lower half, and so on
+#pragma unroll 1
+  for (int half = kLossWarps / 2; half > 0; half /= 2) {
+    if (warp >= half && warp < 2 * half) {
 #pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) {
-        const int e = R::expert(t, lane);
-        s_sum[e] = w == 0 ? acc[t] : s_sum[e] + acc[t];
-      }
+      for (int t = 0; t < PER_LANE; ++t) s_sum[warp - half][R::expert(t, lane)] = acc[t];
+    }
+    __syncthreads();
+    if (warp < half) {
+#pragma unroll
+      for (int t = 0; t < PER_LANE; ++t) acc[t] += s_sum[warp][R::expert(t, lane)];
     }
     __syncthreads();
   }
-  for (int e = threadIdx.x; e < a.E; e += 32 * kWarps) {
-    a.part_p[(int64_t)blockIdx.x * a.E + e] = s_sum[e];
-    a.part_c[(int64_t)blockIdx.x * a.E + e] = s_count[e];
+  if (warp == 0) {
+#pragma unroll
+    for (int t = 0; t < PER_LANE; ++t) s_sum[0][R::expert(t, lane)] = acc[t];
   }
-  if (threadIdx.x == 0) a.part_t[blockIdx.x] = s_tokens;
+  cluster.sync();
+  // every block joins its share of the experts
+  const int each = (a.E + kCluster - 1) / kCluster, first = rank * each, n = max(0, min(each, a.E - first));
+  const bool alone = gridDim.x == kCluster;
+  const int64_t part = blockIdx.x / kCluster;
+  int tokens = 0;
+#pragma unroll
+  for (int i = 0; i < kCluster; ++i) tokens += *cluster.map_shared_rank(&s_tokens, i);
+  double term = 0.0;
+  if ((int)threadIdx.x < n) {
+    const int e = first + threadIdx.x;
+    float p = 0.f;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kCluster; ++i) {
+      p += cluster.map_shared_rank(&s_sum[0][0], i)[e];
+      c += cluster.map_shared_rank(&s_count[0], i)[e];
+    }
+    if (alone) {
+      const float mean = tokens > 0 ? p / (float)tokens : 0.f;
+      a.mean[e] = mean;
+      a.counts[e] = c;
+      term = (double)c * (double)mean;
+    } else {
+      a.part_p[part * a.E + e] = p;
+      a.part_c[part * a.E + e] = c;
+    }
+  }
+  if (!alone) {
+    if (rank == 0 && threadIdx.x == 0) a.part_t[part] = tokens;
+    cluster.sync();   // the others' shared memory is read until here
+    return;
+  }
+  // n <= 128: four warps have a share
+  if (warp < 4) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
+  }
+  __shared__ double s_warp_term[4];
+  if (warp < 4 && lane == 0) s_warp_term[warp] = term;
+  __syncthreads();
+  if (threadIdx.x == 0) s_term = (s_warp_term[0] + s_warp_term[1]) + (s_warp_term[2] + s_warp_term[3]);
+  cluster.sync();
+  if (rank == 0 && threadIdx.x == 0) {
+    double sum = 0.0;
+    for (int i = 0; i < kCluster; ++i) sum += *cluster.map_shared_rank(&s_term, i);
+    write_loss(a, sum, tokens);
+  }
+  cluster.sync();
 }
 
-// Adds the partial rows up: thread (g, e) takes every G-th block of expert e.
+// Adds the clusters' rows up: thread (g, e) takes every G-th row of expert e.
 __global__ void __launch_bounds__(1024)
 balance_join_kernel(LossArgs a) {
   __shared__ float s_p[1024];
@@ -161,15 +242,20 @@ balance_join_kernel(LossArgs a) {
   const int E = a.E, G = 1024 / E, tid = threadIdx.x, g = tid / E, e = tid - g * E;
   if (tid == 0) s_tokens = 0;
   __syncthreads();
+  chain_wait();
+  // (written by the kernel that this one overlaps: no read-only loads)
+  const volatile float* part_p = a.part_p;
+  const volatile int32_t *part_c = a.part_c, *part_t = a.part_t;
   int t = 0;
-  for (int b = tid; b < a.blocks; b += 1024) t += a.part_t[b];
+  for (int b = tid; b < a.parts; b += 1024) t += part_t[b];
   if (t != 0) atomicAdd(&s_tokens, t);
   float p = 0.f;
   int c = 0;
   if (g < G) {
-    for (int b = g; b < a.blocks; b += G) {
-      p += a.part_p[(int64_t)b * E + e];
-      c += a.part_c[(int64_t)b * E + e];
+#pragma unroll 8
+    for (int b = g; b < a.parts; b += G) {
+      p += part_p[b * E + e];
+      c += part_c[b * E + e];
     }
   }
   s_p[tid] = p;
@@ -188,11 +274,11 @@ balance_join_kernel(LossArgs a) {
   for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
   if ((tid & 31) == 0) s_loss[tid >> 5] = term;
   __syncthreads();
-  if (tid == 0) {
-    double sum = 0.0;
-    for (int i = 0; i < 32; ++i) sum += s_loss[i];
-    *a.loss = T > 0 && a.k > 0 ? (float)(sum * E / ((double)a.k * T)) : 0.f;
-    *a.tokens = T;
+  if (tid < 32) {
+    double sum = s_loss[tid];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (tid == 0) write_loss(a, sum, T);
   }
 }
 
@@ -217,80 +303,97 @@ __global__ void __launch_bounds__(32 * kWarps)
 router_grad_kernel(GateArgs a) {
   using R = Row<T, PER_LANE, P>;
   __shared__ float s_share[32 * PER_LANE];          // the balance loss's part of dp
-  __shared__ float s_row[kWarps][32 * PER_LANE];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* row = s_row[warp];
-  if (a.counts != nullptr) {
+  const bool balance = a.counts != nullptr, weights = a.g_w != nullptr;
+  if (balance) {
     const float n = a.tokens != nullptr ? (float)*a.tokens : (float)a.M;
     const float g = (a.g_loss != nullptr ? *a.g_loss : 1.f) * a.scale;
     const float f = n > 0.f && a.k > 0 ? g * (float)a.E / ((float)a.k * n) / n : 0.f;
     for (int e = threadIdx.x; e < 32 * PER_LANE; e += 32 * kWarps) s_share[e] = e < a.E ? f * (float)a.counts[e] : 0.f;
+    __syncthreads();
   }
-  __syncthreads();
   for (int64_t m = (int64_t)blockIdx.x * kWarps + warp; m < a.M; m += (int64_t)gridDim.x * kWarps) {
-    float p[PER_LANE], dp[PER_LANE];
-    R::load(static_cast<const T*>(a.gating) + m * a.E, a.E, lane, p);
-    const bool counted = a.counts != nullptr && (a.mask == nullptr || a.mask[m] != 0);
+    const T* row = static_cast<const T*>(a.gating) + m * a.E;
+    T* out = static_cast<T*>(a.out) + m * a.E;
+    float x[PER_LANE], max, inv;
+    R::load(row, a.E, lane, x);
+    // slot `lane` of the first 32: expert (-1: none), gradient, logit
+    int e = -1;
+    float g = 0.f, xe = 0.f;
+    if (weights && lane < a.k) {
+      e = a.ids[m * a.k + lane];
+      if (e < 0 || e >= a.E) e = -1;
+      else {
+        g = a.g_w[m * a.k + lane];
+        xe = to_float(row[e]);
+      }
+    }
+    const bool counted = balance && (a.mask == nullptr || a.mask[m] != 0);
     if (!counted) {   // a row that nothing comes back to (padding) has gradient 0, whatever its logits are
-      bool any = false;
-      for (int j = lane; j < a.k && a.g_w != nullptr; j += 32) any |= a.g_w[m * a.k + j] != 0.f;
+      bool any = g != 0.f;
+      if (weights)
+        for (int j = lane + 32; j < a.k; j += 32) {
+          const int o = a.ids[m * a.k + j];
+          any |= o >= 0 && o < a.E && a.g_w[m * a.k + j] != 0.f;
+        }
       if (!__any_sync(0xffffffffu, any)) {
 #pragma unroll
-        for (int t = 0; t < PER_LANE; ++t) p[t] = 0.f;
-        R::store(static_cast<T*>(a.out) + m * a.E, a.E, lane, p);
+        for (int t = 0; t < PER_LANE; ++t) x[t] = 0.f;
+        R::store(out, a.E, lane, x);
         continue;
       }
     }
-    R::softmax(p);
-#pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) dp[t] = counted ? s_share[R::expert(t, lane)] : 0.f;
-    if (a.g_w != nullptr) {
-      __syncwarp();
-#pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) row[R::expert(t, lane)] = p[t];
-      __syncwarp();
-      float sel = 0.f, dot = 0.f;   // of the slots: sum of probabilities, sum of gradient x probability
-      for (int j = lane; j < a.k; j += 32) {
-        const int e = a.ids[m * a.k + j];
-        if (e < 0 || e >= a.E) continue;
-        sel += row[e];
-        dot = fmaf(a.g_w[m * a.k + j], row[e], dot);
+    R::exponentials(x, max, inv);
+    // the chosen probabilities: their sum and their product with the gradients; the balance loss's sum_e p_e a_e
+    float p = e >= 0 ? exp_of(xe - max) * inv : 0.f, sel = p, dot = p * g, even = 0.f;
+    if (weights)
+      for (int j = lane + 32; j < a.k; j += 32) {
+        const int o = a.ids[m * a.k + j];
+        if (o < 0 || o >= a.E) continue;
+        const float po = exp_of(to_float(row[o]) - max) * inv;
+        sel += po;
+        dot = fmaf(po, a.g_w[m * a.k + j], dot);
       }
-      sel = warp_add(sel);
-      dot = warp_add(dot);
-      __syncwarp();
+    if (counted) {
 #pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) row[R::expert(t, lane)] = dp[t];
-      __syncwarp();
-      for (int j0 = 0; j0 < a.k; j0 += 32) {
-        const int j = j0 + lane;
-        int e = -1;
-        float q = 0.f;
-        if (j < a.k) {
-          e = a.ids[m * a.k + j];
-          if (e < 0 || e >= a.E) e = -1;
-          else q = a.g_w[m * a.k + j];
-        }
-        if (a.renorm) q = sel == 0.f ? 0.f : (q - dot / sel) / sel;
-        // an expert that several slots chose takes them one after the other
-        const unsigned same = __match_any_sync(0xffffffffu, e);
-        const int before = __popc(same & ((1u << lane) - 1u));
-        const int rounds = __reduce_max_sync(0xffffffffu, e >= 0 ? before : 0);
-        for (int i = 0; i <= rounds; ++i) {
-          if (e >= 0 && before == i) row[e] += q;
-          __syncwarp();
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) dp[t] = row[R::expert(t, lane)];
+      for (int t = 0; t < PER_LANE; ++t) even = fmaf(x[t], s_share[R::expert(t, lane)], even);
+      even = warp_add(even) * inv;
     }
-    float s = 0.f;
+    if (weights) {
+      dot = warp_add(dot);
+      if (a.renorm) sel = warp_add(sel);
+    }
+    const float s = even + (a.renorm ? 0.f : dot);
 #pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) s = fmaf(p[t], dp[t], s);
-    s = warp_add(s);
-#pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) p[t] *= dp[t] - s;
-    R::store(static_cast<T*>(a.out) + m * a.E, a.E, lane, p);
+    for (int t = 0; t < PER_LANE; ++t) x[t] = x[t] * inv * ((counted ? s_share[R::expert(t, lane)] : 0.f) - s);
+    R::store(out, a.E, lane, x);
+    if (!weights) continue;
+    // q of a slot; an expert that several slots chose takes all of them, in their order
+    const float ratio = dot / sel;
+    auto q_of = [&](float gj) -> float { return !a.renorm ? gj : sel == 0.f ? 0.f : (gj - ratio) / sel; };
+    __syncwarp();   // the stores below come after the row's
+    const float q = e >= 0 ? q_of(g) : 0.f;
+    if (a.k <= 32) {
+      float own = q;
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      if (__any_sync(0xffffffffu, e >= 0 && (same & (same - 1)) != 0)) {
+        own = 0.f;
+        for (int j = 0; j < a.k; ++j) {
+          const float qj = __shfl_sync(0xffffffffu, q, j);
+          if (same >> j & 1) own += qj;
+        }
+      }
+      if (e >= 0) out[e] = of_float<T>(p * ((counted ? s_share[e] : 0.f) + own - s));
+    } else {
+      for (int j = lane; j < a.k; j += 32) {
+        const int o = a.ids[m * a.k + j];
+        if (o < 0 || o >= a.E) continue;
+        float own = 0.f;
+        for (int i = 0; i < a.k; ++i)
+          if (a.ids[m * a.k + i] == o) own += q_of(a.g_w[m * a.k + i]);
+        out[o] = of_float<T>(exp_of(to_float(row[o]) - max) * inv * ((counted ? s_share[o] : 0.f) + own - s));
+      }
+    }
   }
 }
 
@@ -321,8 +424,18 @@ template <typename T> struct LaunchLoss {
   const LossArgs& a;
   cudaStream_t s;
   template <int PER_LANE, int P> int operator()() const {
-    balance_partial_kernel<T, PER_LANE, P><<<a.blocks, 32 * kWarps, 0, s>>>(a);
-    XKB_CHECK_LAUNCH("balance_partial_kernel");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.parts * kCluster));
+    cfg.blockDim = dim3(32 * kLossWarps);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, balance_kernel<T, PER_LANE, P>, a));
+    XKB_CHECK_LAUNCH("balance_kernel");
     return XKB_OK;
   }
 };
@@ -337,10 +450,13 @@ template <typename T> struct LaunchGrad {
   }
 };
 
-constexpr int64_t kMostBlocks = 2 * 148;
-int64_t loss_blocks(int64_t M) {
-  const int64_t b = ceil_div(M, (int64_t)kWarps);
-  return b < 1 ? 1 : b > kMostBlocks ? kMostBlocks : b;
+// Clusters of the loss kernel: one, which needs no second kernel, up to eight rows a warp; two blocks per SM at most.
+constexpr int64_t kMostParts = 2 * 148 / kCluster;
+int64_t loss_parts(int64_t M) {
+  const int64_t rows = kCluster * kLossWarps;
+  if (M <= 8 * rows) return 1;
+  const int64_t p = ceil_div(M, rows);
+  return p > kMostParts ? kMostParts : p;
 }
 
 }  // namespace
@@ -349,8 +465,8 @@ int64_t loss_blocks(int64_t M) {
 extern "C" int64_t xkb_moe_balance_loss_workspace_bytes(int64_t M, int E) {
   using namespace xkb;
   if (M < 0 || E < 1 || E > kMaxExperts) return -1;
-  const int64_t blocks = loss_blocks(M);
-  return 2 * align_up(blocks * E * 4, 256) + align_up(blocks * 4, 256);
+  const int64_t parts = loss_parts(M);
+  return 2 * align_up(parts * E * 4, 256) + align_up(parts * 4, 256);
 }
 
 extern "C" int xkb_moe_balance_loss(const void* gating_output, int dtype, const int32_t* topk_ids, const uint8_t* token_mask,
@@ -366,12 +482,12 @@ extern "C" int xkb_moe_balance_loss(const void* gating_output, int dtype, const 
     return fail(XKB_ERR_WORKSPACE, "moe_balance_loss: the workspace needs %lld bytes (got %lld)",
                 (long long)xkb_moe_balance_loss_workspace_bytes(M, E), (long long)(workspace ? workspace_bytes : 0));
   XKB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "moe_balance_loss: misaligned workspace");
-  const int64_t blocks = loss_blocks(M);
+  const int64_t parts = loss_parts(M);
   Carver ws(workspace);
-  LossArgs a{gating_output, topk_ids, token_mask, nullptr, nullptr, nullptr, loss, counts, mean_probs, tokens, M, E, top_k, (int)blocks};
-  a.part_p = ws.take<float>(blocks * E);
-  a.part_c = ws.take<int32_t>(blocks * E);
-  a.part_t = ws.take<int32_t>(blocks);
+  LossArgs a{gating_output, topk_ids, token_mask, nullptr, nullptr, nullptr, loss, counts, mean_probs, tokens, M, E, top_k, (int)parts};
+  a.part_p = ws.take<float>(parts * E);
+  a.part_c = ws.take<int32_t>(parts * E);
+  a.part_t = ws.take<int32_t>(parts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const uintptr_t bits = reinterpret_cast<uintptr_t>(gating_output);
   int rc;
@@ -380,8 +496,8 @@ extern "C" int xkb_moe_balance_loss(const void* gating_output, int dtype, const 
     case XKB_F32: rc = with_shape<float>(E, bits, LaunchLoss<float>{a, s}); break;
     default: rc = with_shape<__half>(E, bits, LaunchLoss<__half>{a, s}); break;
   }
-  if (rc != XKB_OK) return rc;
-  balance_join_kernel<<<1, 1024, 0, s>>>(a);
+  if (rc != XKB_OK || parts == 1) return rc;
+  XKB_CHECK_CUDA(launch_chained(balance_join_kernel, dim3(1), dim3(1024), 0, s, a));
   XKB_CHECK_LAUNCH("balance_join_kernel");
   return XKB_OK;
 }

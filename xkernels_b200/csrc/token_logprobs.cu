@@ -51,6 +51,31 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 
+// Two fp32 values side by side: one instruction does both.
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair_of(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ Pair pair_of(float v) { return pair_of(v, v); }
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+
 // What a type of logits needs: N elements in 16 bytes, a running maximum of whole vectors, ordered keys.
 //   kClamp: smaller elements count as this, which keeps -inf out of the products.  A row whose maximum is not between kLow
 //   and kHigh, where a clamped element would count or x log2(e) is too coarse, takes the slow pass.
@@ -58,7 +83,7 @@ __device__ __forceinline__ float warp_add(float v) {
 template <typename T> struct Elem;
 
 template <> struct Elem<float> {
-  static constexpr int N = 4, kKeyBits = 32;
+  static constexpr int N = 4;
   static constexpr float kClamp = -1e8f, kLow = -1e6f, kHigh = 1e6f;
   using Max = float;
   static __device__ __forceinline__ Max lowest() { return -INFINITY; }
@@ -92,7 +117,7 @@ template <> struct Elem<float> {
 };
 
 template <> struct Elem<__nv_bfloat16> {
-  static constexpr int N = 8, kKeyBits = 16;
+  static constexpr int N = 8;
   static constexpr float kClamp = -1e8f, kLow = -1e6f, kHigh = 1e6f;
   using Max = __nv_bfloat162;
   static __device__ __forceinline__ Max as2(uint32_t u) { return *reinterpret_cast<Max*>(&u); }
@@ -133,7 +158,7 @@ template <> struct Elem<__nv_bfloat16> {
 };
 
 template <> struct Elem<__half> {
-  static constexpr int N = 8, kKeyBits = 16;
+  static constexpr int N = 8;
   static constexpr float kClamp = -65504.f, kLow = -60000.f, kHigh = 1e6f;
   using Max = __half2;
   static __device__ __forceinline__ Max as2(uint32_t u) { return *reinterpret_cast<Max*>(&u); }
@@ -221,39 +246,67 @@ struct Sums {
   }
 };
 
+// S and T of the even and of the odd places of a vector
+struct PairSums { Pair S, T; };
+
 template <typename T>
-__device__ __forceinline__ void add_vector(const uint4& q, Sums& s) {
+__device__ __forceinline__ void add_vector(const uint4& q, Pair minus_c, PairSums& s) {
   constexpr int N = Elem<T>::N;
   float v[N];
   Elem<T>::clamped(q, v);
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = fmaf(v[i], kLog2e, -s.c), e = exp2_fast(y);
-    s.S += e;
-    s.T = fmaf(e, y, s.T);
+  for (int i = 0; i < N; i += 2) {
+    const Pair y = fma2(pair_of(v[i], v[i + 1]), pair_of(kLog2e), minus_c);
+    float y0, y1;
+    split(y, y0, y1);
+    const Pair e = pair_of(exp2_fast(y0), exp2_fast(y1));
+    s.S = add2(s.S, e);
+    s.T = fma2(e, y, s.T);
   }
 }
 
-// The largest key t of which at least k of the block's keys are >= t (one key a thread; 0 if there are fewer than k above 0).
-template <int BITS>
-__device__ __forceinline__ uint32_t kth_largest(uint32_t key, int k) {
-  uint32_t t = 0;
-#pragma unroll 1
-  for (int b = BITS - 1; b >= 0; --b) {
-    const uint32_t trial = t | (1u << b);
-    if (__syncthreads_count(key >= trial) >= k) t = trial;
+// The largest key t of which at least k of the n keys are >= t (0 if fewer than k are above 0): a search by two bits at a time
+// from the first one in which the keys differ, by one warp that holds the keys in registers.
+template <int THREADS>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t* keys, int k) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[THREADS / 32], most = 0, least = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) {
+    key[i] = keys[i * 32 + lane];
+    most = max(most, key[i]);
+    least = min(least, key[i]);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (most == least) return most;
+  int b = (31 - __clz(most ^ least)) & ~1;         // the upper of two bits is b + 1
+  uint32_t t = b == 30 ? 0u : most >> (b + 2) << (b + 2);
+  for (; b >= 0; b -= 2) {
+    uint32_t n = 0;   // how many reach t + 1, t + 2, t + 3 in units of this step: fields of ten bits (THREADS < 1024)
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+      // (equal bits above the step: everything that is not below t)
+      const uint32_t d = key[i] >= t ? min((key[i] - t) >> b, 3u) : 0u;
+      n += d == 0 ? 0u : d == 1 ? 1u : d == 2 ? 1u + (1u << 10) : 1u + (1u << 10) + (1u << 20);
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    const uint32_t step = (int)(n >> 20) >= k ? 3u : (int)(n >> 10 & 1023u) >= k ? 2u : (int)(n & 1023u) >= k ? 1u : 0u;
+    t += step << b;
   }
   return t;
 }
 
-constexpr int kBatch = 4;   // vectors a thread requests before it uses the first
+constexpr int kBatch = 4;   // vectors a thread requests before it uses the first (select_top names them one by one)
 
 template <int THREADS>
 struct TopScratch {
   uint64_t cand[8 * THREADS + kMaxTop];   // value key, ~column: all different, larger is better
   uint64_t top[kMaxTop];                  // the CTA's best ones, in order
+  uint32_t key[THREADS];                  // of every thread
   int owner[THREADS];                     // threads whose elements are read again
-  int n, owners;
+  int n, owners, want;
+  uint32_t bound;
 };
 template <int THREADS> struct NoScratch {};
 
@@ -305,12 +358,24 @@ template <typename T, int THREADS>
 __device__ void select_top(const RowView<T>& r, int lo, int hi, uint32_t best, int k, TopScratch<THREADS>& s) {
   constexpr int N = Elem<T>::N;
   const int tid = threadIdx.x, per = (hi - lo + THREADS - 1) / THREADS;   // vectors of a thread, at most
-  const uint32_t bound = kth_largest<Elem<T>::kKeyBits>(best, k);
-  // Equal maxima: of more threads than are needed those count whose first element of that value comes first.
+  s.key[tid] = best;
+  __syncthreads();
+  if (tid < 32) {
+    const uint32_t t = kth_largest<THREADS>(s.key, k);
+    if (tid == 0) {
+      s.bound = t;
+      s.n = s.owners = s.want = 0;
+    }
+  }
+  __syncthreads();
+  const uint32_t bound = s.bound;
+  // Several threads may share the bound.  A few too many are taken; of a crowd (rows of equal logits) only those whose first
+  // element of that value comes first, which each looks for in its own vectors.
   uint32_t last = 0xffffffffu;   // an element equal to the bound counts up to this column
   bool mine = best > 0 && best >= bound;
-  const int above = __syncthreads_count(best > bound), ties = __syncthreads_count(best > 0 && best == bound);
-  if (bound > 0 && above + ties > k) {
+  const int reach = __syncthreads_count(mine);
+  if (bound > 0 && reach > 2 * k + 32) {
+    const int above = __syncthreads_count(best > bound);
     uint32_t at = 0xffffffffu;
     if (best == bound) {
       for (int j = lo + tid; j < hi && at == 0xffffffffu; j += THREADS) {
@@ -323,40 +388,79 @@ __device__ void select_top(const RowView<T>& r, int lo, int hi, uint32_t best, i
         }
       }
     }
-    last = ~kth_largest<32>(best == bound ? ~at : 0u, k - above);
+    s.key[tid] = best == bound ? ~at : 0u;
+    __syncthreads();
+    if (tid < 32) {
+      const uint32_t t = kth_largest<THREADS>(s.key, k - above);
+      if (tid == 0) s.bound = t;
+    }
+    __syncthreads();
+    last = ~s.bound;
     mine = best > bound || (best == bound && at <= last);
   }
-  if (tid == 0) s.n = s.owners = 0;
-  __syncthreads();
   if (mine) s.owner[atomicAdd(&s.owners, 1)] = tid;
   __syncthreads();
   const int items = s.owners * per;
-  for (int base = 0; base < items; base += THREADS) {
-    if (base > 0) {   // room for a whole round: what is there is cut down to k
-      __syncthreads();
-      const int have = s.n;
-      __syncthreads();
-      if (have > kMaxTop) keep_best<THREADS>(s, k);
-    }
-    const int it = base + tid;
-    if (it < items) {
-      const int j = lo + s.owner[it / per] + it % per * THREADS;
-      if (j < hi) {
-        float v[N];
-        Elem<T>::unpack(r.load(j, 0.f), v);
+  auto counts = [&](float v, int col) -> bool {
+    const uint32_t key = Elem<T>::key_of(v);
+    return col >= 0 && col < r.V && (key > bound || (key == bound && (uint32_t)col <= last));
+  };
+  auto push = [&](float v, int col) {
+    s.cand[atomicAdd(&s.n, 1)] = (uint64_t)Elem<T>::key_of(v) << 32 | (uint32_t)~(uint32_t)col;
+  };
+  for (int base = 0; base < items; base += kBatch * THREADS) {
+    // some vectors of every thread at once, their candidates counted before any is put down
+    uint4 q[kBatch];
+    int at[kBatch], n = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t key = Elem<T>::key_of(v[i]);
-          const int col = r.column(j) + i;
-          if (col >= 0 && col < r.V && (key > bound || (key == bound && (uint32_t)col <= last)))
-            s.cand[atomicAdd(&s.n, 1)] = (uint64_t)key << 32 | (uint32_t)~(uint32_t)col;
+    for (int u = 0; u < kBatch; ++u) {
+      const int it = base + u * THREADS + tid;
+      at[u] = -1;
+      if (it < items) {
+        const int j = lo + s.owner[it / per] + it % per * THREADS;
+        if (j < hi) {
+          at[u] = j;
+          q[u] = r.load(j, 0.f);
         }
       }
     }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (at[u] < 0) continue;
+      float v[N];
+      Elem<T>::unpack(q[u], v);
+#pragma unroll
+      for (int i = 0; i < N; ++i) n += counts(v[i], r.column(at[u]) + i);
+    }
+    if (n > 0) atomicAdd(&s.want, n);
+    __syncthreads();
+    const int have = s.n, want = s.want;
+    __syncthreads();
+    if (tid == 0) s.want = 0;
+    const bool fits = have + want <= 8 * THREADS + kMaxTop;
+#pragma unroll 1
+    for (int u = 0; u < kBatch; ++u) {
+      if (!fits) {   // one vector a thread at a time, what is there cut down to k before
+        __syncthreads();
+        const int now = s.n;
+        __syncthreads();
+        if (now > kMaxTop) keep_best<THREADS>(s, k);
+      }
+      const int j = u == 0 ? at[0] : u == 1 ? at[1] : u == 2 ? at[2] : at[3];
+      if (j < 0 || n == 0) continue;
+      const uint4 w = u == 0 ? q[0] : u == 1 ? q[1] : u == 2 ? q[2] : q[3];
+      float v[N];
+      Elem<T>::unpack(w, v);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (counts(v[i], r.column(j) + i)) push(v[i], r.column(j) + i);
+    }
+    __syncthreads();
   }
+  const int found = s.n;
   __syncthreads();
-  if (s.n > THREADS) keep_best<THREADS>(s, k);
-  rank_all<THREADS>(s.cand, s.n, k, s.top);
+  if (found > THREADS) keep_best<THREADS>(s, k);
+  rank_all<THREADS>(s.cand, found > THREADS ? k : found, k, s.top);
 }
 
 struct LogprobArgs {
@@ -388,17 +492,14 @@ token_logprobs_kernel(LogprobArgs a) {
   const RowView<T> r(static_cast<const T*>(a.logits) + m * a.ld, a.V);
   const int per = (r.vectors + C - 1) / C, lo = rank * per, hi = min(lo + per, r.vectors);
 
-  // the given token's logit, early
-  float given = 0.f;
+  // the given token: requested here, its logit behind the pass, both used at the end
   int64_t id = 0;
-  if (rank == 0 && tid == 0) {
-    id = id_at(a.ids, a.ids64, m);
-    if (id >= 0 && id < a.V) given = Elem<T>::load(r.row + id);
-  }
+  if (rank == 0 && tid == 0) id = id_at(a.ids, a.ids64, m);
 
   using Max = typename Elem<T>::Max;
   Max best = Elem<T>::lowest();
-  Sums s{Elem<T>::kLow * kLog2e, 0.f, 0.f};
+  float c = Elem<T>::kLow * kLog2e;
+  PairSums sums{pair_of(0.f), pair_of(0.f)};
   float move = -INFINITY;   // a maximum above this moves c
   for (int j0 = lo; j0 < hi; j0 += kBatch * THREADS) {
     uint4 q[kBatch];
@@ -426,10 +527,25 @@ token_logprobs_kernel(LogprobArgs a) {
     const float top = Elem<T>::value(here);
     if (top > move) {
       move = top + kSlack;
-      s.move_to(fmaxf(top, Elem<T>::kLow) * kLog2e);
+      const float to = fmaxf(top, Elem<T>::kLow) * kLog2e, d = c - to;
+      const Pair f = pair_of(exp2_fast(d));
+      sums.T = mul2(fma2(pair_of(d), sums.S, sums.T), f);
+      sums.S = mul2(sums.S, f);
+      c = to;
     }
+    const Pair minus_c = pair_of(-c);
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) add_vector<T>(q[u], s);
+    for (int u = 0; u < kBatch; ++u) add_vector<T>(q[u], minus_c, sums);
+  }
+  float given = 0.f;
+  if (rank == 0 && tid == 0 && id >= 0 && id < a.V) given = Elem<T>::load(r.row + id);
+  Sums s{c, 0.f, 0.f};
+  {
+    float s0, s1, t0, t1;
+    split(sums.S, s0, s1);
+    split(sums.T, t0, t1);
+    s.S = s0 + s1;
+    s.T = t0 + t1;
   }
 
   // the CTA's sums, at the reference of its maximum
@@ -458,13 +574,15 @@ token_logprobs_kernel(LogprobArgs a) {
   }
   __syncthreads();
 
-  // the row's
-  float row_max = s_part.x;
+  // the row's: the parts of all CTAs, one a lane
+  float4 part = s_part;
   if (C > 1) {
     cluster.sync();
-    row_max = -INFINITY;
-    for (int i = 0; i < C; ++i) row_max = max_nan(row_max, cluster.map_shared_rank(&s_part, i)->x);
+    part = none;
+    if (lane < C) part = *cluster.map_shared_rank(&s_part, lane);
+    part = joined(part);
   }
+  const float row_max = part.x;
   float l, H;
   const bool odd = row_max != row_max || row_max == INFINITY, dead = row_max == -INFINITY;
   if (!odd && !dead && (row_max < Elem<T>::kLow || row_max > Elem<T>::kHigh)) {
@@ -505,19 +623,13 @@ token_logprobs_kernel(LogprobArgs a) {
   } else if (dead) {
     l = H = 0.f;
   } else {
-    const float c = row_max * kLog2e;
-    float S = 0.f, Tl = 0.f;
-    for (int i = 0; i < C; ++i) {
-      const float4 p = C > 1 ? *cluster.map_shared_rank(&s_part, i) : s_part;
-      Sums t{p.y, p.z, p.w};
-      t.move_to(c);
-      S += t.S;
-      Tl += t.T;
-    }
-    // c is row_max log2(e) but for its rounding, which is in every e: ln sum exp(x - row_max) = ln2 (log2 S + c - row_max log2(e))
-    const float off = -fmaf(row_max, kLog2e, -c), log2s = log2f(S);
+    const float at_max = row_max * kLog2e;
+    Sums t{part.y, part.z, part.w};
+    t.move_to(at_max);
+    // at_max is row_max log2(e) but for its rounding, which is in every e: ln sum exp(x - row_max) = ln2 (log2 S + at_max - row_max log2(e))
+    const float off = -fmaf(row_max, kLog2e, -at_max), log2s = log2f(t.S);
     l = (log2s + off) * kLn2;
-    H = fmaxf((log2s - Tl / S) * kLn2, 0.f);
+    H = fmaxf((log2s - t.T / t.S) * kLn2, 0.f);
   }
   if (rank == 0 && tid == 0) {
     float lp = given - row_max - l;
@@ -610,13 +722,19 @@ token_logprobs_grad_kernel(GradArgs a) {
   __syncthreads();
   float G = 0.f;
   for (int i = 0; i <= a.top_k; ++i) G += s_g[i];
-  const float base = fmaf(gh, h, G);
+  // -p (G + gh (ln p + h)) with ln p = x - mx - l: any value
   const bool dead = mx == -INFINITY;
+  const float base = fmaf(gh, h, G);
   auto gradient = [&](float x) -> float {
-    const float lp = max_nan(x - mx - l, -200.f);   // 2^-288 is 0
-    const float p = exp2_fast(lp * kLog2e);
-    return dead ? 0.f : -p * fmaf(gh, lp, base);
+    const float lp = max_nan(x - mx - l, -200.f);   // e^-200 is 0
+    return dead ? 0.f : -exp2_fast(lp * kLog2e) * fmaf(gh, lp, base);
   };
+  // The same as 2^y (slope y + level), y = x log2(e) - c: half the instructions, for maxima whose log2(e) multiple is fine
+  // enough.  c is mx log2(e) rounded; what the rounding left, and e^-l, are in the factor.
+  const bool near = mx >= Elem<T>::kLow && mx <= Elem<T>::kHigh;
+  const float c = mx * kLog2e, rest = -fmaf(mx, kLog2e, -c);
+  const float scale = -exp2f(rest) * expf(-l);
+  const Pair slope = pair_of(scale * gh * kLn2), level = pair_of(scale * fmaf(gh, fmaf(rest, kLn2, -l) + h, G)), minus_c = pair_of(-c);
   for (int j0 = lo; j0 < hi; j0 += kBatch * kGradThreads) {
     uint4 q[kBatch];
 #pragma unroll
@@ -629,9 +747,20 @@ token_logprobs_grad_kernel(GradArgs a) {
       const int j = j0 + u * kGradThreads + tid;
       if (j >= hi) continue;
       float v[N];
-      Elem<T>::unpack(q[u], v);
+      if (near) {
+        Elem<T>::clamped(q[u], v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = gradient(v[i]);
+        for (int i = 0; i < N; i += 2) {
+          const Pair y = fma2(pair_of(v[i], v[i + 1]), pair_of(kLog2e), minus_c);
+          float y0, y1;
+          split(y, y0, y1);
+          split(mul2(pair_of(exp2_fast(y0), exp2_fast(y1)), fma2(y, slope, level)), v[i], v[i + 1]);
+        }
+      } else {
+        Elem<T>::unpack(q[u], v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = gradient(v[i]);
+      }
       if (r.whole(j)) {
         *(reinterpret_cast<uint4*>(out - r.skew) + j) = Elem<T>::pack(v);
       } else {

@@ -1,7 +1,7 @@
-// The call path of the small ops (router, routing sort, top-k reduce) from Python: checks, output tensors and the
-// C-ABI call in one native function.
+// The call path of the small ops (router, routing sort, top-k reduce, losses and gradients) from Python: checks, output
+// tensors and the C-ABI call in one native function.
 //
-// These ops take 3 to 10 us on the device and a call through Python and ctypes 9 to 18 us of host time, which therefore
+// These ops often take 3 to 10 us on the device and a call through Python and ctypes 9 to 18 us of host time, which therefore
 // was what a caller waited for.  A function here serves the plain call - ordinary contiguous CUDA tensors on the current
 // device, arguments of the plain Python types, no dispatch or function mode - and returns None for any other, which the
 // Python form then handles or refuses as it always has.  A failing C call returns its status.
@@ -25,16 +25,22 @@ decltype(&xkb_topk_softmax) g_topk_softmax;
 decltype(&xkb_moe_align_block_size) g_align;
 decltype(&xkb_moe_align_workspace_bytes) g_align_bytes;
 decltype(&xkb_moe_sum_reduce) g_sum_reduce;
+decltype(&xkb_token_logprobs) g_logprobs;
+decltype(&xkb_token_logprobs_backward) g_logprobs_grad;
+decltype(&xkb_moe_balance_loss) g_balance;
+decltype(&xkb_moe_balance_loss_workspace_bytes) g_balance_bytes;
+decltype(&xkb_moe_router_backward) g_router_grad;
+decltype(&xkb_moe_sum_reduce_backward) g_sum_reduce_grad;
 
 bool modes_active() {
   return at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set();
 }
 
 // The tensor behind `obj` if it is a plain one, else nullptr.
-const at::Tensor* plain(PyObject* obj) {
+const at::Tensor* plain(PyObject* obj, bool contiguous = true) {
   if (!THPVariable_CheckExact(obj)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(obj);
-  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || !t.is_contiguous() || t.is_neg() ||
+  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || (contiguous && !t.is_contiguous()) || t.is_neg() ||
       t.is_conj() || t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                                               c10::DispatchKey::FuncTorchGradWrapper,
                                                               c10::DispatchKey::Functionalize})) ||
@@ -52,6 +58,48 @@ bool plain_int(PyObject* obj, int64_t* value) {
   int overflow = 0;
   *value = PyLong_AsLongLongAndOverflow(obj, &overflow);
   return overflow == 0;
+}
+
+// None, or a plain tensor of this type and shape (shape[1] < 0: a vector); false for anything else
+bool optional(PyObject* obj, at::ScalarType type, int64_t rows, int64_t cols, const at::Tensor** out) {
+  *out = nullptr;
+  if (obj == Py_None) return true;
+  const at::Tensor* t = plain(obj);
+  if (t == nullptr || t->scalar_type() != type || t->dim() != (cols < 0 ? 1 : 2) || t->size(0) != rows ||
+      (cols >= 0 && t->size(1) != cols))
+    return false;
+  *out = t;
+  return true;
+}
+// the same with one element, whatever the dimensions
+bool optional_scalar(PyObject* obj, at::ScalarType type, const at::Tensor** out) {
+  *out = nullptr;
+  if (obj == Py_None) return true;
+  const at::Tensor* t = plain(obj);
+  if (t == nullptr || t->scalar_type() != type || t->numel() != 1) return false;
+  *out = t;
+  return true;
+}
+template <typename T> const T* data(const at::Tensor* t) { return t == nullptr ? nullptr : static_cast<const T*>(t->const_data_ptr()); }
+
+// A head's logits [M, V], rows of neighbouring columns, and the tokens [M] given for them.
+const at::Tensor* head(PyObject* obj) {
+  const at::Tensor* t = plain(obj, false);
+  return t != nullptr && t->dim() == 2 && t->size(1) >= 1 && t->stride(1) == 1 && code_of(t->scalar_type()) >= 0 ? t : nullptr;
+}
+bool tokens_of(PyObject* obj, int64_t M, const at::Tensor** out) {
+  return optional(obj, at::kLong, M, -1, out) || optional(obj, at::kInt, M, -1, out);
+}
+const at::Tensor* gating(PyObject* obj) {
+  const at::Tensor* t = plain(obj);
+  return t != nullptr && t->dim() == 2 && t->size(1) >= 1 && t->size(1) <= 1024 && code_of(t->scalar_type()) >= 0 ? t : nullptr;
+}
+const at::Tensor* chosen(PyObject* obj, int64_t M) {
+  const at::Tensor* t = plain(obj);
+  return t != nullptr && t->dim() == 2 && t->size(0) == M && t->size(1) <= 0x7fffffff && t->scalar_type() == at::kInt ? t : nullptr;
+}
+bool mask_of(PyObject* obj, int64_t M, const at::Tensor** out) {
+  return optional(obj, at::kBool, M, -1, out) || optional(obj, at::kByte, M, -1, out);
 }
 
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -156,11 +204,166 @@ PyObject* moe_sum_reduce(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(topk_softmax, align, align_workspace_bytes, sum_reduce): the library's functions, as addresses
+// token_logprobs(logits [M, V], token_ids [M], top_k) -> (logprobs, entropy, stats, top_logprobs, top_ids)
+PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  int64_t top_k;
+  const at::Tensor* ids;
+  if (n != 3 || modes_active() || !plain_int(args[2], &top_k)) Py_RETURN_NONE;
+  const at::Tensor* x = head(args[0]);
+  if (x == nullptr || args[1] == Py_None || !tokens_of(args[1], x->size(0), &ids)) Py_RETURN_NONE;
+  const int64_t M = x->size(0), V = x->size(1);
+  if (top_k < 0 || top_k > 64 || top_k > V) Py_RETURN_NONE;
+  const at::TensorOptions f = x->options().dtype(at::kFloat);
+  at::Tensor lp = at::empty({M}, f), entropy = at::empty({M}, f), stats = at::empty({M, 2}, f), top_lp = at::empty({M, top_k}, f),
+             top_ids = at::empty({M, top_k}, f.dtype(at::kInt));
+  const int code = code_of(x->scalar_type()), ids64 = ids->scalar_type() == at::kLong;
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_logprobs(x->const_data_ptr(), code, x->stride(0), ids->const_data_ptr(), ids64, static_cast<float*>(lp.mutable_data_ptr()),
+                      static_cast<float*>(entropy.mutable_data_ptr()), static_cast<float*>(stats.mutable_data_ptr()),
+                      static_cast<float*>(top_lp.mutable_data_ptr()), static_cast<int32_t*>(top_ids.mutable_data_ptr()), M, V,
+                      (int)top_k, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  return tuple_of(THPVariable_Wrap(std::move(lp)), THPVariable_Wrap(std::move(entropy)), THPVariable_Wrap(std::move(stats)),
+                  THPVariable_Wrap(std::move(top_lp)), THPVariable_Wrap(std::move(top_ids)));
+  END_HANDLE_TH_ERRORS
+}
+
+// token_logprobs_backward(logits, token_ids, stats, entropy, grad_logprobs, grad_entropy, top_ids, grad_top_logprobs)
+// -> [M, V]; rows that do not start on 16 bytes are the Python form's
+PyObject* token_logprobs_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || modes_active() || (args[4] == Py_None && args[5] == Py_None && args[7] == Py_None)) Py_RETURN_NONE;
+  const at::Tensor *ids, *stats, *entropy, *g_lp, *g_entropy, *top_ids = nullptr, *g_top = nullptr;
+  const at::Tensor* x = head(args[0]);
+  if (x == nullptr) Py_RETURN_NONE;
+  const int64_t M = x->size(0), V = x->size(1), es = x->element_size();
+  if (args[2] == Py_None || !tokens_of(args[1], M, &ids) || !optional(args[2], at::kFloat, M, 2, &stats) ||
+      !optional(args[4], at::kFloat, M, -1, &g_lp) || !optional(args[5], at::kFloat, M, -1, &g_entropy) ||
+      !optional(args[3], at::kFloat, M, -1, &entropy) || (g_lp != nullptr && ids == nullptr) || (g_entropy != nullptr && entropy == nullptr))
+    Py_RETURN_NONE;
+  int64_t top_k = 0;
+  if (args[7] != Py_None) {
+    g_top = plain(args[7]);
+    if (g_top == nullptr || g_top->dim() != 2 || g_top->size(0) != M || g_top->size(1) > 64 || g_top->scalar_type() != at::kFloat ||
+        args[6] == Py_None || !optional(args[6], at::kInt, M, g_top->size(1), &top_ids))
+      Py_RETURN_NONE;
+    top_k = g_top->size(1);
+  }
+  if (reinterpret_cast<uintptr_t>(x->const_data_ptr()) % 16 != 0 || (M > 1 && (x->stride(0) - V) * es % 16 != 0)) Py_RETURN_NONE;
+  at::Tensor out = at::empty({M, V}, x->options());
+  const int code = code_of(x->scalar_type()), ids64 = ids != nullptr && ids->scalar_type() == at::kLong;
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_logprobs_grad(x->const_data_ptr(), code, x->stride(0), data<void>(ids), ids64, data<float>(stats),
+                           g_entropy != nullptr ? data<float>(entropy) : nullptr, data<float>(g_lp), data<float>(g_entropy),
+                           top_k != 0 ? data<int32_t>(top_ids) : nullptr, top_k != 0 ? data<float>(g_top) : nullptr, (int)top_k,
+                           out.mutable_data_ptr(), V, M, V, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// moe_balance_loss(gating [M, E], topk_ids [M, top_k], token_mask [M] or None) -> (loss, counts, mean_probs, tokens)
+PyObject* moe_balance_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* mask;
+  if (n != 3 || modes_active()) Py_RETURN_NONE;
+  const at::Tensor* x = gating(args[0]);
+  const at::Tensor* ids = x == nullptr ? nullptr : chosen(args[1], x->size(0));
+  if (ids == nullptr || !mask_of(args[2], x->size(0), &mask)) Py_RETURN_NONE;
+  const int64_t M = x->size(0), E = x->size(1), ws_bytes = g_balance_bytes(M, (int)E);
+  const at::TensorOptions f = x->options().dtype(at::kFloat), i = f.dtype(at::kInt);
+  at::Tensor loss = at::empty({}, f), counts = at::empty({E}, i), mean = at::empty({E}, f), tokens = at::empty({}, i),
+             ws = at::empty({ws_bytes}, f.dtype(at::kByte));
+  const int code = code_of(x->scalar_type()), top_k = (int)ids->size(1);
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_balance(x->const_data_ptr(), code, data<int32_t>(ids), data<uint8_t>(mask), static_cast<float*>(loss.mutable_data_ptr()),
+                     static_cast<int32_t*>(counts.mutable_data_ptr()), static_cast<float*>(mean.mutable_data_ptr()),
+                     static_cast<int32_t*>(tokens.mutable_data_ptr()), M, (int)E, top_k, ws.mutable_data_ptr(), ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  return tuple_of(THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(counts)), THPVariable_Wrap(std::move(mean)),
+                  THPVariable_Wrap(std::move(tokens)));
+  END_HANDLE_TH_ERRORS
+}
+
+// moe_router_backward(gating, topk_ids, grad_weights, renormalize, counts, tokens, grad_loss, token_mask) -> [M, E]
+PyObject* moe_router_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *g_w, *counts, *tokens, *g_loss, *mask;
+  if (n != 8 || modes_active() || !PyBool_Check(args[3]) || (args[2] == Py_None && args[4] == Py_None)) Py_RETURN_NONE;
+  const at::Tensor* x = gating(args[0]);
+  const at::Tensor* ids = x == nullptr ? nullptr : chosen(args[1], x->size(0));
+  if (ids == nullptr) Py_RETURN_NONE;
+  const int64_t M = x->size(0), E = x->size(1);
+  float scale = 1.f;
+  PyObject* loss = args[6];
+  if (PyFloat_CheckExact(loss)) {
+    scale = (float)PyFloat_AS_DOUBLE(loss);
+    loss = Py_None;
+  }
+  if (!optional(args[2], at::kFloat, M, ids->size(1), &g_w) || !optional(args[4], at::kInt, E, -1, &counts) ||
+      !optional_scalar(args[5], at::kInt, &tokens) || !optional_scalar(loss, at::kFloat, &g_loss) || !mask_of(args[7], M, &mask) ||
+      (counts == nullptr && (args[5] != Py_None || args[6] != Py_None)))
+    Py_RETURN_NONE;
+  at::Tensor out = at::empty({M, E}, x->options());
+  const int code = code_of(x->scalar_type()), renorm = args[3] == Py_True, top_k = (int)ids->size(1);
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_router_grad(x->const_data_ptr(), code, data<int32_t>(ids), data<float>(g_w), renorm, data<int32_t>(counts),
+                         data<int32_t>(tokens), data<float>(g_loss), scale, data<uint8_t>(mask), out.mutable_data_ptr(), M, (int)E,
+                         top_k, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// moe_sum_reduce_backward(grad_out [M, H], y [M, top_k, H], w or None, factor, need_grad_y, need_grad_w) -> (grad_y, grad_w)
+PyObject* moe_sum_reduce_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || modes_active() || !PyFloat_CheckExact(args[3]) || !PyBool_Check(args[4]) || !PyBool_Check(args[5])) Py_RETURN_NONE;
+  const at::Tensor *y = plain(args[1]), *w = nullptr, *go;
+  if (y == nullptr || y->dim() != 3 || (y->scalar_type() != at::kBFloat16 && y->scalar_type() != at::kFloat)) Py_RETURN_NONE;
+  const int64_t M = y->size(0), top_k = y->size(1), H = y->size(2);
+  if (args[0] == Py_None || !optional(args[0], y->scalar_type(), M, H, &go) || top_k > 0x7fffffff ||
+      !(optional(args[2], at::kFloat, M, top_k, &w) || optional(args[2], at::kBFloat16, M, top_k, &w)))
+    Py_RETURN_NONE;
+  const bool need_y = args[4] == Py_True, need_w = args[5] == Py_True && w != nullptr;
+  at::Tensor gy, gw;
+  if (need_y) gy = at::empty({M, top_k, H}, y->options());
+  if (need_w) gw = at::empty({M, top_k}, w->options());
+  const int code = code_of(y->scalar_type()), w_code = w == nullptr ? XKB_F32 : code_of(w->scalar_type());
+  const float factor = (float)PyFloat_AS_DOUBLE(args[3]);
+  void* const stream = stream_of(*y);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_sum_reduce_grad(go->const_data_ptr(), code, need_w ? y->const_data_ptr() : nullptr, data<void>(w), w_code,
+                             need_y ? gy.mutable_data_ptr() : nullptr, need_w ? gw.mutable_data_ptr() : nullptr, M, (int)top_k, H,
+                             factor, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  PyObject* a = need_y ? THPVariable_Wrap(std::move(gy)) : Py_NewRef(Py_None);
+  PyObject* b = need_w ? THPVariable_Wrap(std::move(gw)) : Py_NewRef(Py_None);
+  return tuple_of(a, b);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(...): the library's functions, as addresses, in the order of the pointers above
+constexpr Py_ssize_t kFunctions = 10;
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 4) { PyErr_SetString(PyExc_TypeError, "bind: four addresses expected"); return nullptr; }
-  void* p[4];
-  for (int i = 0; i < 4; ++i) {
+  if (n != kFunctions) { PyErr_SetString(PyExc_TypeError, "bind: another number of addresses expected"); return nullptr; }
+  void* p[kFunctions];
+  for (Py_ssize_t i = 0; i < kFunctions; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (p[i] == nullptr) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
@@ -171,6 +374,12 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_align = reinterpret_cast<decltype(g_align)>(p[1]);
   g_align_bytes = reinterpret_cast<decltype(g_align_bytes)>(p[2]);
   g_sum_reduce = reinterpret_cast<decltype(g_sum_reduce)>(p[3]);
+  g_logprobs = reinterpret_cast<decltype(g_logprobs)>(p[4]);
+  g_logprobs_grad = reinterpret_cast<decltype(g_logprobs_grad)>(p[5]);
+  g_balance = reinterpret_cast<decltype(g_balance)>(p[6]);
+  g_balance_bytes = reinterpret_cast<decltype(g_balance_bytes)>(p[7]);
+  g_router_grad = reinterpret_cast<decltype(g_router_grad)>(p[8]);
+  g_sum_reduce_grad = reinterpret_cast<decltype(g_sum_reduce_grad)>(p[9]);
   Py_RETURN_NONE;
 }
 
@@ -179,7 +388,10 @@ PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)), METH_FASTCALL, nullptr};
 }
 PyMethodDef g_methods[] = {method<topk_softmax>("topk_softmax"), method<moe_align_block_size>("moe_align_block_size"),
-                           method<moe_sum_reduce>("moe_sum_reduce"), method<bind>("bind"), {nullptr, nullptr, 0, nullptr}};
+                           method<moe_sum_reduce>("moe_sum_reduce"), method<token_logprobs>("token_logprobs"),
+                           method<token_logprobs_backward>("token_logprobs_backward"), method<moe_balance_loss>("moe_balance_loss"),
+                           method<moe_router_backward>("moe_router_backward"),
+                           method<moe_sum_reduce_backward>("moe_sum_reduce_backward"), method<bind>("bind"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -347,6 +347,11 @@ def moe_sum_reduce_backward(grad_out, y, w=None, routed_scaling_factor=1.0, need
     order.  What is not wanted, and ``grad_w`` without ``w``, is None.  No reference counterpart: the reference's
     pure-torch form is differentiated by torch.
     """
+    got = (_lib._calls or _lib.load_calls()).moe_sum_reduce_backward(grad_out, y, w, routed_scaling_factor, need_grad_y, need_grad_w)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_moe_sum_reduce_backward")
+        return got
     lib = _lib.load()
     dev = _require_cuda("moe_sum_reduce_backward", grad_out, y, w)
     if y.dim() != 3:
@@ -394,6 +399,11 @@ def moe_balance_loss(gating_output, topk_ids, token_mask=None):
     The same bits in every run.  The gradient: :func:`moe_router_backward`; in a data-parallel job ``counts`` and ``tokens`` may be
     summed over the ranks before it, which makes it the gradient of the whole batch's loss.  No reference counterpart.
     """
+    got = (_lib._calls or _lib.load_calls()).moe_balance_loss(gating_output, topk_ids, token_mask)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_moe_balance_loss")
+        return BalanceLoss._make(got)
     lib = _lib.load()
     dev = _require_cuda("moe_balance_loss", gating_output, topk_ids, token_mask)
     if topk_ids is None:
@@ -424,6 +434,12 @@ def moe_router_backward(gating_output, topk_ids, grad_weights=None, renormalize=
     left out.  Ids outside ``[0, E)`` are dropped slots.  A row that neither brings a gradient to is 0, whatever its
     logits.  No reference counterpart: the reference's pure-torch router is differentiated by torch.
     """
+    got = (_lib._calls or _lib.load_calls()).moe_router_backward(
+        gating_output, topk_ids, grad_weights, renormalize, counts, tokens, grad_loss, token_mask)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_moe_router_backward")
+        return got
     lib = _lib.load()
     name = "moe_router_backward"
     on_device = grad_loss if isinstance(grad_loss, torch.Tensor) else None
@@ -494,6 +510,11 @@ def token_logprobs(logits, token_ids, top_k=0):
     logits are all -inf has log-probabilities -inf and entropy 0, a row with a NaN or a +inf is NaN.  The same bits in every
     run.  The gradient: :func:`token_logprobs_backward`.  No reference counterpart.
     """
+    got = (_lib._calls or _lib.load_calls()).token_logprobs(logits, token_ids, top_k)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_token_logprobs")
+        return TokenLogprobs._make(got)
     lib = _lib.load()
     name = "token_logprobs"
     dev = _require_cuda(name, logits, token_ids)
@@ -525,6 +546,12 @@ def token_logprobs_backward(logits, token_ids, stats, entropy=None, grad_logprob
     Gradients that are left out count as 0; one at least is needed.  Padding tokens (negative ids) have no gradient.  The
     result is contiguous, or, where the logits' rows do not start on 16 bytes, a view of rows that start like theirs.
     """
+    got = (_lib._calls or _lib.load_calls()).token_logprobs_backward(
+        logits, token_ids, stats, entropy, grad_logprobs, grad_entropy, top_ids, grad_top_logprobs)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_token_logprobs_backward")
+        return got
     lib = _lib.load()
     name = "token_logprobs_backward"
     dev = _require_cuda(name, logits, token_ids, stats, entropy, grad_logprobs, grad_entropy, top_ids, grad_top_logprobs)

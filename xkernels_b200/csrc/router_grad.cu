@@ -25,7 +25,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxExperts = 1024;
-constexpr int kWarps = 8;          // of a block of the gradient kernel
+constexpr int kWarps = 8;   // of a block of the gradient kernel
 constexpr float kLog2e = 1.44269504088896340736f;
 
 template <typename T> __device__ __forceinline__ float to_float(T v);
@@ -60,17 +60,21 @@ struct Row {
   static constexpr int kPieces = PER_LANE / P;
   static __device__ __forceinline__ int expert(int t, int lane) { return (t / P * 32 + lane) * P + t % P; }
   // logits, -inf behind the row
-  static __device__ __forceinline__ void load(const T* row, int E, int lane, float (&x)[PER_LANE]) {
-    Piece q[kPieces];
+  struct Raw { Piece q[kPieces]; };
+  static __device__ __forceinline__ Raw load(const T* row, int E, int lane) {
+    Raw r;
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
       const bool in = (c * 32 + lane) * P < E;
 #pragma unroll
-      for (int i = 0; i < P; ++i) q[c].x[i] = of_float<T>(-INFINITY);
-      if (in) q[c] = reinterpret_cast<const Piece*>(row)[c * 32 + lane];
+      for (int i = 0; i < P; ++i) r.q[c].x[i] = of_float<T>(-INFINITY);
+      if (in) r.q[c] = reinterpret_cast<const Piece*>(row)[c * 32 + lane];
     }
+    return r;
+  }
+  static __device__ __forceinline__ void values(const Raw& r, float (&x)[PER_LANE]) {
 #pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) x[t] = to_float(q[t / P].x[t % P]);
+    for (int t = 0; t < PER_LANE; ++t) x[t] = to_float(r.q[t / P].x[t % P]);
   }
   static __device__ __forceinline__ void store(T* row, int E, int lane, const float (&x)[PER_LANE]) {
 #pragma unroll
@@ -81,25 +85,30 @@ struct Row {
       if ((c * 32 + lane) * P < E) reinterpret_cast<Piece*>(row)[c * 32 + lane] = q;
     }
   }
-  // logits -> e^(x - max); their maximum (0 for a row without a live logit) and 1 / sum (0 for such a row).  NaN and +inf make
-  // the row NaN.
-  static __device__ __forceinline__ void exponentials(float (&x)[PER_LANE], float& max, float& inv) {
-    float mx = -INFINITY;
+  // logits -> e^(x - max), the maximum (0 for a row without a live logit, whose values become 0) and this lane's sum.  NaN and
+  // +inf make the row NaN.
+  static __device__ __forceinline__ float exponentials(float (&x)[PER_LANE], float& max) {
+    float mx = x[0];
 #pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(x[t]));
+    for (int t = 1; t < PER_LANE; ++t) asm("max.NaN.f32 %0, %0, %1;" : "+f"(mx) : "f"(x[t]));
     mx = warp_max_nan(mx);
-    const bool dead = mx == -INFINITY;
-    max = dead ? 0.f : mx;
+    max = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < PER_LANE; ++t) {
       x[t] = exp_of(x[t] - max);
       sum += x[t];
     }
-    sum = warp_add(sum);
-    inv = dead ? 0.f : 1.f / sum;
+    return sum;
   }
 };
+
+// 1 / s to 1 ulp; 0 for 0 (a row or a choice without a live logit).  The sums here are 0 or 2^-126 to 2^10, or NaN.
+__device__ __forceinline__ float inverse(float s) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return s == 0.f ? 0.f : r;
+}
 
 // ---- loss ---------------------------------------------------------------------------------------------------------
 struct LossArgs {
@@ -117,119 +126,124 @@ struct LossArgs {
   int E, k, parts;
 };
 
-constexpr int kLossWarps = 16;
 constexpr int kCluster = 8;
+constexpr int loss_warps(int per_lane) { return per_lane > 16 ? 8 : 16; }   // their sums take shared memory side by side
 
-__device__ __forceinline__ void write_loss(const LossArgs& a, double sum, int T) {
-  *a.loss = T > 0 && a.k > 0 ? (float)(sum * a.E / ((double)a.k * T)) : 0.f;
+__device__ __forceinline__ void write_loss(const LossArgs& a, float sum, int T) {   // sum of counts x means
+  *a.loss = T > 0 && a.k > 0 ? sum * (float)a.E / ((float)a.k * (float)T) : 0.f;
   *a.tokens = T;
 }
 
 template <typename T, int PER_LANE, int P>
-__global__ void __launch_bounds__(32 * kLossWarps)
+__global__ void __launch_bounds__(32 * loss_warps(PER_LANE))
 balance_kernel(LossArgs a) {
   using R = Row<T, PER_LANE, P>;
-  constexpr int kPlaces = 32 * PER_LANE;
-  __shared__ float s_sum[kLossWarps / 2][kPlaces];
+  constexpr int kPlaces = 32 * PER_LANE, kWarps = loss_warps(PER_LANE), kThreads = 32 * kWarps;
+  __shared__ float s_sum[kWarps][kPlaces];
+  __shared__ float s_total[kPlaces];
   __shared__ int s_count[kPlaces];
   __shared__ int s_tokens;
-  __shared__ double s_term;
+  __shared__ float s_term[4];
   cg::cluster_group cluster = cg::this_cluster();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = (int)cluster.block_rank();
   chain_trigger();   // the joining kernel may become resident
-  for (int e = threadIdx.x; e < kPlaces; e += 32 * kLossWarps) s_count[e] = 0;
-  if (threadIdx.x == 0) {
-    s_tokens = 0;
-    s_term = 0.0;
-  }
+  for (int e = threadIdx.x; e < kPlaces; e += kThreads) s_count[e] = 0;
+  if (threadIdx.x == 0) s_tokens = 0;
   __syncthreads();
   float acc[PER_LANE];
 #pragma unroll
   for (int t = 0; t < PER_LANE; ++t) acc[t] = 0.f;
   int mine = 0;
-  const int64_t step = (int64_t)gridDim.x * kLossWarps;
-#pragma unroll 2
-  for (int64_t m = (int64_t)blockIdx.x * kLossWarps + warp; m < a.M; m += step) {
-    if (a.mask != nullptr && a.mask[m] == 0) continue;
-    ++mine;
-    float x[PER_LANE], max, inv;
-    R::load(static_cast<const T*>(a.gating) + m * a.E, a.E, lane, x);
-    for (int j = lane; j < a.k; j += 32) {
-      const int e = a.ids[m * a.k + j];
-      if (e >= 0 && e < a.E) atomicAdd(&s_count[e], 1);
+  const int64_t step = (int64_t)gridDim.x * kWarps, m0 = (int64_t)blockIdx.x * kWarps + warp;
+  const T* row = static_cast<const T*>(a.gating) + m0 * a.E;
+  const int32_t* ids = a.ids + m0 * a.k + lane;
+  auto requested = [&](int64_t m) -> bool { return m < a.M && (a.mask == nullptr || a.mask[m] != 0); };
+  bool on = requested(m0);
+  typename R::Raw next;
+  int e = -1;
+  if (on) {
+    next = R::load(row, a.E, lane);
+    if (lane < a.k) e = *ids;
+  }
+  for (int64_t m = m0; m < a.M; m += step) {
+    const bool now = on;
+    const int en = e;
+    float x[PER_LANE];
+    if (now) R::values(next, x);
+    // the next row is on its way while this one is computed
+    row += step * a.E;
+    ids += step * a.k;
+    on = requested(m + step);
+    e = -1;
+    if (on) {
+      next = R::load(row, a.E, lane);
+      if (lane < a.k) e = *ids;
     }
-    R::exponentials(x, max, inv);
+    if (!now) continue;
+    ++mine;
+    if (en >= 0 && en < a.E) atomicAdd(&s_count[en], 1);
+    for (int j = lane + 32; j < a.k; j += 32) {
+      const int o = a.ids[m * a.k + j];
+      if (o >= 0 && o < a.E) atomicAdd(&s_count[o], 1);
+    }
+    float max;
+    const float inv = inverse(warp_add(R::exponentials(x, max)));
 #pragma unroll
     for (int t = 0; t < PER_LANE; ++t) acc[t] = fmaf(x[t], inv, acc[t]);
   }
   if (lane == 0 && mine != 0) atomicAdd(&s_tokens, mine);
-  // the upper half of the warps hands its sums to the lower half, and so on
-#pragma unroll 1
-  for (int half = kLossWarps / 2; half > 0; half /= 2) {
-    if (warp >= half && warp < 2 * half) {
 #pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) s_sum[warp - half][R::expert(t, lane)] = acc[t];
-    }
-    __syncthreads();
-    if (warp < half) {
+  for (int t = 0; t < PER_LANE; ++t) s_sum[warp][R::expert(t, lane)] = acc[t];
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.E; i += kThreads) {
+    float sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) acc[t] += s_sum[warp][R::expert(t, lane)];
-    }
-    __syncthreads();
-  }
-  if (warp == 0) {
-#pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) s_sum[0][R::expert(t, lane)] = acc[t];
+    for (int w = 0; w < kWarps; ++w) sum += s_sum[w][i];
+    s_total[i] = sum;
   }
   cluster.sync();
-  // every block joins its share of the experts
+  // every block joins its share of the experts: 128 at most
   const int each = (a.E + kCluster - 1) / kCluster, first = rank * each, n = max(0, min(each, a.E - first));
   const bool alone = gridDim.x == kCluster;
   const int64_t part = blockIdx.x / kCluster;
-  int tokens = 0;
-#pragma unroll
-  for (int i = 0; i < kCluster; ++i) tokens += *cluster.map_shared_rank(&s_tokens, i);
-  double term = 0.0;
-  if ((int)threadIdx.x < n) {
-    const int e = first + threadIdx.x;
-    float p = 0.f;
+  if (warp < 4) {
+    int tokens = lane < kCluster ? *cluster.map_shared_rank(&s_tokens, lane) : 0;
+    float p = 0.f, term = 0.f;
     int c = 0;
+    const int i = first + threadIdx.x;
+    if ((int)threadIdx.x < n) {
 #pragma unroll
-    for (int i = 0; i < kCluster; ++i) {
-      p += cluster.map_shared_rank(&s_sum[0][0], i)[e];
-      c += cluster.map_shared_rank(&s_count[0], i)[e];
+      for (int b = 0; b < kCluster; ++b) {
+        p += cluster.map_shared_rank(&s_total[0], b)[i];
+        c += cluster.map_shared_rank(&s_count[0], b)[i];
+      }
     }
+    tokens = __reduce_add_sync(0xffffffffu, tokens);
     if (alone) {
       const float mean = tokens > 0 ? p / (float)tokens : 0.f;
-      a.mean[e] = mean;
-      a.counts[e] = c;
-      term = (double)c * (double)mean;
-    } else {
-      a.part_p[part * a.E + e] = p;
-      a.part_c[part * a.E + e] = c;
+      if ((int)threadIdx.x < n) {
+        a.mean[i] = mean;
+        a.counts[i] = c;
+        term = (float)c * mean;
+      }
+      term = warp_add(term);
+      if (lane == 0) s_term[warp] = term;
+    } else if ((int)threadIdx.x < n) {
+      a.part_p[part * a.E + i] = p;
+      a.part_c[part * a.E + i] = c;
     }
+    if (threadIdx.x == 0) mine = tokens;   // (used by thread 0 alone)
   }
-  if (!alone) {
-    if (rank == 0 && threadIdx.x == 0) a.part_t[part] = tokens;
-    cluster.sync();   // the others' shared memory is read until here
-    return;
+  if (alone) {
+    cluster.sync();   // the terms are there: four of eight blocks, one a lane
+    if (rank == 0 && warp == 0) {
+      const float term = warp_add(cluster.map_shared_rank(&s_term[0], lane >> 2)[lane & 3]);
+      if (lane == 0) write_loss(a, term, mine);
+    }
+  } else if (rank == 0 && threadIdx.x == 0) {
+    a.part_t[part] = mine;
   }
-  // n <= 128: four warps have a share
-  if (warp < 4) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
-  }
-  __shared__ double s_warp_term[4];
-  if (warp < 4 && lane == 0) s_warp_term[warp] = term;
-  __syncthreads();
-  if (threadIdx.x == 0) s_term = (s_warp_term[0] + s_warp_term[1]) + (s_warp_term[2] + s_warp_term[3]);
-  cluster.sync();
-  if (rank == 0 && threadIdx.x == 0) {
-    double sum = 0.0;
-    for (int i = 0; i < kCluster; ++i) sum += *cluster.map_shared_rank(&s_term, i);
-    write_loss(a, sum, tokens);
-  }
-  cluster.sync();
+  cluster.sync();   // the others' shared memory is read until here
 }
 
 // Adds the clusters' rows up: thread (g, e) takes every G-th row of expert e.
@@ -237,47 +251,43 @@ __global__ void __launch_bounds__(1024)
 balance_join_kernel(LossArgs a) {
   __shared__ float s_p[1024];
   __shared__ int s_c[1024];
-  __shared__ double s_loss[32];
-  __shared__ int s_tokens;
+  __shared__ float s_loss[32];
+  __shared__ int s_tokens[2];
   const int E = a.E, G = 1024 / E, tid = threadIdx.x, g = tid / E, e = tid - g * E;
-  if (tid == 0) s_tokens = 0;
-  __syncthreads();
   chain_wait();
-  // (written by the kernel that this one overlaps: no read-only loads)
-  const volatile float* part_p = a.part_p;
-  const volatile int32_t *part_c = a.part_c, *part_t = a.part_t;
-  int t = 0;
-  for (int b = tid; b < a.parts; b += 1024) t += part_t[b];
-  if (t != 0) atomicAdd(&s_tokens, t);
+  // (written by the kernel that this one overlaps: loads from the L2)
   float p = 0.f;
   int c = 0;
   if (g < G) {
-#pragma unroll 8
-    for (int b = g; b < a.parts; b += G) {
-      p += part_p[b * E + e];
-      c += part_c[b * E + e];
+    const float* pp = a.part_p + g * E + e;
+    const int32_t* pc = a.part_c + g * E + e;
+    const int step = G * E;
+#pragma unroll 10
+    for (int b = g; b < a.parts; b += G, pp += step, pc += step) {
+      p += __ldcg(pp);
+      c += __ldcg(pc);
     }
   }
+  int t = tid < a.parts ? __ldcg(a.part_t + tid) : 0;   // parts <= 64
+  if (tid < 64) t = __reduce_add_sync(0xffffffffu, t);
+  if (tid == 0 || tid == 32) s_tokens[tid >> 5] = t;
   s_p[tid] = p;
   s_c[tid] = c;
   __syncthreads();
-  const int T = s_tokens;
-  double term = 0.0;
+  const int T = s_tokens[0] + s_tokens[1];
+  float term = 0.f;
   if (tid < E) {
     for (int i = 1; i < G; ++i) { p += s_p[tid + i * E]; c += s_c[tid + i * E]; }
     const float mean = T > 0 ? p / (float)T : 0.f;
     a.mean[tid] = mean;
     a.counts[tid] = c;
-    term = (double)c * (double)mean;
+    term = (float)c * mean;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) term += __shfl_xor_sync(0xffffffffu, term, o);
+  term = warp_add(term);
   if ((tid & 31) == 0) s_loss[tid >> 5] = term;
   __syncthreads();
   if (tid < 32) {
-    double sum = s_loss[tid];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float sum = warp_add(s_loss[tid]);
     if (tid == 0) write_loss(a, sum, T);
   }
 }
@@ -312,86 +322,102 @@ router_grad_kernel(GateArgs a) {
     for (int e = threadIdx.x; e < 32 * PER_LANE; e += 32 * kWarps) s_share[e] = e < a.E ? f * (float)a.counts[e] : 0.f;
     __syncthreads();
   }
-  for (int64_t m = (int64_t)blockIdx.x * kWarps + warp; m < a.M; m += (int64_t)gridDim.x * kWarps) {
-    const T* row = static_cast<const T*>(a.gating) + m * a.E;
-    T* out = static_cast<T*>(a.out) + m * a.E;
-    float x[PER_LANE], max, inv;
-    R::load(row, a.E, lane, x);
+  float share[PER_LANE];   // of the lane's experts: the same for all rows
+#pragma unroll
+  for (int t = 0; t < PER_LANE; ++t) share[t] = balance ? s_share[R::expert(t, lane)] : 0.f;
+  // lanes over which the first 32 slots' sums run
+  int span = 1;
+  while (span < a.k && span < 32) span *= 2;
+  if (a.k > 32 || !a.renorm) span = 32;
+
+  const int64_t step = (int64_t)gridDim.x * kWarps, m0 = (int64_t)blockIdx.x * kWarps + warp;
+  const T* row = static_cast<const T*>(a.gating) + m0 * a.E;
+  T* out = static_cast<T*>(a.out) + m0 * a.E;
+  const int32_t* ids = a.ids + m0 * a.k;
+  const float* g_w = a.g_w + m0 * a.k;
+  for (int64_t m = m0; m < a.M; m += step, row += step * a.E, out += step * a.E, ids += step * a.k, g_w += step * a.k) {
+    const typename R::Raw raw = R::load(row, a.E, lane);
     // slot `lane` of the first 32: expert (-1: none), gradient, logit
     int e = -1;
-    float g = 0.f, xe = 0.f;
+    float g = 0.f, xe = -INFINITY;
     if (weights && lane < a.k) {
-      e = a.ids[m * a.k + lane];
-      if (e < 0 || e >= a.E) e = -1;
-      else {
-        g = a.g_w[m * a.k + lane];
+      e = ids[lane];
+      g = g_w[lane];
+      if ((unsigned)e < (unsigned)a.E) {
         xe = to_float(row[e]);
+      } else {
+        e = -1;
+        g = 0.f;
       }
     }
     const bool counted = balance && (a.mask == nullptr || a.mask[m] != 0);
     if (!counted) {   // a row that nothing comes back to (padding) has gradient 0, whatever its logits are
       bool any = g != 0.f;
       if (weights)
-        for (int j = lane + 32; j < a.k; j += 32) {
-          const int o = a.ids[m * a.k + j];
-          any |= o >= 0 && o < a.E && a.g_w[m * a.k + j] != 0.f;
-        }
+        for (int j = lane + 32; j < a.k; j += 32) any |= (unsigned)ids[j] < (unsigned)a.E && g_w[j] != 0.f;
       if (!__any_sync(0xffffffffu, any)) {
+        float none[PER_LANE];
 #pragma unroll
-        for (int t = 0; t < PER_LANE; ++t) x[t] = 0.f;
-        R::store(out, a.E, lane, x);
+        for (int t = 0; t < PER_LANE; ++t) none[t] = 0.f;
+        R::store(out, a.E, lane, none);
         continue;
       }
     }
-    R::exponentials(x, max, inv);
-    // the chosen probabilities: their sum and their product with the gradients; the balance loss's sum_e p_e a_e
-    float p = e >= 0 ? exp_of(xe - max) * inv : 0.f, sel = p, dot = p * g, even = 0.f;
+    float x[PER_LANE], max;
+    R::values(raw, x);
+    float sum = R::exponentials(x, max);
+    // of the slots: sum of exponentials and of exponential x gradient; the balance loss's sum_e e^x_e a_e
+    const float ex = e >= 0 ? exp_of(xe - max) : 0.f;
+    float sel = ex, dot = ex * g, even = 0.f;
     if (weights)
       for (int j = lane + 32; j < a.k; j += 32) {
-        const int o = a.ids[m * a.k + j];
-        if (o < 0 || o >= a.E) continue;
-        const float po = exp_of(to_float(row[o]) - max) * inv;
-        sel += po;
-        dot = fmaf(po, a.g_w[m * a.k + j], dot);
+        const int o = ids[j];
+        if ((unsigned)o >= (unsigned)a.E) continue;
+        const float eo = exp_of(to_float(row[o]) - max);
+        sel += eo;
+        dot = fmaf(eo, g_w[j], dot);
       }
-    if (counted) {
+    if (balance) {
 #pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) even = fmaf(x[t], s_share[R::expert(t, lane)], even);
-      even = warp_add(even) * inv;
+      for (int t = 0; t < PER_LANE; ++t) even = fmaf(x[t], share[t], even);
     }
-    if (weights) {
-      dot = warp_add(dot);
-      if (a.renorm) sel = warp_add(sel);
-    }
-    const float s = even + (a.renorm ? 0.f : dot);
 #pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) x[t] = x[t] * inv * ((counted ? s_share[R::expert(t, lane)] : 0.f) - s);
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (balance) even += __shfl_xor_sync(0xffffffffu, even, o);
+      if (weights && o < span) {
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        sel += __shfl_xor_sync(0xffffffffu, sel, o);
+      }
+    }
+    const float inv = inverse(sum), s = (counted ? even * inv : 0.f) + (a.renorm ? 0.f : dot * inv);
+#pragma unroll
+    for (int t = 0; t < PER_LANE; ++t) x[t] = x[t] * inv * ((counted ? share[t] : 0.f) - s);
     R::store(out, a.E, lane, x);
     if (!weights) continue;
-    // q of a slot; an expert that several slots chose takes all of them, in their order
-    const float ratio = dot / sel;
-    auto q_of = [&](float gj) -> float { return !a.renorm ? gj : sel == 0.f ? 0.f : (gj - ratio) / sel; };
+    // A slot's part is e^x scale (gradient - level); an expert that several slots chose takes all of them, in their order.
+    const float scale = a.renorm ? inverse(sel) : inv, level = a.renorm ? dot * scale : 0.f;
     __syncwarp();   // the stores below come after the row's
-    const float q = e >= 0 ? q_of(g) : 0.f;
     if (a.k <= 32) {
-      float own = q;
+      float own = e >= 0 ? g - level : 0.f;
       const unsigned same = __match_any_sync(0xffffffffu, e);
       if (__any_sync(0xffffffffu, e >= 0 && (same & (same - 1)) != 0)) {
+        const float q = own;
         own = 0.f;
         for (int j = 0; j < a.k; ++j) {
           const float qj = __shfl_sync(0xffffffffu, q, j);
           if (same >> j & 1) own += qj;
         }
       }
-      if (e >= 0) out[e] = of_float<T>(p * ((counted ? s_share[e] : 0.f) + own - s));
+      if (e >= 0) out[e] = of_float<T>(ex * (inv * ((counted ? s_share[e] : 0.f) - s) + scale * own));
     } else {
       for (int j = lane; j < a.k; j += 32) {
-        const int o = a.ids[m * a.k + j];
-        if (o < 0 || o >= a.E) continue;
+        const int o = ids[j];
+        if ((unsigned)o >= (unsigned)a.E) continue;
         float own = 0.f;
         for (int i = 0; i < a.k; ++i)
-          if (a.ids[m * a.k + i] == o) own += q_of(a.g_w[m * a.k + i]);
-        out[o] = of_float<T>(exp_of(to_float(row[o]) - max) * inv * ((counted ? s_share[o] : 0.f) + own - s));
+          if (ids[i] == o) own += g_w[i] - level;
+        out[o] = of_float<T>(exp_of(to_float(row[o]) - max) * (inv * ((counted ? s_share[o] : 0.f) - s) + scale * own));
       }
     }
   }
@@ -426,7 +452,7 @@ template <typename T> struct LaunchLoss {
   template <int PER_LANE, int P> int operator()() const {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.parts * kCluster));
-    cfg.blockDim = dim3(32 * kLossWarps);
+    cfg.blockDim = dim3(32 * loss_warps(PER_LANE));
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -452,8 +478,9 @@ template <typename T> struct LaunchGrad {
 
 // Clusters of the loss kernel: one, which needs no second kernel, up to eight rows a warp; two blocks per SM at most.
 constexpr int64_t kMostParts = 2 * 148 / kCluster;
+static_assert(kMostParts <= 64, "the joining kernel reads the clusters' tokens with 64 threads");
 int64_t loss_parts(int64_t M) {
-  const int64_t rows = kCluster * kLossWarps;
+  const int64_t rows = kCluster * 16;
   if (M <= 8 * rows) return 1;
   const int64_t p = ceil_div(M, rows);
   return p > kMostParts ? kMostParts : p;

@@ -41,9 +41,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if one of 
   return r;
 }
 __device__ __forceinline__ float warp_max_nan(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 __device__ __forceinline__ float warp_add(float v) {
 #pragma unroll
@@ -79,7 +84,7 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
 // What a type of logits needs: N elements in 16 bytes, a running maximum of whole vectors, ordered keys.
 //   kClamp: smaller elements count as this, which keeps -inf out of the products.  A row whose maximum is not between kLow
 //   and kHigh, where a clamped element would count or x log2(e) is too coarse, takes the slow pass.
-//   key_of: ascending with the value; NaN above all, -0 as +0, never 0 (that is "no element").
+//   key_of: ascending with the value; NaN above all, -0 as +0, never 0 (that is "no element") nor the largest word.
 template <typename T> struct Elem;
 
 template <> struct Elem<float> {
@@ -106,12 +111,12 @@ template <> struct Elem<float> {
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
   static __device__ __forceinline__ uint32_t key_of(float v) {
-    if (v != v) return 0xffffffffu;
+    if (v != v) return 0xfffffffeu;
     const uint32_t u = __float_as_uint(v + 0.f);
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
   }
   static __device__ __forceinline__ float of_key(uint32_t k) {
-    if (k == 0xffffffffu) return kNan;
+    if (k >= 0xfffffffeu) return kNan;
     return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
   }
 };
@@ -246,6 +251,21 @@ struct Sums {
   }
 };
 
+// Parts are (maximum, c, S, T).  Two of them in one, and those of a warp's lanes in one, at the largest c: no factor exceeds 1.
+__device__ __forceinline__ float4 joined(float4 p, float4 q) {
+  const float to = fmaxf(p.y, q.y);
+  Sums a{p.y, p.z, p.w}, b{q.y, q.z, q.w};
+  a.move_to(to);
+  b.move_to(to);
+  return make_float4(max_nan(p.x, q.x), to, a.S + b.S, a.T + b.T);
+}
+__device__ __noinline__ float4 joined(float4 p) {
+  const float mx = warp_max_nan(p.x), to = warp_max(p.y);
+  Sums t{p.y, p.z, p.w};
+  t.move_to(to);
+  return make_float4(mx, to, warp_add(t.S), warp_add(t.T));
+}
+
 // S and T of the even and of the odd places of a vector
 struct PairSums { Pair S, T; };
 
@@ -265,54 +285,54 @@ __device__ __forceinline__ void add_vector(const uint4& q, Pair minus_c, PairSum
   }
 }
 
-// The largest key t of which at least k of the n keys are >= t (0 if fewer than k are above 0): a search by two bits at a time
-// from the first one in which the keys differ, by one warp that holds the keys in registers.
-template <int THREADS>
-__device__ __forceinline__ uint32_t kth_largest(const uint32_t* keys, int k) {
-  const int lane = threadIdx.x & 31;
-  uint32_t key[THREADS / 32], most = 0, least = 0xffffffffu;
+// The largest key that at least k of the warp's 32 PER keys reach (0 if fewer than k are above 0), bit by bit from the first
+// one in which the keys differ.
+template <int PER>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[PER], int k) {
+  uint32_t most = 0, least = 0xffffffffu;
 #pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) {
-    key[i] = keys[i * 32 + lane];
+  for (int i = 0; i < PER; ++i) {
     most = max(most, key[i]);
     least = min(least, key[i]);
   }
   most = __reduce_max_sync(0xffffffffu, most);
   least = __reduce_min_sync(0xffffffffu, least);
   if (most == least) return most;
-  int b = (31 - __clz(most ^ least)) & ~1;         // the upper of two bits is b + 1
-  uint32_t t = b == 30 ? 0u : most >> (b + 2) << (b + 2);
-  for (; b >= 0; b -= 2) {
-    uint32_t n = 0;   // how many reach t + 1, t + 2, t + 3 in units of this step: fields of ten bits (THREADS < 1024)
+  uint32_t bit = 0x80000000u >> __clz(most ^ least), t = most & ~(2u * bit - 1u);
+#pragma unroll 1
+  for (; bit != 0; bit >>= 1) {
+    const uint32_t trial = t | bit;
+    int n = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) {
-      // (equal bits above the step: everything that is not below t)
-      const uint32_t d = key[i] >= t ? min((key[i] - t) >> b, 3u) : 0u;
-      n += d == 0 ? 0u : d == 1 ? 1u : d == 2 ? 1u + (1u << 10) : 1u + (1u << 10) + (1u << 20);
-    }
-    n = __reduce_add_sync(0xffffffffu, n);
-    const uint32_t step = (int)(n >> 20) >= k ? 3u : (int)(n >> 10 & 1023u) >= k ? 2u : (int)(n & 1023u) >= k ? 1u : 0u;
-    t += step << b;
+    for (int i = 0; i < PER; ++i) n += key[i] >= trial;
+    if (__reduce_add_sync(0xffffffffu, n) >= k) t = trial;
   }
   return t;
 }
 
-constexpr int kBatch = 4;   // vectors a thread requests before it uses the first (select_top names them one by one)
+constexpr int kBatch = 4;   // vectors a thread requests before it uses the first
 
 template <int THREADS>
 struct TopScratch {
-  uint64_t cand[8 * THREADS + kMaxTop];   // value key, ~column: all different, larger is better
-  uint64_t top[kMaxTop];                  // the CTA's best ones, in order
-  uint32_t key[THREADS];                  // of every thread
-  int owner[THREADS];                     // threads whose elements are read again
-  int n, owners, want;
+  static constexpr int kRoom = 8 * THREADS + kMaxTop, kGroups = THREADS < 128 ? THREADS : 128;
+  static constexpr int kRanked = 32;         // candidates that are ranked side by side: the places behind the last one hold 0
+  uint64_t cand[kRoom];                      // value key, ~column: all different, larger is better
+  uint64_t top[kMaxTop];                     // the best ones, in order
+  alignas(16) uint32_t group[kGroups];       // the maxima of the row's groups of threads
+  uint32_t key[THREADS];                     // (long way) of every thread
+  int owner[THREADS];                        // (long way) threads whose elements are read again
+  int ties[THREADS / 32];                    // of a warp
+  uint32_t least[kGroups / 32];              // of a warp
+  int n, owners;
   uint32_t bound;
 };
 template <int THREADS> struct NoScratch {};
 
-// Leaves the k largest of the n candidates (n > k) at the front, in any order.
+// Leaves the k largest of the n candidates (n > k) at the front, in any order, and 0 in the places behind them.
 template <int THREADS>
 __device__ __noinline__ void keep_best(TopScratch<THREADS>& s, int k) {
+  constexpr int kEach = (TopScratch<THREADS>::kRoom + THREADS - 1) / THREADS;
+  static_assert(kEach < 16, "counts of four bits");
   const int n = s.n;
   uint64_t t = 0;
 #pragma unroll 1
@@ -320,14 +340,13 @@ __device__ __noinline__ void keep_best(TopScratch<THREADS>& s, int k) {
     const uint64_t trial = t | (1ull << b);
     int mine = 0, all = 0;
     for (int i = threadIdx.x; i < n; i += THREADS) mine += s.cand[i] >= trial;
-    // (at most 9 a thread: four counts of one bit)
 #pragma unroll
     for (int w = 0; w < 4; ++w) all += __syncthreads_count((mine >> w) & 1) << w;
     if (all >= k) t = trial;
   }
-  uint64_t mine[9];   // 9 THREADS > 8 THREADS + kMaxTop
+  uint64_t mine[kEach];
 #pragma unroll
-  for (int i = 0; i < 9; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     const int at = threadIdx.x + i * THREADS;
     mine[i] = at < n ? s.cand[at] : 0;
   }
@@ -335,132 +354,212 @@ __device__ __noinline__ void keep_best(TopScratch<THREADS>& s, int k) {
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 9; ++i)
+  for (int i = 0; i < kEach; ++i)
     if (mine[i] != 0 && mine[i] >= t) s.cand[atomicAdd(&s.n, 1)] = mine[i];
   __syncthreads();
+  if ((int)threadIdx.x >= k && threadIdx.x < TopScratch<THREADS>::kRanked) s.cand[threadIdx.x] = 0;
+  __syncthreads();
 }
 
-// The k best of n <= THREADS candidates, in order, to `to`; unfilled places are 0.
+// The k best of the first n <= THREADS candidates to s.top, in order; unfilled places are 0.
 template <int THREADS>
-__device__ __forceinline__ void rank_all(const uint64_t* cand, int n, int k, uint64_t* to) {
-  for (int i = threadIdx.x; i < k; i += THREADS)
-    if (i >= n) to[i] = 0;
-  if ((int)threadIdx.x < n) {
-    const uint64_t mine = cand[threadIdx.x];
+__device__ __forceinline__ void rank_all(TopScratch<THREADS>& s, int n, int k) {
+  const int tid = threadIdx.x;
+  if (tid < k && tid >= n) s.top[tid] = 0;
+  if (n <= 32 && 4 * 32 <= THREADS) {   // four threads a candidate, every fourth place each
+    const int i = tid >> 2;
+    if (i >= 32) return;
+    const uint64_t mine = s.cand[i];
     int rank = 0;
-    for (int i = 0; i < n; ++i) rank += cand[i] > mine;
-    if (rank < k) to[rank] = mine;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) rank += s.cand[j + (tid & 3)] > mine;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if ((tid & 3) == 0 && i < n && rank < k) s.top[rank] = mine;
+    return;
   }
+  if (tid >= n) return;
+  const uint64_t mine = s.cand[tid];
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+  if (rank < k) s.top[rank] = mine;
 }
 
-// The k largest elements of the CTA's vectors [lo, hi) to s.top, ordered; `best` is the maximum of this thread's vectors.
+__device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (uint64_t)key << 32 | (uint32_t)~(uint32_t)col; }
+
 template <typename T, int THREADS>
-__device__ void select_top(const RowView<T>& r, int lo, int hi, uint32_t best, int k, TopScratch<THREADS>& s) {
-  constexpr int N = Elem<T>::N;
-  const int tid = threadIdx.x, per = (hi - lo + THREADS - 1) / THREADS;   // vectors of a thread, at most
-  s.key[tid] = best;
-  __syncthreads();
-  if (tid < 32) {
-    const uint32_t t = kth_largest<THREADS>(s.key, k);
-    if (tid == 0) {
-      s.bound = t;
-      s.n = s.owners = s.want = 0;
-    }
+__device__ __forceinline__ void offer(const RowView<T>& r, int col, uint32_t floor, uint64_t* to, int* n) {
+  const uint32_t key = Elem<T>::key_of(Elem<T>::load(r.row + col));
+  if (key < floor) return;
+  const int place = atomicAdd(n, 1);
+  if (place < TopScratch<THREADS>::kRoom) to[place] = candidate(key, col);
+}
+
+// Once more the vectors of those threads of the warp whose maximum reaches `floor`: their elements from there on to the list
+// `to`, which `n` counts (both perhaps another CTA's).  The warp's lanes share the vectors of an owner, or several small owners.
+// The elements before the row's first and behind its last whole vector are looked at in any case, by the CTA that has them.
+// Nothing is put behind the list's end: the caller sees by the count that it was too short.
+// (This runs a few times in a CTA's life: what costs is latency and fetching the code, so there is one copy of each step.)
+template <typename T, int THREADS>
+__device__ __forceinline__ void collect(const RowView<T>& r, int lo, int hi, uint32_t floor, uint32_t best, uint64_t* to, int* n) {
+  constexpr int N = Elem<T>::N, kLoads = 4;
+  const int lane = threadIdx.x & 31, end = min(hi, r.end_whole);
+  if (threadIdx.x < 2 * N) {
+    const bool head = threadIdx.x < N;   // vector 0 if it is no whole one in front of those, or the one behind them
+    const int j = head ? 0 : r.end_whole, col = r.column(j) + (int)(threadIdx.x & (N - 1));
+    if (j >= lo && j < hi && (head ? r.first_whole > 0 : true) && col >= 0 && col < r.V) offer<T, THREADS>(r, col, floor, to, n);
   }
-  __syncthreads();
-  const uint32_t bound = s.bound;
-  // Several threads may share the bound.  A few too many are taken; of a crowd (rows of equal logits) only those whose first
-  // element of that value comes first, which each looks for in its own vectors.
-  uint32_t last = 0xffffffffu;   // an element equal to the bound counts up to this column
-  bool mine = best > 0 && best >= bound;
-  const int reach = __syncthreads_count(mine);
-  if (bound > 0 && reach > 2 * k + 32) {
-    const int above = __syncthreads_count(best > bound);
-    uint32_t at = 0xffffffffu;
-    if (best == bound) {
-      for (int j = lo + tid; j < hi && at == 0xffffffffu; j += THREADS) {
-        float v[N];
-        Elem<T>::unpack(r.load(j, 0.f), v);
+  unsigned rest = __ballot_sync(0xffffffffu, best > 0 && best >= floor);
+  if (rest == 0) return;
+  const int per = (hi - lo + THREADS - 1) / THREADS, first = lo + (int)(threadIdx.x & ~31u);
+  const float least = Elem<T>::of_key(floor > 0 ? floor : 1u);          // (a NaN, as of key 1, lets everything pass to the keys)
+  const int log = per >= 32 ? 5 : per <= 1 ? 0 : 32 - __clz(per - 1);   // lanes of an owner: a power of two
+  for (int i = lane >> log; i > 0; --i) rest &= rest - 1;               // its lowest bit is this lane's next owner
+#pragma unroll 1
+  while (rest != 0) {
+    int from[kLoads];
 #pragma unroll
-        for (int i = N - 1; i >= 0; --i) {
-          const int col = r.column(j) + i;
-          if (col >= 0 && col < r.V && Elem<T>::key_of(v[i]) == bound) at = (uint32_t)col;
+    for (int u = 0; u < kLoads; ++u) {
+      from[u] = rest != 0 ? first + __ffs(rest) - 1 : end;
+#pragma unroll 1
+      for (int i = 32 >> log; i > 0 && rest != 0; --i) rest &= rest - 1;
+    }
+#pragma unroll 1
+    for (int i = lane & ((1 << log) - 1); i < per; i += 1 << log) {
+      uint4 q[kLoads];
+      unsigned pass = 0;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int j = from[u] + i * THREADS;
+        if (j < end && j >= r.first_whole) {
+          q[u] = r.load_whole(j);
+          pass |= 1u << u;
         }
       }
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+        if ((pass >> u & 1) && Elem<T>::value(Elem<T>::of(q[u])) < least) pass &= ~(1u << u);
+#pragma unroll 1
+      for (; pass != 0; pass &= pass - 1) {   // seldom more than one; the vector comes from the L1 now
+        const int u = __ffs(pass) - 1, j = (u == 0 ? from[0] : u == 1 ? from[1] : u == 2 ? from[2] : from[3]) + i * THREADS;
+        float v[N];
+        Elem<T>::unpack(r.load_whole(j), v);
+        unsigned ok = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) ok |= v[e] < least ? 0u : 1u << e;
+#pragma unroll 1
+        for (; ok != 0; ok &= ok - 1) offer<T, THREADS>(r, r.column(j) + __ffs(ok) - 1, floor, to, n);
+      }
     }
-    s.key[tid] = best == bound ? ~at : 0u;
+  }
+}
+
+// The first k columns of the row whose key is `bound`, to the CTA's list.
+template <typename T, int THREADS>
+__device__ __noinline__ void collect_first(const T* row, int V, uint32_t bound, int k, TopScratch<THREADS>& s) {
+  constexpr int N = Elem<T>::N;
+  const RowView<T> r(row, V);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int found = 0;
+  for (int j0 = 0; j0 < r.vectors && found < k; j0 += THREADS) {
+    const int j = j0 + tid, first = r.column(j);
+    unsigned equal = 0;
+    if (j < r.vectors) {
+      float v[N];
+      Elem<T>::unpack(r.load(j, 0.f), v);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (first + i >= 0 && first + i < r.V && Elem<T>::key_of(v[i]) == bound) equal |= 1u << i;
+    }
+    const int own = __popc(equal);
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += below;
+    }
+    if (lane == 31) s.ties[warp] = upto;
+    __syncthreads();
+    int place = found + upto - own, all = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) place += s.ties[w];
+      all += s.ties[w];
+    }
+    for (; equal != 0 && place < k; equal &= equal - 1, ++place) {
+      const int to = atomicAdd(&s.n, 1);
+      if (to < TopScratch<THREADS>::kRoom) s.cand[to] = candidate(bound, first + __ffs(equal) - 1);
+    }
+    found += all;
+    __syncthreads();
+  }
+}
+
+// The long way, for rows whose candidates do not fit the list: the k largest elements of the whole row to s.top, by one CTA.
+template <typename T, int THREADS>
+__device__ __noinline__ void select_top(const T* row, int V, int k, TopScratch<THREADS>& s) {
+  constexpr int N = Elem<T>::N, kPer = THREADS / 32;
+  const RowView<T> r(row, V);
+  const int tid = threadIdx.x, lane = tid & 31, per = (r.vectors + THREADS - 1) / THREADS;   // vectors of a thread, at most
+  auto search = [&](uint32_t key, int want) -> uint32_t {   // the want-th largest of the threads' keys
+    __syncthreads();
+    s.key[tid] = key;
     __syncthreads();
     if (tid < 32) {
-      const uint32_t t = kth_largest<THREADS>(s.key, k - above);
+      uint32_t keys[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) keys[i] = s.key[i * 32 + lane];
+      const uint32_t t = kth_largest<kPer>(keys, want);
       if (tid == 0) s.bound = t;
     }
     __syncthreads();
-    last = ~s.bound;
+    return s.bound;
+  };
+  // a vector's elements that lie in the row
+  auto each = [&](int j, auto f) {
+    float v[N];
+    Elem<T>::unpack(r.load(j, 0.f), v);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int col = r.column(j) + i;
+      if (col >= 0 && col < r.V) f(Elem<T>::key_of(v[i]), col);
+    }
+  };
+  uint32_t best = 0;
+  for (int j = tid; j < r.vectors; j += THREADS) each(j, [&](uint32_t key, int) { best = max(best, key); });
+  const uint32_t bound = search(best, k);
+  // Of the threads that share the bound those count whose first element of that value comes first, which each looks for.
+  uint32_t last = 0xffffffffu;   // an element equal to the bound counts up to this column
+  bool mine = best > 0 && best >= bound;
+  const int above = __syncthreads_count(best > bound), ties = __syncthreads_count(best > 0 && best == bound);
+  if (bound > 0 && above + ties > k) {
+    uint32_t at = 0xffffffffu;
+    if (best == bound)
+      for (int j = tid; j < r.vectors && at == 0xffffffffu; j += THREADS)
+        each(j, [&](uint32_t key, int col) { if (key == bound) at = min(at, (uint32_t)col); });
+    last = ~search(best == bound ? ~at : 0u, k - above);
     mine = best > bound || (best == bound && at <= last);
   }
+  if (tid == 0) s.n = s.owners = 0;
+  __syncthreads();
   if (mine) s.owner[atomicAdd(&s.owners, 1)] = tid;
   __syncthreads();
   const int items = s.owners * per;
-  auto counts = [&](float v, int col) -> bool {
-    const uint32_t key = Elem<T>::key_of(v);
-    return col >= 0 && col < r.V && (key > bound || (key == bound && (uint32_t)col <= last));
-  };
-  auto push = [&](float v, int col) {
-    s.cand[atomicAdd(&s.n, 1)] = (uint64_t)Elem<T>::key_of(v) << 32 | (uint32_t)~(uint32_t)col;
-  };
-  for (int base = 0; base < items; base += kBatch * THREADS) {
-    // some vectors of every thread at once, their candidates counted before any is put down
-    uint4 q[kBatch];
-    int at[kBatch], n = 0;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int it = base + u * THREADS + tid;
-      at[u] = -1;
-      if (it < items) {
-        const int j = lo + s.owner[it / per] + it % per * THREADS;
-        if (j < hi) {
-          at[u] = j;
-          q[u] = r.load(j, 0.f);
-        }
-      }
+  for (int base = 0; base < items; base += THREADS) {
+    if (base > 0) {   // room for a whole round: what is there is cut down to k
+      __syncthreads();
+      const int have = s.n;
+      __syncthreads();
+      if (have > kMaxTop) keep_best<THREADS>(s, k);
     }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (at[u] < 0) continue;
-      float v[N];
-      Elem<T>::unpack(q[u], v);
-#pragma unroll
-      for (int i = 0; i < N; ++i) n += counts(v[i], r.column(at[u]) + i);
-    }
-    if (n > 0) atomicAdd(&s.want, n);
-    __syncthreads();
-    const int have = s.n, want = s.want;
-    __syncthreads();
-    if (tid == 0) s.want = 0;
-    const bool fits = have + want <= 8 * THREADS + kMaxTop;
-#pragma unroll 1
-    for (int u = 0; u < kBatch; ++u) {
-      if (!fits) {   // one vector a thread at a time, what is there cut down to k before
-        __syncthreads();
-        const int now = s.n;
-        __syncthreads();
-        if (now > kMaxTop) keep_best<THREADS>(s, k);
-      }
-      const int j = u == 0 ? at[0] : u == 1 ? at[1] : u == 2 ? at[2] : at[3];
-      if (j < 0 || n == 0) continue;
-      const uint4 w = u == 0 ? q[0] : u == 1 ? q[1] : u == 2 ? q[2] : q[3];
-      float v[N];
-      Elem<T>::unpack(w, v);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (counts(v[i], r.column(j) + i)) push(v[i], r.column(j) + i);
-    }
-    __syncthreads();
+    const int it = base + tid, j = it < items ? s.owner[it / per] + it % per * THREADS : r.vectors;
+    if (j < r.vectors)
+      each(j, [&](uint32_t key, int col) {
+        if (key > bound || (key == bound && (uint32_t)col <= last)) s.cand[atomicAdd(&s.n, 1)] = candidate(key, col);
+      });
   }
-  const int found = s.n;
   __syncthreads();
-  if (found > THREADS) keep_best<THREADS>(s, k);
-  rank_all<THREADS>(s.cand, found > THREADS ? k : found, k, s.top);
+  keep_best<THREADS>(s, k);
 }
 
 struct LogprobArgs {
@@ -478,19 +577,81 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int ids64, int64_t i) 
   return ids64 ? static_cast<const int64_t*>(ids)[i] : (int64_t)static_cast<const int32_t*>(ids)[i];
 }
 
-template <typename T, int THREADS, bool TOP>
+// The statistics of a row from its part: maximum, l, H; `far`: they have to come from the slow pass.
+__device__ __forceinline__ void statistics(const float4& part, float low, float high, float& row_max, float& l, float& H, bool& far) {
+  row_max = part.x;
+  far = false;
+  if (row_max != row_max || row_max == INFINITY) {
+    l = H = kNan;
+  } else if (row_max == -INFINITY) {
+    l = H = 0.f;
+  } else if (row_max < low || row_max > high) {
+    l = H = 0.f;
+    far = true;
+  } else {
+    const float at_max = row_max * kLog2e;
+    Sums t{part.y, part.z, part.w};
+    t.move_to(at_max);
+    // at_max is row_max log2(e) but for its rounding, which is in every e: ln sum exp(x - row_max) = ln2 (log2 S + at_max - row_max log2(e))
+    const float off = -fmaf(row_max, kLog2e, -at_max), log2s = log2f(t.S);
+    l = (log2s + off) * kLn2;
+    H = fmaxf((log2s - t.T / t.S) * kLn2, 0.f);
+  }
+}
+
+// The slow pass, for a row whose maximum is far from zero: differences from the maximum, in natural units, by one CTA.
+template <typename T, int THREADS>
+__device__ __noinline__ float2 slow_statistics(const T* row, int V, float row_max, float4* s_warp) {   // l, H
+  const RowView<T> r(row, V);
+  const int tid = threadIdx.x;
+  float S = 0.f, Tn = 0.f;
+  for (int j = tid; j < r.vectors; j += THREADS) {
+    float v[Elem<T>::N];
+    Elem<T>::unpack(r.load(j, -INFINITY), v);
+#pragma unroll
+    for (int i = 0; i < Elem<T>::N; ++i) {
+      const float z = v[i] - row_max, e = exp2_fast(z * kLog2e);
+      S += e;
+      if (e > 0.f) Tn = fmaf(e, z, Tn);
+    }
+  }
+  S = warp_add(S);
+  Tn = warp_add(Tn);
+  __syncthreads();
+  if ((tid & 31) == 0) s_warp[tid >> 5] = make_float4(S, Tn, 0.f, 0.f);
+  __syncthreads();
+  S = Tn = 0.f;
+  for (int i = 0; i < THREADS / 32; ++i) {
+    S += s_warp[i].x;
+    Tn += s_warp[i].y;
+  }
+  const float l = logf(S);
+  return make_float2(l, fmaxf(l - Tn / S, 0.f));
+}
+
+constexpr int kMostCluster = 8;
+
+// CLUSTERED: a row belongs to the CTAs of a cluster.  They hand their parts to the first one, and their groups' maxima to each other,
+// by stores into its shared memory; behind the last barrier only the first one runs on.
+template <typename T, int THREADS, bool TOP, bool CLUSTERED>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 token_logprobs_kernel(LogprobArgs a) {
-  constexpr int kWarps = THREADS / 32;
-  __shared__ float4 s_warp[kWarps];                 // a warp's maximum, c, S, T
-  __shared__ float4 s_part;                         // the CTA's
-  __shared__ typename std::conditional<TOP, TopScratch<THREADS>, NoScratch<THREADS>>::type s_top;
+  using Scratch = TopScratch<THREADS>;
+  constexpr int kWarps = THREADS / 32, kGroups = Scratch::kGroups;
+  __shared__ float4 s_parts[CLUSTERED ? kMostCluster * kWarps : kWarps];   // of every warp of the row: maximum, c, S, T
+  __shared__ float4 s_row;                                                 // maximum, l, H, whether they are still to come
+  __shared__ typename std::conditional<TOP, Scratch, NoScratch<THREADS>>::type s_top;
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t m = blockIdx.x / C;
+  const int C = CLUSTERED ? (int)cluster.num_blocks() : 1, rank = CLUSTERED ? (int)cluster.block_rank() : 0;
+  const int64_t m = CLUSTERED ? blockIdx.x / C : blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const RowView<T> r(static_cast<const T*>(a.logits) + m * a.ld, a.V);
-  const int per = (r.vectors + C - 1) / C, lo = rank * per, hi = min(lo + per, r.vectors);
+  const int per = CLUSTERED ? (r.vectors + C - 1) / C : r.vectors, lo = rank * per, hi = min(lo + per, r.vectors);
+  if constexpr (TOP) {
+    if (tid < Scratch::kRanked) s_top.cand[tid] = 0;
+    if (tid == 0) s_top.n = 0;
+  }
+  if constexpr (CLUSTERED) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
 
   // the given token: requested here, its logit behind the pass, both used at the end
   int64_t id = 0;
@@ -539,99 +700,77 @@ token_logprobs_kernel(LogprobArgs a) {
   }
   float given = 0.f;
   if (rank == 0 && tid == 0 && id >= 0 && id < a.V) given = Elem<T>::load(r.row + id);
-  Sums s{c, 0.f, 0.f};
-  {
-    float s0, s1, t0, t1;
-    split(sums.S, s0, s1);
-    split(sums.T, t0, t1);
-    s.S = s0 + s1;
-    s.T = t0 + t1;
-  }
 
-  // the CTA's sums, at the reference of its maximum
   const float own_max = Elem<T>::value(best);
-  auto joined = [](float4 p) -> float4 {   // p: maximum, c, S, T of a lane
-    const float mx = warp_max_nan(p.x);
-    Sums t{p.y, p.z, p.w};
-    float c = p.y;   // the largest c: no factor exceeds 1
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) c = fmaxf(c, __shfl_xor_sync(0xffffffffu, c, o));
-    t.move_to(c);
-    return make_float4(mx, c, warp_add(t.S), warp_add(t.T));
-  };
-  const float4 w = joined(make_float4(own_max, s.c, s.S, s.T));
-  if (lane == 0) s_warp[warp] = w;
-  __syncthreads();
-  const float4 none = make_float4(-INFINITY, Elem<T>::kLow * kLog2e, 0.f, 0.f);
-  if (warp == 0) {
-    const float4 all = joined(lane < kWarps ? s_warp[lane] : none);
-    if (lane == 0) s_part = all;
-  }
+  float s0, s1, t0, t1;
+  split(sums.S, s0, s1);
+  split(sums.T, t0, t1);
+  const float4 part = joined(make_float4(own_max, c, s0 + s1, t0 + t1));
+  if constexpr (CLUSTERED) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");   // the others run: their memory is there
+  if (lane == 0) (CLUSTERED ? cluster.map_shared_rank(&s_parts[0], 0) : s_parts)[rank * kWarps + warp] = part;
+  uint32_t best_key = 0;
   if constexpr (TOP) {
-    // (a thread without elements holds -inf: its key must be 0)
-    const uint32_t key = lo + tid < hi ? Elem<T>::key_of(own_max) : 0u;
-    select_top<T, THREADS>(r, lo, hi, key, a.top_k, s_top);
+    if (lo + tid < hi) best_key = Elem<T>::key_of(own_max);   // (a thread without elements holds -inf and has key 0)
+    const int each = THREADS / kGroups * C;                   // threads of a group: 1 to 16 neighbours
+    uint32_t most = best_key;
+    for (int o = each / 2; o > 0; o /= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int to = lane % each;                               // the group's maximum goes to every CTA
+    if (to < C) (CLUSTERED ? cluster.map_shared_rank(&s_top.group[0], to) : s_top.group)[rank * (kGroups / C) + tid / each] = most;
+  }
+  if constexpr (CLUSTERED) cluster.sync(); else __syncthreads();
+  if constexpr (TOP) {
+    if (tid < kGroups) {   // the k-th largest of the groups' maxima: the smallest that fewer than k exceed
+      const uint32_t mine = s_top.group[tid];
+      int more[4] = {0, 0, 0, 0};
+#pragma unroll 8
+      for (int i = 0; i < kGroups; i += 4) {
+        const uint4 g = *reinterpret_cast<const uint4*>(s_top.group + i);
+        more[0] += g.x > mine;
+        more[1] += g.y > mine;
+        more[2] += g.z > mine;
+        more[3] += g.w > mine;
+      }
+      const uint32_t least = __reduce_min_sync(0xffffffffu, more[0] + more[1] + (more[2] + more[3]) < a.top_k ? mine : 0xffffffffu);
+      if (lane == 0) s_top.least[warp] = least;
+    }
+  } else {
+    if (rank != 0) return;
+  }
+  if (warp == kWarps - 1 && rank == 0) {
+    const int n = C * kWarps;
+    const float4 none = make_float4(-INFINITY, Elem<T>::kLow * kLog2e, 0.f, 0.f);
+    float4 p = lane < n ? s_parts[lane] : none;
+    if (CLUSTERED && n > 32) p = joined(p, lane + 32 < n ? s_parts[lane + 32] : none);
+    p = joined(p);
+    float row_max, l, H;
+    bool far;
+    statistics(p, Elem<T>::kLow, Elem<T>::kHigh, row_max, l, H, far);
+    if (lane == 0) s_row = make_float4(row_max, l, H, far ? 1.f : 0.f);
   }
   __syncthreads();
-
-  // the row's: the parts of all CTAs, one a lane
-  float4 part = s_part;
-  if (C > 1) {
-    cluster.sync();
-    part = none;
-    if (lane < C) part = *cluster.map_shared_rank(&s_part, lane);
-    part = joined(part);
-  }
-  const float row_max = part.x;
-  float l, H;
-  const bool odd = row_max != row_max || row_max == INFINITY, dead = row_max == -INFINITY;
-  if (!odd && !dead && (row_max < Elem<T>::kLow || row_max > Elem<T>::kHigh)) {
-    // slow pass: differences from the maximum, natural units
-    if (C > 1) cluster.sync();   // everyone has read the maxima
-    float S = 0.f, Tn = 0.f;
-    for (int j = lo + tid; j < hi; j += THREADS) {
-      float v[Elem<T>::N];
-      Elem<T>::unpack(r.load(j, -INFINITY), v);
+  if constexpr (TOP) {
+    const uint32_t bound = __reduce_min_sync(0xffffffffu, s_top.least[lane % (kGroups / 32)]);
+    // Many groups that share the bound (rows of equal logits, few live ones): of the elements that equal it the first k are enough.
+    int reach = 0;
 #pragma unroll
-      for (int i = 0; i < Elem<T>::N; ++i) {
-        const float z = v[i] - row_max, e = exp2_fast(z * kLog2e);
-        S += e;
-        if (e > 0.f) Tn = fmaf(e, z, Tn);
-      }
-    }
-    S = warp_add(S);
-    Tn = warp_add(Tn);
-    __syncthreads();
-    if (lane == 0) s_warp[warp] = make_float4(0.f, 0.f, S, Tn);
-    __syncthreads();
-    if (tid == 0) {
-      S = Tn = 0.f;
-      for (int i = 0; i < kWarps; ++i) { S += s_warp[i].z; Tn += s_warp[i].w; }
-      s_part = make_float4(row_max, 0.f, S, Tn);
-    }
-    if (C > 1) cluster.sync(); else __syncthreads();
-    S = Tn = 0.f;
-    for (int i = 0; i < C; ++i) {
-      const float4 p = C > 1 ? *cluster.map_shared_rank(&s_part, i) : s_part;
-      S += p.z;
-      Tn += p.w;
-    }
-    l = logf(S);
-    H = fmaxf(l - Tn / S, 0.f);
-  } else if (odd) {
-    l = H = kNan;
-  } else if (dead) {
-    l = H = 0.f;
-  } else {
-    const float at_max = row_max * kLog2e;
-    Sums t{part.y, part.z, part.w};
-    t.move_to(at_max);
-    // at_max is row_max log2(e) but for its rounding, which is in every e: ln sum exp(x - row_max) = ln2 (log2 S + at_max - row_max log2(e))
-    const float off = -fmaf(row_max, kLog2e, -at_max), log2s = log2f(t.S);
-    l = (log2s + off) * kLn2;
-    H = fmaxf((log2s - t.T / t.S) * kLn2, 0.f);
+    for (int i = 0; i < kGroups; i += 32) reach += s_top.group[i + lane] >= bound;
+    const bool ties = bound > 0 && __reduce_add_sync(0xffffffffu, reach) > 2 * a.top_k + 32;
+    collect<T, THREADS>(r, lo, hi, bound + ties, best_key, CLUSTERED ? cluster.map_shared_rank(&s_top.cand[0], 0) : s_top.cand,
+                        CLUSTERED ? cluster.map_shared_rank(&s_top.n, 0) : &s_top.n);
+    if (ties && rank == 0) collect_first<T, THREADS>(r.row, r.V, bound, a.top_k, s_top);
+    if constexpr (CLUSTERED) cluster.sync(); else __syncthreads();
+    if (rank != 0) return;
   }
-  if (rank == 0 && tid == 0) {
+  const float4 row = s_row;
+  const float row_max = row.x;
+  float l = row.y, H = row.z;
+  if (row.w != 0.f) {
+    const float2 slow = slow_statistics<T, THREADS>(r.row, r.V, row_max, s_parts);
+    l = slow.x;
+    H = slow.y;
+  }
+  const bool odd = row_max != row_max || row_max == INFINITY, dead = row_max == -INFINITY;
+  if (tid == 0) {
     float lp = given - row_max - l;
     if (odd || id >= a.V) lp = kNan;
     else if (dead) lp = -INFINITY;
@@ -643,30 +782,22 @@ token_logprobs_kernel(LogprobArgs a) {
   }
   if constexpr (TOP) {
     const int k = a.top_k;
-    if (rank == 0) {
-      const uint64_t* best_of_row = s_top.top;
-      if (C > 1) {   // the CTAs' best ones, ranked once more
-        for (int i = tid; i < C * k; i += THREADS) s_top.cand[i] = cluster.map_shared_rank(s_top.top, i / k)[i % k];
-        __syncthreads();
-        uint64_t* to = s_top.cand + 8 * kMaxTop;
-        for (int i = tid; i < C * k; i += THREADS) {   // (places a CTA did not fill are 0 and come last)
-          const uint64_t mine = s_top.cand[i];
-          int above = 0;
-          for (int n = 0; n < C * k; ++n) above += s_top.cand[n] > mine;
-          if (mine != 0 && above < k) to[above] = mine;
-        }
-        __syncthreads();
-        best_of_row = to;
-      }
-      for (int i = tid; i < k; i += THREADS) {
-        const uint64_t key = best_of_row[i];
-        const float x = Elem<T>::of_key((uint32_t)(key >> 32));
-        a.top_ids[m * k + i] = (int32_t)~(uint32_t)key;
-        a.top_logprobs[m * k + i] = odd ? kNan : dead ? -INFINITY : x - row_max - l;
-      }
+    int n = s_top.n;
+    if (n > THREADS) {
+      __syncthreads();   // everyone has read the count
+      if (n > Scratch::kRoom) select_top<T, THREADS>(r.row, r.V, k, s_top);
+      else keep_best<THREADS>(s_top, k);
+      n = k;
+    }
+    rank_all<THREADS>(s_top, n, k);
+    __syncthreads();
+    for (int i = tid; i < k; i += THREADS) {
+      const uint64_t key = s_top.top[i];
+      const float x = Elem<T>::of_key((uint32_t)(key >> 32));
+      a.top_ids[m * k + i] = (int32_t)~(uint32_t)key;
+      a.top_logprobs[m * k + i] = odd ? kNan : dead ? -INFINITY : x - row_max - l;
     }
   }
-  if (C > 1) cluster.sync();   // the others' shared memory is read until here
 }
 
 // ---- gradient -----------------------------------------------------------------------------------------------------
@@ -802,7 +933,7 @@ int launch_forward(const LogprobArgs& a, int C, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = C > 1 ? 1 : 0;
-  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, THREADS, TOP>, a));
+  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, C > 1 ? token_logprobs_kernel<T, THREADS, TOP, true> : token_logprobs_kernel<T, THREADS, TOP, false>, a));
   XKB_CHECK_LAUNCH("token_logprobs_kernel");
   return XKB_OK;
 }
@@ -812,7 +943,7 @@ constexpr int kThreads = 256;
 // CTAs per row: few rows are cut so that the chip is full, as long as a piece keeps some vectors for every thread.
 int cluster_of(int64_t M, int64_t bytes) {
   int C = 1;
-  while (C < 8 && M * C * 2 <= 148 * (1024 / kThreads) && bytes / (2 * C) >= 16 * kThreads) C *= 2;
+  while (C < kMostCluster && M * C * 2 <= 148 * (1024 / kThreads) && bytes / (2 * C) >= 16 * kThreads) C *= 2;
   return C;
 }
 

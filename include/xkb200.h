@@ -143,7 +143,7 @@ int xkb_moe_sum_reduce(const void* y, int y_dtype, const void* w, int w_dtype,
  * grad_out [M, H], y [M, top_k, H] and grad_y of one dtype (XKB_BF16 or
  * XKB_F32), w NULL or [M, top_k] (w_dtype), grad_w of w_dtype.  grad_y and
  * grad_w may each be NULL (not wanted); y is read for grad_w only.  fp32 sums in
- * a fixed order.  One launch, no workspace.
+ * a fixed order.  M * top_k < 2^31, H < 2^28.  One launch, no workspace.
  * ---------------------------------------------------------------------- */
 int xkb_moe_sum_reduce_backward(const void* grad_out, int dtype, const void* y,
                                 const void* w, int w_dtype, void* grad_y,
@@ -161,7 +161,8 @@ int xkb_moe_sum_reduce_backward(const void* grad_out, int dtype, const void* y,
  * bytes: tokens with 0 count for nothing.  A row whose logits are all -inf has no
  * probabilities (adds 0); NaN and +inf make mean_probs and loss NaN.  Outputs:
  * loss [1] fp32, counts [E] int32, mean_probs [E] fp32, tokens [1] int32 (T).
- * T = 0: loss 0.  M * top_k < 2^31.  Two launches; the same bits in every run.
+ * T = 0: loss 0.  M * top_k < 2^31.  One launch without workspace for up to 512
+ * tokens (the query then says 0), two for more; the same bits in every run.
  * ---------------------------------------------------------------------- */
 int64_t xkb_moe_balance_loss_workspace_bytes(int64_t M, int E);
 int xkb_moe_balance_loss(const void* gating_output, int dtype,

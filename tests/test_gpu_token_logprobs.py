@@ -53,6 +53,35 @@ def test_rows(M, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [297, 593, 1185, 2369, 4000])
+def test_many_rows(M, dtype, cuda_device):
+    """Around the numbers of rows where a row gets fewer threads, and the widths and alternatives that decide with them."""
+    for V, k in ((8, 3), (100, 10), (1000, 0), (2049, 11), (4100, 21), (9001, 22)):
+        x, ids = head(M, V, dtype, cuda_device)
+        check(x, ids, k)
+    x, ids = head(M, 600, dtype, cuda_device)
+    x[::3] = -math.inf
+    x[1::3, 7:] = torch.finfo(dtype).min
+    x[2::6] = 1.0
+    x[5::12, 300:] = -math.inf
+    x[-1, 5] = math.nan
+    for k in (1, 10, 21, 64):
+        check(x, ids, k)
+
+
+@pytest.mark.parametrize("M,k", [(4000, 10), (2000, 20), (1000, 42)])
+def test_more_candidates_than_a_small_list_holds(M, k, cuda_device):
+    """As below for CTAs of 32, 64 and 128 threads: rows whose large values lie in the vectors of few threads."""
+    V = 3000
+    g = torch.Generator(device=cuda_device).manual_seed(7)
+    n = torch.arange(V, device=cuda_device)
+    for step, few in ((32, 9), (64, 19), (128, 40)):
+        value = torch.where((n // 4) % step < few, torch.rand(V, generator=g, device=cuda_device) + 9, 0.0)
+        x = (value + 0.001 * torch.rand(M, V, generator=g, device=cuda_device))
+        check(x, torch.zeros(M, dtype=torch.int64, device=cuda_device), k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("start,V,pitch", [(0, 1000, 1024), (3, 1001, 1024), (5, 77, 83), (1, 20000, 20003)])
 def test_rows_that_lie_apart(dtype, start, V, pitch, cuda_device):
     base, ids = head(9, pitch, dtype, cuda_device)

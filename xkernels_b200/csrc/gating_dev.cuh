@@ -1,0 +1,155 @@
+// Rows of gating logits in registers, shared by the balance loss and the gradient of the gating logits.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "softmax_dev.cuh"
+
+namespace xkb {
+
+constexpr int kMaxExperts = 1024;
+
+template <typename T> __device__ __forceinline__ float to_float(T v);
+template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T of_float(float v);
+template <> __device__ __forceinline__ float of_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 of_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half of_float<__half>(float v) { return __float2half_rn(v); }
+
+// The larger of two pairs of 16-bit values, NaN where one of them is.
+template <typename T> __device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Over each group of LANES neighbouring lanes.
+template <int LANES> __device__ __forceinline__ float lanes_add(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <int LANES> __device__ __forceinline__ float lanes_max_nan(float v) {
+  if constexpr (LANES == 32) {
+    return warp_max_nan(v);
+  } else {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  }
+}
+
+// 1 / s to 1 ulp; 0 for 0 (a row or a choice without a live logit).  The sums here are 0 or 2^-126 to 2^10, or NaN.
+__device__ __forceinline__ float inverse(float s) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return s == 0.f ? 0.f : r;
+}
+
+// e^(x - max) of one logit
+__device__ __forceinline__ float exponential(float x, float max) { return exp2_fast((x - max) * kLog2e); }
+
+// A row over LANES lanes, in pieces of P neighbouring experts: a lane's t-th value belongs to expert (t / P * LANES + lane) * P + t % P.
+// 8 lanes are a quarter of a warp, which then has four rows.
+template <typename T, int LANES, int PER_LANE, int P>
+struct Row {
+  struct alignas(P * sizeof(T)) Piece { T x[P]; };
+  static constexpr int kPieces = PER_LANE / P;
+  struct Raw { Piece q[kPieces]; };
+  static __device__ __forceinline__ int expert(int t, int lane) { return (t / P * LANES + lane) * P + t % P; }
+  // logits; -inf behind the row, and everywhere if there is none
+  static __device__ __forceinline__ Raw load(const T* row, int E, int lane, bool there) {
+    Raw r;
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) r.q[c].x[i] = of_float<T>(-INFINITY);
+      if (there && (c * LANES + lane) * P < E) r.q[c] = reinterpret_cast<const Piece*>(row)[c * LANES + lane];
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void store(T* row, int E, int lane, const float (&x)[PER_LANE]) {
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      Piece q;
+#pragma unroll
+      for (int i = 0; i < P; ++i) q.x[i] = of_float<T>(x[c * P + i]);
+      if ((c * LANES + lane) * P < E) reinterpret_cast<Piece*>(row)[c * LANES + lane] = q;
+    }
+  }
+  // the lane's maximum, NaN if one of its logits is
+  static __device__ __forceinline__ float lane_max(const Raw& r, const float (&x)[PER_LANE]) {
+    if constexpr (sizeof(T) == 2 && P >= 2) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+      uint32_t m = w[0];
+#pragma unroll
+      for (int i = 1; i < PER_LANE / 2; ++i) m = larger2<T>(m, w[i]);
+      const T* two = reinterpret_cast<const T*>(&m);
+      return max_nan(to_float(two[0]), to_float(two[1]));
+    } else {
+      float m = x[0];
+#pragma unroll
+      for (int t = 1; t < PER_LANE; ++t) m = max_nan(m, x[t]);
+      return m;
+    }
+  }
+  // logits -> e^(x - max), the row's maximum (0 for a row without a live logit, whose values become 0) and this lane's sum.  NaN and
+  // +inf make the row NaN.  Two values an instruction.
+  static __device__ __forceinline__ float exponentials(const Raw& r, float (&x)[PER_LANE], float& max) {
+#pragma unroll
+    for (int t = 0; t < PER_LANE; ++t) x[t] = to_float(r.q[t / P].x[t % P]);
+    const float mx = lanes_max_nan<LANES>(lane_max(r, x));
+    max = mx == -INFINITY ? 0.f : mx;
+    if constexpr (PER_LANE == 1) {
+      x[0] = exponential(x[0], max);
+      return x[0];
+    } else {
+      Pair sum = pair_of(0.f);
+      const Pair minus = pair_of(-max), scale = pair_of(kLog2e);
+#pragma unroll
+      for (int t = 0; t < PER_LANE; t += 2) {
+        const Pair y = mul2(add2(pair_of(x[t], x[t + 1]), minus), scale);
+        float y0, y1;
+        split(y, y0, y1);
+        x[t] = exp2_fast(y0);
+        x[t + 1] = exp2_fast(y1);
+        sum = add2(sum, pair_of(x[t], x[t + 1]));
+      }
+      float s0, s1;
+      split(sum, s0, s1);
+      return s0 + s1;
+    }
+  }
+};
+
+// Calls f<LANES, PER_LANE, P>() with the fewest values per lane that cover the row and the widest piece that the row and its
+// address allow.  Quarter warps take up to 64 experts, if their 8 lanes also have a lane for each slot.
+template <typename T, int LANES, int PER_LANE, typename F>
+int with_piece(int E, uintptr_t bits, F f) {   // bits: the addresses of all rows, or'ed
+  constexpr int kMost = PER_LANE < (int)(16 / sizeof(T)) ? PER_LANE : (int)(16 / sizeof(T));
+  auto fits = [&](int P) { return E % P == 0 && bits % (P * sizeof(T)) == 0; };
+  if constexpr (kMost > 2) if (fits(kMost)) return f.template operator()<LANES, PER_LANE, kMost>();
+  if constexpr (kMost >= 2) if (fits(2)) return f.template operator()<LANES, PER_LANE, 2>();
+  return f.template operator()<LANES, PER_LANE, 1>();
+}
+template <typename T, typename F>
+int with_shape(int E, int top_k, uintptr_t bits, F f) {
+  if (top_k <= 8) {
+    if (E <= 8) return with_piece<T, 8, 1>(E, bits, f);
+    if (E <= 16) return with_piece<T, 8, 2>(E, bits, f);
+    if (E <= 32) return with_piece<T, 8, 4>(E, bits, f);
+    if (E <= 64) return with_piece<T, 8, 8>(E, bits, f);
+  }
+  if (E <= 128) return with_piece<T, 32, 4>(E, bits, f);
+  if (E <= 256) return with_piece<T, 32, 8>(E, bits, f);
+  if (E <= 512) return with_piece<T, 32, 16>(E, bits, f);
+  return with_piece<T, 32, 32>(E, bits, f);
+}
+
+}  // namespace xkb

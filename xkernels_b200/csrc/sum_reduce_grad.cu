@@ -3,7 +3,8 @@
 //   dy[m, k, :] = f w[m, k] g[m, :]          dw[m, k] = f sum_h g[m, h] y[m, k, h]          (fp32 sums)
 //
 // HBM-bound: y is read once, dy written once, g read once.  A block is some slots of one token: a thread holds a piece of g
-// and requests the same piece of all its slots' rows before it uses the first.  The sum over h runs in a fixed order (thread,
+// and requests the same piece of all its slots' rows before it uses the first.  Rows whose ends lie anywhere go in narrower
+// accesses, several at once.  The sum over h runs in a fixed order (thread,
 // warp, block), so the result is the same in every run.
 #include "common.cuh"
 
@@ -15,31 +16,38 @@ __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162f
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// 16 bytes of a row
-template <typename T> struct Vec16;
-template <> struct Vec16<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
-    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
-  }
-  static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  }
-};
-template <> struct Vec16<__nv_bfloat16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+// N neighbouring elements, one access
+template <int BYTES> struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<2> { using type = unsigned short; };
+template <typename T, int N> using word = typename Word<N * (int)sizeof(T)>::type;
+
+template <int N> __device__ __forceinline__ void unpack(const word<float, N>& q, float (&v)[N], float) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(u[i] << 16);
-      v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    }
+  for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const float*>(&q)[i];
+}
+template <int N> __device__ __forceinline__ void unpack(const word<__nv_bfloat16, N>& q, float (&v)[N], __nv_bfloat16) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = bf16_bits_to_float(reinterpret_cast<const unsigned short*>(&q)[i]);
+}
+template <int N> __device__ __forceinline__ word<float, N> pack(const float (&v)[N], float) {
+  word<float, N> q;
+#pragma unroll
+  for (int i = 0; i < N; ++i) reinterpret_cast<float*>(&q)[i] = v[i];
+  return q;
+}
+template <int N> __device__ __forceinline__ word<__nv_bfloat16, N> pack(const float (&v)[N], __nv_bfloat16) {
+  word<__nv_bfloat16, N> q;
+  if constexpr (N == 1) {
+    q = (unsigned short)pack_bf16(v[0], 0.f);   // (the conversion of a single value runs on the special-function unit)
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) reinterpret_cast<uint32_t*>(&q)[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
   }
-  static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
-    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-  }
-};
+  return q;
+}
 
 struct Args {
   const void *go, *y, *w;
@@ -52,62 +60,84 @@ struct Args {
 
 constexpr int kMaxThreads = 256;
 
-// SLOTS slots of a token per block.  y (and gw) or gy may be missing.
-template <typename T, typename TW, int SLOTS>
+// SLOTS slots of a token per block, N elements per access (rows of an odd number of elements start anywhere), COLS accesses at once.
+// y (and gw) or gy may be missing.
+template <typename T, typename TW, int SLOTS, int N, int COLS>
 __global__ void __launch_bounds__(kMaxThreads)
 sum_reduce_grad_kernel(Args a) {
-  constexpr int N = Vec16<T>::N;
+  using W = word<T, N>;
   __shared__ float s_part[kMaxThreads / 32][SLOTS];
   const int64_t m = blockIdx.x / a.groups;
   const int k0 = (int)(blockIdx.x - m * a.groups) * SLOTS, n = min(SLOTS, a.top_k - k0);
-  const int64_t slot0 = m * a.top_k + k0, hv = a.H / N;
-  const uint4* g = reinterpret_cast<const uint4*>(static_cast<const T*>(a.go) + m * a.H);
-  const uint4* y = reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + slot0 * a.H);
-  uint4* gy = reinterpret_cast<uint4*>(static_cast<T*>(a.gy) + slot0 * a.H);
+  const int64_t slot0 = m * a.top_k + k0;
+  const unsigned hv = (unsigned)(a.H / N);   // SLOTS rows of it stay below 2^31
+  const W* g = reinterpret_cast<const W*>(static_cast<const T*>(a.go) + m * a.H);
+  const W* y = reinterpret_cast<const W*>(static_cast<const T*>(a.y) + slot0 * a.H);
+  W* gy = reinterpret_cast<W*>(static_cast<T*>(a.gy) + slot0 * a.H);
   float wk[SLOTS], acc[SLOTS];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) {
     acc[k] = 0.f;
     wk[k] = a.f * (a.w != nullptr && k < n ? as_float(static_cast<const TW*>(a.w)[slot0 + k]) : 1.f);
   }
-  for (int64_t i = threadIdx.x; i < hv; i += blockDim.x) {
-    uint4 q[SLOTS];
-    const uint4 gq = g[i];
-    if (a.gw != nullptr) {
+  for (unsigned i0 = threadIdx.x; i0 < hv; i0 += COLS * blockDim.x) {
+    W q[COLS][SLOTS], gq[COLS];
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k)
-        if (k < n) q[k] = __ldcs(y + k * hv + i);
-    }
-    float gv[N];
-    Vec16<T>::unpack(gq, gv);
-    if (a.gy != nullptr) {
+    for (int c = 0; c < COLS; ++c) {
+      const unsigned i = i0 + c * blockDim.x;
+      if (i >= hv) continue;
+      gq[c] = g[i];
+      if (a.gw != nullptr) {
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k) {
-        if (k >= n) break;
-        float v[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = gv[e] * wk[k];
-        __stcs(gy + k * hv + i, Vec16<T>::pack(v));
+        for (int k = 0; k < SLOTS; ++k)
+          if (k < n) q[c][k] = __ldcs(y + k * hv + i);
       }
     }
-    if (a.gw != nullptr) {
 #pragma unroll
-      for (int k = 0; k < SLOTS; ++k) {
-        if (k >= n) break;
-        float v[N];
-        Vec16<T>::unpack(q[k], v);
+    for (int c = 0; c < COLS; ++c) {
+      const unsigned i = i0 + c * blockDim.x;
+      if (i >= hv) continue;
+      float gv[N];
+      unpack<N>(gq[c], gv, T());
+      if (a.gy != nullptr) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[k] = fmaf(gv[e], v[e], acc[k]);
+        for (int k = 0; k < SLOTS; ++k) {
+          if (k >= n) break;
+          float v[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = gv[e] * wk[k];
+          __stcs(gy + k * hv + i, pack<N>(v, T()));
+        }
+      }
+      if (a.gw != nullptr) {
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+          if (k >= n) break;
+          float v[N];
+          unpack<N>(q[c][k], v, T());
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[k] = fmaf(gv[e], v[e], acc[k]);
+        }
       }
     }
   }
   if (a.gw == nullptr) return;
+  // Over the lanes: each step halves the slots that a lane adds up, until it has one, then the lanes of that slot.
+  const int lane = threadIdx.x & 31;
+  int o = 16, slot = 0;
 #pragma unroll
-  for (int k = 0; k < SLOTS; ++k) {
+  for (int have = SLOTS; have > 1; have /= 2, o /= 2) {
+    const bool upper = lane & o;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
-    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5][k] = acc[k];
+    for (int k = 0; k < have / 2; ++k) {
+      const float send = upper ? acc[k] : acc[k + have / 2], keep = upper ? acc[k + have / 2] : acc[k];
+      acc[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+    if (upper) slot += have / 2;
   }
+#pragma unroll
+  for (; o > 0; o /= 2) acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+  if ((lane & (32 / SLOTS - 1)) == 0) s_part[threadIdx.x >> 5][slot] = acc[0];
   __syncthreads();
   if ((int)threadIdx.x < n) {
     float sum = 0.f;
@@ -116,54 +146,40 @@ sum_reduce_grad_kernel(Args a) {
   }
 }
 
-// Any H, any alignment: a warp per slot.
-template <typename T, typename TW>
-__global__ void __launch_bounds__(256)
-sum_reduce_grad_scalar_kernel(Args a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t slots = a.M * a.top_k, warps = (int64_t)gridDim.x * 8;
-  for (int64_t s = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); s < slots; s += warps) {
-    const T* g = static_cast<const T*>(a.go) + s / a.top_k * a.H;
-    const float w = a.f * (a.w != nullptr ? as_float(static_cast<const TW*>(a.w)[s]) : 1.f);
-    float acc = 0.f;
-    for (int64_t h = lane; h < a.H; h += 32) {
-      const float x = as_float(g[h]);
-      if (a.gy != nullptr) put(static_cast<T*>(a.gy) + s * a.H + h, x * w);
-      if (a.gw != nullptr) acc = fmaf(x, as_float(static_cast<const T*>(a.y)[s * a.H + h]), acc);
-    }
-    if (a.gw == nullptr) continue;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0) put(static_cast<TW*>(a.gw) + s, acc * a.f);
-  }
-}
-
-template <typename T, typename TW, int SLOTS>
+template <typename T, typename TW, int SLOTS, int N>
 int launch_slots(Args a, cudaStream_t s) {
-  const int64_t hv = a.H / Vec16<T>::N;
+  constexpr int kCols = 16 / (N * (int)sizeof(T)) > 4 ? 4 : 16 / (N * (int)sizeof(T));
+  const int64_t hv = a.H / N;
   a.groups = (unsigned)ceil_div(a.top_k, SLOTS);
-  const int64_t steps = ceil_div(hv, (int64_t)kMaxThreads);   // as few threads as take the row in as many steps
-  const unsigned threads = (unsigned)align_up(ceil_div(hv, steps), 32);
-  sum_reduce_grad_kernel<T, TW, SLOTS><<<(unsigned)(a.M * a.groups), threads, 0, s>>>(a);
+  const int64_t steps = ceil_div(hv, (int64_t)kMaxThreads * kCols);   // as few threads as take the row in as many steps
+  const unsigned threads = (unsigned)align_up(ceil_div(hv, steps * kCols), 32);
+  sum_reduce_grad_kernel<T, TW, SLOTS, N, kCols><<<(unsigned)(a.M * a.groups), threads, 0, s>>>(a);
   XKB_CHECK_LAUNCH("sum_reduce_grad_kernel");
   return XKB_OK;
 }
 
+template <typename T, typename TW, int N>
+int launch_width(const Args& a, cudaStream_t s) {
+  // slots per block: all of them where the tokens fill the chip
+  if (a.top_k > 4 && a.M * ceil_div(a.top_k, 8) >= 2 * 148) return launch_slots<T, TW, 8, N>(a, s);
+  if (a.top_k > 2 && a.M * ceil_div(a.top_k, 4) >= 2 * 148) return launch_slots<T, TW, 4, N>(a, s);
+  if (a.top_k > 1 && a.M * ceil_div(a.top_k, 2) >= 2 * 148) return launch_slots<T, TW, 2, N>(a, s);
+  return launch_slots<T, TW, 1, N>(a, s);
+}
+
 template <typename T, typename TW>
 int launch(const Args& a, cudaStream_t s) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.go) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.gy);
-  if (a.H % Vec16<T>::N == 0 && bits % 16 == 0 && a.M * a.top_k <= 0x7fffffff) {
-    // slots per block: all of them where the tokens fill the chip
-    if (a.top_k > 4 && a.M * ceil_div(a.top_k, 8) >= 2 * 148) return launch_slots<T, TW, 8>(a, s);
-    if (a.top_k > 2 && a.M * ceil_div(a.top_k, 4) >= 2 * 148) return launch_slots<T, TW, 4>(a, s);
-    if (a.top_k > 1 && a.M * ceil_div(a.top_k, 2) >= 2 * 148) return launch_slots<T, TW, 2>(a, s);
-    return launch_slots<T, TW, 1>(a, s);
+  XKB_REQUIRE(a.M * a.top_k <= 0x7fffffff && a.H < (1 << 28), "moe_sum_reduce_backward: M * top_k must be below 2^31 and H below 2^28");
+  // the widest access whose boundaries all rows start on
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.go) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.gy) |
+                         (uintptr_t)(a.H * (int64_t)sizeof(T));
+  XKB_REQUIRE(bits % sizeof(T) == 0, "moe_sum_reduce_backward: misaligned tensor");
+  if (bits % 16 == 0) return launch_width<T, TW, 16 / sizeof(T)>(a, s);
+  if (bits % 8 == 0) return launch_width<T, TW, 8 / sizeof(T)>(a, s);
+  if constexpr (sizeof(T) == 2) {
+    if (bits % 4 == 0) return launch_width<T, TW, 2>(a, s);
   }
-  int64_t blocks = ceil_div(a.M * a.top_k, (int64_t)8);
-  if (blocks > 148 * 32) blocks = 148 * 32;
-  sum_reduce_grad_scalar_kernel<T, TW><<<(unsigned)blocks, 256, 0, s>>>(a);
-  XKB_CHECK_LAUNCH("sum_reduce_grad_scalar_kernel");
-  return XKB_OK;
+  return launch_width<T, TW, 1>(a, s);
 }
 
 }  // namespace

@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "softmax_dev.cuh"
 
 namespace xkb {
 namespace {
@@ -25,62 +26,14 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxTop = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kSlack = 11.f;              // 2^16
 constexpr float kNan = __builtin_nanf("");
 
-__device__ __forceinline__ float exp2_fast(float x) {   // 2 ulp; subnormal results are 0
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if one of them is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float warp_max_nan(float v) {
-  float r;
-  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float warp_max(float v) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ float warp_add(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Two fp32 values side by side: one instruction does both.
-struct Pair { uint64_t v; };
-__device__ __forceinline__ Pair pair_of(float lo, float hi) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
-  return p;
-}
-__device__ __forceinline__ Pair pair_of(float v) { return pair_of(v, v); }
-__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v)); }
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-
 // What a type of logits needs: N elements in 16 bytes, a running maximum of whole vectors, ordered keys.
 //   kClamp: smaller elements count as this, which keeps -inf out of the products.  A row whose maximum is not between kLow
 //   and kHigh, where a clamped element would count or x log2(e) is too coarse, takes the slow pass.
@@ -90,6 +43,7 @@ template <typename T> struct Elem;
 template <> struct Elem<float> {
   static constexpr int N = 4;
   static constexpr float kClamp = -1e8f, kLow = -1e6f, kHigh = 1e6f;
+  static constexpr uint32_t kMaskKey = 0x00800000u;   // of the lowest finite value: one above that of -inf
   using Max = float;
   static __device__ __forceinline__ Max lowest() { return -INFINITY; }
   static __device__ __forceinline__ Max larger(Max a, Max b) { return max_nan(a, b); }
@@ -124,6 +78,7 @@ template <> struct Elem<float> {
 template <> struct Elem<__nv_bfloat16> {
   static constexpr int N = 8;
   static constexpr float kClamp = -1e8f, kLow = -1e6f, kHigh = 1e6f;
+  static constexpr uint32_t kMaskKey = 0x0080u;
   using Max = __nv_bfloat162;
   static __device__ __forceinline__ Max as2(uint32_t u) { return *reinterpret_cast<Max*>(&u); }
   static __device__ __forceinline__ Max lowest() { return as2(0xff80ff80u); }
@@ -165,6 +120,7 @@ template <> struct Elem<__nv_bfloat16> {
 template <> struct Elem<__half> {
   static constexpr int N = 8;
   static constexpr float kClamp = -65504.f, kLow = -60000.f, kHigh = 1e6f;
+  static constexpr uint32_t kMaskKey = 0x0400u;
   using Max = __half2;
   static __device__ __forceinline__ Max as2(uint32_t u) { return *reinterpret_cast<Max*>(&u); }
   static __device__ __forceinline__ Max lowest() { return as2(0xfc00fc00u); }
@@ -321,6 +277,7 @@ struct TopScratch {
   alignas(16) uint32_t group[kGroups];       // the maxima of the row's groups of threads
   uint32_t key[THREADS];                     // (long way) of every thread
   int owner[THREADS];                        // (long way) threads whose elements are read again
+  int digits[256], digit, before, inside;    // (too many candidates) how many have a digit, and where the k-th is
   int ties[THREADS / 32];                    // of a warp
   uint32_t least[kGroups / 32];              // of a warp
   int n, owners;
@@ -328,36 +285,67 @@ struct TopScratch {
 };
 template <int THREADS> struct NoScratch {};
 
-// Leaves the k largest of the n candidates (n > k) at the front, in any order, and 0 in the places behind them.
+// Leaves the k largest of the n candidates (n >= k) at the front, in any order, and 0 in the places behind them: digits of
+// eight bits from the top, until the k-th's digit is one that all who share it are needed.
 template <int THREADS>
 __device__ __noinline__ void keep_best(TopScratch<THREADS>& s, int k) {
   constexpr int kEach = (TopScratch<THREADS>::kRoom + THREADS - 1) / THREADS;
-  static_assert(kEach < 16, "counts of four bits");
-  const int n = s.n;
-  uint64_t t = 0;
-#pragma unroll 1
-  for (int b = 63; b >= 0; --b) {
-    const uint64_t trial = t | (1ull << b);
-    int mine = 0, all = 0;
-    for (int i = threadIdx.x; i < n; i += THREADS) mine += s.cand[i] >= trial;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) all += __syncthreads_count((mine >> w) & 1) << w;
-    if (all >= k) t = trial;
-  }
+  const int n = s.n, tid = threadIdx.x;
   uint64_t mine[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    const int at = threadIdx.x + i * THREADS;
+    const int at = tid + i * THREADS;
     mine[i] = at < n ? s.cand[at] : 0;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) s.n = 0;
+  uint64_t floor = 0, known = 0;   // digits so far, which bits they are
+  int need = k;                    // of those that share them
+#pragma unroll 1
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    for (int i = tid; i < 256; i += THREADS) s.digits[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (mine[i] != 0 && (mine[i] & known) == floor) atomicAdd(&s.digits[mine[i] >> shift & 255], 1);
+    __syncthreads();
+    if (tid < 32) {   // the digit whose suffix sum reaches `need`: lane l has digits 8 l .. 8 l + 7
+      int count[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += count[i] = s.digits[tid * 8 + i];
+      int above = sum;             // of the lanes from this one on, then of those behind it
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int more = __shfl_down_sync(0xffffffffu, above, d);
+        if (tid + d < 32) above += more;
+      }
+      above -= sum;
+      if (above < need && above + sum >= need) {
+        int digit = 7;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+          digit = i;
+          if (above + count[i] >= need) break;
+          above += count[i];
+        }
+        s.digit = tid * 8 + digit;
+        s.before = above;
+        s.inside = s.digits[tid * 8 + digit];
+      }
+    }
+    __syncthreads();
+    floor |= (uint64_t)s.digit << shift;
+    known |= 255ull << shift;
+    need -= s.before;
+    const bool all = s.inside == need;
+    __syncthreads();
+    if (all) break;
+  }
+  if (tid == 0) s.n = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
-    if (mine[i] != 0 && mine[i] >= t) s.cand[atomicAdd(&s.n, 1)] = mine[i];
+    if (mine[i] != 0 && (mine[i] & known) >= floor) s.cand[atomicAdd(&s.n, 1)] = mine[i];
   __syncthreads();
-  if ((int)threadIdx.x >= k && threadIdx.x < TopScratch<THREADS>::kRanked) s.cand[threadIdx.x] = 0;
+  if (tid >= k && tid < TopScratch<THREADS>::kRanked) s.cand[tid] = 0;
   __syncthreads();
 }
 
@@ -366,13 +354,17 @@ template <int THREADS>
 __device__ __forceinline__ void rank_all(TopScratch<THREADS>& s, int n, int k) {
   const int tid = threadIdx.x;
   if (tid < k && tid >= n) s.top[tid] = 0;
-  if (n <= 32 && 4 * 32 <= THREADS) {   // four threads a candidate, every fourth place each
+  if (4 * n <= THREADS && THREADS >= 128) {   // four threads a candidate, every fourth place each
     const int i = tid >> 2;
-    if (i >= 32) return;
     const uint64_t mine = s.cand[i];
     int rank = 0;
+    if (n <= 32) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) rank += s.cand[j + (tid & 3)] > mine;
+      for (int j = 0; j < 32; j += 4) rank += s.cand[j + (tid & 3)] > mine;
+    } else {
+#pragma unroll 4
+      for (int j = tid & 3; j < n; j += 4) rank += s.cand[j] > mine;
+    }
     rank += __shfl_xor_sync(0xffffffffu, rank, 1);
     rank += __shfl_xor_sync(0xffffffffu, rank, 2);
     if ((tid & 3) == 0 && i < n && rank < k) s.top[rank] = mine;
@@ -750,11 +742,12 @@ token_logprobs_kernel(LogprobArgs a) {
   __syncthreads();
   if constexpr (TOP) {
     const uint32_t bound = __reduce_min_sync(0xffffffffu, s_top.least[lane % (kGroups / 32)]);
-    // Many groups that share the bound (rows of equal logits, few live ones): of the elements that equal it the first k are enough.
+    // Where many groups share the bound (rows of equal logits), or it is what masks are made of, the first k of the elements that
+    // equal it are enough.
     int reach = 0;
 #pragma unroll
     for (int i = 0; i < kGroups; i += 32) reach += s_top.group[i + lane] >= bound;
-    const bool ties = bound > 0 && __reduce_add_sync(0xffffffffu, reach) > 2 * a.top_k + 32;
+    const bool ties = bound > 0 && (bound <= Elem<T>::kMaskKey || __reduce_add_sync(0xffffffffu, reach) > 2 * a.top_k + 32);
     collect<T, THREADS>(r, lo, hi, bound + ties, best_key, CLUSTERED ? cluster.map_shared_rank(&s_top.cand[0], 0) : s_top.cand,
                         CLUSTERED ? cluster.map_shared_rank(&s_top.n, 0) : &s_top.n);
     if (ties && rank == 0) collect_first<T, THREADS>(r.row, r.V, bound, a.top_k, s_top);
@@ -816,43 +809,58 @@ struct GradArgs {
   int per;           // vectors of a CTA
 };
 
-constexpr int kGradThreads = 256;
+constexpr int kGradThreads = 256;   // at most
 
-// A CTA is a piece of a row: element by element from the saved statistics, then the columns that were given a gradient of
-// their own once more, so that each is rounded once.
-template <typename T>
+// A CTA is a piece of a row: element by element from the saved statistics.  A column that was given a gradient of its own is rounded
+// once: the token's is added where its thread comes by, the alternatives' columns are computed once more at the end.
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(kGradThreads)
 token_logprobs_grad_kernel(GradArgs a) {
-  constexpr int N = Elem<T>::N;
-  __shared__ int s_id[kMaxTop + 1];
-  __shared__ float s_g[kMaxTop + 1];
+  constexpr int N = Elem<T>::N, kGiven = TOP ? kMaxTop + 1 : 1;
+  __shared__ int s_id[kGiven];
+  __shared__ float s_g[kGiven];
   const int64_t m = blockIdx.x / a.chunks;
-  const int chunk = (int)(blockIdx.x - m * a.chunks), tid = threadIdx.x;
+  const int chunk = (int)(blockIdx.x - m * a.chunks), tid = threadIdx.x, threads = blockDim.x;
   const RowView<T> r(static_cast<const T*>(a.logits) + m * a.ld, a.V);
   T* out = static_cast<T*>(a.out) + m * a.ldo;   // at the same place within 16 bytes as the row
   const int lo = chunk * a.per, hi = min(lo + a.per, r.vectors);
 
-  // the row's coefficients; entry 0 is the given token, 1 .. top_k the alternatives
-  for (int i = tid; i <= a.top_k; i += kGradThreads) {
+  // the first logits are on their way before the row's coefficients are asked for
+  uint4 q[kBatch];
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    const int j = lo + u * threads + tid;
+    if (j < hi) q[u] = r.load(j, 0.f);
+  }
+  // what entry i was given: 0 is the token, 1 .. top_k the alternatives
+  auto given = [&](int i, int& column, float& g) {
     int64_t id = -1;
-    float g = 0.f;
+    g = 0.f;
     if (i == 0) {
       if (a.g_lp != nullptr) { id = id_at(a.ids, a.ids64, m); g = a.g_lp[m]; }
-    } else if (a.g_top != nullptr) {
+    } else {
       id = a.top_ids[m * a.top_k + i - 1];
       g = a.g_top[m * a.top_k + i - 1];
     }
     if (id < 0) g = 0.f;
     if (id >= a.V) g = kNan;
-    s_id[i] = id >= 0 && id < a.V ? (int)id : -1;
-    s_g[i] = g;
-  }
+    column = id >= 0 && id < a.V ? (int)id : -1;
+  };
   const float mx = a.stats[2 * m], l = a.stats[2 * m + 1];
   const float gh = a.g_entropy != nullptr ? a.g_entropy[m] : 0.f;
   const float h = a.g_entropy != nullptr ? a.entropy[m] : 0.f;
-  __syncthreads();
-  float G = 0.f;
-  for (int i = 0; i <= a.top_k; ++i) G += s_g[i];
+  int column = -1;
+  float own = 0.f, G = 0.f;
+  if constexpr (TOP) {
+    for (int i = tid; i <= a.top_k; i += threads) given(i, s_id[i], s_g[i]);
+    __syncthreads();
+    for (int i = 0; i <= a.top_k; ++i) G += s_g[i];
+  } else {
+    given(0, column, own);
+    G = own;
+  }
+  const int own_vector = column < 0 ? -1 : (column + r.skew) / N, own_place = (column + r.skew) % N;
+
   // -p (G + gh (ln p + h)) with ln p = x - mx - l: any value
   const bool dead = mx == -INFINITY;
   const float base = fmaf(gh, h, G);
@@ -866,16 +874,17 @@ token_logprobs_grad_kernel(GradArgs a) {
   const float c = mx * kLog2e, rest = -fmaf(mx, kLog2e, -c);
   const float scale = -exp2f(rest) * expf(-l);
   const Pair slope = pair_of(scale * gh * kLn2), level = pair_of(scale * fmaf(gh, fmaf(rest, kLn2, -l) + h, G)), minus_c = pair_of(-c);
-  for (int j0 = lo; j0 < hi; j0 += kBatch * kGradThreads) {
-    uint4 q[kBatch];
+  for (int j0 = lo; j0 < hi; j0 += kBatch * threads) {
+    if (j0 > lo) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int j = j0 + u * kGradThreads + tid;
-      if (j < hi) q[u] = r.load(j, 0.f);
+      for (int u = 0; u < kBatch; ++u) {
+        const int j = j0 + u * threads + tid;
+        if (j < hi) q[u] = r.load(j, 0.f);
+      }
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int j = j0 + u * kGradThreads + tid;
+      const int j = j0 + u * threads + tid;
       if (j >= hi) continue;
       float v[N];
       if (near) {
@@ -892,6 +901,10 @@ token_logprobs_grad_kernel(GradArgs a) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = gradient(v[i]);
       }
+      if (!TOP && j == own_vector) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += i == own_place ? own : 0.f;
+      }
       if (r.whole(j)) {
         *(reinterpret_cast<uint4*>(out - r.skew) + j) = Elem<T>::pack(v);
       } else {
@@ -903,25 +916,49 @@ token_logprobs_grad_kernel(GradArgs a) {
       }
     }
   }
-  __syncthreads();   // the columns below were written by other threads of this block
-  if (tid <= a.top_k) {
-    const int id = s_id[tid];
-    const int j = id < 0 ? -1 : (id + r.skew) / N;
-    if (id >= 0 && j >= lo && j < hi) {
+  if constexpr (TOP) {
+    __syncthreads();   // the columns below were written by other threads of this block
+    for (int n = tid; n <= a.top_k; n += threads) {
+      const int id = s_id[n];
+      const int j = id < 0 ? -1 : (id + r.skew) / N;
+      if (id < 0 || j < lo || j >= hi) continue;
       bool first = true;
-      float own = 0.f;
+      float sum = 0.f;
       for (int i = 0; i <= a.top_k; ++i) {   // a column may have been given more than one
         if (s_id[i] != id) continue;
-        if (i < tid) first = false;
-        own += s_g[i];
+        if (i < n) first = false;
+        sum += s_g[i];
       }
-      if (first) Elem<T>::store(out + id, gradient(Elem<T>::load(r.row + id)) + own);
+      if (first) Elem<T>::store(out + id, gradient(Elem<T>::load(r.row + id)) + sum);
     }
   }
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
-template <typename T, int THREADS, bool TOP>
+// Threads of a CTA, which is one row.  A small CTA lets more rows overlap their ends with each other's passes, a large one takes
+// a row in fewer steps.  So: halved while the rows fill the chip twice over with half the threads (a wave is 148 x 1024) and
+// a thread has less than 16 vectors (15 without alternatives).  us, 96 MB of bf16 rows, top 5, 32 / 64 / 128 / 256 threads: V=1000 64 / 123 /
+// 263 / 407, 4000 30 / 40 / 69 / 108, 8000 27 / 29 / 43 / 57, 16000 29 / 26 / 30 / 38, 32000 38 / 28 / 26 / 28, 128000 100 / 55 / 34 / 26; no
+// alternatives, V=8000 21.2 / 20.2 / 22.3 / 28.9, 16000 23.6 / 21.1 / 20.3 / 23.2; 128 rows of 4000, top 5, 6.3 / 5.3 / 5.0 / 4.8.
+// Below 128 threads, the number of groups is theirs, and top_k at most a third of it, or the bound lets too much through.
+int threads_of(int64_t M, int64_t vectors, int top_k) {
+  int threads = 256;
+  while (threads > 32 && (threads == 256 || 3 * top_k <= threads / 2) && M * threads > 148 * 512 && vectors < (top_k > 0 ? 16 : 15) * threads) threads /= 2;
+  return threads;
+}
+
+// CTAs of a row: long rows are cut, into as many as half fill the chip, or fill it if a piece stays long.  The barriers
+// of a cluster cost 1.5 us (less without alternatives), and every piece an end.  us, bf16, top 20, 1 / 2 / 4 / 8: 16 rows of 50001 9.1 / 7.8 / 7.1 / 6.7 (of 32000, top 5,
+// 6.0 / 6.7 / 6.2 / 6.7); 64 of 128000 14.7 / 11.2 / 9.4 / 10.6; 128 of 50001 9.9 / 9.8 / 11.1 / 16.5; 300 of 128000 25.4 / 22.9 / 26.5 / 38.5;
+// 509 of 50001 17.2 / 22.1 / 33.0 / 54.4.
+int cluster_of(int64_t M, int64_t bytes, int top_k) {
+  int C = 1;
+  if (bytes >= (top_k > 0 ? 64 : 32) * 1024)
+    while (C < kMostCluster && (M * C * 2 <= 2 * 148 || (M * C * 2 <= 4 * 148 && bytes / (2 * C) >= 96 * 1024))) C *= 2;
+  return C;
+}
+
+template <typename T, int THREADS, bool CLUSTERED>
 int launch_forward(const LogprobArgs& a, int C, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.M * C));
@@ -932,25 +969,23 @@ int launch_forward(const LogprobArgs& a, int C, cudaStream_t s) {
   attr[0].val.clusterDim.x = (unsigned)C;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = C > 1 ? 1 : 0;
-  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, C > 1 ? token_logprobs_kernel<T, THREADS, TOP, true> : token_logprobs_kernel<T, THREADS, TOP, false>, a));
+  cfg.numAttrs = CLUSTERED ? 1 : 0;
+  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, a.top_k > 0 ? token_logprobs_kernel<T, THREADS, true, CLUSTERED>
+                                                      : token_logprobs_kernel<T, THREADS, false, CLUSTERED>, a));
   XKB_CHECK_LAUNCH("token_logprobs_kernel");
   return XKB_OK;
 }
 
-constexpr int kThreads = 256;
-
-// CTAs per row: few rows are cut so that the chip is full, as long as a piece keeps some vectors for every thread.
-int cluster_of(int64_t M, int64_t bytes) {
-  int C = 1;
-  while (C < kMostCluster && M * C * 2 <= 148 * (1024 / kThreads) && bytes / (2 * C) >= 16 * kThreads) C *= 2;
-  return C;
-}
-
 template <typename T>
 int forward_typed(const LogprobArgs& a, cudaStream_t s) {
-  const int C = cluster_of(a.M, (int64_t)a.V * (int64_t)sizeof(T));
-  return a.top_k > 0 ? launch_forward<T, kThreads, true>(a, C, s) : launch_forward<T, kThreads, false>(a, C, s);
+  const int64_t bytes = (int64_t)a.V * (int64_t)sizeof(T);
+  switch (threads_of(a.M, ceil_div(bytes, (int64_t)16), a.top_k)) {
+    case 32: return launch_forward<T, 32, false>(a, 1, s);
+    case 64: return launch_forward<T, 64, false>(a, 1, s);
+    case 128: return launch_forward<T, 128, false>(a, 1, s);
+  }
+  const int C = cluster_of(a.M, bytes, a.top_k);
+  return C > 1 ? launch_forward<T, 256, true>(a, C, s) : launch_forward<T, 256, false>(a, 1, s);
 }
 
 template <typename T>
@@ -959,6 +994,7 @@ int backward_typed(GradArgs a, int64_t M, cudaStream_t s) {
                   (M == 1 || (a.ld - a.ldo) * (int64_t)sizeof(T) % 16 == 0),
               "token_logprobs_backward: a row of grad_logits must start at the same place within 16 bytes as the row of logits");
   XKB_REQUIRE(reinterpret_cast<uintptr_t>(a.logits) % sizeof(T) == 0, "token_logprobs_backward: misaligned logits");
+  // Pieces of two batches a thread, halved where the rows are few; short rows take as many threads as hold them in one batch.
   const int64_t vectors = ceil_div((int64_t)a.V + Elem<T>::N - 1, Elem<T>::N);
   int64_t per = 2 * kBatch * kGradThreads;
   while (per > kGradThreads && M * ceil_div(vectors, per) < 4 * 148) per /= 2;
@@ -966,7 +1002,9 @@ int backward_typed(GradArgs a, int64_t M, cudaStream_t s) {
   XKB_REQUIRE(M * chunks <= 0x7fffffff, "token_logprobs_backward: %lld rows of %d columns do not fit a grid", (long long)M, a.V);
   a.chunks = (unsigned)chunks;
   a.per = (int)per;
-  token_logprobs_grad_kernel<T><<<(unsigned)(M * chunks), kGradThreads, 0, s>>>(a);
+  const int64_t need = align_up(ceil_div(vectors < per ? vectors : per, (int64_t)kBatch), 32);
+  const unsigned threads = need < kGradThreads ? (unsigned)need : kGradThreads;
+  (a.top_k > 0 ? token_logprobs_grad_kernel<T, true> : token_logprobs_grad_kernel<T, false>)<<<(unsigned)(M * chunks), threads, 0, s>>>(a);
   XKB_CHECK_LAUNCH("token_logprobs_grad_kernel");
   return XKB_OK;
 }

@@ -204,6 +204,22 @@ PyObject* moe_sum_reduce(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Several small outputs are pieces of one allocation (an allocation takes as long as a short kernel): ordinary tensors over
+// disjoint pieces of one storage, each on 16 bytes.
+struct Pieces {
+  const at::Tensor base;
+  int64_t at = 0;
+  static int64_t room(int64_t elements) { return (elements * 4 + 15) / 16 * 16; }   // of 4-byte elements
+  Pieces(int64_t bytes, const at::TensorOptions& options) : base(at::empty({bytes}, options.dtype(at::kByte))) {}
+  at::Tensor take(at::ScalarType type, at::IntArrayRef sizes) {   // of 4-byte elements
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+    impl->set_sizes_contiguous(sizes);
+    impl->set_storage_offset(at / 4);
+    at += room(impl->numel());
+    return at::Tensor(std::move(impl));
+  }
+};
+
 // token_logprobs(logits [M, V], token_ids [M], top_k) -> (logprobs, entropy, stats, top_logprobs, top_ids)
 PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -214,9 +230,9 @@ PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (x == nullptr || args[1] == Py_None || !tokens_of(args[1], x->size(0), &ids)) Py_RETURN_NONE;
   const int64_t M = x->size(0), V = x->size(1);
   if (top_k < 0 || top_k > 64 || top_k > V) Py_RETURN_NONE;
-  const at::TensorOptions f = x->options().dtype(at::kFloat);
-  at::Tensor lp = at::empty({M}, f), entropy = at::empty({M}, f), stats = at::empty({M, 2}, f), top_lp = at::empty({M, top_k}, f),
-             top_ids = at::empty({M, top_k}, f.dtype(at::kInt));
+  Pieces pieces(2 * Pieces::room(M) + Pieces::room(2 * M) + 2 * Pieces::room(M * top_k), x->options());
+  at::Tensor lp = pieces.take(at::kFloat, {M}), entropy = pieces.take(at::kFloat, {M}), stats = pieces.take(at::kFloat, {M, 2}),
+             top_lp = pieces.take(at::kFloat, {M, top_k}), top_ids = pieces.take(at::kInt, {M, top_k});
   const int code = code_of(x->scalar_type()), ids64 = ids->scalar_type() == at::kLong;
   void* const stream = stream_of(*x);
   int status;
@@ -278,16 +294,17 @@ PyObject* moe_balance_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* ids = x == nullptr ? nullptr : chosen(args[1], x->size(0));
   if (ids == nullptr || !mask_of(args[2], x->size(0), &mask)) Py_RETURN_NONE;
   const int64_t M = x->size(0), E = x->size(1), ws_bytes = g_balance_bytes(M, (int)E);
-  const at::TensorOptions f = x->options().dtype(at::kFloat), i = f.dtype(at::kInt);
-  at::Tensor loss = at::empty({}, f), counts = at::empty({E}, i), mean = at::empty({E}, f), tokens = at::empty({}, i),
-             ws = at::empty({ws_bytes}, f.dtype(at::kByte));
+  Pieces pieces(2 * Pieces::room(1) + 2 * Pieces::room(E), x->options());
+  at::Tensor loss = pieces.take(at::kFloat, {}), tokens = pieces.take(at::kInt, {}), counts = pieces.take(at::kInt, {E}),
+             mean = pieces.take(at::kFloat, {E}), ws;
+  if (ws_bytes > 0) ws = at::empty({ws_bytes}, x->options().dtype(at::kByte));
   const int code = code_of(x->scalar_type()), top_k = (int)ids->size(1);
   void* const stream = stream_of(*x);
   int status;
   Py_BEGIN_ALLOW_THREADS
   status = g_balance(x->const_data_ptr(), code, data<int32_t>(ids), data<uint8_t>(mask), static_cast<float*>(loss.mutable_data_ptr()),
                      static_cast<int32_t*>(counts.mutable_data_ptr()), static_cast<float*>(mean.mutable_data_ptr()),
-                     static_cast<int32_t*>(tokens.mutable_data_ptr()), M, (int)E, top_k, ws.mutable_data_ptr(), ws_bytes, stream);
+                     static_cast<int32_t*>(tokens.mutable_data_ptr()), M, (int)E, top_k, ws.defined() ? ws.mutable_data_ptr() : nullptr, ws_bytes, stream);
   Py_END_ALLOW_THREADS
   if (status != 0) return PyLong_FromLong(status);
   return tuple_of(THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(counts)), THPVariable_Wrap(std::move(mean)),

@@ -271,7 +271,8 @@ constexpr int kBatch = 4;   // vectors a thread requests before it uses the firs
 template <int THREADS>
 struct TopScratch {
   static constexpr int kRoom = 8 * THREADS + kMaxTop, kGroups = THREADS < 128 ? THREADS : 128;
-  static constexpr int kRanked = 32;         // candidates that are ranked side by side: the places behind the last one hold 0
+  static constexpr int kRanked = 32;         // so many candidates are ranked in one step: the places behind the last one hold 0
+  static constexpr int kFew = THREADS < 128 ? 128 : THREADS;   // more are cut down to k first
   uint64_t cand[kRoom];                      // value key, ~column: all different, larger is better
   uint64_t top[kMaxTop];                     // the best ones, in order
   alignas(16) uint32_t group[kGroups];       // the maxima of the row's groups of threads
@@ -349,11 +350,11 @@ __device__ __noinline__ void keep_best(TopScratch<THREADS>& s, int k) {
   __syncthreads();
 }
 
-// The k best of the first n <= THREADS candidates to s.top, in order; unfilled places are 0.
+// The k best of the first n candidates to s.top, in order; unfilled places are 0.
 template <int THREADS>
 __device__ __forceinline__ void rank_all(TopScratch<THREADS>& s, int n, int k) {
   const int tid = threadIdx.x;
-  if (tid < k && tid >= n) s.top[tid] = 0;
+  for (int i = n + tid; i < k; i += THREADS) s.top[i] = 0;
   if (4 * n <= THREADS && THREADS >= 128) {   // four threads a candidate, every fourth place each
     const int i = tid >> 2;
     const uint64_t mine = s.cand[i];
@@ -370,12 +371,14 @@ __device__ __forceinline__ void rank_all(TopScratch<THREADS>& s, int n, int k) {
     if ((tid & 3) == 0 && i < n && rank < k) s.top[rank] = mine;
     return;
   }
-  if (tid >= n) return;
-  const uint64_t mine = s.cand[tid];
-  int rank = 0;
+#pragma unroll 1
+  for (int i = tid; i < n; i += THREADS) {
+    const uint64_t mine = s.cand[i];
+    int rank = 0;
 #pragma unroll 8
-  for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
-  if (rank < k) s.top[rank] = mine;
+    for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+    if (rank < k) s.top[rank] = mine;
+  }
 }
 
 __device__ __forceinline__ uint64_t candidate(uint32_t key, int col) { return (uint64_t)key << 32 | (uint32_t)~(uint32_t)col; }
@@ -626,7 +629,7 @@ constexpr int kMostCluster = 8;
 // CLUSTERED: a row belongs to the CTAs of a cluster.  They hand their parts to the first one, and their groups' maxima to each other,
 // by stores into its shared memory; behind the last barrier only the first one runs on.
 template <typename T, int THREADS, bool TOP, bool CLUSTERED>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS, (TOP || THREADS < 64 ? 1024 : 1280) / THREADS)   // (4096 x 128000: 182 us with 1024 threads an SM, 176 with 1280, 180 with 1536)
 token_logprobs_kernel(LogprobArgs a) {
   using Scratch = TopScratch<THREADS>;
   constexpr int kWarps = THREADS / 32, kGroups = Scratch::kGroups;
@@ -776,7 +779,7 @@ token_logprobs_kernel(LogprobArgs a) {
   if constexpr (TOP) {
     const int k = a.top_k;
     int n = s_top.n;
-    if (n > THREADS) {
+    if (n > Scratch::kFew) {
       __syncthreads();   // everyone has read the count
       if (n > Scratch::kRoom) select_top<T, THREADS>(r.row, r.V, k, s_top);
       else keep_best<THREADS>(s_top, k);
@@ -814,7 +817,7 @@ constexpr int kGradThreads = 256;   // at most
 // A CTA is a piece of a row: element by element from the saved statistics.  A column that was given a gradient of its own is rounded
 // once: the token's is added where its thread comes by, the alternatives' columns are computed once more at the end.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kGradThreads)
+__global__ void __launch_bounds__(kGradThreads, 4)
 token_logprobs_grad_kernel(GradArgs a) {
   constexpr int N = Elem<T>::N, kGiven = TOP ? kMaxTop + 1 : 1;
   __shared__ int s_id[kGiven];
@@ -906,7 +909,7 @@ token_logprobs_grad_kernel(GradArgs a) {
         for (int i = 0; i < N; ++i) v[i] += i == own_place ? own : 0.f;
       }
       if (r.whole(j)) {
-        *(reinterpret_cast<uint4*>(out - r.skew) + j) = Elem<T>::pack(v);
+        __stcs(reinterpret_cast<uint4*>(out - r.skew) + j, Elem<T>::pack(v));
       } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -940,10 +943,16 @@ token_logprobs_grad_kernel(GradArgs a) {
 // a thread has less than 16 vectors (15 without alternatives).  us, 96 MB of bf16 rows, top 5, 32 / 64 / 128 / 256 threads: V=1000 64 / 123 /
 // 263 / 407, 4000 30 / 40 / 69 / 108, 8000 27 / 29 / 43 / 57, 16000 29 / 26 / 30 / 38, 32000 38 / 28 / 26 / 28, 128000 100 / 55 / 34 / 26; no
 // alternatives, V=8000 21.2 / 20.2 / 22.3 / 28.9, 16000 23.6 / 21.1 / 20.3 / 23.2; 128 rows of 4000, top 5, 6.3 / 5.3 / 5.0 / 4.8.
-// Below 128 threads, the number of groups is theirs, and top_k at most a third of it, or the bound lets too much through.
+// Below 128 threads, which are then the groups, a top_k above a third of them lets more candidates through, and it pays for short
+// rows alone (48 MB, top 20, 32 / 64 threads: V=1000 48 / 70, 2000 34 / 39, 4000 28 / 25), above 5/8 not at all (top 32 122 / 83).
 int threads_of(int64_t M, int64_t vectors, int top_k) {
   int threads = 256;
-  while (threads > 32 && (threads == 256 || 3 * top_k <= threads / 2) && M * threads > 148 * 512 && vectors < (top_k > 0 ? 16 : 15) * threads) threads /= 2;
+  while (threads > 32 && M * threads > 148 * 512) {
+    const int groups = threads / 2;
+    const int least = top_k == 0 ? 15 : groups >= 128 || 3 * top_k <= groups ? 16 : 8 * top_k <= 5 * groups ? 6 : 0;
+    if (vectors >= least * threads) break;
+    threads /= 2;
+  }
   return threads;
 }
 
@@ -954,7 +963,7 @@ int threads_of(int64_t M, int64_t vectors, int top_k) {
 int cluster_of(int64_t M, int64_t bytes, int top_k) {
   int C = 1;
   if (bytes >= (top_k > 0 ? 64 : 32) * 1024)
-    while (C < kMostCluster && (M * C * 2 <= 2 * 148 || (M * C * 2 <= 4 * 148 && bytes / (2 * C) >= 96 * 1024))) C *= 2;
+    while (C < kMostCluster && (M * C * 2 <= 2 * 148 || (M * C * 2 <= 4 * 148 && bytes / (2 * C) >= 64 * 1024))) C *= 2;
   return C;
 }
 
@@ -994,11 +1003,19 @@ int backward_typed(GradArgs a, int64_t M, cudaStream_t s) {
                   (M == 1 || (a.ld - a.ldo) * (int64_t)sizeof(T) % 16 == 0),
               "token_logprobs_backward: a row of grad_logits must start at the same place within 16 bytes as the row of logits");
   XKB_REQUIRE(reinterpret_cast<uintptr_t>(a.logits) % sizeof(T) == 0, "token_logprobs_backward: misaligned logits");
-  // Pieces of two batches a thread, halved where the rows are few; short rows take as many threads as hold them in one batch.
-  const int64_t vectors = ceil_div((int64_t)a.V + Elem<T>::N - 1, Elem<T>::N);
-  int64_t per = 2 * kBatch * kGradThreads;
-  while (per > kGradThreads && M * ceil_div(vectors, per) < 4 * 148) per /= 2;
-  const int64_t chunks = ceil_div(vectors, per);
+  // Pieces of a row: few, for every one costs as much as 128 vectors before it has begun, but a whole number of waves of four CTAs
+  // per SM.  Pieces are at most eight batches (4096 rows of 128000 bf16 in a loop of calls, where power decides: one batch 377 us,
+  // two 357, eight 340, sixteen 346).  Short rows take as many threads as hold them in one batch.
+  const int64_t vectors = ceil_div((int64_t)a.V + Elem<T>::N - 1, Elem<T>::N), most = 8 * kBatch * kGradThreads;
+  int64_t chunks = 1, per = vectors, least = INT64_MAX;
+  for (int64_t c = ceil_div(vectors, most), end = c + 63; c <= end && (c == 1 || ceil_div(vectors, c) >= kGradThreads); ++c) {
+    const int64_t p = align_up(ceil_div(vectors, c), kGradThreads), cost = ceil_div(M * c, (int64_t)4 * 148) * (p + 128);
+    if (cost < least) {
+      least = cost;
+      chunks = c;
+      per = ceil_div(vectors, c);
+    }
+  }
   XKB_REQUIRE(M * chunks <= 0x7fffffff, "token_logprobs_backward: %lld rows of %d columns do not fit a grid", (long long)M, a.V);
   a.chunks = (unsigned)chunks;
   a.per = (int)per;

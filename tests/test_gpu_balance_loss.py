@@ -90,6 +90,15 @@ def test_dropped_slots_and_masked_tokens(dtype, cuda_device):
     assert not bool(check_grad(x, ids, None, True, r.counts, r.tokens, 1.0, none).any())
 
 
+def test_wide_ids_are_dropped_slots_too(cuda_device):
+    """int64 ids that no int32 holds do not wrap around to an expert."""
+    x, ids, g_w, _ = case(40, 16, 4, torch.float32, cuda_device)
+    wide = ids.long()
+    wide[::3, 0], wide[1::3, 1] = 2 ** 32 + 3, -(2 ** 33)
+    check_loss(x, wide)
+    check_grad(x, wide, g_w, True)
+
+
 def test_padding_may_hold_anything(cuda_device):
     """Rows behind the mask, and rows that no gradient comes back to, are not looked at."""
     x, ids, g_w, mask = case(200, 64, 4, torch.float32, cuda_device)

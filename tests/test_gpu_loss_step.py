@@ -163,6 +163,18 @@ def test_the_differentiable_forms_refuse_capture(cuda_device):
     assert torch.equal(at, xkb.topk_softmax(x, 2)[1])
 
 
+def test_nor_does_their_backward_pass_run_in_one(cuda_device, monkeypatch):
+    """(The answer of a capturing stream is put in its place: a captured backward pass is not started.)"""
+    x, ids, y = torch.randn(8, 16, device=cuda_device), torch.zeros(8, dtype=torch.int64, device=cuda_device), torch.randn(8, 2, 4, device=cuda_device)
+    leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+    w, at = xka.topk_softmax(leaf(x), 2)
+    outs = [w, xka.token_logprobs(leaf(x), ids).logprobs, xka.moe_balance_loss(leaf(x), at).loss, xka.moe_sum_reduce(leaf(y), w.detach())]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for out in outs:
+        with pytest.raises(RuntimeError, match="captured"):
+            out.sum().backward()
+
+
 def test_on_another_stream(cuda_device):
     """Inputs made on the stream that the calls run on, nothing waits for the default stream."""
     want = functional_step(*inputs(cuda_device, 4))

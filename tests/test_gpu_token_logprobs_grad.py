@@ -92,6 +92,11 @@ def test_the_same_column_again(cuda_device):
     want, err = ref.token_grad(x, ids, False, g_lp, None, at, g)
     want[2] = math.nan                       # 500 is no column
     ref.assert_near(got, want, err)
+    wide = at.long()
+    wide[1, 0], wide[1, 3] = -(2 ** 33), 2 ** 32 + 3      # nor are these, one no token and one behind the row
+    got = xkb.token_logprobs_backward(x, ids, torch.stack([m, l], dim=1).float(), grad_logprobs=g_lp, top_ids=wide, grad_top_logprobs=g)
+    want[1] = math.nan
+    ref.assert_near(got, want, err)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -162,6 +167,7 @@ def test_no_rows_and_refusals(cuda_device):
                         (lambda: f(x.double(), ids, r.stats, grad_logprobs=kw["g_lp"]), TypeError),
                         (lambda: f(x, ids, r.stats.cpu(), grad_logprobs=kw["g_lp"]), RuntimeError),
                         (lambda: f(x, ids, r.stats, top_ids=r.top_ids[:, :2], grad_top_logprobs=kw["g_top"]), ValueError),
+                        (lambda: f(x, ids, r.stats, top_ids=r.top_ids.float(), grad_top_logprobs=kw["g_top"]), TypeError),
                         (lambda: f(x, ids, r.stats, top_ids=ids[:, None].expand(4, 65), grad_top_logprobs=x[:, :65]), ValueError)):
         with pytest.raises(error):
             call()

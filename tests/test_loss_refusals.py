@@ -89,6 +89,10 @@ def test_there_is_no_cpu_path(lib):
                  lambda: xka.moe_sum_reduce(y)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+    for call in (lambda: xka.token_logprobs(x.requires_grad_(), ids[:, 0]), lambda: xka.topk_softmax(x, 2)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    x = x.detach()
     for call in (lambda: xkb.token_logprobs([1.0], ids), lambda: xkb.moe_balance_loss(None, [1]), lambda: xkb.moe_sum_reduce_backward(3, y)):
         with pytest.raises(TypeError):
             call()

@@ -5,8 +5,8 @@ gradient ops there.  First derivatives only.
 
 They are not for stream capture: torch ties the accumulation of a leaf's gradient to the stream that first used the
 leaf, and a captured backward pass that meets it on another stream ends the process.  A call that would record a
-gradient while its stream is being captured is refused; a captured step calls the gradient ops themselves
-(``ops.moe_router_backward`` and so on), which are ordinary stream-ordered launches.
+gradient while its stream is being captured is refused, and so is its backward pass there; a captured step calls the
+gradient ops themselves (``ops.moe_router_backward`` and so on), which are ordinary stream-ordered launches.
 """
 
 from __future__ import annotations
@@ -18,8 +18,12 @@ from . import ops
 
 
 def _not_captured(name: str, *inputs) -> None:
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs) \
-            and torch.cuda.is_current_stream_capturing():
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.is_cuda and t.requires_grad for t in inputs):
+        _not_capturing(name)
+
+
+def _not_capturing(name: str) -> None:
+    if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name}: the differentiable form cannot be captured; call the gradient op of xkernels_b200.ops")
 
 
@@ -36,6 +40,7 @@ class _TopkSoftmax(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_w, _):
+        _not_capturing("topk_softmax")
         if grad_w is None:
             return None, None, None
         gating, ids = ctx.saved_tensors
@@ -61,6 +66,7 @@ class _SumReduce(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
+        _not_capturing("moe_sum_reduce")
         if grad_out is None:
             return None, None, None
         y, w = ctx.saved_tensors
@@ -90,6 +96,7 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_loss, *_):
+        _not_capturing("moe_balance_loss")
         if grad_loss is None:
             return None, None, None
         gating, ids, mask, counts, tokens = ctx.saved_tensors
@@ -114,6 +121,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_lp, grad_entropy, _, grad_top, __):
+        _not_capturing("token_logprobs")
         if grad_lp is None and grad_entropy is None and grad_top is None:
             return None, None, None
         logits, ids, stats, entropy, top_ids = ctx.saved_tensors

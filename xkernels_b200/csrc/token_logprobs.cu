@@ -963,7 +963,7 @@ int threads_of(int64_t M, int64_t vectors, int top_k) {
 int cluster_of(int64_t M, int64_t bytes, int top_k) {
   int C = 1;
   if (bytes >= (top_k > 0 ? 64 : 32) * 1024)
-    while (C < kMostCluster && (M * C * 2 <= 2 * 148 || (M * C * 2 <= 4 * 148 && bytes / (2 * C) >= 64 * 1024))) C *= 2;
+    while (C < kMostCluster && (M * C * 2 <= 2 * 148 || (M * C * 2 <= 4 * 148 && bytes / (2 * C) >= 48 * 1024))) C *= 2;
   return C;
 }
 
@@ -1026,7 +1026,7 @@ int backward_typed(GradArgs a, int64_t M, cudaStream_t s) {
   return XKB_OK;
 }
 
-constexpr int64_t kMaxColumns = 0x7fffffff - 64;
+constexpr int64_t kMaxColumns = 0x7fffffff - 4096;   // columns behind the row's end, of threads without a vector, are numbers too
 
 }  // namespace
 }  // namespace xkb

@@ -336,6 +336,8 @@ def _gating(name, gating_output, topk_ids):
             raise ValueError(f"{name}: topk_ids must be [{M}, top_k], got {list(topk_ids.shape)}")
         if topk_ids.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"{name}: topk_ids must be int32 or int64, got {topk_ids.dtype}")
+        if topk_ids.dtype == torch.int64:       # what no int32 holds stays outside [0, E)
+            topk_ids = topk_ids.clamp(-1, E)
         topk_ids = topk_ids.to(torch.int32).contiguous()
     return gating_output.contiguous(), topk_ids, M, E
 
@@ -569,7 +571,11 @@ def token_logprobs_backward(logits, token_ids, stats, entropy=None, grad_logprob
         entropy = _typed(name, "entropy", entropy, (M,), torch.float32)
     top_k = 0
     if grad_top_logprobs is not None:
-        top_k = int(top_ids.shape[-1])
+        top_k = int(top_ids.shape[-1]) if top_ids.dim() else 0
+        if top_ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: top_ids must be int32 or int64, got {top_ids.dtype}")
+        if top_ids.dtype == torch.int64:
+            top_ids = top_ids.clamp(-1, V)
         top_ids = _typed(name, "top_ids", top_ids, (M, top_k), torch.int32)
         grad_top_logprobs = _typed(name, "grad_top_logprobs", grad_top_logprobs, (M, top_k), torch.float32)
         if top_k > 64:

@@ -91,17 +91,8 @@ balance_kernel(LossArgs a) {
     // (a group without a row holds -inf and adds 0)
     float x[PER_LANE], max;
     const float inv = inverse(lanes_add<LANES>(R::exponentials(raw, x, max)));
-    if constexpr (PER_LANE == 1) {
-      acc[0] = fmaf(x[0], inv, acc[0]);
-    } else {
 #pragma unroll
-      for (int t = 0; t < PER_LANE; t += 2) {
-        float a0, a1;
-        split(fma2(pair_of(x[t], x[t + 1]), pair_of(inv), pair_of(acc[t], acc[t + 1])), a0, a1);
-        acc[t] = a0;
-        acc[t + 1] = a1;
-      }
-    }
+    for (int t = 0; t < PER_LANE; ++t) acc[t] = fmaf(x[t], inv, acc[t]);
   }
   mine = __reduce_add_sync(0xffffffffu, sub == 0 ? mine : 0);
   if (lane == 0 && mine != 0) atomicAdd(&s_tokens, mine);

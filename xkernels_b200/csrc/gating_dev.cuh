@@ -29,6 +29,26 @@ template <typename T> __device__ __forceinline__ uint32_t larger2(uint32_t a, ui
   return r;
 }
 
+// Two values in a word, and a word's two values.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16(lo, hi);
+  }
+}
+template <typename T> __device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x;
+    hi = f.y;
+  } else {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+  }
+}
+
 // Over each group of LANES neighbouring lanes.
 template <int LANES> __device__ __forceinline__ float lanes_add(float v) {
 #pragma unroll
@@ -45,15 +65,19 @@ template <int LANES> __device__ __forceinline__ float lanes_max_nan(float v) {
   }
 }
 
-// 1 / s to 1 ulp; 0 for 0 (a row or a choice without a live logit).  The sums here are 0 or 2^-126 to 2^10, or NaN.
+// 1 / s to 1 ulp; 0 for 0 (a row or a choice without a live logit).  The sums here are 0 or 2^-127 to 2^11, or NaN.
 __device__ __forceinline__ float inverse(float s) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(s));
   return s == 0.f ? 0.f : r;
 }
 
-// e^(x - max) of one logit
-__device__ __forceinline__ float exponential(float x, float max) { return exp2_fast((x - max) * kLog2e); }
+// e^(x - max), but for a factor that all terms of a row share: 2^(x log2(e) - c) with c = max log2(e) rounded, one multiply-add.  Where
+// the rounding could come near 1 the difference is taken first.
+constexpr float kNear = 1e6f;
+__device__ __forceinline__ float exponential(float x, float max) {
+  return exp2_fast(fabsf(max) <= kNear ? fmaf(x, kLog2e, -(max * kLog2e)) : (x - max) * kLog2e);
+}
 
 // A row over LANES lanes, in pieces of P neighbouring experts: a lane's t-th value belongs to expert (t / P * LANES + lane) * P + t % P.
 // 8 lanes are a quarter of a warp, which then has four rows.
@@ -68,8 +92,13 @@ struct Row {
     Raw r;
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
+      if constexpr (sizeof(T) == 2 && P >= 2) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) r.q[c].x[i] = of_float<T>(-INFINITY);
+        for (int i = 0; i < P / 2; ++i) reinterpret_cast<uint32_t*>(&r.q[c])[i] = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) r.q[c].x[i] = of_float<T>(-INFINITY);
+      }
       if (there && (c * LANES + lane) * P < E) r.q[c] = reinterpret_cast<const Piece*>(row)[c * LANES + lane];
     }
     return r;
@@ -78,8 +107,13 @@ struct Row {
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
       Piece q;
+      if constexpr (sizeof(T) == 2 && P >= 2) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) q.x[i] = of_float<T>(x[c * P + i]);
+        for (int i = 0; i < P; i += 2) reinterpret_cast<uint32_t*>(&q)[i / 2] = pack2<T>(x[c * P + i], x[c * P + i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) q.x[i] = of_float<T>(x[c * P + i]);
+      }
       if ((c * LANES + lane) * P < E) reinterpret_cast<Piece*>(row)[c * LANES + lane] = q;
     }
   }
@@ -99,26 +133,35 @@ struct Row {
       return m;
     }
   }
-  // logits -> e^(x - max), the row's maximum (0 for a row without a live logit, whose values become 0) and this lane's sum.  NaN and
-  // +inf make the row NaN.  Two values an instruction.
+  // logits -> exponential(x, max), the row's maximum (0 for a row without a live logit, whose values become 0) and this lane's sum.
+  // NaN and +inf make the row NaN.
   static __device__ __forceinline__ float exponentials(const Raw& r, float (&x)[PER_LANE], float& max) {
+    if constexpr (sizeof(T) == 2 && P >= 2) {
 #pragma unroll
-    for (int t = 0; t < PER_LANE; ++t) x[t] = to_float(r.q[t / P].x[t % P]);
+      for (int t = 0; t < PER_LANE; t += 2) unpack2<T>(reinterpret_cast<const uint32_t*>(&r)[t / 2], x[t], x[t + 1]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < PER_LANE; ++t) x[t] = to_float(r.q[t / P].x[t % P]);
+    }
     const float mx = lanes_max_nan<LANES>(lane_max(r, x));
     max = mx == -INFINITY ? 0.f : mx;
     if constexpr (PER_LANE == 1) {
       x[0] = exponential(x[0], max);
       return x[0];
     } else {
+      if (fabsf(max) <= kNear) {   // (NaN: below)
+        const Pair scale = pair_of(kLog2e), minus_c = pair_of(-(max * kLog2e));
+#pragma unroll
+        for (int t = 0; t < PER_LANE; t += 2) split(fma2(pair_of(x[t], x[t + 1]), scale, minus_c), x[t], x[t + 1]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < PER_LANE; ++t) x[t] = (x[t] - max) * kLog2e;
+      }
       Pair sum = pair_of(0.f);
-      const Pair minus = pair_of(-max), scale = pair_of(kLog2e);
 #pragma unroll
       for (int t = 0; t < PER_LANE; t += 2) {
-        const Pair y = mul2(add2(pair_of(x[t], x[t + 1]), minus), scale);
-        float y0, y1;
-        split(y, y0, y1);
-        x[t] = exp2_fast(y0);
-        x[t + 1] = exp2_fast(y1);
+        x[t] = exp2_fast(x[t]);
+        x[t + 1] = exp2_fast(x[t + 1]);
         sum = add2(sum, pair_of(x[t], x[t + 1]));
       }
       float s0, s1;

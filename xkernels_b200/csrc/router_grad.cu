@@ -14,6 +14,10 @@ namespace xkb {
 namespace {
 
 constexpr int kWarps = 8;
+// Resident blocks, and the grid: a block that follows another has to ask for the counts again.  us, bf16, both gradients: 16384 x 256 with
+// 4 / 5 / 6 blocks 7.7 / 8.7 / 10.2, with a grid of twice as many 8.2; 65536 x 512 65 with 3, 46 with 4; 16384 x 1024 36 / 21 with 1 / 2.
+// (Asking for the next row while one is computed: 9.2, for the registers that it takes.)
+constexpr int blocks_per_sm(int per_lane) { return per_lane > 16 ? 2 : 4; }
 
 struct GateArgs {
   const void* gating;
@@ -31,7 +35,7 @@ struct GateArgs {
 };
 
 template <typename T, int LANES, int PER_LANE, int P, bool BALANCE>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(PER_LANE))
 router_grad_kernel(GateArgs a) {
   using R = Row<T, LANES, PER_LANE, P>;
   constexpr int kRows = 32 / LANES, kPlaces = LANES * PER_LANE;
@@ -73,9 +77,8 @@ router_grad_kernel(GateArgs a) {
         g = 0.f;
       }
     }
-    const bool more = LANES == 32 && weights && a.k > LANES;   // (quarter warps have a lane for each slot)
     const bool counted = BALANCE && there && (a.mask == nullptr || a.mask[m] != 0);
-    // a row that nothing comes back to (padding) has gradient 0, whatever its logits are
+    const bool more = LANES == 32 && weights && a.k > LANES;   // (quarter warps have a lane for each slot)
     bool live = counted || g != 0.f;
     if (more)
       for (int j = sub + LANES; j < a.k; j += LANES) live |= (unsigned)ids[j] < (unsigned)a.E && g_w[j] != 0.f;
@@ -95,8 +98,16 @@ router_grad_kernel(GateArgs a) {
         dot = fmaf(eo, g_w[j], dot);
       }
     if constexpr (BALANCE) {
+      if constexpr (PER_LANE == 1) {
+        even = x[0] * share[0];
+      } else {
+        Pair sums = pair_of(0.f);
 #pragma unroll
-      for (int t = 0; t < PER_LANE; ++t) even = fmaf(x[t], share[t], even);
+        for (int t = 0; t < PER_LANE; t += 2) sums = fma2(pair_of(x[t], x[t + 1]), pair_of(share[t], share[t + 1]), sums);
+        float e0, e1;
+        split(sums, e0, e1);
+        even = e0 + e1;
+      }
     }
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -108,15 +119,16 @@ router_grad_kernel(GateArgs a) {
     const float inv = inverse(sum), s = (counted ? even * inv : 0.f) + (a.renorm ? 0.f : dot * inv);
     // e^x (inv share - inv s)
     const float f = counted ? inv : 0.f, f0 = -inv * s;
-    if constexpr (PER_LANE == 1) {
-      x[0] = live ? x[0] * (BALANCE ? fmaf(f, share[0], f0) : f0) : 0.f;
+    if (!live) {   // a row that nothing comes back to (padding) has gradient 0, whatever its logits are
+#pragma unroll
+      for (int t = 0; t < PER_LANE; ++t) x[t] = 0.f;
+    } else if constexpr (PER_LANE == 1) {
+      x[0] *= BALANCE ? fmaf(f, share[0], f0) : f0;
     } else {
 #pragma unroll
       for (int t = 0; t < PER_LANE; t += 2) {
         const Pair d = BALANCE ? fma2(pair_of(f), pair_of(share[t], share[t + 1]), pair_of(f0)) : pair_of(f0);
         split(mul2(pair_of(x[t], x[t + 1]), d), x[t], x[t + 1]);
-        x[t] = live ? x[t] : 0.f;
-        x[t + 1] = live ? x[t + 1] : 0.f;
       }
     }
     if (there) R::store(out, a.E, sub, x);
@@ -154,7 +166,7 @@ template <typename T> struct LaunchGrad {
   const GateArgs& a;
   cudaStream_t s;
   template <int LANES, int PER_LANE, int P> int operator()() const {
-    const int64_t want = ceil_div(a.M, (int64_t)kWarps * 32 / LANES), most = 148 * 8;
+    const int64_t want = ceil_div(a.M, (int64_t)kWarps * 32 / LANES), most = 148 * blocks_per_sm(PER_LANE);
     const unsigned blocks = (unsigned)(want < most ? want : most);
     (a.counts != nullptr ? router_grad_kernel<T, LANES, PER_LANE, P, true>
                          : router_grad_kernel<T, LANES, PER_LANE, P, false>)<<<blocks, 32 * kWarps, 0, s>>>(a);

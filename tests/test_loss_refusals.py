@@ -81,6 +81,39 @@ def test_sum_reduce_backward(lib):
         assert b"moe_sum_reduce_backward" in lib.xkb_last_error()
 
 
+def test_misaligned_tensors_and_counts_beyond_64_bits(lib):
+    f1 = ctypes.c_float(1.0)
+
+    def logprobs(x=P, dtype=0, ids=P, ids64=0, o=(P, P, P, P, P)):
+        return lib.xkb_token_logprobs(x, dtype, 100, ids, ids64, *o, 4, 100, 5, None)
+
+    def logprobs_grad(ids=P, ids64=0, p=(P, P, P, P, P, P), M=4):
+        return lib.xkb_token_logprobs_backward(P, 0, 100, ids, ids64, *p[:4], *p[4:], 5, P, 100, M, 100, None)
+
+    def balance(g=P, dtype=0, p=(P, P, P, P, P), M=4, k=2):
+        return lib.xkb_moe_balance_loss(g, dtype, p[0], None, *p[1:], M, 8, k, P, 1 << 20, None)
+
+    def router(g=P, dtype=0, p=(P, P, P, P, P), out=P):
+        return lib.xkb_moe_router_backward(g, dtype, p[0], p[1], 1, p[2], p[3], p[4], f1, None, out, 4, 8, 2, None)
+
+    def combine(w=P, wd=1, gw=P, M=4, k=2, H=8):
+        return lib.xkb_moe_sum_reduce_backward(P, 0, P, w, wd, P, gw, M, k, H, f1, None)
+
+    assert logprobs(ids=P + 4, ids64=1) == -1 and logprobs(ids=P + 2) == -1
+    assert logprobs_grad(ids=P + 4, ids64=1) == -1 and logprobs_grad(ids=P + 2) == -1 and logprobs_grad(M=2 ** 62) == -1
+    for i in range(6):
+        p = tuple(P + 2 if j == i else P for j in range(6))
+        assert logprobs_grad(p=p) == -1, i
+        if i < 5:
+            assert logprobs(o=p[:5]) == balance(p=p[:5]) == router(p=p[:5]) == -1, i
+    for dtype, off in ((0, 1), (1, 2), (2, 1)):
+        assert balance(g=P + off, dtype=dtype) == router(g=P + off, dtype=dtype) == router(out=P + off, dtype=dtype) == -1
+        assert b"misaligned" in lib.xkb_last_error()
+    assert balance(M=2 ** 62, k=8) == balance(M=2 ** 40, k=0) == -1
+    assert combine(w=P + 2) == combine(gw=P + 2) == combine(w=P + 1, wd=0) == -1
+    assert combine(M=2 ** 62, k=8) == combine(M=2 ** 62, k=8, H=0) == -1
+
+
 def test_there_is_no_cpu_path(lib):
     x, ids, y = torch.randn(4, 8), torch.zeros(4, 2, dtype=torch.int32), torch.randn(4, 2, 8)
     for call in (lambda: xkb.token_logprobs(x, ids[:, 0]), lambda: xkb.token_logprobs_backward(x, ids[:, 0], y[0]), lambda: xkb.moe_balance_loss(x, ids),

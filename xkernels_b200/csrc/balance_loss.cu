@@ -266,7 +266,7 @@ extern "C" int xkb_moe_balance_loss(const void* gating_output, int dtype, const 
                                     int top_k, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace xkb;
   XKB_REQUIRE(M >= 0 && E >= 1 && E <= kMaxExperts, "moe_balance_loss: bad shape M=%lld E=%d (at most %d experts)", (long long)M, E, kMaxExperts);
-  XKB_REQUIRE(top_k >= 0 && M * top_k <= 0x7fffffff, "moe_balance_loss: M * top_k must fit 31 bits (M=%lld, top_k=%d)", (long long)M, top_k);
+  XKB_REQUIRE(top_k >= 0 && M <= 0x7fffffff / (top_k > 0 ? top_k : 1), "moe_balance_loss: M * top_k must fit 31 bits (M=%lld, top_k=%d)", (long long)M, top_k);
   XKB_REQUIRE(dtype == XKB_BF16 || dtype == XKB_F32 || dtype == XKB_F16, "moe_balance_loss: unsupported logits dtype code %d", dtype);
   XKB_REQUIRE(loss && counts && mean_probs && tokens && (M == 0 || gating_output) && (M * top_k == 0 || topk_ids),
               "moe_balance_loss: null pointer");
@@ -274,7 +274,9 @@ extern "C" int xkb_moe_balance_loss(const void* gating_output, int dtype, const 
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(XKB_ERR_WORKSPACE, "moe_balance_loss: the workspace needs %lld bytes (got %lld)", (long long)need,
                 (long long)(workspace ? workspace_bytes : 0));
-  XKB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "moe_balance_loss: misaligned workspace");
+  XKB_REQUIRE(address_bits(workspace) % 4 == 0, "moe_balance_loss: misaligned workspace");
+  XKB_REQUIRE(address_bits(gating_output) % (dtype == XKB_F32 ? 4 : 2) == 0 && address_bits(topk_ids, loss, counts, mean_probs, tokens) % 4 == 0,
+              "moe_balance_loss: a misaligned tensor");
   const int64_t parts = loss_parts(M);
   LossArgs a{gating_output, topk_ids, token_mask, nullptr, nullptr, nullptr, loss, counts, mean_probs, tokens, M, E, top_k, (int)parts};
   if (parts > 0) {
@@ -284,7 +286,7 @@ extern "C" int xkb_moe_balance_loss(const void* gating_output, int dtype, const 
     a.part_t = ws.take<int32_t>(parts);
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(gating_output);
+  const uintptr_t bits = address_bits(gating_output);
   int rc;
   switch (dtype) {
     case XKB_BF16: rc = with_shape<__nv_bfloat16>(E, top_k, bits, LaunchLoss<__nv_bfloat16>{a, s}); break;

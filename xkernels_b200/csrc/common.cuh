@@ -44,6 +44,9 @@ inline void count_launch(int n = 1) { g_launches.fetch_add(n, std::memory_order_
 inline int64_t align_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// The or of some addresses: a multiple of n (a power of two) if all are.
+template <typename... P> inline uintptr_t address_bits(P... p) { return (reinterpret_cast<uintptr_t>(p) | ...); }
+
 // Bump allocator over the caller's workspace (256-byte aligned slices).
 struct Carver {
   char* base;

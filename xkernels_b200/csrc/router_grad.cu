@@ -188,10 +188,13 @@ extern "C" int xkb_moe_router_backward(const void* gating_output, int dtype, con
   XKB_REQUIRE(dtype == XKB_BF16 || dtype == XKB_F32 || dtype == XKB_F16, "moe_router_backward: unsupported logits dtype code %d", dtype);
   if (M == 0) return XKB_OK;
   XKB_REQUIRE(gating_output && grad_gating && (grad_weights == nullptr || top_k == 0 || topk_ids), "moe_router_backward: null pointer");
+  XKB_REQUIRE(address_bits(gating_output, grad_gating) % (dtype == XKB_F32 ? 4 : 2) == 0 &&
+                  address_bits(topk_ids, grad_weights, counts, tokens, grad_loss) % 4 == 0,
+              "moe_router_backward: a misaligned tensor");
   const GateArgs a{gating_output, topk_ids, top_k == 0 ? nullptr : grad_weights, renormalize, counts, tokens, grad_loss, loss_scale,
                    token_mask, grad_gating, M, E, top_k};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(gating_output) | reinterpret_cast<uintptr_t>(grad_gating);
+  const uintptr_t bits = address_bits(gating_output, grad_gating);
   switch (dtype) {
     case XKB_BF16: return with_shape<__nv_bfloat16>(E, top_k, bits, LaunchGrad<__nv_bfloat16>{a, s});
     case XKB_F32: return with_shape<float>(E, top_k, bits, LaunchGrad<float>{a, s});

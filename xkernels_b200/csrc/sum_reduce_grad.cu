@@ -169,11 +169,10 @@ int launch_width(const Args& a, cudaStream_t s) {
 
 template <typename T, typename TW>
 int launch(const Args& a, cudaStream_t s) {
-  XKB_REQUIRE(a.M * a.top_k <= 0x7fffffff && a.H < (1 << 28), "moe_sum_reduce_backward: M * top_k must be below 2^31 and H below 2^28");
+  XKB_REQUIRE(a.H < (1 << 28), "moe_sum_reduce_backward: H must be below 2^28");
   // the widest access whose boundaries all rows start on
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.go) | reinterpret_cast<uintptr_t>(a.y) | reinterpret_cast<uintptr_t>(a.gy) |
-                         (uintptr_t)(a.H * (int64_t)sizeof(T));
-  XKB_REQUIRE(bits % sizeof(T) == 0, "moe_sum_reduce_backward: misaligned tensor");
+  const uintptr_t bits = address_bits(a.go, a.y, a.gy) | (uintptr_t)(a.H * (int64_t)sizeof(T));
+  XKB_REQUIRE(bits % sizeof(T) == 0 && address_bits(a.w, a.gw) % sizeof(TW) == 0, "moe_sum_reduce_backward: misaligned tensor");
   if (bits % 16 == 0) return launch_width<T, TW, 16 / sizeof(T)>(a, s);
   if (bits % 8 == 0) return launch_width<T, TW, 8 / sizeof(T)>(a, s);
   if constexpr (sizeof(T) == 2) {
@@ -194,6 +193,7 @@ extern "C" int xkb_moe_sum_reduce_backward(const void* grad_out, int dtype, cons
   XKB_REQUIRE(grad_w == nullptr || w != nullptr, "moe_sum_reduce_backward: grad_w without w");
   if (M == 0 || top_k == 0 || (grad_y == nullptr && grad_w == nullptr)) return XKB_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  XKB_REQUIRE(M <= 0x7fffffff / top_k, "moe_sum_reduce_backward: M * top_k must be below 2^31");
   if (H == 0) {   // empty sums
     if (grad_w != nullptr) XKB_CHECK_CUDA(cudaMemsetAsync(grad_w, 0, (size_t)(M * top_k) * (w_dtype == XKB_BF16 ? 2 : 4), s));
     return XKB_OK;

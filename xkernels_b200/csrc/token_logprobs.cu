@@ -1058,6 +1058,8 @@ extern "C" int xkb_token_logprobs(const void* logits, int dtype, int64_t ld, con
   XKB_REQUIRE(logits && token_ids && logprobs && entropy && stats && (top_k == 0 || (top_logprobs && top_ids)),
               "token_logprobs: null pointer");
   XKB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == XKB_F32 ? 4 : 2) == 0, "token_logprobs: misaligned logits");
+  XKB_REQUIRE(address_bits(token_ids) % (ids64 ? 8 : 4) == 0 && address_bits(logprobs, entropy, stats, top_logprobs, top_ids) % 4 == 0,
+              "token_logprobs: a misaligned tensor");
   const LogprobArgs a{logits, ld, token_ids, ids64, logprobs, entropy, stats, top_logprobs, top_ids, M, (int)V, top_k};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
@@ -1078,11 +1080,14 @@ extern "C" int xkb_token_logprobs_backward(const void* logits, int dtype, int64_
               "token_logprobs_backward: unsupported logits dtype code %d", dtype);
   XKB_REQUIRE(ids64 == 0 || ids64 == 1, "token_logprobs_backward: ids64 must be 0 or 1");
   if (M == 0) return XKB_OK;
-  XKB_REQUIRE(ld >= 0 && (M == 1 || ld_grad >= V), "token_logprobs_backward: bad row stride");
+  XKB_REQUIRE(ld >= 0 && (M == 1 || ld_grad >= V) && M <= 0x7fffffff, "token_logprobs_backward: bad row stride or too many rows");
   XKB_REQUIRE(logits && stats && grad_logits, "token_logprobs_backward: null pointer");
   XKB_REQUIRE(grad_logprobs == nullptr || token_ids != nullptr, "token_logprobs_backward: grad_logprobs without token_ids");
   XKB_REQUIRE(grad_entropy == nullptr || entropy != nullptr, "token_logprobs_backward: grad_entropy without entropy");
   XKB_REQUIRE(grad_top_logprobs == nullptr || top_k == 0 || top_ids != nullptr, "token_logprobs_backward: grad_top_logprobs without top_ids");
+  XKB_REQUIRE(address_bits(token_ids) % (ids64 ? 8 : 4) == 0 &&
+                  address_bits(stats, entropy, grad_logprobs, grad_entropy, top_ids, grad_top_logprobs) % 4 == 0,
+              "token_logprobs_backward: a misaligned tensor");
   GradArgs a{logits, ld, token_ids, ids64, stats, entropy, grad_logprobs, grad_entropy, grad_top_logprobs, top_ids,
              grad_top_logprobs == nullptr ? 0 : top_k, grad_logits, ld_grad, (int)V, 0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -133,6 +133,20 @@ def test_an_expert_named_twice(renorm, cuda_device):
     check_grad(x, ids, g_w, renorm)
 
 
+@pytest.mark.parametrize("E,k", [(65, 8), (128, 8), (128, 9), (97, 16), (128, 17), (130, 16), (256, 16), (255, 17), (258, 16), (512, 16), (512, 17),
+                                 (513, 16)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_parts_of_warps(E, k, dtype, cuda_device):
+    """The layouts of a row over 8, 16 and 32 lanes, with several rounds of rows and experts named twice."""
+    for M in (3, 20011 if E <= 256 else 12007):
+        x, ids, g_w, mask = case(M, E, k, dtype, cuda_device)
+        ids[::3, 1] = ids[::3, 0]
+        ids[1::5, k - 1] = ids[1::5, 2]
+        r = check_loss(x, ids, mask)
+        check_grad(x, ids, g_w, True, r.counts, r.tokens, 0.3, mask)
+        check_grad(x, ids, g_w, False)
+
+
 def test_sharp_rows(cuda_device):
     """Probabilities down to 0, selected ones among them."""
     x, ids, g_w, _ = case(64, 64, 8, torch.float32, cuda_device)

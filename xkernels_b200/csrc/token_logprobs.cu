@@ -10,8 +10,9 @@
 // no workspace, no atomics on floats, the same result in every run.
 //
 // Top alternatives: every thread keeps the maximum of its elements, which the pass needs anyway.  The k-th largest of
-// these maxima, taken by groups of threads, bounds the row's k-th largest element from below, and only threads that reach it can hold one of the k:
-// their elements (4 % of a row at k = 20) are read again, out of the L2, and what reaches the bound is ranked.
+// these maxima, taken by groups of threads, bounds the row's k-th largest element from below, and only threads that reach
+// it can hold one of the k: their elements (a tenth of a row at k = 20) are read again, mostly out of the L2, and what
+// reaches the bound is ranked.
 //
 // Forward: HBM-bound where rows fill the chip: 4096 x 128000 bf16 159 us, 6.6 TB/s (182 in a loop of calls, at the power limit).  Few rows are
 // bound by latency, half of it behind the pass where alternatives are wanted: 1 x 128000 with 20 of them 6.0 us, 64 x 128000 fp32 with

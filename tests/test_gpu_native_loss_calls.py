@@ -129,3 +129,32 @@ def test_the_same_refusals(cuda_device):
                 else:
                     with mode:
                         call()
+
+
+def test_outputs_are_ordinary_tensors(served, cuda_device):
+    """What the native path makes of its own storage: usable, in and out of inference mode, apart from each other."""
+    x = torch.randn(8, 100, device=cuda_device)
+    ids = torch.randint(0, 100, (8, 2), device=cuda_device, dtype=torch.int32)
+    w, y, go = torch.rand(8, 2, device=cuda_device), torch.randn(8, 2, 100, device=cuda_device), torch.randn(8, 100, device=cuda_device)
+    def calls():
+        r = xkb.token_logprobs(x, ids[:, 0].contiguous(), 3)
+        b = xkb.moe_balance_loss(x, ids)
+        return [*r, *b, xkb.token_logprobs_backward(x, ids[:, 0].contiguous(), r.stats, grad_logprobs=r.logprobs),
+                xkb.moe_router_backward(x, ids, grad_weights=w), *xkb.moe_sum_reduce_backward(go, y, w)]
+    want = [t.clone() for t in calls()]
+    got = calls()
+    for t, v in zip(got, want):
+        assert t.device == x.device and t.is_contiguous() and not t.requires_grad and t.grad_fn is None and not t.is_inference()
+        assert torch.equal(t, v) and torch.equal(t.cpu(), v.cpu())
+    for i, t in enumerate(got):
+        t.zero_()
+        assert all(torch.equal(u, v) for u, v in zip(got[i + 1:], want[i + 1:]))
+        if t.is_floating_point():
+            t.requires_grad_()
+            (t * 2).sum().backward()
+            assert bool((t.grad == 2).all())
+    with torch.inference_mode():
+        assert all(t.is_inference() and torch.equal(t, v) for t, v in zip(calls(), want))
+    a = torch.cuda.memory_allocated(cuda_device)
+    calls()
+    assert torch.cuda.memory_allocated(cuda_device) == a   # and given back

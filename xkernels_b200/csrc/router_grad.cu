@@ -15,9 +15,11 @@ namespace xkb {
 namespace {
 
 constexpr int kWarps = 8;
-// Resident blocks, and the grid: a block that follows another has to ask for the counts again.  us, bf16, both gradients: 65536 x 256 with
-// 3 / 4 blocks 17.8 / 22.5 (their 85 and 64 registers a thread), 16384 x 1024 with 1 / 2 36 / 21.
-constexpr int blocks_per_sm(int per_lane, bool balance) { return per_lane > 16 ? 2 : per_lane == 16 && balance ? 3 : 4; }
+// Resident blocks, and the grid: a block that follows another has to ask for the counts again.  us, bf16, top 8, 3 / 4 blocks (which leave 85 and 64
+// registers a thread): 65536 x 256 with both gradients 16.5 / 22.5, with the weights' alone 12.8 / 13.9, 65536 x 64 7.5 / 7.9, 16384 x 128 fp32
+// 3.8 / 3.7; 16384 x 1024 with 1 / 2 36 / 21.
+constexpr int blocks_per_sm(int per_lane) { return per_lane > 16 ? 2 : per_lane >= 8 ? 3 : 4; }
+constexpr float kFewest = 0x1p-20f;   // of the chosen experts' exponentials, relative to the row's largest
 
 struct GateArgs {
   const void* gating;
@@ -35,7 +37,7 @@ struct GateArgs {
 };
 
 template <typename T, int LANES, int PER_LANE, int P, bool BALANCE>
-__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(PER_LANE, BALANCE))
+__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm(PER_LANE))
 router_grad_kernel(GateArgs a) {
   using R = Row<T, LANES, PER_LANE, P>;
   constexpr int kRows = 32 / LANES, kPlaces = LANES * PER_LANE;
@@ -140,6 +142,8 @@ router_grad_kernel(GateArgs a) {
     if (!weights) continue;
     // A slot's part is e^x scale (gradient - level); an expert that several slots chose takes all of them, in their order.
     const float scale = a.renorm ? inverse(sel) : inv, level = a.renorm ? dot * scale : 0.f;
+    // (a row of dropped slots alone has none: 65536 x 256 with a tenth of such rows 16.9 us, 23.8 if they counted)
+    const bool few = a.renorm && live && sel < kFewest && (more || e >= 0);
     __syncwarp();   // the stores below come after the row's
     if (!more) {
       float own = e >= 0 ? g - level : 0.f;
@@ -147,7 +151,8 @@ router_grad_kernel(GateArgs a) {
       // 9.9 us instead of 7.2, the time goes with the number of different values.)
       if (e >= 0) s_who[warp][group][e] = (unsigned char)lane;
       __syncwarp();
-      if (__any_sync(0xffffffffu, e >= 0 && s_who[warp][group][e] != lane)) {
+      const bool seldom = __any_sync(0xffffffffu, (e >= 0 && s_who[warp][group][e] != lane) || few);
+      if (seldom) {
         const unsigned same = __match_any_sync(0xffffffffu, e < 0 ? -1 : group << 16 | e);
         const float q = own;
         own = 0.f;
@@ -157,8 +162,9 @@ router_grad_kernel(GateArgs a) {
           if (same >> j & 1) own += qj;
         }
       }
-      if (e >= 0 && live) out[e] = of_float<T>(ex * ((BALANCE ? fmaf(f, s_share[BALANCE ? e : 0], f0) : f0) + scale * own));
-    } else if (live) {
+      if (e >= 0 && live && !few) out[e] = of_float<T>(ex * ((BALANCE ? fmaf(f, s_share[BALANCE ? e : 0], f0) : f0) + scale * own));
+      if (!seldom) continue;
+    } else if (live && !few) {
       for (int j = sub; j < a.k; j += LANES) {
         const int o = ids[j];
         if ((unsigned)o >= (unsigned)a.E) continue;
@@ -168,6 +174,36 @@ router_grad_kernel(GateArgs a) {
         out[o] = of_float<T>(exponential(to_float(row[o]), max) * ((BALANCE ? fmaf(f, s_share[BALANCE ? o : 0], f0) : f0) + scale * own));
       }
     }
+    if (!__any_sync(0xffffffffu, few)) continue;
+    // Renormalised weights depend on the chosen logits alone.  Where these have less than kFewest of the row's largest exponential (a choice
+    // under a bias or within a group), theirs are taken relative to the largest of themselves: relative to the row's they
+    // could all be 0, or have a sum whose inverse overflows.  (65536 x 256, top 8, all rows such ones: 40 us instead of 17.)
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int j = sub; few && j < a.k; j += LANES)
+      if ((unsigned)ids[j] < (unsigned)a.E) top = fmaxf(top, to_float(row[ids[j]]));   // (no NaN: that row's sum is NaN)
+    top = lanes_max_nan<LANES>(top);
+    if (top == -INFINITY) top = 0.f;   // no chosen logit is live: their weights are 0
+    sel = dot = 0.f;
+#pragma unroll 1
+    for (int j = sub; few && j < a.k; j += LANES) {
+      if ((unsigned)ids[j] >= (unsigned)a.E) continue;
+      const float eo = exponential(to_float(row[ids[j]]), top);
+      sel += eo;
+      dot = fmaf(eo, g_w[j], dot);
+    }
+    const float own_scale = inverse(lanes_add<LANES>(sel)), own_level = lanes_add<LANES>(dot) * own_scale;
+#pragma unroll 1
+    for (int j = sub; few && j < a.k; j += LANES) {
+      const int o = ids[j];
+      if ((unsigned)o >= (unsigned)a.E) continue;
+      float own = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < a.k; ++i)
+        if (ids[i] == o) own += g_w[i] - own_level;
+      const float xo = to_float(row[o]), part = exponential(xo, max) * (BALANCE ? fmaf(f, s_share[BALANCE ? o : 0], f0) : f0);
+      out[o] = of_float<T>(fmaf(exponential(xo, top), own_scale * own, part));   // (part is NaN in a row with +inf)
+    }
   }
 }
 
@@ -175,7 +211,7 @@ template <typename T> struct LaunchGrad {
   const GateArgs& a;
   cudaStream_t s;
   template <int LANES, int PER_LANE, int P> int operator()() const {
-    const int64_t want = ceil_div(a.M, (int64_t)kWarps * 32 / LANES), most = 148 * blocks_per_sm(PER_LANE, a.counts != nullptr);
+    const int64_t want = ceil_div(a.M, (int64_t)kWarps * 32 / LANES), most = 148 * blocks_per_sm(PER_LANE);
     const unsigned blocks = (unsigned)(want < most ? want : most);
     (a.counts != nullptr ? router_grad_kernel<T, LANES, PER_LANE, P, true>
                          : router_grad_kernel<T, LANES, PER_LANE, P, false>)<<<blocks, 32 * kWarps, 0, s>>>(a);

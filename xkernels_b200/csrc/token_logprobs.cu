@@ -883,8 +883,9 @@ token_logprobs_grad_kernel(GradArgs a) {
   }
   const int own_vector = column < 0 ? -1 : (column + r.skew) / N, own_place = (column + r.skew) % N;
 
-  // -p (G + gh (ln p + h)) with ln p = x - mx - l: any value
-  const bool dead = mx == -INFINITY;
+  // -p (G + gh (ln p + h)) with ln p = x - mx - l: any value.  A row without a live logit has p = 0; NaN in G, of a token that is no column,
+  // is kept there too.
+  const bool dead = mx == -INFINITY && G == G;
   const float base = fmaf(gh, h, G);
   auto gradient = [&](float x) -> float {
     const float lp = max_nan(x - mx - l, -200.f);   // e^-200 is 0

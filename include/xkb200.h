@@ -178,6 +178,11 @@ int xkb_moe_balance_loss(const void* gating_output, int dtype,
  *   grad = p * (dp - sum_e p dp),   p = softmax(gating) in fp32.
  * grad_weights NULL or [M, top_k] fp32, renormalize as in topk_softmax; ids
  * outside [0, E) are dropped slots, an expert named twice takes both.
+ * Renormalised weights are p_j / sum p over the slots that are not dropped.  Where
+ * slots are dropped after topk_softmax, which divides by the sum over all of
+ * them, topk_ids are its ids as they were, with grad_weights 0 for those slots.
+ * Weights depend on the chosen logits alone, wherever these lie in the row; a
+ * choice without a live logit has none.
  * counts NULL or [E]: adds the gradient of loss_scale * grad_loss * loss
  * (grad_loss NULL: 1), with counts and tokens (NULL: M) as moe_balance_loss left
  * them, or summed over the ranks of a data-parallel job; token_mask as there.

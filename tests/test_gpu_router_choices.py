@@ -8,6 +8,7 @@ import torch
 
 import xkernels_b200 as xkb
 from tests import loss_util as ref
+from xkernels_b200 import autograd as xka
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -135,3 +136,66 @@ def test_against_differences(cuda_device):
         v, h = torch.randn(30, 40, generator=g, device=cuda_device, dtype=torch.float64), 1e-5
         want = (f(x.double() + h * v) - f(x.double() - h * v)) / (2 * h)
         assert abs(float((got * v).sum() - want)) <= float(((err + ref.U24 * got.abs() + 1e-9) * v.abs()).sum())
+
+
+# ---- slots that are dropped behind the router -------------------------------------------------------------------
+def routing64(leaf, ids):
+    p = torch.softmax(leaf, dim=1).gather(1, ids.long())
+    return p / p.sum(dim=1, keepdim=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_slots_dropped_behind_the_router(dtype, cuda_device):
+    """topk_softmax, then a slot is dropped (an expert's capacity): the weights were formed over all top_k slots, so the gradient takes the
+    ids that topk_softmax gave and 0 for what was dropped.  The balance loss counts the kept slots alone.  Against autograd
+    of that composition in 64 bits."""
+    M, E, k = 300, 48, 6
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    x = (torch.randn(M, E, generator=g, device=cuda_device) * 1.5).to(dtype)
+    keep = torch.rand(M, k, generator=g, device=cuda_device) < 0.7
+    keep[0] = False
+    g_w = torch.randn(M, k, generator=g, device=cuda_device)
+    _, ids = xkb.topk_softmax(x, k)
+    kept_ids = torch.where(keep, ids, -1)
+    r = xkb.moe_balance_loss(x, kept_ids)
+    got = xkb.moe_router_backward(x, ids, grad_weights=torch.where(keep, g_w, 0.0), counts=r.counts, tokens=r.tokens, grad_loss=0.3)
+
+    leaf = x.double().requires_grad_()
+    loss = (routing64(leaf, ids) * keep * g_w.double()).sum()
+    (loss + 0.3 * E * (r.counts.double() / (k * M) * torch.softmax(leaf, dim=1).mean(dim=0)).sum()).backward()
+    _, err = ref.router_grad(x, ids, torch.where(keep, g_w, 0.0), True, r.counts, r.tokens, 0.3)
+    ref.assert_near(got, leaf.grad, err, "gradient")
+
+
+def test_slots_dropped_through_autograd(cuda_device):
+    """The differentiable router keeps its own ids: dropping is a matter of what becomes of the weights."""
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    x = torch.randn(200, 32, generator=g, device=cuda_device)
+    keep = torch.rand(200, 4, generator=g, device=cuda_device) < 0.7
+    g_w = torch.randn(200, 4, generator=g, device=cuda_device)
+    own, plain = x.clone().requires_grad_(), x.double().requires_grad_()
+    w, ids = xka.topk_softmax(own, 4)
+    (w * keep * g_w).sum().backward()
+    (routing64(plain, ids) * keep * g_w.double()).sum().backward()
+    _, err = ref.router_grad(x, ids, torch.where(keep, g_w, 0.0), True)
+    ref.assert_near(own.grad, plain.grad, err + 2 ** -23 * plain.grad.abs())
+    w, ids = xka.topk_softmax(own, 4)
+    ids[~keep] = -1                            # the ids that the gradient needs: torch refuses
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        w.sum().backward()
+
+
+def test_weights_of_the_kept_slots(cuda_device):
+    """Ids outside [0, E) mean weights that were formed over the kept slots: p_j by the sum of the kept p."""
+    g = torch.Generator(device=cuda_device).manual_seed(10)
+    x = torch.randn(200, 32, generator=g, device=cuda_device)
+    _, ids = xkb.topk_softmax(x, 4)
+    keep = torch.rand(200, 4, generator=g, device=cuda_device) < 0.7
+    keep[:, 0] = True
+    g_w = torch.randn(200, 4, generator=g, device=cuda_device)
+    kept_ids = torch.where(keep, ids, 32)
+    leaf = x.double().requires_grad_()
+    p = torch.softmax(leaf, dim=1).gather(1, ids.long()) * keep
+    (p / p.sum(dim=1, keepdim=True) * g_w.double()).sum().backward()
+    _, err = ref.router_grad(x, kept_ids, g_w, True)
+    ref.assert_near(xkb.moe_router_backward(x, kept_ids, grad_weights=g_w), leaf.grad, err)

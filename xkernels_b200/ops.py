@@ -431,10 +431,12 @@ def moe_router_backward(gating_output, topk_ids, grad_weights=None, renormalize=
     """The gradient of the gating logits, ``[M, E]`` of their dtype, in one pass.
 
     From the routing weights: ``grad_weights`` ``[M, top_k]``, the gradient of :func:`topk_softmax`'s weights for
-    ``topk_ids`` (``renormalize`` as there).  From :func:`moe_balance_loss`: ``counts`` and ``tokens`` (None: M) as it returned them,
-    ``grad_loss`` the loss's gradient (a number or a one-element CUDA tensor; None: 1), ``token_mask`` as there.  Either may be
-    left out.  Ids outside ``[0, E)`` are dropped slots.  A row that neither brings a gradient to is 0, whatever its
-    logits.  No reference counterpart: the reference's pure-torch router is differentiated by torch.
+    ``topk_ids`` (``renormalize`` as there).  Ids outside ``[0, E)`` are dropped slots, and renormalised weights are taken to be
+    ``p_j`` by the sum over the other slots.  A caller that drops slots behind :func:`topk_softmax`, which divided by the sum over all of
+    them, therefore passes the ids as they were, and a gradient of 0 for what was dropped.  From :func:`moe_balance_loss`: ``counts`` and
+    ``tokens`` (None: M) as it returned them, ``grad_loss`` the loss's gradient (a number or a one-element CUDA tensor; None: 1),
+    ``token_mask`` as there.  Either may be left out.  A row that neither brings a gradient to is 0, whatever its logits.  No
+    reference counterpart: the reference's pure-torch router is differentiated by torch.
     """
     got = (_lib._calls or _lib.load_calls()).moe_router_backward(
         gating_output, topk_ids, grad_weights, renormalize, counts, tokens, grad_loss, token_mask)

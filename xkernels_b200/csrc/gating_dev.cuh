@@ -193,13 +193,13 @@ struct Row {
 // experts) and have a lane for each slot.  us, gradient of both, bf16 top 8, 32 lanes / here: 16384 x 128 6.3 / 4.4, 16384 x 256 7.2 / 6.0,
 // 65536 x 256 25 / 18, 65536 x 512 36 / 32.  But 32 lanes above 256 experts where pieces are of one (5003 x 327 6.0 over 16 lanes, 5.1
 // over 32; balance loss of 1021 x 271 8.8 / 7.3).  (65536 x 256 over 8 lanes: 16.2, but 16384 x 255 9.8 instead of 7.5.)
-template <typename T, int LANES, int PER_LANE, typename F>
-int with_piece(int E, uintptr_t bits, F f) {   // bits: the addresses of all rows, or'ed
+template <typename T, int LANES, int PER_LANE, int LEAST = 1, typename F>
+int with_piece(int E, uintptr_t bits, F f) {   // bits: the addresses of all rows, or'ed; pieces of LEAST always fit
   constexpr int kMost = PER_LANE < (int)(16 / sizeof(T)) ? PER_LANE : (int)(16 / sizeof(T));
   auto fits = [&](int P) { return E % P == 0 && bits % (P * sizeof(T)) == 0; };
   if constexpr (kMost > 2) if (fits(kMost)) return f.template operator()<LANES, PER_LANE, kMost>();
-  if constexpr (kMost >= 2) if (fits(2)) return f.template operator()<LANES, PER_LANE, 2>();
-  return f.template operator()<LANES, PER_LANE, 1>();
+  if constexpr (kMost >= 2 && LEAST == 1) if (fits(2)) return f.template operator()<LANES, PER_LANE, 2>();
+  return f.template operator()<LANES, PER_LANE, LEAST>();
 }
 template <typename T, typename F>
 int with_shape(int E, int top_k, uintptr_t bits, F f) {
@@ -213,7 +213,7 @@ int with_shape(int E, int top_k, uintptr_t bits, F f) {
   if (top_k <= 16) {
     if (E <= 128) return with_piece<T, 16, 8>(E, bits, f);
     if (E <= 256) return with_piece<T, 16, 16>(E, bits, f);
-    if (E <= 512 && E % 2 == 0 && bits % (2 * sizeof(T)) == 0) return with_piece<T, 16, 32>(E, bits, f);
+    if (E <= 512 && E % 2 == 0 && bits % (2 * sizeof(T)) == 0) return with_piece<T, 16, 32, 2>(E, bits, f);
   }
   if (E <= 128) return with_piece<T, 32, 4>(E, bits, f);
   if (E <= 256) return with_piece<T, 32, 8>(E, bits, f);

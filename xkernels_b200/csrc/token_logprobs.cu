@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <cstddef>
 #include <type_traits>
 
 #include "common.cuh"
@@ -291,6 +292,10 @@ struct TopScratch {
   uint32_t bound;
 };
 template <int THREADS> struct NoScratch {};
+// `group` is read in words of 16 bytes, at multiples of four
+template <int THREADS> constexpr bool kWordsOfGroups = alignof(TopScratch<THREADS>) % 16 == 0 && offsetof(TopScratch<THREADS>, group) % 16 == 0 &&
+                                                       TopScratch<THREADS>::kGroups % 32 == 0;
+static_assert(kWordsOfGroups<32> && kWordsOfGroups<64> && kWordsOfGroups<128> && kWordsOfGroups<256>, "misaligned");
 
 // Leaves the k largest of the n candidates (n >= k) at the front, in any order, and 0 in the places behind them: digits of
 // eight bits from the top, until the k-th's digit is one that all who share it are needed.

@@ -199,3 +199,20 @@ def test_weights_of_the_kept_slots(cuda_device):
     (p / p.sum(dim=1, keepdim=True) * g_w.double()).sum().backward()
     _, err = ref.router_grad(x, kept_ids, g_w, True)
     ref.assert_near(xkb.moe_router_backward(x, kept_ids, grad_weights=g_w), leaf.grad, err)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_both_losses_on_the_same_logits(dtype, cuda_device):
+    """Through the differentiable forms the two gradients are results of their own, each rounded, and torch rounds their sum."""
+    M, E, k = 333, 60, 6
+    g = torch.Generator(device=cuda_device).manual_seed(12)
+    x = (torch.randn(M, E, generator=g, device=cuda_device) * 1.5).to(dtype)
+    g_w = torch.randn(M, k, generator=g, device=cuda_device)
+    mask = torch.rand(M, generator=g, device=cuda_device) < 0.8
+    leaf = x.clone().requires_grad_()
+    w, ids = xka.topk_softmax(leaf, k)
+    b = xka.moe_balance_loss(leaf, ids, mask)
+    ((w * g_w).sum() + 300.0 * b.loss).backward()
+    parts = [ref.router_grad(x, ids, g_w, True), ref.router_grad(x, ids, None, True, b.counts, b.tokens, 300.0, mask)]
+    err = sum(e + ref.half_step(dtype) * (d.abs() + e) + ref.TINY[dtype] for d, e in parts)
+    ref.assert_near(leaf.grad, parts[0][0] + parts[1][0], err + ref.half_step(dtype) * err)

@@ -5,10 +5,12 @@
 // A warp has one row of up to 1024 experts in registers, two of up to 512 or four of up to 128.  Warps take rows in turn, the next one on its way
 // while one is computed, and keep the sum of every expert's probability in registers; a block adds its warps up.  A few rows
 // are one block, or one cluster of eight, joined through distributed shared memory, and one launch; more are a block per SM that leaves a row
-// of partial sums each, which a second kernel of eight blocks, resident by then, adds up.  Floats are added in a fixed
-// order, only counts by atomics: the same bits in every run.
-// 16384 x 256 bf16 8.8 us: 2.2 of launch, 2.5 for the second kernel, else the rows' instructions (65536 rows 16.4 us, 2.2 TB/s).  333 x 48 fp32
-// 4.3 us: launch, the cluster's barriers, the chain of sums.
+// of partial sums each, which a second kernel of eight blocks adds up.  It is launched early, but its blocks (46 registers, 1024
+// threads) do not fit an SM beside one of the first kernel's (63 to 128 registers, 512 threads): where there is one on every SM
+// they start as those end.  Floats are added in a fixed order, only counts by atomics: the same bits in every run.
+// 16384 x 256 bf16 8.8 us: 2.2 of launch, 2.5 for the second kernel, else latency: a lane group has one row's chain of maximum, exponentials, sum and
+// reciprocal, and 1.7 of 4 instructions a cycle are issued (65536 rows 16.5 us, 2.2 TB/s).  333 x 48 fp32 4.3 us: launch, the
+// cluster's barriers, the chain of sums.
 #include <cooperative_groups.h>
 
 #include "gating_dev.cuh"
@@ -55,7 +57,7 @@ balance_kernel(LossArgs a) {
   __shared__ int s_tokens;
   __shared__ float s_term[kCluster * kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LANES;
-  chain_trigger();   // the joining kernel may become resident
+  chain_trigger();   // the joining kernel may start where there is room for it
   float acc[PER_LANE];
 #pragma unroll
   for (int t = 0; t < PER_LANE; ++t) acc[t] = 0.f;

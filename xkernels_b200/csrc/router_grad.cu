@@ -5,10 +5,11 @@
 //   a_e = g_loss E c_e / (k T^2)
 //
 // A warp has one row of up to 1024 experts in registers, two of up to 512 or four of up to 128, as the number of slots allows.  Bound by
-// instructions, so no row goes through shared memory: sum_e p dp splits into sum_e p_e a_e and the slots' part, which is sum_j p_j g_j for raw weights and nothing
-// for renormalised ones (they do not change along p); the row is written with the first part alone, and the lanes that hold a
-// slot put the chosen experts' gradients in afterwards, from logits that they loaded themselves.
-// Both gradients, bf16, top 8: 16384 x 256 6.1 us (2 of them launch), 65536 x 256 17.8 us (4.0 TB/s), 77 x 60 fp32 1.9 us.
+// instructions and latency (183 instructions a row, 2.6 of 4 a cycle at a third of the warps), so no row goes through shared memory: sum_e p
+// dp splits into sum_e p_e a_e and the slots' part, which is sum_j p_j g_j for raw weights and nothing for renormalised ones (they
+// do not change along p); the row is written with the first part alone, and the lanes that hold a slot put the chosen experts'
+// gradients in afterwards, from logits that they loaded themselves.
+// Both gradients, bf16, top 8: 16384 x 256 6.1 us (2 of them launch), 65536 x 256 16.7 us (4.3 TB/s), 77 x 60 fp32 1.9 us.
 #include "gating_dev.cuh"
 
 namespace xkb {
@@ -16,7 +17,7 @@ namespace {
 
 constexpr int kWarps = 8;
 // Resident blocks, and the grid: a block that follows another has to ask for the counts again.  us, bf16, top 8, 3 / 4 blocks (which leave 85 and 64
-// registers a thread): 65536 x 256 with both gradients 16.5 / 22.5, with the weights' alone 12.8 / 13.9, 65536 x 64 7.5 / 7.9, 16384 x 128 fp32
+// registers a thread): 65536 x 256 with both gradients 16.5 / 22.5, with the weights' alone 13.2 / 13.9, 65536 x 64 7.4 / 7.9, 16384 x 128 fp32
 // 3.8 / 3.7; 16384 x 1024 with 1 / 2 36 / 21.
 constexpr int blocks_per_sm(int per_lane) { return per_lane > 16 ? 2 : per_lane >= 8 ? 3 : 4; }
 constexpr float kFewest = 0x1p-20f;   // of the chosen experts' exponentials, relative to the row's largest

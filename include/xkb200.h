@@ -236,6 +236,83 @@ int xkb_token_logprobs_backward(const void* logits, int dtype, int64_t ld,
                                 void* grad_logits, int64_t ld_grad, int64_t M,
                                 int64_t V, void* stream);
 
+/* ------------------------------------------------------------------------
+ * linear_cross_entropy: the loss of given tokens from hidden states, the head's
+ * logits z = hidden weight^T (fp32) never stored: m = max z, l = ln sum exp(z - m),
+ * lse = m + l, loss = lse - z[label].  No reference counterpart.
+ * hidden [M, H] (row stride ld_hidden, any alignment of 2 bytes), weight [V, H]
+ * (row stride ld_weight a multiple of 8, first row on 16 bytes), both bf16 or fp16;
+ * labels [M] int32, or int64 with ids64 = 1; loss, lse [M] and stats [M, 2] = (m, l)
+ * fp32.  A row with a negative label is padding: it is not read, and its results are
+ * 0; a label >= V gives a loss of NaN; a row whose logits hold a NaN or +inf is NaN.
+ * M, V < 2^28.  Three launches; the same bits in every run.
+ * ---------------------------------------------------------------------- */
+int64_t xkb_linear_cross_entropy_workspace_bytes(int64_t M, int64_t H, int64_t V);
+int xkb_linear_cross_entropy(const void* hidden, int64_t ld_hidden, int dtype,
+                             const void* weight, int64_t ld_weight,
+                             const void* labels, int ids64, float* loss,
+                             float* lse, float* stats, int64_t M, int64_t H,
+                             int64_t V, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * linear_cross_entropy_backward: the gradients of hidden [M, H] and weight [V, H]
+ * (contiguous, of their dtype; NULL: not wanted) from grad_loss and grad_lse [M]
+ * fp32 (NULL: 0; one is needed) and the forward call's stats,
+ *   d = p (grad_loss + grad_lse) - grad_loss onehot(label),  p = exp(z - m - l),
+ *   grad_hidden = d weight,  grad_weight = d^T hidden.
+ * z is multiplied again, a piece of the vocabulary at a time; d is rounded to dtype
+ * (fp16: times a power of two that keeps small probabilities).  Padding rows are not
+ * read and have a gradient of 0; a label >= V makes its row of d NaN.  The workspace
+ * holds one piece of d, 256 MiB at most (or 256 columns of it).
+ * ---------------------------------------------------------------------- */
+int64_t xkb_linear_cross_entropy_backward_workspace_bytes(int64_t M, int64_t H, int64_t V);
+int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_hidden, int dtype,
+                                      const void* weight, int64_t ld_weight,
+                                      const void* labels, int ids64,
+                                      const float* stats, const float* grad_loss,
+                                      const float* grad_lse, void* grad_hidden,
+                                      void* grad_weight, int64_t M, int64_t H,
+                                      int64_t V, void* workspace,
+                                      int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * gated_ffn: a dense feed-forward block, the shared expert of a routed layer,
+ *   out = (silu(gate) * up) w2^T,  [gate up] = x w13^T.
+ * x [M, H], w13 [2 I, H] (gate rows first, as in the fused calls), w2 [H, I], all
+ * bf16 or fp16, row strides multiples of 8 elements and first rows on 16 bytes.
+ * limit > 0: gate is cut off at limit, up at +-limit (as in fused_moe_mxfp4).
+ * Products are added up in fp32; silu(gate) * up is rounded to dtype once.
+ * out [M, H] and, if not NULL, gate_up [M, 2 I] (before the limit), contiguous.
+ * No reference counterpart.  Two launches.
+ * ---------------------------------------------------------------------- */
+int64_t xkb_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I);
+int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void* w13,
+                  int64_t ld_w13, const void* w2, int64_t ld_w2, float limit,
+                  void* out, void* gate_up, int64_t M, int64_t H, int64_t I,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * gated_ffn_backward: the gradients of x [M, H], w13 [2 I, H] and w2 [H, I]
+ * (contiguous; NULL: not wanted) from grad_out [M, H].  gate_up [M, 2 I] contiguous
+ * as gated_ffn left it, or NULL: multiplied again (recompute = 1 in the query).
+ * A gate above the limit, an up beyond +-limit has a gradient of 0.
+ * The gradients of gate and up, and silu(gate) * up, are rounded to dtype once.
+ * ---------------------------------------------------------------------- */
+int64_t xkb_gated_ffn_backward_workspace_bytes(int64_t M, int64_t H, int64_t I, int recompute);
+int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_grad_out, int dtype,
+                           const void* x, int64_t ld_x, const void* w13,
+                           int64_t ld_w13, const void* w2, int64_t ld_w2,
+                           const void* gate_up, float limit, void* grad_x,
+                           void* grad_w13, void* grad_w2, int64_t M, int64_t H,
+                           int64_t I, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
+/* Synchronises `stream` and reports (XKB_ERR_DEVICE) whether a kernel of the four calls
+ * above ever gave up a bounded wait on the current device. */
+int xkb_dense_status(void* stream);
+
+
 /* The token tile (positions of a token block) that a fused call picks on the
  * tensor cores, from its number of slots; no GPU is needed to ask.  INT4: 16,
  * 32, 64 or 128.  MXFP4, with weights on 32 bytes: 8, 16 or 32 of the

@@ -14,6 +14,14 @@ Losses of a routed model and their gradients (no reference counterparts):
 * :func:`token_logprobs`, :func:`token_logprobs_backward` (given tokens, entropy, top alternatives)
 * :func:`moe_balance_loss` (with per-expert counts), :func:`moe_router_backward` (gating logits)
 * :func:`moe_sum_reduce_backward`
+* :func:`linear_cross_entropy`, :func:`linear_cross_entropy_backward` (a head's loss from hidden states, without its logits)
+
+The shared expert beside the routed ones (no reference counterpart):
+
+* :func:`gated_ffn`, :func:`gated_ffn_backward`
+
+And
+
 * :mod:`xkernels_b200.autograd`: the same as differentiable functions
 
 ``plugin.install()`` registers them as the ``backend="cuda"`` cards of an
@@ -22,10 +30,15 @@ installed ``xkernels`` package.
 
 from .ops import (  # noqa: F401
     BalanceLoss,
+    LinearCrossEntropy,
     TokenLogprobs,
     fused_moe_int4_ffn,
     fused_moe_int4_w4a16,
     fused_moe_mxfp4,
+    gated_ffn,
+    gated_ffn_backward,
+    linear_cross_entropy,
+    linear_cross_entropy_backward,
     moe_align_block_size,
     moe_balance_loss,
     moe_router_backward,
@@ -38,10 +51,15 @@ from .ops import (  # noqa: F401
 
 __all__ = [
     "BalanceLoss",
+    "LinearCrossEntropy",
     "TokenLogprobs",
     "fused_moe_int4_ffn",
     "fused_moe_int4_w4a16",
     "fused_moe_mxfp4",
+    "gated_ffn",
+    "gated_ffn_backward",
+    "linear_cross_entropy",
+    "linear_cross_entropy_backward",
     "moe_align_block_size",
     "moe_balance_loss",
     "moe_router_backward",

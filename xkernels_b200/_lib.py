@@ -73,6 +73,31 @@ SIGNATURES = {
         [c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
          c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p],
     ),
+    "xkb_linear_cross_entropy_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "xkb_linear_cross_entropy": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "xkb_linear_cross_entropy_backward_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "xkb_linear_cross_entropy_backward": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "xkb_gated_ffn_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "xkb_gated_ffn": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p, c_int64, c_int64,
+         c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "xkb_gated_ffn_backward_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "xkb_gated_ffn_backward": (
+        c_int,
+        [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_void_p,
+         c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "xkb_dense_status": (c_int, [c_void_p]),
     "xkb_fused_moe_int4_w4a16_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
     "xkb_fused_moe_int4_w4a16": (
         c_int,

@@ -1,0 +1,172 @@
+// Host side of the dense products: tensor maps, which tile a product gets, launches.
+#include <mutex>
+
+#include "dense_dev.cuh"
+#include "tensor_map.h"
+
+namespace xkb {
+extern std::atomic<int> g_sm_margin;
+
+namespace dense {
+
+// Status of the last wait that ran out on this device (0: none).  The calls have no workspace of their caller's that
+// would outlive them, so it is the library's.
+__device__ int g_dense_status;
+
+namespace {
+
+int sm_count(int* out) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  XKB_CHECK_CUDA(cudaGetDevice(&dev));
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    XKB_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return XKB_OK;
+}
+
+int status_word(int** out) {
+  static std::atomic<int*> known[64];
+  int dev = 0;
+  XKB_CHECK_CUDA(cudaGetDevice(&dev));
+  int* p = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (p == nullptr) {
+    void* at = nullptr;
+    XKB_CHECK_CUDA(cudaGetSymbolAddress(&at, g_dense_status));
+    p = static_cast<int*>(at);
+    if (dev < 64) known[dev].store(p, std::memory_order_relaxed);
+  }
+  *out = p;
+  return XKB_OK;
+}
+
+struct Shape { int cg, bn, split; };
+
+// Which tile.  The cost of a shape is its rounds of tiles times the time of a tile, which is K times the clocks of a
+// stage: 512 for 256 x 256 on a pair (MMA rate), 330 for 256 x 128 (operand traffic), 300 to 400 for 128 x 128 on one CTA.
+// A cluster that splits K pays for adding its parts up.
+Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, int count, bool paired, bool may_split, int sms) {
+  Shape best{2, 256, 1};
+  double best_cost = 1e300;
+  auto consider = [&](Shape s, double cost) {
+    if (cost < best_cost * 0.999) best_cost = cost, best = s;
+  };
+  for (int bn : {256, 128}) {
+    const int64_t tile_n = paired ? bn / 2 : bn;
+    double work = 0;
+    int64_t tiles = 0, longest = 0;
+    for (int i = 0; i < count; ++i) {
+      const int64_t t = ceil_div(M[i], 256) * ceil_div(N[i], tile_n), kb = ceil_div(K[i], kBK);
+      tiles += t;
+      work += (double)t * kb;
+      longest = kb > longest ? kb : longest;
+    }
+    const double mean = work / (double)(tiles > 0 ? tiles : 1);
+    const int64_t rounds = ceil_div(tiles, sms / 2);
+    consider({2, bn, 1}, (double)rounds * mean * (bn == 256 ? 512 : 330) + (bn == 256 ? 6000 : 3000));
+  }
+  if (count == 1 && may_split) {
+    const int64_t tile_n = paired ? 64 : 128, tiles = ceil_div(M[0], kRows) * ceil_div(N[0], tile_n), kb = ceil_div(K[0], kBK);
+    const int64_t rows = M[0] < kRows ? align_up(M[0], 8) : kRows;
+    const double stage = 256 + rows;
+    for (int s : {1, 2, 4, 8}) {
+      if (s > 1 && (s > kb || tiles * s > sms / s * s)) continue;
+      consider({1, 128, s}, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage + (s > 1 ? 4000 : 2000));
+    }
+  }
+  return best;
+}
+
+int vec_of(const void* p, int64_t ld, int64_t extra = 0) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * 2) | (uintptr_t)(extra * 2);
+  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
+}
+
+}  // namespace
+
+int ce_parts(int64_t M, int64_t N, int64_t K) {
+  int sms = 148;
+  if (sm_count(&sms) != XKB_OK) sms = 148;
+  const Shape s = shape_of(&M, &N, &K, 1, false, true, sms);
+  return (int)(ceil_div(N, s.bn) * s.split * 2);
+}
+
+int launch(const Product* products, int count, int end, int dtype, bool chained, bool early_b, cudaStream_t stream) {
+  XKB_REQUIRE(count >= 1 && count <= kMaxProblems, "dense products: %d products", count);
+  int sms = 0, rc = sm_count(&sms);
+  if (rc != XKB_OK) return rc;
+  Params p = {};
+  rc = status_word(&p.status);
+  if (rc != XKB_OK) return rc;
+  const bool b_mn = products[0].b.k_rows;
+  int64_t M[kMaxProblems], N[kMaxProblems], K[kMaxProblems];
+  bool any_a_mn = false;
+  for (int i = 0; i < count; ++i) {
+    M[i] = products[i].M, N[i] = products[i].N, K[i] = products[i].K;
+    any_a_mn |= products[i].a.k_rows;
+    XKB_REQUIRE(M[i] > 0 && N[i] > 0 && K[i] > 0 && M[i] < (1ll << 30) && N[i] < (1ll << 30) && K[i] < (1ll << 30),
+                "dense products: sizes out of range");
+  }
+  const Shape s = shape_of(M, N, K, count, end == kSwiglu, !any_a_mn, sms);
+  const int a_rows = s.cg == 1 && !any_a_mn && M[0] < kRows ? (int)align_up(M[0], 8) : kRows;
+  const CUtensorMapDataType dt = dtype == XKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  p.count = count;
+  p.fmt = dtype == XKB_BF16 ? 1 : 0;
+  p.split = s.split;
+  p.a_bytes = a_rows * 128;
+  p.early_b = early_b ? 1 : 0;
+  int64_t tiles = 0;
+  const int tile_m = kRows * s.cg, tile_n = end == kSwiglu ? s.bn / 2 : s.bn;
+  for (int i = 0; i < count; ++i) {
+    const Product& q = products[i];
+    DevProduct& d = p.prod[i];
+    rc = make_map_2d_pitched(&d.a, dt, q.a.base, q.a.rows, q.a.cols, (uint64_t)q.a.pitch * 2, q.a.k_rows ? 64 : a_rows, 64,
+                             CU_TENSOR_MAP_SWIZZLE_128B, "left operand");
+    if (rc != XKB_OK) return rc;
+    rc = make_map_2d_pitched(&d.b, dt, q.b.base, q.b.rows, q.b.cols, (uint64_t)q.b.pitch * 2, b_mn ? 64 : s.bn / 2, 64,
+                             CU_TENSOR_MAP_SWIZZLE_128B, "right operand");
+    if (rc != XKB_OK) return rc;
+    d.M = (int)q.M, d.N = (int)q.N, d.K = (int)q.K, d.b_row0 = (int)q.b.row0;
+    d.live = q.live;
+    d.live_is_k = d.a_mn = q.a.k_rows;
+    d.group = 16 / s.cg;
+    d.end = q.end;
+    d.end.vec_out = vec_of(q.end.out, q.end.ld, end == kDswiglu ? q.end.half : 0);
+    d.end.vec_h = vec_of(q.end.h, q.end.ld_h);
+    d.end.vec_gu = vec_of(q.end.gate_up, q.end.ld_gu, q.end.half);
+    tiles += ceil_div(q.M, tile_m) * ceil_div(q.N, tile_n);
+  }
+  Launch l;
+  l.cg = s.cg, l.bn = s.bn, l.split = s.split, l.chained = chained, l.stream = stream;
+  const int margin = g_sm_margin.load(std::memory_order_relaxed);
+  if (s.split > 1) {
+    l.grid = (int)tiles * s.split;     // one tile a cluster
+  } else {
+    int64_t most = (sms - margin) / s.cg;
+    if (most < 1) most = 1;
+    l.grid = (int)(tiles < most ? tiles : most) * s.cg;
+  }
+  if (end == kStore) return run_store(b_mn, p, l);
+  if (end == kSwiglu || end == kDswiglu) return run_ffn(end, p, l);
+  return run_ce(end, p, l);
+}
+
+}  // namespace dense
+}  // namespace xkb
+
+extern "C" int xkb_dense_status(void* stream_) {
+  using namespace xkb;
+  int* word = nullptr;
+  const int rc = dense::status_word(&word);
+  if (rc != XKB_OK) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int host = 0;
+  XKB_CHECK_CUDA(cudaMemcpyAsync(&host, word, sizeof(int), cudaMemcpyDeviceToHost, stream));
+  XKB_CHECK_CUDA(cudaStreamSynchronize(stream));
+  if (host != 0)
+    return fail(XKB_ERR_DEVICE, "a kernel of a dense product gave up a bounded wait: status 0x%x (wait site %d)", host, host >> 8);
+  return XKB_OK;
+}

@@ -1,0 +1,68 @@
+// Dense products of 16-bit matrices with a fused end, on tcgen05 (dense_dev.cuh): what their callers hand over.
+#pragma once
+#include <cuda.h>
+#include "common.cuh"
+
+namespace xkb {
+namespace dense {
+
+// What a product's accumulators become.
+constexpr int kStore = 0;     // D, rounded to 16 bits; or kept / added to in fp32
+constexpr int kSwiglu = 1;    // gate and up of the same column side by side: silu(gate) * up, and both if they are kept
+constexpr int kDswiglu = 2;   // D is the gradient of silu(gate) * up: the gradients of both, and the product itself
+constexpr int kCeStats = 3;   // D are logits: maximum and sum of exponentials of a row's piece, the label's logit
+constexpr int kCeGrad = 4;    // D are logits: their gradient, rounded to 16 bits
+
+constexpr int kMaxProblems = 3;
+
+// One product D[M, N] = A[M, K] B[N, K]^T.  Either operand lies in memory as its own rows (K contiguous) or as K rows
+// (its own index contiguous).
+struct Operand {
+  const void* base;
+  int64_t pitch;      // elements from one row in memory to the next, a multiple of 8; the base is 16-byte aligned
+  bool k_rows;        // rows in memory are K
+  int64_t row0;       // first row in memory (B of a piece of the vocabulary)
+  int64_t rows, cols; // extents in memory; what lies outside reads as 0
+};
+
+struct End {
+  void* out;            // 16-bit
+  int64_t ld;
+  const int32_t* row_map;   // row of `out` for every row of D, nullptr: the same
+  const float* scale;       // factor of D on the device, nullptr: 1
+  float* acc;               // fp32 [M, acc_ld]
+  int64_t acc_ld;
+  int acc_in, acc_out;      // add what acc holds; write there and not to out
+  // kSwiglu, kDswiglu
+  void* h;
+  int64_t ld_h;
+  void* gate_up;            // [M, 2 * half]
+  int64_t ld_gu;
+  int half;                 // columns of gate, which are in front of those of up
+  float limit;
+  // kCeStats, kCeGrad: arrays over the rows of D
+  const int32_t* labels;
+  float2* part;             // [parts, part_ld]
+  int64_t part_ld;
+  float* given;
+  const float4* coef;       // m, l, factor of p, what is taken off at the label
+  int col0;                 // first column of the piece in the vocabulary
+  // which vector accesses their rows allow (bytes: 32, 16, or 2), set by the launcher
+  int vec_out, vec_h, vec_gu;
+};
+
+struct Product {
+  Operand a, b;
+  int64_t M, N, K;
+  const int32_t* live;  // on the device: how many of M's rows (of K's, if a.k_rows) there are, nullptr: all
+  End end;
+};
+
+// Launches `count` products with the same end and the same orientation of B as one kernel.  `chained`: may start while
+// its predecessor on the stream runs (common.cuh); `early_b`: B is no output of a kernel of the same call.
+int launch(const Product* products, int count, int end, int dtype, bool chained, bool early_b, cudaStream_t stream);
+// How many pieces a row's statistics come in (kCeStats).
+int ce_parts(int64_t M, int64_t N, int64_t K);
+
+}  // namespace dense
+}  // namespace xkb

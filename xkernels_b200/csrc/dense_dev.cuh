@@ -1,0 +1,737 @@
+// The kernel of the dense products (dense.h): D = A B^T on tcgen05 with fp32 accumulators in tensor memory.
+//
+// A tile is 128 rows of D per CTA and BN columns; with CG = 2 the two CTAs of a pair hold 128 rows of A and half of the
+// columns' rows of B each and one instruction multiplies both halves, so that every SM loads half of B.  Warps: one feeds
+// stages of 64 K by TMA, one issues the MMAs, two warpgroups read accumulators out while the next tile is multiplied
+// (two accumulator sets).  CTAs (pairs) are persistent and take tiles in turn.  Where there are few tiles (CG = 1), up to
+// eight CTAs of a cluster share one: each multiplies a part of K, and adds up a part of the columns in the order of the CTAs.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "dense.h"
+#include "softmax_dev.cuh"
+#include "tc_common.cuh"
+
+namespace xkb {
+namespace dense {
+
+constexpr int kBK = 64;             // K of a stage: 128 bytes, one swizzle row
+constexpr int kRows = 128;          // rows of D per CTA
+constexpr int kThreads = 384;       // warps 0: TMA, 1: MMA, 2: tensor memory, 4 to 11: read-out
+constexpr int kReadWarps = 8;
+constexpr int kABytes = kRows * 128;
+constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
+// The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, so a long sum drifts towards 0
+// (2^-24 of it a step of 16 K: 5e-6 of the logits at K = 7168).  Where the result stays fp32 (kCeStats) an accumulator takes
+// 512 K, and the read-out adds them up in registers while the next is filled: 5e-7, as an fp32 sum on the ordinary cores.
+constexpr int kPartBlocks = 8;
+template <int END> __device__ __forceinline__ int parts_of(int kb) {
+  return END == kCeStats ? (kb + kPartBlocks - 1) / kPartBlocks : 1;
+}
+
+struct DevProduct {
+  CUtensorMap a, b;
+  int M, N, K, b_row0;
+  const int32_t* live;
+  int live_is_k, a_mn;
+  int group;          // row tiles that are walked side by side
+  End end;
+};
+
+struct Params {
+  DevProduct prod[kMaxProblems];
+  int count, fmt;       // fmt: 1 bf16, 0 fp16
+  int split;            // CTAs that share a tile (CG = 1)
+  int a_bytes;          // bytes of A that a stage loads
+  int early_b;
+  int* status;
+};
+
+struct Shared {
+  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+  int abort_flag;
+  uint32_t tmem;
+  int m_tiles[kMaxProblems], n_tiles[kMaxProblems], kb[kMaxProblems], rows[kMaxProblems], first[kMaxProblems + 1];
+};
+
+template <int CG, int BN> struct Cfg {
+  static constexpr int kBBytes = BN / CG * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = (200 * 1024 / kStageBytes) < 8 ? (200 * 1024 / kStageBytes) : 8;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static_assert(kStages >= 4 && kStages <= 8, "");
+};
+
+// ---- instructions that tc_common.cuh has no form of ----------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t smem_addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if constexpr (CG == 2)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this address (in both CTAs of a pair) once the MMAs issued so far are done.
+template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+  else
+    tc::tc_commit(bar);
+}
+template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t* result, uint32_t cols) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(result)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tc::tmem_alloc(result, cols);
+  }
+}
+template <int CG> __device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  else
+    tc::tmem_dealloc(addr, cols);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Operand in shared memory, 128-byte swizzle.  K contiguous: rows of 64 K, groups of eight rows 1024 bytes apart.  Own
+// index contiguous: boxes of 64 elements by 64 K rows, 8192 bytes from box to box, groups of eight K rows 1024 apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool k_rows) {
+  const uint64_t lbo = k_rows ? (kBoxBytes >> 4) : 1;
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (lbo << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// ---- 16-bit rows ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t pack16(int fmt, float lo, float hi) {
+  if (fmt) return pack_bf16(lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void unpack16(int fmt, uint32_t p, float& lo, float& hi) {
+  if (fmt) {
+    lo = __uint_as_float(p << 16);
+    hi = __uint_as_float(p & 0xFFFF0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    lo = f.x;
+    hi = f.y;
+  }
+}
+// CW consecutive elements of a row, the first n of which exist; vec: what the addresses allow.
+template <int CW> __device__ __forceinline__ void store_row(void* base, int64_t at, const uint32_t (&w)[CW / 2], int n, int vec) {
+  uint16_t* p = static_cast<uint16_t*>(base) + at;
+  if (n >= CW && CW % 16 == 0 && vec == 32) {
+#pragma unroll
+    for (int i = 0; i < CW / 2; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                   ::"l"(p + 2 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
+                     "r"(w[i + 7]) : "memory");
+  } else if (n >= CW && vec >= 16) {
+#pragma unroll
+    for (int i = 0; i < CW / 2; i += 4) *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < CW; ++i)
+      if (i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+template <int CW> __device__ __forceinline__ void load_row(const void* base, int64_t at, uint32_t (&w)[CW / 2], int n, int vec) {
+  const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+  if (n >= CW && vec >= 16) {
+#pragma unroll
+    for (int i = 0; i < CW / 2; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p + 2 * i);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < CW; i += 2)
+      w[i / 2] = (i < n ? (uint32_t)p[i] : 0u) | (i + 1 < n ? (uint32_t)p[i + 1] << 16 : 0u);
+  }
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + exp2_fast(-kLog2e * x)); }
+
+// ---- what becomes of CW columns of a row ---------------------------------------------------------------------
+struct RowState {
+  float m, s;       // kCeStats: maximum so far, sum of exponentials against it
+  int label;        // column of the label within the piece
+  float4 coef;      // kCeGrad
+};
+
+template <int END> __device__ __forceinline__ void row_begin(const End& e, int row, bool live, RowState& st) {
+  if constexpr (END == kCeStats || END == kCeGrad) {
+    st.m = -INFINITY;
+    st.s = 0.f;
+    st.label = live ? e.labels[row] - e.col0 : -1;
+    if constexpr (END == kCeGrad) st.coef = live ? e.coef[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+}
+template <int END> __device__ __forceinline__ void row_end(const End& e, int row, bool live, int part, const RowState& st) {
+  if constexpr (END == kCeStats)
+    if (live) e.part[(int64_t)part * e.part_ld + row] = make_float2(st.m, st.s);
+}
+
+// v: columns col .. col + CW of D (kSwiglu: of gate, w: of up), n of which exist
+template <int END, int CW>
+__device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool live, int col, int n, float scale, float (&v)[CW],
+                                          float (&w)[CW], RowState& st) {
+  uint32_t o[CW / 2];
+  if constexpr (END == kStore) {
+    if (!live) return;
+    float4* acc = reinterpret_cast<float4*>(e.acc + (int64_t)row * e.acc_ld + col);
+    if (e.acc_in) {
+#pragma unroll
+      for (int j = 0; j < CW; j += 4) {
+        const float4 f = acc[j / 4];
+        v[j] += f.x, v[j + 1] += f.y, v[j + 2] += f.z, v[j + 3] += f.w;
+      }
+    }
+    if (e.acc_out) {
+#pragma unroll
+      for (int j = 0; j < CW; j += 4) acc[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      return;
+    }
+    if (scale != 1.f) {
+#pragma unroll
+      for (int j = 0; j < CW; ++j) v[j] *= scale;
+    }
+#pragma unroll
+    for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, v[j], v[j + 1]);
+    const int64_t to = e.row_map != nullptr ? e.row_map[row] : row;
+    store_row<CW>(e.out, to * e.ld + col, o, n, e.vec_out);
+  } else if constexpr (END == kSwiglu) {
+    if (!live) return;
+    if (e.gate_up != nullptr) {
+#pragma unroll
+      for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, v[j], v[j + 1]);
+      store_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + col, o, n, e.vec_gu);
+#pragma unroll
+      for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, w[j], w[j + 1]);
+      store_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + e.half + col, o, n, e.vec_gu);
+    }
+    if (e.h == nullptr) return;
+#pragma unroll
+    for (int j = 0; j < CW; j += 2) {
+      float h[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float g = v[j + i], u = w[j + i];
+        if (e.limit > 0.f) {      // (a NaN stays one)
+          g = g > e.limit ? e.limit : g;
+          u = u > e.limit ? e.limit : u < -e.limit ? -e.limit : u;
+        }
+        h[i] = g * sigmoid(g) * u;
+      }
+      o[j / 2] = pack16(fmt, h[0], h[1]);
+    }
+    store_row<CW>(e.h, (int64_t)row * e.ld_h + col, o, n, e.vec_h);
+  } else if constexpr (END == kDswiglu) {
+    if (!live) return;
+    uint32_t ug[CW / 2], uu[CW / 2];
+    const int64_t half = e.half;
+    load_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + col, ug, n, e.vec_gu);
+    load_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + half + col, uu, n, e.vec_gu);
+#pragma unroll
+    for (int j = 0; j < CW; j += 2) {
+      float g[2], u[2], dg[2], du[2], h[2];
+      unpack16(fmt, ug[j / 2], g[0], g[1]);
+      unpack16(fmt, uu[j / 2], u[0], u[1]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float gc = g[i], uc = u[i];
+        if (e.limit > 0.f) {
+          gc = gc > e.limit ? e.limit : gc;
+          uc = uc > e.limit ? e.limit : uc < -e.limit ? -e.limit : uc;
+        }
+        const float s = sigmoid(gc), gs = gc * s, d = v[j + i];
+        dg[i] = d * uc * (s + gs * (1.f - s));
+        du[i] = d * gs;
+        h[i] = gs * uc;
+        if (e.limit > 0.f) {
+          if (g[i] > e.limit) dg[i] = 0.f;
+          if (fabsf(u[i]) > e.limit) du[i] = 0.f;
+        }
+      }
+      o[j / 2] = pack16(fmt, h[0], h[1]);
+      ug[j / 2] = pack16(fmt, dg[0], dg[1]);
+      uu[j / 2] = pack16(fmt, du[0], du[1]);
+    }
+    store_row<CW>(e.out, (int64_t)row * e.ld + col, ug, n, e.vec_out);
+    store_row<CW>(e.out, (int64_t)row * e.ld + half + col, uu, n, e.vec_out);
+    if (e.h != nullptr) store_row<CW>(e.h, (int64_t)row * e.ld_h + col, o, n, e.vec_h);
+  } else if constexpr (END == kCeStats) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < CW; ++j) {
+      if (j >= n) v[j] = -INFINITY;
+      top = fmaxf(top, v[j]);
+    }
+    if (top > st.m) {
+      st.s *= exp2_fast((st.m - top) * kLog2e);
+      st.m = top;
+    }
+    const float ref = st.m == -INFINITY ? 0.f : st.m;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < CW; j += 2) {
+      s0 += exp2_fast((v[j] - ref) * kLog2e);
+      s1 += exp2_fast((v[j + 1] - ref) * kLog2e);
+    }
+    st.s += s0 + s1;
+    const int at = st.label - col;
+    if (at >= 0 && at < n && at < CW) {
+      float x = v[0];
+#pragma unroll
+      for (int j = 1; j < CW; ++j)
+        if (j == at) x = v[j];
+      e.given[row] = x;
+    }
+  } else {
+    const float4 c = st.coef;
+    const int at = st.label - col;
+#pragma unroll
+    for (int j = 0; j < CW; j += 2) {
+      float d[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        d[i] = exp2_fast(((v[j + i] - c.x) - c.y) * kLog2e) * c.z;
+        if (j + i == at) d[i] -= c.w;
+        if (!live) d[i] = 0.f;
+      }
+      o[j / 2] = pack16(fmt, d[0], d[1]);
+    }
+    store_row<CW>(e.out, (int64_t)row * e.ld + col, o, n, e.vec_out);
+  }
+}
+
+// ---- the kernel ----------------------------------------------------------------------------------------------
+struct Tile { int prod, m, n; };
+
+__device__ __forceinline__ bool tile_of(const Params& p, const Shared& sh, int t, Tile& out) {
+  if (t >= sh.first[p.count]) return false;
+  int i = 0;
+  while (i + 1 < p.count && t >= sh.first[i + 1]) ++i;
+  const int r = t - sh.first[i], G = p.prod[i].group, nt = sh.n_tiles[i];
+  const int g = r / (G * nt), in = r - g * G * nt;
+  const int wide = min(G, sh.m_tiles[i] - g * G);
+  out.prod = i;
+  out.n = in / wide;
+  out.m = g * G + (in - out.n * wide);
+  return true;
+}
+
+template <int CG, int BN, bool BMN, int END>
+__global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<CG, BN>;
+  constexpr bool kPaired = END == kSwiglu;
+  constexpr int kTileN = kPaired ? BN / 2 : BN;    // columns of the result
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Shared sh;
+  const uint32_t ring = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = CG == 1 ? p.split : 1;
+  const int width = CG == 2 ? 2 : split;           // CTAs of a cluster
+  const uint32_t rank = width > 1 ? cluster_rank() : 0;
+  const int cluster = blockIdx.x / width, clusters = gridDim.x / width;
+  tc::Guard guard{&sh.abort_flag, p.status};
+
+  if (!p.early_b) chain_wait();
+  chain_trigger();
+  if (threadIdx.x == 0) {
+    sh.abort_flag = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      tc::mbar_init(&sh.full[s], 1);
+      tc::mbar_init(&sh.empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      tc::mbar_init(&sh.acc_full[a], 1);
+      tc::mbar_init(&sh.acc_empty[a], kReadWarps * CG);
+    }
+    tc::mbar_fence_init();
+    int first = 0;
+    for (int i = 0; i < p.count; ++i) {
+      const DevProduct& q = p.prod[i];
+      int M = q.M, K = q.K;
+      if (q.live != nullptr) {
+        const int live = *q.live;
+        if (q.live_is_k) K = min(live, K);
+        else M = min(live, M);
+      }
+      sh.rows[i] = M;
+      sh.m_tiles[i] = (M + kRows * CG - 1) / (kRows * CG);
+      sh.n_tiles[i] = (q.N + kTileN - 1) / kTileN;
+      sh.kb[i] = (K + kBK - 1) / kBK;
+      sh.first[i] = first;
+      first += sh.m_tiles[i] * sh.n_tiles[i];
+    }
+    sh.first[p.count] = first;
+    for (int i = 0; i < p.count; ++i) {
+      tc::prefetch_tensormap(&p.prod[i].a);
+      tc::prefetch_tensormap(&p.prod[i].b);
+    }
+  }
+  if (warp == 2) tmem_alloc<CG>(&sh.tmem, 2 * BN);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (width > 1) cluster_sync();
+  tc::tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      const uint32_t bytes = (uint32_t)(p.a_bytes + C::kBBytes) * CG;
+      Tile t;
+      bool early = p.early_b != 0, ok = true;
+      for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+        const DevProduct& q = p.prod[t.prod];
+        const int kb = sh.kb[t.prod];
+        const int k0 = kb * (int)(CG == 1 ? rank : 0) / split, k1 = kb * ((int)(CG == 1 ? rank : 0) + 1) / split;
+        const int m0 = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0);
+        auto load_a = [&](uint32_t s, uint32_t bar, int k) {
+          const uint32_t dst = ring + s * C::kStageBytes;
+          if (!q.a_mn) {
+            tma_2d<CG>(dst, &q.a, bar, k * kBK, m0);
+          } else {
+            tma_2d<CG>(dst, &q.a, bar, m0, k * kBK);
+            tma_2d<CG>(dst + kBoxBytes, &q.a, bar, m0 + 64, k * kBK);
+          }
+        };
+        auto load_b = [&](uint32_t s, uint32_t bar, int k) {
+          const uint32_t dst = ring + s * C::kStageBytes + kABytes;
+          if constexpr (!BMN) {
+#pragma unroll
+            for (int j = 0; j < 2 / CG; ++j) {
+              const int part = CG == 2 ? (int)rank : j;
+              const int row = kPaired ? part * q.end.half + t.n * (BN / 2) : t.n * BN + part * (BN / 2);
+              tma_2d<CG>(dst + j * (BN / 2) * 128, &q.b, bar, k * kBK, q.b_row0 + row);
+            }
+          } else {
+            const int n0 = t.n * BN + (CG == 2 ? (int)rank * (BN / 2) : 0);
+#pragma unroll
+            for (int j = 0; j < BN / CG / 64; ++j) tma_2d<CG>(dst + j * kBoxBytes, &q.b, bar, n0 + 64 * j, q.b_row0 + k * kBK);
+          }
+        };
+        auto bar_of = [&](uint32_t s) {
+          const uint32_t bar = tc::smem_u32(&sh.full[s]);
+          return CG == 2 ? map_to(bar, 0) : bar;
+        };
+        int k = k0;
+        if (early) {      // B is there before the predecessor has finished
+          const int n = min(C::kStages, k1 - k0);
+          for (int i = 0; i < n; ++i) {
+            if (CG == 1 || rank == 0) tc::mbar_expect_tx(&sh.full[i], bytes);
+            load_b(i, bar_of(i), k0 + i);
+          }
+          chain_wait();
+          for (int i = 0; i < n; ++i) load_a(i, bar_of(i), k0 + i);
+          k += n;
+          it += n;
+          early = false;
+        }
+        for (; k < k1; ++k, ++it) {
+          const uint32_t s = it % C::kStages, phase = (it / C::kStages) & 1;
+          if (!tc::mbar_wait(&sh.empty[s], phase ^ 1, guard, 1)) { ok = false; break; }
+          if (CG == 1 || rank == 0) tc::mbar_expect_tx(&sh.full[s], bytes);
+          load_a(s, bar_of(s), k);
+          load_b(s, bar_of(s), k);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (CG == 1 || rank == 0) {
+      const uint32_t base_idesc = (1u << 4) | ((uint32_t)p.fmt << 7) | ((uint32_t)p.fmt << 10) | ((BMN ? 1u : 0u) << 16) |
+                                  ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((kRows * CG) >> 4) << 24);
+      const bool leader = tc::elect_one();
+      uint32_t it = 0, sets = 0;
+      Tile t;
+      bool ok = true;
+      for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+        const bool a_mn = p.prod[t.prod].a_mn != 0;
+        const uint32_t idesc = base_idesc | ((a_mn ? 1u : 0u) << 15);
+        const uint32_t a_step = a_mn ? 128 : 2, b_step = BMN ? 128 : 2;    // 16 K further, in units of 16 bytes
+        const int kb = sh.kb[t.prod];
+        const int k0 = kb * (int)(CG == 1 ? rank : 0) / split, k1 = kb * ((int)(CG == 1 ? rank : 0) + 1) / split;
+        const int parts = parts_of<END>(k1 - k0);
+        for (int part = 0; ok && part < parts; ++part, ++sets) {
+          const uint32_t set = sets & 1, d = tmem + set * BN;
+          if (!tc::mbar_wait(&sh.acc_empty[set], ((sets >> 1) & 1) ^ 1, guard, 2)) { ok = false; break; }
+          tc::tc_fence_after();
+          const int b0 = END == kCeStats ? k0 + part * kPartBlocks : k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, k1) : k1;
+          for (int k = b0; k < b1; ++k, ++it) {
+            const uint32_t s = it % C::kStages, phase = (it / C::kStages) & 1;
+            if (!tc::mbar_wait(&sh.full[s], phase, guard, 3)) { ok = false; break; }
+            tc::tc_fence_after();
+            if (leader) {
+              const uint32_t addr = ring + s * C::kStageBytes;
+              const uint64_t a = operand_desc(addr, a_mn), b = operand_desc(addr + kABytes, BMN);
+#pragma unroll
+              for (int i = 0; i < kBK / 16; ++i)
+                mma_ss<CG>(d, a + i * a_step, b + i * b_step, idesc, (k > b0 || i > 0) ? 1u : 0u);
+              commit<CG>(&sh.empty[s]);
+            }
+            __syncwarp();
+          }
+          if (ok && leader) commit<CG>(&sh.acc_full[set]);
+          __syncwarp();
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    const int wg = (warp - 4) >> 2, quad = warp & 3;
+    const int in_tile = quad * 32 + lane;
+    constexpr int kMine = kTileN / 2;       // columns of a warpgroup
+    if (p.early_b) chain_wait();
+    uint32_t sets = 0;
+    Tile t;
+    bool ok = true;
+    for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+      const End& e = p.prod[t.prod].end;
+      const int N = p.prod[t.prod].N, kb = sh.kb[t.prod];
+      const int row = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0) + in_tile;
+      const bool live = row < sh.rows[t.prod];
+      const bool warp_live = row - lane < sh.rows[t.prod];
+      auto hand_back = [&](uint32_t set) {      // all loads from the accumulators have come back
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) remote_arrive(map_to(tc::smem_u32(&sh.acc_empty[set]), CG == 2 ? 0 : rank));
+      };
+      auto park = [&](int c, float x) {         // this CTA's part of a sum, columns of 128 rows, where the stages were
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (c * kRows + in_tile) * 4), "f"(x) : "memory");
+      };
+      RowState st;
+      row_begin<END>(e, row, live && split == 1, st);
+      const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
+      if constexpr (END == kCeStats) {
+        const int parts = parts_of<END>(kb * ((int)(CG == 1 ? rank : 0) + 1) / split - kb * (int)(CG == 1 ? rank : 0) / split);
+        float sum[kMine];
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
+        for (int part = 0; part < parts; ++part, ++sets) {
+          const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16) + wg * kMine;
+          if (!tc::mbar_wait(&sh.acc_full[set], (sets >> 1) & 1, guard, 4)) { ok = false; break; }
+          tc::tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < kMine; c += 16) {
+            uint32_t v[16];
+            tc::tmem_ld_32x16(from + c, v);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(v[j]);
+          }
+          hand_back(set);
+        }
+        if (!ok) break;
+        if (split > 1) {
+          if (warp_live)
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) park(wg * kMine + j, sum[j]);
+          break;
+        }
+#pragma unroll
+        for (int c = 0; c < kMine; c += 32) {
+          const int col = t.n * kTileN + wg * kMine + c;
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
+          if (N - col > 0) row_piece<END, 32>(e, p.fmt, row, live, col, N - col, scale, v, v, st);
+        }
+        row_end<END>(e, row, live, t.n * 2 + wg, st);
+      } else {
+        const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16);
+        ++sets;
+        if (!tc::mbar_wait(&sh.acc_full[set], ((sets - 1) >> 1) & 1, guard, 4)) break;
+        tc::tc_fence_after();
+        if (split > 1) {
+          if (warp_live) {
+            for (int c = wg * (BN / 2); c < (wg + 1) * (BN / 2); c += 32) {
+              float v[32];
+              tmem_ld32(from + c, v);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) park(c + j, v[j]);
+            }
+          }
+          break;
+        }
+#pragma unroll 1
+        for (int c = wg * kMine; c < (wg + 1) * kMine; c += 32) {
+          const int col = t.n * kTileN + c, n = N - col;
+          if (n <= 0) break;
+          float v[32], w[32];
+          tmem_ld32(from + c, v);
+          if constexpr (kPaired) tmem_ld32(from + BN / 2 + c, w);
+          tc::tmem_wait_ld();
+          if (kb == 0) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = w[j] = 0.f;
+          }
+          row_piece<END, 32>(e, p.fmt, row, live, col, n, scale, v, w, st);
+        }
+        hand_back(set);
+      }
+    }
+  }
+  __syncwarp();
+
+  if (split > 1) {
+    cluster_sync();       // every CTA's part is in its shared memory
+    Tile t;
+    if (warp >= 4 && tile_of(p, sh, cluster, t) && !guard.aborted()) {
+      const End& e = p.prod[t.prod].end;
+      const int wg = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
+      const int row = t.m * kRows + in_tile;
+      const bool live = row < sh.rows[t.prod];
+      if (t.m * kRows + (warp & 3) * 32 < sh.rows[t.prod]) {
+        RowState st;
+        row_begin<END>(e, row, live, st);
+        const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
+        const int mine = kTileN / split;     // columns of this CTA
+#pragma unroll 1
+        for (int c = (int)rank * mine + wg * 8; c < ((int)rank + 1) * mine; c += 16) {
+          const int col = t.n * kTileN + c, n = p.prod[t.prod].N - col;
+          if (n <= 0) break;
+          float v[8], w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
+          for (int from = 0; from < split; ++from) {
+            const uint32_t base = map_to(ring + (c * kRows + in_tile) * 4, from);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              v[j] += ld_cluster(base + j * kRows * 4);
+              if constexpr (kPaired) w[j] += ld_cluster(base + (BN / 2 + j) * kRows * 4);
+            }
+          }
+          row_piece<END, 8>(e, p.fmt, row, live, col, n, scale, v, w, st);
+        }
+        row_end<END>(e, row, live, (t.n * split + (int)rank) * 2 + wg, st);
+      } else if (END == kCeGrad && t.m * kRows < sh.rows[t.prod]) {
+        // rows behind the last: zeros, they are K of the next product
+        RowState st;
+        row_begin<END>(e, row, false, st);
+        const int mine = kTileN / split;
+        for (int c = (int)rank * mine + wg * 8; c < ((int)rank + 1) * mine; c += 16) {
+          const int col = t.n * kTileN + c, n = p.prod[t.prod].N - col;
+          if (n <= 0) break;
+          float v[8], w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
+          row_piece<END, 8>(e, p.fmt, row, false, col, n, 1.f, v, w, st);
+        }
+      }
+    }
+  }
+  // A wait that ran out leaves copies and MMAs in flight: they land within microseconds.
+  if (guard.aborted())
+    for (int i = 0; i < 100; ++i) __nanosleep(20000);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (width > 1) cluster_sync();
+  if (warp == 2) {
+    tc::tc_fence_after();
+    tmem_dealloc<CG>(tmem, 2 * BN);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------
+struct Launch {
+  int cg, bn, split, grid;
+  bool chained;
+  cudaStream_t stream;
+};
+
+template <int CG, int BN, bool BMN, int END>
+int run_kernel(const Params& p, const Launch& l) {
+  using C = Cfg<CG, BN>;
+  static std::atomic<uint64_t> ready{0};      // devices on which this instance is set up
+  int dev = 0;
+  XKB_CHECK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit == 0 || !(ready.load(std::memory_order_acquire) & bit)) {
+    XKB_CHECK_CUDA(cudaFuncSetAttribute(dense_kernel<CG, BN, BMN, END>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    ready.fetch_or(bit, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(l.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = l.stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (CG == 2 || l.split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = CG == 2 ? 2 : l.split;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (l.chained) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dense_kernel<CG, BN, BMN, END>, p));
+  XKB_CHECK_LAUNCH("dense_kernel");
+  return XKB_OK;
+}
+
+template <bool BMN, int END>
+int run_variant(const Params& p, const Launch& l) {
+  if (l.cg == 2) return l.bn == 256 ? run_kernel<2, 256, BMN, END>(p, l) : run_kernel<2, 128, BMN, END>(p, l);
+  return run_kernel<1, 128, BMN, END>(p, l);
+}
+
+// one per translation unit
+int run_ffn(int end, const Params& p, const Launch& l);
+int run_store(bool b_mn, const Params& p, const Launch& l);
+int run_ce(int end, const Params& p, const Launch& l);
+
+}  // namespace dense
+}  // namespace xkb

@@ -9,4 +9,8 @@ namespace xkb {
 int make_map_2d(CUtensorMap* map, CUtensorMapDataType dt, int elem_bits, const void* base, uint64_t rows,
                 uint64_t cols, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swz, const char* what);
 
+// The same with rows `pitch_bytes` apart (a multiple of 16).
+int make_map_2d_pitched(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t rows, uint64_t cols,
+                        uint64_t pitch_bytes, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swz, const char* what);
+
 }  // namespace xkb

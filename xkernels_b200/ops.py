@@ -602,6 +602,190 @@ def token_logprobs_backward(logits, token_ids, stats, entropy=None, grad_logprob
 
 
 # ---------------------------------------------------------------------------
+_HALF_DT = {torch.bfloat16: _lib.XKB_BF16, torch.float16: _lib.XKB_F16}
+
+
+def _matrix(name, what, t, shape, dtype):
+    """``t`` as an operand of a dense product: of ``dtype``, rows a multiple of 16 bytes apart, the first on 16 bytes.  Read in
+    place where it is one already (a slice of wider rows too); else laid out once more."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: {what} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: {what} must be {dtype} like the first argument, got {t.dtype}")
+    rows, cols = shape
+    if (cols == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(0) >= cols:
+        return t, t.stride(0)
+    ld = -(-cols // 8) * 8
+    buf = torch.empty((rows, ld), dtype=dtype, device=t.device)
+    buf[:, :cols].copy_(t)
+    return buf, ld
+
+
+class LinearCrossEntropy(NamedTuple):
+    """What :func:`linear_cross_entropy` returns."""
+
+    loss: torch.Tensor    # [M] fp32
+    lse: torch.Tensor     # [M] fp32: log-sum-exp of the logits
+    stats: torch.Tensor   # [M, 2] fp32: row maximum m, ln sum exp(z - m)
+
+
+def _linear_head(name, hidden, weight, labels):
+    if hidden.dim() != 2 or weight.dim() != 2 or hidden.shape[1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"{name}: hidden must be [M, H] and weight [V, H]")
+    if hidden.dtype not in _HALF_DT:
+        raise TypeError(f"{name}: hidden must be bf16 or fp16, got {hidden.dtype}")
+    if labels.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: labels must be int32 or int64, got {labels.dtype}")
+    M, H = hidden.shape
+    if tuple(labels.shape) != (M,):
+        raise ValueError(f"{name}: labels must be [{M}], got {list(labels.shape)}")
+    if H > 1 and hidden.stride(1) != 1:
+        hidden = hidden.contiguous()
+    return hidden, labels.contiguous(), M, H, weight.shape[0]
+
+
+def linear_cross_entropy(hidden, weight, labels):
+    """Cross entropy of a head: ``loss[i] = lse(z[i]) - z[i, labels[i]]`` with ``z = hidden @ weight.T``, which is never stored.
+
+    ``hidden`` ``[M, H]`` and ``weight`` ``[V, H]`` bf16 or fp16 (products are added up in fp32), ``labels`` ``[M]`` int32 or int64.
+    A negative label is padding: the row is not read, its results are 0, and it costs next to nothing.  A label of V or more gives
+    a loss of NaN, a row whose logits hold a NaN or +inf is NaN.  The same bits in every run.  Where :func:`token_logprobs` takes
+    logits, this takes what they are made from; its gradient is :func:`linear_cross_entropy_backward`.  No reference counterpart.
+    """
+    lib = _lib.load()
+    name = "linear_cross_entropy"
+    dev = _require_cuda(name, hidden, weight, labels)
+    hidden, labels, M, H, V = _linear_head(name, hidden, weight, labels)
+    with _on(dev):
+        weight, ld_w = _matrix(name, "weight", weight, (V, H), hidden.dtype)
+        loss = torch.empty((M,), dtype=torch.float32, device=dev)
+        lse = torch.empty((M,), dtype=torch.float32, device=dev)
+        stats = torch.empty((M, 2), dtype=torch.float32, device=dev)
+        ws_bytes = _bytes("xkb_linear_cross_entropy_workspace_bytes", M, H, V)      # of this call alone: calls may overlap
+        ws = torch.empty((max(ws_bytes, 0),), dtype=torch.uint8, device=dev)
+        _lib.check(
+            lib.xkb_linear_cross_entropy(_ptr(hidden), hidden.stride(0), _HALF_DT[hidden.dtype], _ptr(weight), ld_w, _ptr(labels),
+                                         1 if labels.dtype == torch.int64 else 0, _ptr(loss), _ptr(lse), _ptr(stats), M, H, V,
+                                         _ptr(ws), ws_bytes, _stream(dev)),
+            "xkb_linear_cross_entropy")
+    return LinearCrossEntropy(loss, lse, stats)
+
+
+def linear_cross_entropy_backward(hidden, weight, labels, stats, grad_loss=None, grad_lse=None, need_grad_hidden=True,
+                                  need_grad_weight=True):
+    """The gradients of :func:`linear_cross_entropy`: ``(grad_hidden, grad_weight)``, of ``hidden``'s and ``weight``'s shape and
+    dtype; what is not wanted is None.
+
+    ``stats`` is what the forward call returned; ``grad_loss`` and ``grad_lse`` ``[M]`` are the gradients of its outputs (one at
+    least is needed; the other counts as 0; of padding rows they are not read).  The logits are multiplied once more, a piece of the
+    vocabulary at a time, so no more than 256 MiB of their gradient are ever held.  Sums are fp32; the gradient of the logits is
+    rounded to ``hidden``'s dtype as the operand of the next products.  The same bits in every run.
+    """
+    lib = _lib.load()
+    name = "linear_cross_entropy_backward"
+    dev = _require_cuda(name, hidden, weight, labels, stats, grad_loss, grad_lse)
+    if grad_loss is None and grad_lse is None:
+        raise ValueError(f"{name}: no gradient is given")
+    hidden, labels, M, H, V = _linear_head(name, hidden, weight, labels)
+    stats = _typed(name, "stats", stats, (M, 2), torch.float32)
+    if grad_loss is not None:
+        grad_loss = _typed(name, "grad_loss", grad_loss, (M,), torch.float32)
+    if grad_lse is not None:
+        grad_lse = _typed(name, "grad_lse", grad_lse, (M,), torch.float32)
+    with _on(dev):
+        weight, ld_w = _matrix(name, "weight", weight, (V, H), hidden.dtype)
+        grad_hidden = torch.empty((M, H), dtype=hidden.dtype, device=dev) if need_grad_hidden else None
+        grad_weight = torch.empty((V, H), dtype=hidden.dtype, device=dev) if need_grad_weight else None
+        ws_bytes = _bytes("xkb_linear_cross_entropy_backward_workspace_bytes", M, H, V)
+        ws = torch.empty((max(ws_bytes, 0),), dtype=torch.uint8, device=dev)
+        _lib.check(
+            lib.xkb_linear_cross_entropy_backward(
+                _ptr(hidden), hidden.stride(0), _HALF_DT[hidden.dtype], _ptr(weight), ld_w, _ptr(labels), 1 if labels.dtype == torch.int64 else 0,
+                _ptr(stats), _ptr(grad_loss), _ptr(grad_lse), _ptr(grad_hidden), _ptr(grad_weight), M, H, V, _ptr(ws), ws_bytes,
+                _stream(dev)),
+            "xkb_linear_cross_entropy_backward")
+    return grad_hidden, grad_weight
+
+
+def _gated_sizes(name, x, w13, w2):
+    if x.dim() != 2 or w13.dim() != 2 or w2.dim() != 2:
+        raise ValueError(f"{name}: x must be [M, H], w13 [2*I, H] and w2 [H, I]")
+    if x.dtype not in _HALF_DT:
+        raise TypeError(f"{name}: x must be bf16 or fp16, got {x.dtype}")
+    (M, H), I = x.shape, w2.shape[1]
+    if H < 1 or I < 1:
+        raise ValueError(f"{name}: empty weights")
+    return M, H, I
+
+
+def gated_ffn(x, w13, w2, swiglu_limit=None, save_gate_up=False):
+    """A dense gated feed-forward block, such as the shared expert beside the routed ones: ``(silu(gate) * up) @ w2.T`` with
+    ``gate, up = x @ w13.T``.
+
+    ``x`` ``[M, H]``, ``w13`` ``[2*I, H]`` (gate rows first, as in :func:`fused_moe_mxfp4`), ``w2`` ``[H, I]``, all bf16 or all fp16;
+    rows may lie apart.  ``swiglu_limit`` (None or 0: none) cuts gate off at the limit and up at plus and minus it, as there.
+    Products are added up in fp32, and ``silu(gate) * up`` is rounded to ``x``'s dtype once, as the operand of the second product.
+    Returns ``out`` ``[M, H]``, or ``(out, gate_up)`` with ``save_gate_up``: ``[M, 2*I]`` before the limit, for
+    :func:`gated_ffn_backward`.  The same bits in every run.  No reference counterpart.
+    """
+    lib = _lib.load()
+    name = "gated_ffn"
+    dev = _require_cuda(name, x, w13, w2)
+    M, H, I = _gated_sizes(name, x, w13, w2)
+    limit = 0.0 if swiglu_limit is None else float(swiglu_limit)
+    with _on(dev):
+        dt = x.dtype
+        x, ld_x = _matrix(name, "x", x, (M, H), dt)
+        w13, ld_13 = _matrix(name, "w13", w13, (2 * I, H), dt)
+        w2, ld_2 = _matrix(name, "w2", w2, (H, I), dt)
+        out = torch.empty((M, H), dtype=dt, device=dev)
+        gate_up = torch.empty((M, 2 * I), dtype=dt, device=dev) if save_gate_up else None
+        ws_bytes = _bytes("xkb_gated_ffn_workspace_bytes", M, H, I)                 # of this call alone: calls may overlap
+        ws = torch.empty((max(ws_bytes, 0),), dtype=torch.uint8, device=dev)
+        _lib.check(
+            lib.xkb_gated_ffn(_ptr(x), ld_x, _HALF_DT[dt], _ptr(w13), ld_13, _ptr(w2), ld_2, limit, _ptr(out), _ptr(gate_up), M, H, I,
+                              _ptr(ws), ws_bytes, _stream(dev)),
+            "xkb_gated_ffn")
+    return (out, gate_up) if save_gate_up else out
+
+
+def gated_ffn_backward(grad_out, x, w13, w2, gate_up=None, swiglu_limit=None, need_grad_x=True, need_grad_w13=True,
+                       need_grad_w2=True):
+    """The gradients of :func:`gated_ffn`: ``(grad_x, grad_w13, grad_w2)``, of their shapes and dtype; what is not wanted is None.
+
+    ``gate_up`` is what the forward call saved; without it the first product is multiplied once more (and what the limit cuts off is
+    then decided on its result rounded to ``x``'s dtype, as with the saved one).  Gradients of gate and up and ``silu(gate) * up`` are
+    rounded to ``x``'s dtype once, as operands of the next products; all sums are fp32.  The same bits in every run.
+    """
+    lib = _lib.load()
+    name = "gated_ffn_backward"
+    dev = _require_cuda(name, grad_out, x, w13, w2, gate_up)
+    M, H, I = _gated_sizes(name, x, w13, w2)
+    limit = 0.0 if swiglu_limit is None else float(swiglu_limit)
+    dt = x.dtype
+    if gate_up is not None:
+        if gate_up.dtype != dt:
+            raise TypeError(f"{name}: gate_up must be {dt} like x, got {gate_up.dtype}")
+        gate_up = _typed(name, "gate_up", gate_up, (M, 2 * I), dt)
+    with _on(dev):
+        grad_out, ld_go = _matrix(name, "grad_out", grad_out, (M, H), dt)
+        x, ld_x = _matrix(name, "x", x, (M, H), dt)
+        w13, ld_13 = _matrix(name, "w13", w13, (2 * I, H), dt)
+        w2, ld_2 = _matrix(name, "w2", w2, (H, I), dt)
+        grad_x = torch.empty((M, H), dtype=dt, device=dev) if need_grad_x else None
+        grad_w13 = torch.empty((2 * I, H), dtype=dt, device=dev) if need_grad_w13 else None
+        grad_w2 = torch.empty((H, I), dtype=dt, device=dev) if need_grad_w2 else None
+        ws_bytes = _bytes("xkb_gated_ffn_backward_workspace_bytes", M, H, I, 0 if gate_up is not None else 1)
+        ws = torch.empty((max(ws_bytes, 0),), dtype=torch.uint8, device=dev)
+        _lib.check(
+            lib.xkb_gated_ffn_backward(
+                _ptr(grad_out), ld_go, _HALF_DT[dt], _ptr(x), ld_x, _ptr(w13), ld_13, _ptr(w2), ld_2, _ptr(gate_up), limit, _ptr(grad_x),
+                _ptr(grad_w13), _ptr(grad_w2), M, H, I, _ptr(ws), ws_bytes, _stream(dev)),
+            "xkb_gated_ffn_backward")
+    return grad_x, grad_w13, grad_w2
+
+
+# ---------------------------------------------------------------------------
 _checked_scales: dict[tuple[int, int], int] = {}
 _INT4_SCALE_LIMIT = float(2 ** 24)
 

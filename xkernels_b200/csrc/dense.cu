@@ -132,7 +132,7 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     d.M = (int)q.M, d.N = (int)q.N, d.K = (int)q.K, d.b_row0 = (int)q.b.row0;
     d.live = q.live;
     d.live_is_k = d.a_mn = q.a.k_rows;
-    d.group = 16 / s.cg;
+    d.group = 16;
     d.end = q.end;
     d.end.vec_out = vec_of(q.end.out, q.end.ld, end == kDswiglu ? q.end.half : 0);
     d.end.vec_h = vec_of(q.end.h, q.end.ld_h);

@@ -58,7 +58,7 @@ struct Shared {
 template <int CG, int BN> struct Cfg {
   static constexpr int kBBytes = BN / CG * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = (200 * 1024 / kStageBytes) < 8 ? (200 * 1024 / kStageBytes) : 8;
+  static constexpr int kStages = (225 * 1024 / kStageBytes) < 8 ? (225 * 1024 / kStageBytes) : 8;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
   static_assert(kStages >= 4 && kStages <= 8, "");
 };
@@ -99,12 +99,40 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // Arrives on the barrier at this address (in both CTAs of a pair) once the MMAs issued so far are done.
-template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
+template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
   if constexpr (CG == 2)
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
+                 ::"r"(bar), "h"((uint16_t)3) : "memory");
   else
-    tc::tc_commit(bar);
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Barriers by their address.  A wait is bounded (tc_common.cuh).
+__device__ __forceinline__ bool probe(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, tc::Guard g, int where) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (probe(bar, parity)) return true;
+    if ((i & 63u) == 0u) {
+      if (g.aborted()) return false;
+      const uint64_t now = tc::globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > tc::kWaitBudgetNs) break;
+    }
+  }
+  g.raise(tc::kErrWaitTimeout + (where << 8));
+  return false;
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, const tc::Guard& g, int where) {
+  return probe(bar, parity) || wait_slow(bar, parity, g, where);
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 template <int CG> __device__ __forceinline__ void tmem_alloc(uint32_t* result, uint32_t cols) {
   if constexpr (CG == 2) {
@@ -374,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   const uint32_t ring = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = CG == 1 ? p.split : 1;
   const int width = CG == 2 ? 2 : split;           // CTAs of a cluster
   const uint32_t rank = width > 1 ? cluster_rank() : 0;
@@ -423,64 +451,70 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   tc::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      const uint32_t bytes = (uint32_t)(p.a_bytes + C::kBBytes) * CG;
-      Tile t;
-      bool early = p.early_b != 0, ok = true;
-      for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
-        const DevProduct& q = p.prod[t.prod];
-        const int kb = sh.kb[t.prod];
-        const int k0 = kb * (int)(CG == 1 ? rank : 0) / split, k1 = kb * ((int)(CG == 1 ? rank : 0) + 1) / split;
+  const uint32_t part_rank = CG == 1 ? rank : 0;      // which part of K
+  auto k_from = [&](int kb, uint32_t r) { return split == 1 ? (r == 0 ? 0 : kb) : kb * (int)r / split; };
+  if (warp == 0 || warp == 3) {
+    // Warp 0 feeds A, warp 3 feeds B.  The whole warp runs the loop and one lane issues: operands then sit in uniform
+    // registers (in a loop of one lane a copy took its issuer 200 clocks, and both operands' 600 a stage where the MMAs
+    // take 512).
+    const bool leader = tc::elect_one(), feeds_a = warp == 0;
+    if (p.early_b && feeds_a) chain_wait();
+    const uint32_t bytes = (uint32_t)(p.a_bytes + C::kBBytes) * CG;
+    const bool expects = leader && (CG == 1 || rank == 0);
+    const uint32_t empty = tc::smem_u32(sh.empty);
+    const uint32_t mine = tc::smem_u32(sh.full), full = CG == 2 ? map_to(mine, 0) : mine;   // the first CTA's count
+    uint32_t slot = 0, parity = 1, dst = ring + (feeds_a ? 0 : kABytes);
+    bool ok = true;
+    auto next = [&]() {
+      dst += C::kStageBytes;
+      if (++slot == C::kStages) slot = 0, parity ^= 1, dst -= C::kStages * C::kStageBytes;
+    };
+    Tile t;
+    for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+      const DevProduct& q = p.prod[t.prod];
+      const int kb = sh.kb[t.prod];
+      const int k0 = k_from(kb, part_rank), k1 = k_from(kb, part_rank + 1);
+      if (feeds_a) {
+        const CUtensorMap* map = &q.a;
         const int m0 = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0);
-        auto load_a = [&](uint32_t s, uint32_t bar, int k) {
-          const uint32_t dst = ring + s * C::kStageBytes;
-          if (!q.a_mn) {
-            tma_2d<CG>(dst, &q.a, bar, k * kBK, m0);
-          } else {
-            tma_2d<CG>(dst, &q.a, bar, m0, k * kBK);
-            tma_2d<CG>(dst + kBoxBytes, &q.a, bar, m0 + 64, k * kBK);
-          }
-        };
-        auto load_b = [&](uint32_t s, uint32_t bar, int k) {
-          const uint32_t dst = ring + s * C::kStageBytes + kABytes;
-          if constexpr (!BMN) {
-#pragma unroll
-            for (int j = 0; j < 2 / CG; ++j) {
-              const int part = CG == 2 ? (int)rank : j;
-              const int row = kPaired ? part * q.end.half + t.n * (BN / 2) : t.n * BN + part * (BN / 2);
-              tma_2d<CG>(dst + j * (BN / 2) * 128, &q.b, bar, k * kBK, q.b_row0 + row);
+        const bool mn = q.a_mn != 0;
+        for (int k = k0 * kBK; k < k1 * kBK; k += kBK) {
+          if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
+          if (expects) expect_tx(mine + 8 * slot, bytes);
+          if (leader) {
+            if (!mn) {
+              tma_2d<CG>(dst, map, full + 8 * slot, k, m0);
+            } else {
+              tma_2d<CG>(dst, map, full + 8 * slot, m0, k);
+              tma_2d<CG>(dst + kBoxBytes, map, full + 8 * slot, m0 + 64, k);
             }
-          } else {
-            const int n0 = t.n * BN + (CG == 2 ? (int)rank * (BN / 2) : 0);
-#pragma unroll
-            for (int j = 0; j < BN / CG / 64; ++j) tma_2d<CG>(dst + j * kBoxBytes, &q.b, bar, n0 + 64 * j, q.b_row0 + k * kBK);
           }
-        };
-        auto bar_of = [&](uint32_t s) {
-          const uint32_t bar = tc::smem_u32(&sh.full[s]);
-          return CG == 2 ? map_to(bar, 0) : bar;
-        };
-        int k = k0;
-        if (early) {      // B is there before the predecessor has finished
-          const int n = min(C::kStages, k1 - k0);
-          for (int i = 0; i < n; ++i) {
-            if (CG == 1 || rank == 0) tc::mbar_expect_tx(&sh.full[i], bytes);
-            load_b(i, bar_of(i), k0 + i);
-          }
-          chain_wait();
-          for (int i = 0; i < n; ++i) load_a(i, bar_of(i), k0 + i);
-          k += n;
-          it += n;
-          early = false;
+          next();
         }
-        for (; k < k1; ++k, ++it) {
-          const uint32_t s = it % C::kStages, phase = (it / C::kStages) & 1;
-          if (!tc::mbar_wait(&sh.empty[s], phase ^ 1, guard, 1)) { ok = false; break; }
-          if (CG == 1 || rank == 0) tc::mbar_expect_tx(&sh.full[s], bytes);
-          load_a(s, bar_of(s), k);
-          load_b(s, bar_of(s), k);
+      } else {
+        const CUtensorMap* map = &q.b;
+        if constexpr (!BMN) {
+          const int part = CG == 2 ? (int)rank : 0;
+          const int r0 = q.b_row0 + (kPaired ? part * q.end.half + t.n * (BN / 2) : t.n * BN + part * (BN / 2));
+          const int r1 = r0 + (kPaired ? q.end.half : BN / 2);      // (CG = 1: the other half of the columns)
+          for (int k = k0 * kBK; k < k1 * kBK; k += kBK) {
+            if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
+            if (leader) {
+              tma_2d<CG>(dst, map, full + 8 * slot, k, r0);
+              if constexpr (CG == 1) tma_2d<CG>(dst + (BN / 2) * 128, map, full + 8 * slot, k, r1);
+            }
+            next();
+          }
+        } else {
+          const int n0 = t.n * BN + (CG == 2 ? (int)rank * (BN / 2) : 0), base = q.b_row0;
+          for (int k = k0 * kBK; k < k1 * kBK; k += kBK) {
+            if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
+            if (leader) {
+#pragma unroll
+              for (int j = 0; j < BN / CG / 64; ++j) tma_2d<CG>(dst + j * kBoxBytes, map, full + 8 * slot, n0 + 64 * j, base + k);
+            }
+            next();
+          }
         }
       }
     }
@@ -489,37 +523,46 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       const uint32_t base_idesc = (1u << 4) | ((uint32_t)p.fmt << 7) | ((uint32_t)p.fmt << 10) | ((BMN ? 1u : 0u) << 16) |
                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((kRows * CG) >> 4) << 24);
       const bool leader = tc::elect_one();
-      uint32_t it = 0, sets = 0;
+      const uint32_t full = tc::smem_u32(sh.full), empty = tc::smem_u32(sh.empty);
+      const uint32_t acc_full = tc::smem_u32(sh.acc_full), acc_empty = tc::smem_u32(sh.acc_empty);
+      const uint64_t b_first = operand_desc(ring + kABytes, BMN);
+      uint32_t slot = 0, parity = 0, off = 0, set = 0, set_parity = 1;
       Tile t;
       bool ok = true;
       for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
         const bool a_mn = p.prod[t.prod].a_mn != 0;
+        const uint64_t a_first = operand_desc(ring, a_mn);
         const uint32_t idesc = base_idesc | ((a_mn ? 1u : 0u) << 15);
         const uint32_t a_step = a_mn ? 128 : 2, b_step = BMN ? 128 : 2;    // 16 K further, in units of 16 bytes
         const int kb = sh.kb[t.prod];
-        const int k0 = kb * (int)(CG == 1 ? rank : 0) / split, k1 = kb * ((int)(CG == 1 ? rank : 0) + 1) / split;
+        const int k0 = k_from(kb, part_rank), k1 = k_from(kb, part_rank + 1);
         const int parts = parts_of<END>(k1 - k0);
-        for (int part = 0; ok && part < parts; ++part, ++sets) {
-          const uint32_t set = sets & 1, d = tmem + set * BN;
-          if (!tc::mbar_wait(&sh.acc_empty[set], ((sets >> 1) & 1) ^ 1, guard, 2)) { ok = false; break; }
+        for (int part = 0; ok && part < parts; ++part) {
+          const uint32_t d = tmem + set * BN;
+          if (!wait(acc_empty + 8 * set, set_parity, guard, 2)) { ok = false; break; }
           tc::tc_fence_after();
           const int b0 = END == kCeStats ? k0 + part * kPartBlocks : k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, k1) : k1;
-          for (int k = b0; k < b1; ++k, ++it) {
-            const uint32_t s = it % C::kStages, phase = (it / C::kStages) & 1;
-            if (!tc::mbar_wait(&sh.full[s], phase, guard, 3)) { ok = false; break; }
+          uint32_t accumulate = 0;
+          for (int k = b0; k < b1; ++k) {
+            if (!wait(full + 8 * slot, parity, guard, 3)) { ok = false; break; }
             tc::tc_fence_after();
             if (leader) {
-              const uint32_t addr = ring + s * C::kStageBytes;
-              const uint64_t a = operand_desc(addr, a_mn), b = operand_desc(addr + kABytes, BMN);
+              const uint64_t a = a_first + off, b = b_first + off;
 #pragma unroll
-              for (int i = 0; i < kBK / 16; ++i)
-                mma_ss<CG>(d, a + i * a_step, b + i * b_step, idesc, (k > b0 || i > 0) ? 1u : 0u);
-              commit<CG>(&sh.empty[s]);
+              for (int i = 0; i < kBK / 16; ++i) {
+                mma_ss<CG>(d, a + i * a_step, b + i * b_step, idesc, accumulate);
+                accumulate = 1;
+              }
+              commit<CG>(empty + 8 * slot);
             }
-            __syncwarp();
+            accumulate = 1;
+            off += C::kStageBytes >> 4;
+            if (++slot == C::kStages) slot = 0, parity ^= 1, off = 0;
           }
-          if (ok && leader) commit<CG>(&sh.acc_full[set]);
+          if (ok && leader) commit<CG>(acc_full + 8 * set);
           __syncwarp();
+          set ^= 1;
+          if (set == 0) set_parity ^= 1;
         }
       }
     }
@@ -549,13 +592,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       row_begin<END>(e, row, live && split == 1, st);
       const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
       if constexpr (END == kCeStats) {
-        const int parts = parts_of<END>(kb * ((int)(CG == 1 ? rank : 0) + 1) / split - kb * (int)(CG == 1 ? rank : 0) / split);
+        const int parts = parts_of<END>(k_from(kb, part_rank + 1) - k_from(kb, part_rank));
         float sum[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
         for (int part = 0; part < parts; ++part, ++sets) {
           const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16) + wg * kMine;
-          if (!tc::mbar_wait(&sh.acc_full[set], (sets >> 1) & 1, guard, 4)) { ok = false; break; }
+          if (!wait(tc::smem_u32(&sh.acc_full[set]), (sets >> 1) & 1, guard, 4)) { ok = false; break; }
           tc::tc_fence_after();
 #pragma unroll
           for (int c = 0; c < kMine; c += 16) {
@@ -586,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       } else {
         const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16);
         ++sets;
-        if (!tc::mbar_wait(&sh.acc_full[set], ((sets - 1) >> 1) & 1, guard, 4)) break;
+        if (!wait(tc::smem_u32(&sh.acc_full[set]), ((sets - 1) >> 1) & 1, guard, 4)) break;
         tc::tc_fence_after();
         if (split > 1) {
           if (warp_live) {

@@ -48,7 +48,7 @@ struct Shape { int cg, bn, split; };
 // Which tile.  The cost of a shape is its rounds of tiles times the time of a tile, which is K times the clocks of a
 // stage: 512 for 256 x 256 on a pair (MMA rate), 330 for 256 x 128 (operand traffic), 300 to 400 for 128 x 128 on one CTA.
 // A cluster that splits K pays for adding its parts up.
-Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, int count, bool paired, bool may_split, int sms) {
+Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, bool paired, bool may_split, int sms) {
   Shape best{2, 256, 1};
   double best_cost = 1e300;
   auto consider = [&](Shape s, double cost) {
@@ -59,7 +59,7 @@ Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, int count, 
     double work = 0;
     int64_t tiles = 0, longest = 0;
     for (int i = 0; i < count; ++i) {
-      const int64_t t = ceil_div(M[i], 256) * ceil_div(N[i], tile_n), kb = ceil_div(K[i], kBK);
+      const int64_t t = ceil_div(M[i], 256) * ceil_div(N[i], tile_n) * k_parts[i], kb = ceil_div(ceil_div(K[i], kBK), k_parts[i]);
       tiles += t;
       work += (double)t * kb;
       longest = kb > longest ? kb : longest;
@@ -87,10 +87,23 @@ int vec_of(const void* p, int64_t ld, int64_t extra = 0) {
 
 }  // namespace
 
+int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64_t K1) {
+  int sms = 148;
+  if (sm_count(&sms) != XKB_OK) sms = 148;
+  const int64_t pairs = sms / 2, tiles0 = ceil_div(M0, 256) * ceil_div(N0, 256), kb0 = ceil_div(K0, kBK);
+  const int64_t tiles1 = M1 > 0 ? ceil_div(M1, 256) * ceil_div(N1, 256) : 0, kb1 = ceil_div(K1, kBK);
+  // K blocks of a pair if all work is dealt out evenly, and of a pair with the most long tiles
+  const double even = (double)(tiles0 * kb0 + tiles1 * kb1) / (double)pairs;
+  int parts = 1;
+  while (parts < 32 && kb0 / (2 * parts) >= 16 && (double)ceil_div(tiles0 * parts, pairs) * ((double)kb0 / parts) > 1.1 * even) parts *= 2;
+  return parts;
+}
+
 int ce_parts(int64_t M, int64_t N, int64_t K) {
   int sms = 148;
   if (sm_count(&sms) != XKB_OK) sms = 148;
-  const Shape s = shape_of(&M, &N, &K, 1, false, true, sms);
+  const int one = 1;
+  const Shape s = shape_of(&M, &N, &K, &one, 1, false, true, sms);
   return (int)(ceil_div(N, s.bn) * s.split * 2);
 }
 
@@ -103,14 +116,17 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   if (rc != XKB_OK) return rc;
   const bool b_mn = products[0].b.k_rows;
   int64_t M[kMaxProblems], N[kMaxProblems], K[kMaxProblems];
-  bool any_a_mn = false;
+  int k_parts[kMaxProblems];
+  bool any_a_mn = false, parted = false;
   for (int i = 0; i < count; ++i) {
     M[i] = products[i].M, N[i] = products[i].N, K[i] = products[i].K;
     any_a_mn |= products[i].a.k_rows;
+    k_parts[i] = products[i].k_parts > 1 ? products[i].k_parts : 1;
+    parted |= k_parts[i] > 1;
     XKB_REQUIRE(M[i] > 0 && N[i] > 0 && K[i] > 0 && M[i] < (1ll << 30) && N[i] < (1ll << 30) && K[i] < (1ll << 30),
                 "dense products: sizes out of range");
   }
-  const Shape s = shape_of(M, N, K, count, end == kSwiglu, !any_a_mn, sms);
+  const Shape s = shape_of(M, N, K, k_parts, count, end == kSwiglu, !any_a_mn && !parted, sms);
   const int a_rows = s.cg == 1 && !any_a_mn && M[0] < kRows ? (int)align_up(M[0], 8) : kRows;
   const CUtensorMapDataType dt = dtype == XKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   p.count = count;
@@ -133,11 +149,12 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     d.live = q.live;
     d.live_is_k = d.a_mn = q.a.k_rows;
     d.group = 16;
+    d.k_parts = q.k_parts > 1 ? q.k_parts : 1;
     d.end = q.end;
     d.end.vec_out = vec_of(q.end.out, q.end.ld, end == kDswiglu ? q.end.half : 0);
     d.end.vec_h = vec_of(q.end.h, q.end.ld_h);
     d.end.vec_gu = vec_of(q.end.gate_up, q.end.ld_gu, q.end.half);
-    tiles += ceil_div(q.M, tile_m) * ceil_div(q.N, tile_n);
+    tiles += ceil_div(q.M, tile_m) * ceil_div(q.N, tile_n) * d.k_parts;
   }
   Launch l;
   l.cg = s.cg, l.bn = s.bn, l.split = s.split, l.chained = chained, l.stream = stream;

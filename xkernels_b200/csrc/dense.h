@@ -30,8 +30,8 @@ struct End {
   int64_t ld;
   const int32_t* row_map;   // row of `out` for every row of D, nullptr: the same
   const float* scale;       // factor of D on the device, nullptr: 1
-  float* acc;               // fp32 [M, acc_ld]
-  int64_t acc_ld;
+  float* acc;               // fp32 [k_parts, M, acc_ld]
+  int64_t acc_ld, acc_part; // acc_part: elements from one part to the next
   int acc_in, acc_out;      // add what acc holds; write there and not to out
   // kSwiglu, kDswiglu
   void* h;
@@ -42,7 +42,8 @@ struct End {
   float limit;
   // kCeStats, kCeGrad: arrays over the rows of D
   const int32_t* labels;
-  float2* part;             // [parts, part_ld]
+  const int64_t* labels64;  // kCeStats: in place of labels
+  float2* part;             // [M, parts]
   int64_t part_ld;
   float* given;
   const float4* coef;       // m, l, factor of p, what is taken off at the label
@@ -54,6 +55,7 @@ struct End {
 struct Product {
   Operand a, b;
   int64_t M, N, K;
+  int k_parts;          // kStore with acc_out: K is taken in so many parts, a tile each (0: one)
   const int32_t* live;  // on the device: how many of M's rows (of K's, if a.k_rows) there are, nullptr: all
   End end;
 };
@@ -61,6 +63,9 @@ struct Product {
 // Launches `count` products with the same end and the same orientation of B as one kernel.  `chained`: may start while
 // its predecessor on the stream runs (common.cuh); `early_b`: B is no output of a kernel of the same call.
 int launch(const Product* products, int count, int end, int dtype, bool chained, bool early_b, cudaStream_t stream);
+// In how many parts to take K of the first of two products [M0, N0, K0] (few long tiles) and [M1, N1, K1] (many short ones,
+// or none) that one launch deals out, so that the long ones do not outlast the rest.
+int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64_t K1);
 // How many pieces a row's statistics come in (kCeStats).
 int ce_parts(int64_t M, int64_t N, int64_t K);
 

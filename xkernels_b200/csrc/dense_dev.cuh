@@ -36,6 +36,7 @@ struct DevProduct {
   const int32_t* live;
   int live_is_k, a_mn;
   int group;          // row tiles that are walked side by side
+  int k_parts;
   End end;
 };
 
@@ -53,6 +54,7 @@ struct Shared {
   int abort_flag;
   uint32_t tmem;
   int m_tiles[kMaxProblems], n_tiles[kMaxProblems], kb[kMaxProblems], rows[kMaxProblems], first[kMaxProblems + 1];
+  int long_tiles, delta;
 };
 
 template <int CG, int BN> struct Cfg {
@@ -236,23 +238,31 @@ template <int END> __device__ __forceinline__ void row_begin(const End& e, int r
   if constexpr (END == kCeStats || END == kCeGrad) {
     st.m = -INFINITY;
     st.s = 0.f;
-    st.label = live ? e.labels[row] - e.col0 : -1;
+    st.label = -1;
+    if (live) {
+      if (END == kCeStats && e.labels64 != nullptr) {
+        const int64_t label = e.labels64[row];
+        st.label = label >= 0 && label < (1ll << 30) ? (int)label : -1;
+      } else {
+        st.label = e.labels[row] - e.col0;
+      }
+    }
     if constexpr (END == kCeGrad) st.coef = live ? e.coef[row] : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 template <int END> __device__ __forceinline__ void row_end(const End& e, int row, bool live, int part, const RowState& st) {
   if constexpr (END == kCeStats)
-    if (live) e.part[(int64_t)part * e.part_ld + row] = make_float2(st.m, st.s);
+    if (live) e.part[(int64_t)row * e.part_ld + part] = make_float2(st.m, st.s);
 }
 
 // v: columns col .. col + CW of D (kSwiglu: of gate, w: of up), n of which exist
 template <int END, int CW>
-__device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool live, int col, int n, float scale, float (&v)[CW],
+__device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool live, int kpart, int col, int n, float scale, float (&v)[CW],
                                           float (&w)[CW], RowState& st) {
   uint32_t o[CW / 2];
   if constexpr (END == kStore) {
     if (!live) return;
-    float4* acc = reinterpret_cast<float4*>(e.acc + (int64_t)row * e.acc_ld + col);
+    float4* acc = reinterpret_cast<float4*>(e.acc + kpart * e.acc_part + (int64_t)row * e.acc_ld + col);
     if (e.acc_in) {
 #pragma unroll
       for (int j = 0; j < CW; j += 4) {
@@ -379,16 +389,29 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool l
 }
 
 // ---- the kernel ----------------------------------------------------------------------------------------------
-struct Tile { int prod, m, n; };
+struct Tile { int prod, m, n, kpart; };
 
-__device__ __forceinline__ bool tile_of(const Params& p, const Shared& sh, int t, Tile& out) {
+// The i-th tile of a cluster; false: there is none.
+__device__ __forceinline__ bool tile_of(const Params& p, const Shared& sh, int i, int cluster, int clusters, Tile& out) {
+  const int full = sh.long_tiles / clusters, rest = sh.long_tiles - full * clusters, more = cluster < rest ? 1 : 0;
+  int t;
+  if (i < full + more) {
+    t = i * clusters + cluster;
+  } else {
+    const int r = i - full - (more ? 1 - sh.delta : 0);       // round of the other tiles
+    t = sh.long_tiles + (r < sh.delta ? r * (clusters - rest) + cluster - rest
+                                      : sh.delta * (clusters - rest) + (r - sh.delta) * clusters + cluster);
+  }
   if (t >= sh.first[p.count]) return false;
-  int i = 0;
-  while (i + 1 < p.count && t >= sh.first[i + 1]) ++i;
-  const int r = t - sh.first[i], G = p.prod[i].group, nt = sh.n_tiles[i];
+  int q = 0;
+  while (q + 1 < p.count && t >= sh.first[q + 1]) ++q;
+  int r = t - sh.first[q];
+  const int G = p.prod[q].group, nt = sh.n_tiles[q], each = nt * sh.m_tiles[q];
+  out.kpart = 0;
+  if (p.prod[q].k_parts > 1) out.kpart = r / each, r -= out.kpart * each;
   const int g = r / (G * nt), in = r - g * G * nt;
-  const int wide = min(G, sh.m_tiles[i] - g * G);
-  out.prod = i;
+  const int wide = min(G, sh.m_tiles[q] - g * G);
+  out.prod = q;
   out.n = in / wide;
   out.m = g * G + (in - out.n * wide);
   return true;
@@ -436,9 +459,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       sh.n_tiles[i] = (q.N + kTileN - 1) / kTileN;
       sh.kb[i] = (K + kBK - 1) / kBK;
       sh.first[i] = first;
-      first += sh.m_tiles[i] * sh.n_tiles[i];
+      first += sh.m_tiles[i] * sh.n_tiles[i] * q.k_parts;
     }
     sh.first[p.count] = first;
+    // The first product's tiles may be longer than the others': the clusters that have one of them more leave out as many
+    // rounds of the others.
+    sh.long_tiles = p.count > 1 ? sh.first[1] : 0;
+    sh.delta = 1;
+    if (p.count > 1) sh.delta = max(1, (sh.kb[0] / p.prod[0].k_parts + sh.kb[1] / 2) / max(1, sh.kb[1]));
     for (int i = 0; i < p.count; ++i) {
       tc::prefetch_tensormap(&p.prod[i].a);
       tc::prefetch_tensormap(&p.prod[i].b);
@@ -451,8 +479,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   tc::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  const uint32_t part_rank = CG == 1 ? rank : 0;      // which part of K
-  auto k_from = [&](int kb, uint32_t r) { return split == 1 ? (r == 0 ? 0 : kb) : kb * (int)r / split; };
+  // blocks of K of a tile: its part, or what the cluster leaves to this CTA
+  auto k_range = [&](const Tile& t, int& k0, int& k1) {
+    const int kb = sh.kb[t.prod], parts = CG == 1 && split > 1 ? split : p.prod[t.prod].k_parts;
+    const int part = CG == 1 && split > 1 ? (int)rank : t.kpart;
+    k0 = parts == 1 ? 0 : kb * part / parts;
+    k1 = parts == 1 ? kb : kb * (part + 1) / parts;
+  };
   if (warp == 0 || warp == 3) {
     // Warp 0 feeds A, warp 3 feeds B.  The whole warp runs the loop and one lane issues: operands then sit in uniform
     // registers (in a loop of one lane a copy took its issuer 200 clocks, and both operands' 600 a stage where the MMAs
@@ -470,10 +503,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       if (++slot == C::kStages) slot = 0, parity ^= 1, dst -= C::kStages * C::kStageBytes;
     };
     Tile t;
-    for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+    for (int at = 0; ok && tile_of(p, sh, at, cluster, clusters, t); ++at) {
       const DevProduct& q = p.prod[t.prod];
-      const int kb = sh.kb[t.prod];
-      const int k0 = k_from(kb, part_rank), k1 = k_from(kb, part_rank + 1);
+      int k0, k1;
+      k_range(t, k0, k1);
       if (feeds_a) {
         const CUtensorMap* map = &q.a;
         const int m0 = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0);
@@ -529,13 +562,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       uint32_t slot = 0, parity = 0, off = 0, set = 0, set_parity = 1;
       Tile t;
       bool ok = true;
-      for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+      for (int at = 0; ok && tile_of(p, sh, at, cluster, clusters, t); ++at) {
         const bool a_mn = p.prod[t.prod].a_mn != 0;
         const uint64_t a_first = operand_desc(ring, a_mn);
         const uint32_t idesc = base_idesc | ((a_mn ? 1u : 0u) << 15);
         const uint32_t a_step = a_mn ? 128 : 2, b_step = BMN ? 128 : 2;    // 16 K further, in units of 16 bytes
-        const int kb = sh.kb[t.prod];
-        const int k0 = k_from(kb, part_rank), k1 = k_from(kb, part_rank + 1);
+        int k0, k1;
+        k_range(t, k0, k1);
         const int parts = parts_of<END>(k1 - k0);
         for (int part = 0; ok && part < parts; ++part) {
           const uint32_t d = tmem + set * BN;
@@ -574,9 +607,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     uint32_t sets = 0;
     Tile t;
     bool ok = true;
-    for (int at = cluster; ok && tile_of(p, sh, at, t); at += clusters) {
+    for (int at = 0; ok && tile_of(p, sh, at, cluster, clusters, t); ++at) {
       const End& e = p.prod[t.prod].end;
-      const int N = p.prod[t.prod].N, kb = sh.kb[t.prod];
+      const int N = p.prod[t.prod].N;
+      int k0, k1;
+      k_range(t, k0, k1);
       const int row = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0) + in_tile;
       const bool live = row < sh.rows[t.prod];
       const bool warp_live = row - lane < sh.rows[t.prod];
@@ -592,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       row_begin<END>(e, row, live && split == 1, st);
       const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
       if constexpr (END == kCeStats) {
-        const int parts = parts_of<END>(k_from(kb, part_rank + 1) - k_from(kb, part_rank));
+        const int parts = parts_of<END>(k1 - k0);
         float sum[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
@@ -623,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-          if (N - col > 0) row_piece<END, 32>(e, p.fmt, row, live, col, N - col, scale, v, v, st);
+          if (N - col > 0) row_piece<END, 32>(e, p.fmt, row, live, t.kpart, col, N - col, scale, v, v, st);
         }
         row_end<END>(e, row, live, t.n * 2 + wg, st);
       } else {
@@ -651,11 +686,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           tmem_ld32(from + c, v);
           if constexpr (kPaired) tmem_ld32(from + BN / 2 + c, w);
           tc::tmem_wait_ld();
-          if (kb == 0) {
+          if (k1 == k0) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = w[j] = 0.f;
           }
-          row_piece<END, 32>(e, p.fmt, row, live, col, n, scale, v, w, st);
+          row_piece<END, 32>(e, p.fmt, row, live, t.kpart, col, n, scale, v, w, st);
         }
         hand_back(set);
       }
@@ -666,7 +701,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   if (split > 1) {
     cluster_sync();       // every CTA's part is in its shared memory
     Tile t;
-    if (warp >= 4 && tile_of(p, sh, cluster, t) && !guard.aborted()) {
+    if (warp >= 4 && tile_of(p, sh, 0, cluster, clusters, t) && !guard.aborted()) {
       const End& e = p.prod[t.prod].end;
       const int wg = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
       const int row = t.m * kRows + in_tile;
@@ -691,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               if constexpr (kPaired) w[j] += ld_cluster(base + (BN / 2 + j) * kRows * 4);
             }
           }
-          row_piece<END, 8>(e, p.fmt, row, live, col, n, scale, v, w, st);
+          row_piece<END, 8>(e, p.fmt, row, live, t.kpart, col, n, scale, v, w, st);
         }
         row_end<END>(e, row, live, (t.n * split + (int)rank) * 2 + wg, st);
       } else if (END == kCeGrad && t.m * kRows < sh.rows[t.prod]) {
@@ -705,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           float v[8], w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
-          row_piece<END, 8>(e, p.fmt, row, false, col, n, 1.f, v, w, st);
+          row_piece<END, 8>(e, p.fmt, row, false, t.kpart, col, n, 1.f, v, w, st);
         }
       }
     }

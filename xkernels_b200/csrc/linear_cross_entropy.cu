@@ -19,8 +19,10 @@ int run_ce(int end, const Params& p, const Launch& l) {
 
 namespace {
 
-constexpr int kListThreads = 256;
-constexpr int kJoinThreads = 512;
+constexpr int kListThreads = 512;
+constexpr int kListBlocks = 296;                    // two on every SM
+constexpr int kSegment = 2048;                      // elements of a row that a warp copies at a time: eight loads a lane in flight
+constexpr int kJoinThreads = 128;
 constexpr int kRowPad = 256;                       // rows of the row arrays are a multiple of this
 constexpr int64_t kPieceBytes = 256ll << 20;       // of the logits' gradient that is held at a time
 
@@ -37,7 +39,7 @@ struct ListArgs {
   const void* hidden;
   int64_t ld, ld_x;
   const void* labels;
-  int ids64, vec;
+  int ids64, vec, vec_grad;
   int64_t M, H, V;
   const float* stats;
   const float *g_loss, *g_lse;
@@ -53,14 +55,18 @@ __device__ __forceinline__ float size_at(const ListArgs& a, int64_t i) {
   return (a.g_loss != nullptr ? fabsf(a.g_loss[i]) : 0.f) + (a.g_lse != nullptr ? fabsf(a.g_lse[i]) : 0.f);
 }
 
-// A block has some rows in a line.  It counts the labels before them itself (all blocks read all labels, from L2).
-__global__ void __launch_bounds__(kListThreads) list_rows_kernel(const ListArgs a) {
-  __shared__ int warp_sum[2][kListThreads / 32];
-  __shared__ float warp_top[kListThreads / 32];
+// A block has some rows in a line, or with few rows a part of the columns of one.  It counts the labels before them itself
+// (all blocks read all labels, from L2).  Bound by the latency of the copies.
+__global__ void __launch_bounds__(kListThreads) list_rows_kernel(const ListArgs a, const int col_blocks) {
+  chain_trigger();
+  constexpr int kWarps = kListThreads / 32;
+  __shared__ int warp_sum[2][kWarps];
+  __shared__ float warp_top[kWarps];
   __shared__ int place[kListThreads];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = kListThreads / 32;
-  const int64_t per = (a.M + gridDim.x - 1) / gridDim.x;
-  const int64_t r0 = min((int64_t)blockIdx.x * per, a.M), r1 = min(r0 + per, a.M);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row_blocks = gridDim.x / col_blocks, block = blockIdx.x / col_blocks, col_block = blockIdx.x - block * col_blocks;
+  const int64_t per = (a.M + row_blocks - 1) / row_blocks;
+  const int64_t r0 = min((int64_t)block * per, a.M), r1 = min(r0 + per, a.M);
   int before = 0, all = 0;
   float top = 0.f;
   for (int64_t i = tid; i < a.M; i += kListThreads) {
@@ -78,7 +84,7 @@ __global__ void __launch_bounds__(kListThreads) list_rows_kernel(const ListArgs 
   __syncthreads();
   before = all = 0;
   top = 0.f;
-  for (int w = 0; w < warps; ++w) before += warp_sum[0][w], all += warp_sum[1][w], top = max_nan(top, warp_top[w]);
+  for (int w = 0; w < kWarps; ++w) before += warp_sum[0][w], all += warp_sum[1][w], top = max_nan(top, warp_top[w]);
   // fp16 gradients of the logits: times the power of two that brings the largest factor to 2^10 .. 2^11, so that the small
   // probabilities of a large vocabulary do not fall below fp16's steps (2^-24).  |d| <= 2 |a| + |b|: no overflow.
   float scale = 1.f, inv = 1.f;
@@ -92,14 +98,26 @@ __global__ void __launch_bounds__(kListThreads) list_rows_kernel(const ListArgs 
     *a.r.count = all;
     *a.r.inv_scale = inv;
   }
-  // rows of x, a warp each; out: 16 bytes aligned, ld_x a multiple of 8
-  auto copy = [&](const uint16_t* from, uint16_t* to) {
-    if (from == nullptr) {
-      for (int64_t c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
-    } else if (a.vec) {
-      for (int64_t c = lane * 8; c < a.H; c += 256) *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
+  const int segments = (int)((a.H + kSegment - 1) / kSegment);
+  const int mine = (segments - col_block + col_blocks - 1) / col_blocks;     // segments col_block, col_block + col_blocks, ..
+  // a segment of a row of x, by a warp; from nullptr: zeros.  The rows there start on 16 bytes.
+  auto copy = [&](const uint16_t* from, uint16_t* to, int segment) {
+    const int64_t c0 = (int64_t)segment * kSegment;
+    if (from == nullptr || a.vec) {
+      uint4 v[kSegment / 256];
+#pragma unroll
+      for (int j = 0; j < kSegment / 256; ++j) {
+        const int64_t c = c0 + j * 256 + lane * 8;
+        v[j] = from != nullptr && c < a.H ? *reinterpret_cast<const uint4*>(from + c) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < kSegment / 256; ++j) {
+        const int64_t c = c0 + j * 256 + lane * 8;
+        if (c < a.H) *reinterpret_cast<uint4*>(to + c) = v[j];
+      }
     } else {
-      for (int64_t c = lane; c < a.H; c += 32) to[c] = from[c];
+#pragma unroll 8
+      for (int64_t c = c0 + lane; c < min(c0 + kSegment, a.H); c += 32) to[c] = from[c];
     }
   };
   for (int64_t base = r0; base < r1; base += kListThreads) {
@@ -111,12 +129,12 @@ __global__ void __launch_bounds__(kListThreads) list_rows_kernel(const ListArgs 
     if (lane == 0) warp_sum[0][warp] = __popc(vote);
     __syncthreads();
     int at = before + __popc(vote & ((1u << lane) - 1));
-    for (int w = 0; w < warps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       if (w < warp) at += warp_sum[0][w];
       before += warp_sum[0][w];
     }
     place[tid] = on ? at : -1;
-    if (on) {
+    if (on && col_block == 0) {
       a.r.rows[at] = (int32_t)i;
       a.r.labels[at] = (int32_t)(label < a.V ? label : a.V);
       if (a.stats != nullptr) {
@@ -129,71 +147,111 @@ __global__ void __launch_bounds__(kListThreads) list_rows_kernel(const ListArgs 
     }
     __syncthreads();
     const int n = (int)min((int64_t)kListThreads, r1 - base);
-    for (int j = warp; j < n; j += warps) {
+    for (int u = warp; u < n * mine; u += kWarps) {
+      const int j = u / mine, segment = (u - j * mine) * col_blocks + col_block;
       if (place[j] >= 0) {
-        copy(static_cast<const uint16_t*>(a.hidden) + (base + j) * a.ld, a.r.x + (int64_t)place[j] * a.ld_x);
+        copy(static_cast<const uint16_t*>(a.hidden) + (base + j) * a.ld, a.r.x + (int64_t)place[j] * a.ld_x, segment);
       } else if (a.grad_hidden != nullptr) {
-        for (int64_t c = lane; c < a.H; c += 32) a.grad_hidden[(base + j) * a.H + c] = 0;
+        const int64_t c0 = (int64_t)segment * kSegment, c1 = min(c0 + kSegment, a.H);
+        uint16_t* to = a.grad_hidden + (base + j) * a.H;
+        if (a.vec_grad) for (int64_t c = c0 + lane * 8; c < c1; c += 256) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+        else for (int64_t c = c0 + lane; c < c1; c += 32) to[c] = 0;
       }
     }
   }
   // behind the last row: zeros, as far as a product may read
   const int64_t pad = (all + kRowPad - 1) / kRowPad * kRowPad;
-  for (int64_t j = all + blockIdx.x * warps + warp; j < pad; j += (int64_t)gridDim.x * warps) copy(nullptr, a.r.x + j * a.ld_x);
+  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < (pad - all) * segments; u += (int64_t)gridDim.x * kWarps) {
+    const int64_t j = u / segments;
+    copy(nullptr, a.r.x + (all + j) * a.ld_x, (int)(u - j * segments));
+  }
 }
 
 struct JoinArgs {
   const float2* part;
   int parts;
-  int64_t part_ld;
   const float* given;
-  const int32_t *count, *rows, *labels_of_rows;
+  const int32_t *count, *rows;     // nullptr: the rows are the batch's
   const void* labels;
   int ids64;
   int64_t M, V;
   float *loss, *lse, *stats;
 };
 
-// Lane = row (32 rows a block), the warps share its pieces.  Blocks beyond the rows' write the padding rows' zeros.
+// A block a row: thread = piece of the vocabulary, in turn.  Block i also writes the zeros of row i of the batch if it is padding.
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinArgs a) {
   chain_wait();
   constexpr int kWarps = kJoinThreads / 32;
-  __shared__ float sm[kWarps][33], ss[kWarps][33];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t i = (int64_t)blockIdx.x * 32 + lane;      // row of the batch, for the padding; of the list, for the rest
-  if (warp == 0 && i < a.M) {
-    const int64_t label = a.ids64 ? static_cast<const int64_t*>(a.labels)[i] : (int64_t)static_cast<const int32_t*>(a.labels)[i];
-    if (label < 0) a.loss[i] = a.lse[i] = a.stats[2 * i] = a.stats[2 * i + 1] = 0.f;
-  }
-  const int count = *a.count;
-  if ((int64_t)blockIdx.x * 32 >= count) return;
-  const bool on = i < count;
+  __shared__ float sm[kWarps], ss[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t i = blockIdx.x;
+  auto label_of = [&](int64_t r) {
+    return a.ids64 ? static_cast<const int64_t*>(a.labels)[r] : (int64_t)static_cast<const int32_t*>(a.labels)[r];
+  };
+  const bool padding = label_of(i) < 0;
+  if (padding && tid == 0) a.loss[i] = a.lse[i] = a.stats[2 * i] = a.stats[2 * i + 1] = 0.f;
+  if (a.count != nullptr ? i >= *a.count : padding) return;
+  const float2* part = a.part + i * a.parts;
   float m = -INFINITY, s = 0.f;
-  if (on) {
-    for (int q = warp; q < a.parts; q += kWarps) m = fmaxf(m, a.part[q * a.part_ld + i].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    for (int q = warp; q < a.parts; q += kWarps) {
-      const float2 f = a.part[q * a.part_ld + i];
-      s += f.y * exp2_fast((f.x - ref) * kLog2e);
+  for (int q = tid; q < a.parts; q += kJoinThreads) {
+    const float2 f = part[q];
+    const float top = fmaxf(m, f.x), ref = top == -INFINITY ? 0.f : top;
+    // (a piece without a live logit: exp2(-inf) = 0; a NaN or +inf in the row has made its piece's sum a NaN)
+    s = s * exp2_fast((m - ref) * kLog2e) + f.y * exp2_fast((f.x - ref) * kLog2e);
+    m = top;
+  }
+  float top = m;
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  if (lane == 0) sm[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  s = warp_add(s * exp2_fast((m - ref) * kLog2e));
+  if (lane == 0) ss[warp] = s;
+  __syncthreads();
+  if (tid != 0) return;
+  s = 0.f;
+  for (int w = 0; w < kWarps; ++w) s += ss[w];
+  const bool dead = top == -INFINITY && s == 0.f;      // no live logit
+  const float l = dead ? 0.f : logf(s);
+  const int64_t to = a.rows != nullptr ? a.rows[i] : i;
+  a.loss[to] = label_of(to) >= a.V ? NAN : dead ? INFINITY : (top - a.given[i]) + l;
+  a.lse[to] = top + l;
+  a.stats[2 * to] = top;
+  a.stats[2 * to + 1] = l;
+}
+
+struct AddArgs {
+  const float* acc;
+  int64_t acc_ld, acc_part, H;
+  int parts, fmt, vec;
+  const int32_t *count, *rows;
+  const float* scale;
+  uint16_t* out;
+};
+
+// The parts of grad_hidden added up in their order, a block a row.
+__global__ void __launch_bounds__(256) add_parts_kernel(const AddArgs a) {
+  chain_wait();
+  const int64_t i = blockIdx.x;
+  if (i >= *a.count) return;
+  const float scale = *a.scale;
+  uint16_t* to = a.out + (int64_t)a.rows[i] * a.H;
+  for (int64_t c = threadIdx.x * 4; c < a.H; c += 1024) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < a.parts; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(a.acc + q * a.acc_part + i * a.acc_ld + c);
+      s.x += f.x, s.y += f.y, s.z += f.z, s.w += f.w;
+    }
+    const uint32_t lo = dense::pack16(a.fmt, s.x * scale, s.y * scale), hi = dense::pack16(a.fmt, s.z * scale, s.w * scale);
+    if (a.vec) {
+      *reinterpret_cast<uint2*>(to + c) = make_uint2(lo, hi);
+    } else {
+      const uint32_t w[2] = {lo, hi};
+      for (int j = 0; j < 4; ++j)
+        if (c + j < a.H) to[c + j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
     }
   }
-  sm[warp][lane] = m;
-  ss[warp][lane] = s;
-  __syncthreads();
-  if (warp != 0 || !on) return;
-  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm[w][lane]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  s = 0.f;
-  for (int w = 0; w < kWarps; ++w) s += ss[w][lane] * exp2_fast((sm[w][lane] - ref) * kLog2e);
-  // (a piece whose maximum is below all: exp2(-inf) = 0; a NaN or +inf in the row has made its sum a NaN)
-  const bool dead = m == -INFINITY && s == 0.f;      // no live logit
-  const float l = dead ? 0.f : logf(s);
-  const int64_t to = a.rows[i];
-  const bool known = a.labels_of_rows[i] < a.V;
-  a.loss[to] = !known ? NAN : dead ? INFINITY : (m - a.given[i]) + l;
-  a.lse[to] = m + l;
-  a.stats[2 * to] = m;
-  a.stats[2 * to + 1] = l;
 }
 
 int64_t padded(int64_t M) { return align_up(M, kRowPad); }
@@ -220,6 +278,7 @@ struct Work {
   float* given;
   uint16_t* d;
   float* acc;
+  int k_parts;
   int64_t bytes;
 };
 
@@ -236,7 +295,9 @@ Work carve(void* ws, int64_t M, int64_t H, int64_t V, bool backward) {
     w.r.coef = c.take<float4>(P);
     const int64_t piece = piece_of(M, V);
     w.d = c.take<uint16_t>(P * piece);
-    if (piece < V) w.acc = c.take<float>(P * align_up(H, 32));
+    const int64_t n = V < piece ? V : piece;
+    w.k_parts = dense::k_parts_of(M, H, n, n, H, M);
+    if (piece < V || w.k_parts > 1) w.acc = c.take<float>(w.k_parts * P * align_up(H, 32));
   } else {
     w.given = c.take<float>(P);
     w.part = c.take<float2>(dense::ce_parts(M, V, H) * P);
@@ -264,8 +325,9 @@ int check_inputs(const char* name, const void* hidden, int64_t ld_h, const void*
 }
 
 int launch_list(const ListArgs& a, cudaStream_t stream) {
-  const int64_t blocks = a.M < 296 ? a.M : 296;
-  list_rows_kernel<<<(unsigned)blocks, kListThreads, 0, stream>>>(a);
+  const int64_t row_blocks = a.M < kListBlocks ? a.M : kListBlocks, segments = ceil_div(a.H, kSegment);
+  const int64_t spare = kListBlocks / row_blocks, col_blocks = spare < segments ? spare : segments;
+  list_rows_kernel<<<(unsigned)(row_blocks * col_blocks), kListThreads, 0, stream>>>(a, (int)col_blocks);
   XKB_CHECK_LAUNCH("list_rows_kernel");
   return XKB_OK;
 }
@@ -298,28 +360,38 @@ extern "C" int xkb_linear_cross_entropy(const void* hidden, int64_t ld_hidden, i
   const Work w = carve(workspace, M, H, V, false);
   XKB_TRY(check_workspace(name, workspace, workspace_bytes, w.bytes));
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  ListArgs a = {};
-  a.hidden = hidden, a.ld = ld_hidden, a.ld_x = pitch8(H);
-  a.labels = labels, a.ids64 = ids64;
-  a.vec = reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && ld_hidden % 8 == 0 && H % 8 == 0;
-  a.M = M, a.H = H, a.V = V;
-  a.r = w.r;
-  XKB_TRY(launch_list(a, stream));
+  const bool aligned = reinterpret_cast<uintptr_t>(hidden) % 16 == 0 && ld_hidden % 8 == 0;
+  // One row tile takes as long whatever it holds: the hidden states are then read where they are (listing and copying cost 4 us).
+  const bool in_place = M <= dense::kRows && aligned && ld_hidden >= H;
   dense::Product q = {};
-  q.a = {w.r.x, pitch8(H), false, 0, padded(M), H};
   q.b = {weight, ld_weight, false, 0, V, H};
   q.M = M, q.N = V, q.K = H;
-  q.live = w.r.count;
-  q.end.labels = w.r.labels;
-  q.end.part = w.part, q.end.part_ld = padded(M);
+  const int parts = dense::ce_parts(M, V, H);
+  q.end.part = w.part, q.end.part_ld = parts;
   q.end.given = w.given;
-  XKB_TRY(dense::launch(&q, 1, dense::kCeStats, dtype, true, false, stream));
   JoinArgs j = {};
-  j.part = w.part, j.parts = dense::ce_parts(M, V, H), j.part_ld = padded(M);
-  j.given = w.given, j.count = w.r.count, j.rows = w.r.rows, j.labels_of_rows = w.r.labels;
+  if (in_place) {
+    q.a = {hidden, ld_hidden, false, 0, M, H};
+    if (ids64) q.end.labels64 = static_cast<const int64_t*>(labels);
+    else q.end.labels = static_cast<const int32_t*>(labels);
+  } else {
+    ListArgs a = {};
+    a.hidden = hidden, a.ld = ld_hidden, a.ld_x = pitch8(H);
+    a.labels = labels, a.ids64 = ids64;
+    a.vec = aligned && H % 8 == 0;
+    a.M = M, a.H = H, a.V = V;
+    a.r = w.r;
+    XKB_TRY(launch_list(a, stream));
+    q.a = {w.r.x, pitch8(H), false, 0, padded(M), H};
+    q.live = w.r.count;
+    q.end.labels = w.r.labels;
+    j.count = w.r.count, j.rows = w.r.rows;
+  }
+  XKB_TRY(dense::launch(&q, 1, dense::kCeStats, dtype, !in_place, false, stream));
+  j.part = w.part, j.parts = parts, j.given = w.given;
   j.labels = labels, j.ids64 = ids64, j.M = M, j.V = V;
   j.loss = loss, j.lse = lse, j.stats = stats;
-  XKB_CHECK_CUDA(launch_chained(join_kernel, dim3((unsigned)ceil_div(M, 32)), dim3(kJoinThreads), 0, stream, j));
+  XKB_CHECK_CUDA(launch_chained(join_kernel, dim3((unsigned)M), dim3(kJoinThreads), 0, stream, j));
   XKB_CHECK_LAUNCH("join_kernel");
   return XKB_OK;
 }
@@ -355,6 +427,7 @@ extern "C" int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_
   a.stats = stats, a.g_loss = grad_loss, a.g_lse = grad_lse;
   a.fp16 = dtype == XKB_F16;
   a.grad_hidden = static_cast<uint16_t*>(grad_hidden);
+  a.vec_grad = reinterpret_cast<uintptr_t>(grad_hidden) % 16 == 0 && H % 8 == 0;
   a.r = w.r;
   XKB_TRY(launch_list(a, stream));
   const int64_t piece = piece_of(M, V);
@@ -379,8 +452,9 @@ extern "C" int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_
       g.live = w.r.count;
       g.end.out = grad_hidden, g.end.ld = H;
       g.end.row_map = w.r.rows;
-      g.end.acc = w.acc, g.end.acc_ld = align_up(H, 32);
-      g.end.acc_in = v0 > 0, g.end.acc_out = v0 + n < V;
+      g.k_parts = w.k_parts;
+      g.end.acc = w.acc, g.end.acc_ld = align_up(H, 32), g.end.acc_part = padded(M) * align_up(H, 32);
+      g.end.acc_in = v0 > 0, g.end.acc_out = v0 + n < V || w.k_parts > 1;
       if (!g.end.acc_out) g.end.scale = w.r.inv_scale;
     }
     if (grad_weight != nullptr) {
@@ -393,6 +467,16 @@ extern "C" int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_
       g.end.scale = w.r.inv_scale;
     }
     XKB_TRY(dense::launch(q, count, dense::kStore, dtype, true, false, stream));
+  }
+  if (grad_hidden != nullptr && w.k_parts > 1) {
+    AddArgs s = {};
+    s.acc = w.acc, s.acc_ld = align_up(H, 32), s.acc_part = padded(M) * align_up(H, 32), s.H = H;
+    s.parts = w.k_parts, s.fmt = dtype == XKB_BF16 ? 1 : 0;
+    s.vec = reinterpret_cast<uintptr_t>(grad_hidden) % 8 == 0 && H % 4 == 0;
+    s.count = w.r.count, s.rows = w.r.rows, s.scale = w.r.inv_scale;
+    s.out = static_cast<uint16_t*>(grad_hidden);
+    XKB_CHECK_CUDA(launch_chained(add_parts_kernel, dim3((unsigned)M), dim3(256), 0, stream, s));
+    XKB_CHECK_LAUNCH("add_parts_kernel");
   }
   return XKB_OK;
 }

@@ -82,7 +82,7 @@ Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* 
 
 int vec_of(const void* p, int64_t ld, int64_t extra = 0) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * 2) | (uintptr_t)(extra * 2);
-  return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
+  return bits % 16 == 0 ? 16 : 2;
 }
 
 }  // namespace

@@ -48,7 +48,7 @@ struct End {
   float* given;
   const float4* coef;       // m, l, factor of p, what is taken off at the label
   int col0;                 // first column of the piece in the vocabulary
-  // which vector accesses their rows allow (bytes: 32, 16, or 2), set by the launcher
+  // which vector accesses their rows allow (bytes: 16 or 2), set by the launcher
   int vec_out, vec_h, vec_gu;
 };
 

@@ -21,6 +21,7 @@ constexpr int kRows = 128;          // rows of D per CTA
 constexpr int kThreads = 384;       // warps 0: TMA, 1: MMA, 2: tensor memory, 4 to 11: read-out
 constexpr int kReadWarps = 8;
 constexpr int kABytes = kRows * 128;
+constexpr int kRowsOut = 32 * 64;   // a warp's 32 rows of 64 bytes on their way to or from memory
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
 // The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, so a long sum drifts towards 0
 // (2^-24 of it a step of 16 K: 5e-6 of the logits at K = 7168).  Where the result stays fp32 (kCeStats) an accumulator takes
@@ -54,14 +55,15 @@ struct Shared {
   int abort_flag;
   uint32_t tmem;
   int m_tiles[kMaxProblems], n_tiles[kMaxProblems], kb[kMaxProblems], rows[kMaxProblems], first[kMaxProblems + 1];
-  int long_tiles, delta;
+  int long_tiles, delta, rest;
+  uint32_t strip_inv[kMaxProblems], group_inv[kMaxProblems], last_inv[kMaxProblems];
 };
 
 template <int CG, int BN> struct Cfg {
   static constexpr int kBBytes = BN / CG * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = (225 * 1024 / kStageBytes) < 8 ? (225 * 1024 / kStageBytes) : 8;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static constexpr int kStages = (209 * 1024 / kStageBytes) < 8 ? (209 * 1024 / kStageBytes) : 8;
+  static constexpr int kSmem = kStages * kStageBytes + kReadWarps * kRowsOut + 1024;
   static_assert(kStages >= 4 && kStages <= 8, "");
 };
 
@@ -195,13 +197,7 @@ __device__ __forceinline__ void unpack16(int fmt, uint32_t p, float& lo, float& 
 // CW consecutive elements of a row, the first n of which exist; vec: what the addresses allow.
 template <int CW> __device__ __forceinline__ void store_row(void* base, int64_t at, const uint32_t (&w)[CW / 2], int n, int vec) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
-  if (n >= CW && CW % 16 == 0 && vec == 32) {
-#pragma unroll
-    for (int i = 0; i < CW / 2; i += 8)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                   ::"l"(p + 2 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
-                     "r"(w[i + 7]) : "memory");
-  } else if (n >= CW && vec >= 16) {
+  if (n >= CW && vec >= 16) {
 #pragma unroll
     for (int i = 0; i < CW / 2; i += 4) *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   } else {
@@ -225,6 +221,58 @@ template <int CW> __device__ __forceinline__ void load_row(const void* base, int
   }
 }
 
+// 64 bytes of 32 rows, lane = row, to memory: through shared memory, so that four lanes write a row's 64 bytes side by side
+// (a lane that writes its own row touches one sector of 32 lines an instruction: 3500 clocks a tile of 128 x 128 where this
+// takes 900).  to: this lane's row, 16-byte aligned; nullptr: not written.  All lanes of the warp call.
+__device__ __forceinline__ uint32_t rows_at(uint32_t buf, int row, int unit) { return buf + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4); }
+__device__ __forceinline__ void rows_out(uint32_t buf, void* to, const uint32_t* w) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(rows_at(buf, lane, u)), "r"(w[4 * u]), "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3]) : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + (lane >> 2);
+    char* p = reinterpret_cast<char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(to), row));
+    const uint4 v = tc::lds128(rows_at(buf, row, lane & 3));
+    if (p != nullptr) *reinterpret_cast<uint4*>(p + (lane & 3) * 16) = v;
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void rows_in(uint32_t buf, const void* from, uint32_t* w) {
+  const int lane = threadIdx.x & 31;
+  uint4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const char* p = reinterpret_cast<const char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(from), i * 8 + (lane >> 2)));
+    v[i] = p != nullptr ? *reinterpret_cast<const uint4*>(p + (lane & 3) * 16) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(rows_at(buf, i * 8 + (lane >> 2), lane & 3)), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w) : "memory");
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint4 x = tc::lds128(rows_at(buf, lane, u));
+    w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
+  }
+  __syncwarp();
+}
+// CW columns of this lane's row: together where whole pieces of 32 are aligned, else each lane its own.
+template <int CW>
+__device__ __forceinline__ void put_row(uint32_t buf, void* base, int64_t at, bool live, const uint32_t (&w)[CW / 2], int n, int vec) {
+  if (CW == 32 && n >= CW && vec >= 16) rows_out(buf, live ? static_cast<uint16_t*>(base) + at : nullptr, w);
+  else if (live) store_row<CW>(base, at, w, n, vec);
+}
+template <int CW>
+__device__ __forceinline__ void get_row(uint32_t buf, const void* base, int64_t at, bool live, uint32_t (&w)[CW / 2], int n, int vec) {
+  if (CW == 32 && n >= CW && vec >= 16) rows_in(buf, live ? static_cast<const uint16_t*>(base) + at : nullptr, w);
+  else if (live) load_row<CW>(base, at, w, n, vec);
+}
+
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + exp2_fast(-kLog2e * x)); }
 
 // ---- what becomes of CW columns of a row ---------------------------------------------------------------------
@@ -232,6 +280,7 @@ struct RowState {
   float m, s;       // kCeStats: maximum so far, sum of exponentials against it
   int label;        // column of the label within the piece
   float4 coef;      // kCeGrad
+  int64_t to;       // kStore: row of `out`
 };
 
 template <int END> __device__ __forceinline__ void row_begin(const End& e, int row, bool live, RowState& st) {
@@ -249,6 +298,7 @@ template <int END> __device__ __forceinline__ void row_begin(const End& e, int r
     }
     if constexpr (END == kCeGrad) st.coef = live ? e.coef[row] : make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  if constexpr (END == kStore) st.to = live && e.row_map != nullptr ? e.row_map[row] : row;
 }
 template <int END> __device__ __forceinline__ void row_end(const End& e, int row, bool live, int part, const RowState& st) {
   if constexpr (END == kCeStats)
@@ -257,23 +307,34 @@ template <int END> __device__ __forceinline__ void row_end(const End& e, int row
 
 // v: columns col .. col + CW of D (kSwiglu: of gate, w: of up), n of which exist
 template <int END, int CW>
-__device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool live, int kpart, int col, int n, float scale, float (&v)[CW],
+__device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, int row, bool live, int kpart, int col, int n, float scale, float (&v)[CW],
                                           float (&w)[CW], RowState& st) {
   uint32_t o[CW / 2];
   if constexpr (END == kStore) {
-    if (!live) return;
-    float4* acc = reinterpret_cast<float4*>(e.acc + kpart * e.acc_part + (int64_t)row * e.acc_ld + col);
-    if (e.acc_in) {
+    if (e.acc_in || e.acc_out) {
+      float* acc = e.acc + kpart * e.acc_part + (int64_t)row * e.acc_ld + col;
+      constexpr int kHalf = CW == 32 ? 16 : CW;
 #pragma unroll
-      for (int j = 0; j < CW; j += 4) {
-        const float4 f = acc[j / 4];
-        v[j] += f.x, v[j + 1] += f.y, v[j + 2] += f.z, v[j + 3] += f.w;
+      for (int h = 0; h < CW; h += kHalf) {
+        if (e.acc_in) {
+          uint32_t f[16];
+          if constexpr (CW == 32) {
+            rows_in(buf, live ? acc + h : nullptr, f);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) f[j] = live ? __float_as_uint(acc[j]) : 0u;
+          }
+#pragma unroll
+          for (int j = 0; j < kHalf; ++j) v[h + j] += __uint_as_float(f[j]);
+        }
+        if (e.acc_out) {
+          if constexpr (CW == 32) rows_out(buf, live ? acc + h : nullptr, reinterpret_cast<const uint32_t*>(v + h));
+          else if (live)
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) acc[j] = v[j];
+        }
       }
-    }
-    if (e.acc_out) {
-#pragma unroll
-      for (int j = 0; j < CW; j += 4) acc[j / 4] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      return;
+      if (e.acc_out) return;
     }
     if (scale != 1.f) {
 #pragma unroll
@@ -281,17 +342,15 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool l
     }
 #pragma unroll
     for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, v[j], v[j + 1]);
-    const int64_t to = e.row_map != nullptr ? e.row_map[row] : row;
-    store_row<CW>(e.out, to * e.ld + col, o, n, e.vec_out);
+    put_row<CW>(buf, e.out, st.to * e.ld + col, live, o, n, e.vec_out);
   } else if constexpr (END == kSwiglu) {
-    if (!live) return;
     if (e.gate_up != nullptr) {
 #pragma unroll
       for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, v[j], v[j + 1]);
-      store_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + col, o, n, e.vec_gu);
+      put_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + col, live, o, n, e.vec_gu);
 #pragma unroll
       for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, w[j], w[j + 1]);
-      store_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + e.half + col, o, n, e.vec_gu);
+      put_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + e.half + col, live, o, n, e.vec_gu);
     }
     if (e.h == nullptr) return;
 #pragma unroll
@@ -308,13 +367,12 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool l
       }
       o[j / 2] = pack16(fmt, h[0], h[1]);
     }
-    store_row<CW>(e.h, (int64_t)row * e.ld_h + col, o, n, e.vec_h);
+    put_row<CW>(buf, e.h, (int64_t)row * e.ld_h + col, live, o, n, e.vec_h);
   } else if constexpr (END == kDswiglu) {
-    if (!live) return;
     uint32_t ug[CW / 2], uu[CW / 2];
     const int64_t half = e.half;
-    load_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + col, ug, n, e.vec_gu);
-    load_row<CW>(e.gate_up, (int64_t)row * e.ld_gu + half + col, uu, n, e.vec_gu);
+    get_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + col, live, ug, n, e.vec_gu);
+    get_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + half + col, live, uu, n, e.vec_gu);
 #pragma unroll
     for (int j = 0; j < CW; j += 2) {
       float g[2], u[2], dg[2], du[2], h[2];
@@ -340,9 +398,9 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool l
       ug[j / 2] = pack16(fmt, dg[0], dg[1]);
       uu[j / 2] = pack16(fmt, du[0], du[1]);
     }
-    store_row<CW>(e.out, (int64_t)row * e.ld + col, ug, n, e.vec_out);
-    store_row<CW>(e.out, (int64_t)row * e.ld + half + col, uu, n, e.vec_out);
-    if (e.h != nullptr) store_row<CW>(e.h, (int64_t)row * e.ld_h + col, o, n, e.vec_h);
+    put_row<CW>(buf, e.out, (int64_t)row * e.ld + col, live, ug, n, e.vec_out);
+    put_row<CW>(buf, e.out, (int64_t)row * e.ld + half + col, live, uu, n, e.vec_out);
+    if (e.h != nullptr) put_row<CW>(buf, e.h, (int64_t)row * e.ld_h + col, live, o, n, e.vec_h);
   } else if constexpr (END == kCeStats) {
     float top = -INFINITY;
 #pragma unroll
@@ -384,38 +442,64 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, int row, bool l
       }
       o[j / 2] = pack16(fmt, d[0], d[1]);
     }
-    store_row<CW>(e.out, (int64_t)row * e.ld + col, o, n, e.vec_out);
+    put_row<CW>(buf, e.out, (int64_t)row * e.ld + col, true, o, n, e.vec_out);
   }
 }
 
 // ---- the kernel ----------------------------------------------------------------------------------------------
 struct Tile { int prod, m, n, kpart; };
 
-// The i-th tile of a cluster; false: there is none.
-__device__ __forceinline__ bool tile_of(const Params& p, const Shared& sh, int i, int cluster, int clusters, Tile& out) {
-  const int full = sh.long_tiles / clusters, rest = sh.long_tiles - full * clusters, more = cluster < rest ? 1 : 0;
-  int t;
-  if (i < full + more) {
-    t = i * clusters + cluster;
-  } else {
-    const int r = i - full - (more ? 1 - sh.delta : 0);       // round of the other tiles
-    t = sh.long_tiles + (r < sh.delta ? r * (clusters - rest) + cluster - rest
-                                      : sh.delta * (clusters - rest) + (r - sh.delta) * clusters + cluster);
-  }
-  if (t >= sh.first[p.count]) return false;
-  int q = 0;
-  while (q + 1 < p.count && t >= sh.first[q + 1]) ++q;
-  int r = t - sh.first[q];
-  const int G = p.prod[q].group, nt = sh.n_tiles[q], each = nt * sh.m_tiles[q];
-  out.kpart = 0;
-  if (p.prod[q].k_parts > 1) out.kpart = r / each, r -= out.kpart * each;
-  const int g = r / (G * nt), in = r - g * G * nt;
-  const int wide = min(G, sh.m_tiles[q] - g * G);
-  out.prod = q;
-  out.n = in / wide;
-  out.m = g * G + (in - out.n * wide);
-  return true;
+// n / d by a multiplication: inv = (2^32 - 1) / d, at most one too small before the correction
+__device__ __forceinline__ int quotient(int n, int d, uint32_t inv) {
+  const int q = (int)__umulhi((uint32_t)n, inv);
+  return n - q * d >= d ? q + 1 : q;
 }
+__device__ __forceinline__ uint32_t inverse(int d) { return d > 0 ? 0xFFFFFFFFu / (uint32_t)d : 0u; }
+
+// The tiles of a cluster in turn: first its share of the long ones (of the first product), every `clusters`-th; then of the
+// others, where the clusters that have one long tile more than the rest stay out of the first `delta` rounds.
+struct Walk {
+  int cluster, clusters, t, round;
+  __device__ __forceinline__ void place(const Shared& sh) {
+    const int few = clusters - sh.rest;
+    t = sh.long_tiles + (round < sh.delta ? round * few + cluster - sh.rest
+                                          : sh.delta * few + (round - sh.delta) * clusters + cluster);
+  }
+  __device__ __forceinline__ Walk(const Shared& sh, int cluster_, int clusters_) : cluster(cluster_), clusters(clusters_), t(cluster_), round(-1) {
+    if (t >= sh.long_tiles) start(sh);
+  }
+  __device__ __forceinline__ void start(const Shared& sh) {
+    round = cluster < sh.rest ? sh.delta : 0;
+    place(sh);
+  }
+  __device__ __forceinline__ void next(const Shared& sh) {
+    if (round < 0) {
+      t += clusters;
+      if (t >= sh.long_tiles) start(sh);
+    } else {
+      ++round;
+      place(sh);
+    }
+  }
+  __device__ __forceinline__ bool get(const Params& p, const Shared& sh, Tile& out) const {
+    if (t >= sh.first[p.count]) return false;
+    int q = 0;
+    while (q + 1 < p.count && t >= sh.first[q + 1]) ++q;
+    int r = t - sh.first[q];
+    out.kpart = 0;
+    if (p.prod[q].k_parts > 1) {
+      const int each = sh.n_tiles[q] * sh.m_tiles[q];
+      out.kpart = r / each, r -= out.kpart * each;
+    }
+    const int G = p.prod[q].group, strip = G * sh.n_tiles[q];
+    const int g = quotient(r, strip, sh.strip_inv[q]), in = r - g * strip, left = sh.m_tiles[q] - g * G;
+    const int wide = left < G ? left : G;
+    out.prod = q;
+    out.n = quotient(in, wide, left < G ? sh.last_inv[q] : sh.group_inv[q]);
+    out.m = g * G + (in - out.n * wide);
+    return true;
+  }
+};
 
 template <int CG, int BN, bool BMN, int END>
 __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params p) {
@@ -462,11 +546,17 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       first += sh.m_tiles[i] * sh.n_tiles[i] * q.k_parts;
     }
     sh.first[p.count] = first;
-    // The first product's tiles may be longer than the others': the clusters that have one of them more leave out as many
-    // rounds of the others.
+    // The first product's tiles may be longer than the others': in rounds of the others, with the time of a read-out, which
+    // is about that of 12 blocks of K.
     sh.long_tiles = p.count > 1 ? sh.first[1] : 0;
-    sh.delta = 1;
-    if (p.count > 1) sh.delta = max(1, (sh.kb[0] / p.prod[0].k_parts + sh.kb[1] / 2) / max(1, sh.kb[1]));
+    sh.rest = sh.long_tiles % clusters;
+    sh.delta = p.count > 1 ? max(1, (sh.kb[0] / p.prod[0].k_parts + 12 + (sh.kb[1] + 12) / 2) / (sh.kb[1] + 12)) : 1;
+    for (int i = 0; i < p.count; ++i) {
+      const int G = p.prod[i].group;
+      sh.strip_inv[i] = inverse(G * sh.n_tiles[i]);
+      sh.group_inv[i] = inverse(G);
+      sh.last_inv[i] = inverse(sh.m_tiles[i] % G);
+    }
     for (int i = 0; i < p.count; ++i) {
       tc::prefetch_tensormap(&p.prod[i].a);
       tc::prefetch_tensormap(&p.prod[i].b);
@@ -503,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       if (++slot == C::kStages) slot = 0, parity ^= 1, dst -= C::kStages * C::kStageBytes;
     };
     Tile t;
-    for (int at = 0; ok && tile_of(p, sh, at, cluster, clusters, t); ++at) {
+    for (Walk walk(sh, cluster, clusters); ok && walk.get(p, sh, t); walk.next(sh)) {
       const DevProduct& q = p.prod[t.prod];
       int k0, k1;
       k_range(t, k0, k1);
@@ -562,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       uint32_t slot = 0, parity = 0, off = 0, set = 0, set_parity = 1;
       Tile t;
       bool ok = true;
-      for (int at = 0; ok && tile_of(p, sh, at, cluster, clusters, t); ++at) {
+      for (Walk walk(sh, cluster, clusters); ok && walk.get(p, sh, t); walk.next(sh)) {
         const bool a_mn = p.prod[t.prod].a_mn != 0;
         const uint64_t a_first = operand_desc(ring, a_mn);
         const uint32_t idesc = base_idesc | ((a_mn ? 1u : 0u) << 15);
@@ -600,6 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       }
     }
   } else if (warp >= 4) {
+    const uint32_t buf = ring + C::kStages * C::kStageBytes + (warp - 4) * kRowsOut;
     const int wg = (warp - 4) >> 2, quad = warp & 3;
     const int in_tile = quad * 32 + lane;
     constexpr int kMine = kTileN / 2;       // columns of a warpgroup
@@ -607,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     uint32_t sets = 0;
     Tile t;
     bool ok = true;
-    for (int at = 0; ok && tile_of(p, sh, at, cluster, clusters, t); ++at) {
+    for (Walk walk(sh, cluster, clusters); ok && walk.get(p, sh, t); walk.next(sh)) {
       const End& e = p.prod[t.prod].end;
       const int N = p.prod[t.prod].N;
       int k0, k1;
@@ -658,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-          if (N - col > 0) row_piece<END, 32>(e, p.fmt, row, live, t.kpart, col, N - col, scale, v, v, st);
+          if (N - col > 0) row_piece<END, 32>(e, p.fmt, buf, row, live, t.kpart, col, N - col, scale, v, v, st);
         }
         row_end<END>(e, row, live, t.n * 2 + wg, st);
       } else {
@@ -681,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
 #pragma unroll 1
         for (int c = wg * kMine; c < (wg + 1) * kMine; c += 32) {
           const int col = t.n * kTileN + c, n = N - col;
-          if (n <= 0) break;
+          if (n <= 0 || (END != kCeGrad && !warp_live)) break;
           float v[32], w[32];
           tmem_ld32(from + c, v);
           if constexpr (kPaired) tmem_ld32(from + BN / 2 + c, w);
@@ -690,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = w[j] = 0.f;
           }
-          row_piece<END, 32>(e, p.fmt, row, live, t.kpart, col, n, scale, v, w, st);
+          row_piece<END, 32>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
         }
         hand_back(set);
       }
@@ -701,8 +792,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   if (split > 1) {
     cluster_sync();       // every CTA's part is in its shared memory
     Tile t;
-    if (warp >= 4 && tile_of(p, sh, 0, cluster, clusters, t) && !guard.aborted()) {
+    if (warp >= 4 && Walk(sh, cluster, clusters).get(p, sh, t) && !guard.aborted()) {
       const End& e = p.prod[t.prod].end;
+      const uint32_t buf = 0;      // (pieces of eight columns go to memory lane by lane)
       const int wg = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
       const int row = t.m * kRows + in_tile;
       const bool live = row < sh.rows[t.prod];
@@ -726,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
               if constexpr (kPaired) w[j] += ld_cluster(base + (BN / 2 + j) * kRows * 4);
             }
           }
-          row_piece<END, 8>(e, p.fmt, row, live, t.kpart, col, n, scale, v, w, st);
+          row_piece<END, 8>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
         }
         row_end<END>(e, row, live, (t.n * split + (int)rank) * 2 + wg, st);
       } else if (END == kCeGrad && t.m * kRows < sh.rows[t.prod]) {
@@ -740,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           float v[8], w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
-          row_piece<END, 8>(e, p.fmt, row, false, t.kpart, col, n, 1.f, v, w, st);
+          row_piece<END, 8>(e, p.fmt, buf, row, false, t.kpart, col, n, 1.f, v, w, st);
         }
       }
     }

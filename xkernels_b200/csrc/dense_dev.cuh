@@ -50,13 +50,18 @@ struct Params {
   int* status;
 };
 
+// A product in tiles, in shared memory: a role looks a tile up with a handful of loads side by side.
+struct Extent {
+  int first, m_tiles, n_tiles, kb, rows, k_parts, group;      // first: number of its first tile
+  uint32_t strip_inv, group_inv, last_inv;
+};
+
 struct Shared {
   uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
   int abort_flag;
   uint32_t tmem;
-  int m_tiles[kMaxProblems], n_tiles[kMaxProblems], kb[kMaxProblems], rows[kMaxProblems], first[kMaxProblems + 1];
-  int long_tiles, delta, rest;
-  uint32_t strip_inv[kMaxProblems], group_inv[kMaxProblems], last_inv[kMaxProblems];
+  Extent of[kMaxProblems];
+  int tiles, long_tiles, delta, rest;
 };
 
 template <int CG, int BN> struct Cfg {
@@ -82,7 +87,7 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -447,7 +452,7 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
 }
 
 // ---- the kernel ----------------------------------------------------------------------------------------------
-struct Tile { int prod, m, n, kpart; };
+struct Tile { int prod, m, n, kpart, rows, k0, k1; };      // rows: of the product; k0, k1: blocks of K
 
 // n / d by a multiplication: inv = (2^32 - 1) / d, at most one too small before the correction
 __device__ __forceinline__ int quotient(int n, int d, uint32_t inv) {
@@ -481,22 +486,25 @@ struct Walk {
       place(sh);
     }
   }
-  __device__ __forceinline__ bool get(const Params& p, const Shared& sh, Tile& out) const {
-    if (t >= sh.first[p.count]) return false;
-    int q = 0;
-    while (q + 1 < p.count && t >= sh.first[q + 1]) ++q;
-    int r = t - sh.first[q];
+  __device__ __forceinline__ bool get(const Shared& sh, Tile& out) const {
+    if (t >= sh.tiles) return false;
+    const int q = (t >= sh.of[1].first) + (t >= sh.of[2].first);
+    const Extent e = sh.of[q];
+    int r = t - e.first;
+    out.prod = q;
     out.kpart = 0;
-    if (p.prod[q].k_parts > 1) {
-      const int each = sh.n_tiles[q] * sh.m_tiles[q];
+    if (e.k_parts > 1) {
+      const int each = e.n_tiles * e.m_tiles;
       out.kpart = r / each, r -= out.kpart * each;
     }
-    const int G = p.prod[q].group, strip = G * sh.n_tiles[q];
-    const int g = quotient(r, strip, sh.strip_inv[q]), in = r - g * strip, left = sh.m_tiles[q] - g * G;
-    const int wide = left < G ? left : G;
-    out.prod = q;
-    out.n = quotient(in, wide, left < G ? sh.last_inv[q] : sh.group_inv[q]);
-    out.m = g * G + (in - out.n * wide);
+    const int strip = e.group * e.n_tiles;
+    const int g = quotient(r, strip, e.strip_inv), in = r - g * strip, left = e.m_tiles - g * e.group;
+    const int wide = left < e.group ? left : e.group;
+    out.n = quotient(in, wide, left < e.group ? e.last_inv : e.group_inv);
+    out.m = g * e.group + (in - out.n * wide);
+    out.rows = e.rows;
+    out.k0 = 0, out.k1 = e.kb;
+    if (e.k_parts > 1) out.k0 = e.kb * out.kpart / e.k_parts, out.k1 = e.kb * (out.kpart + 1) / e.k_parts;
     return true;
   }
 };
@@ -530,7 +538,10 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     }
     tc::mbar_fence_init();
     int first = 0;
-    for (int i = 0; i < p.count; ++i) {
+    for (int i = 0; i < kMaxProblems; ++i) {
+      Extent& x = sh.of[i];
+      x.first = 0x7FFFFFFF;
+      if (i >= p.count) continue;
       const DevProduct& q = p.prod[i];
       int M = q.M, K = q.K;
       if (q.live != nullptr) {
@@ -538,25 +549,24 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         if (q.live_is_k) K = min(live, K);
         else M = min(live, M);
       }
-      sh.rows[i] = M;
-      sh.m_tiles[i] = (M + kRows * CG - 1) / (kRows * CG);
-      sh.n_tiles[i] = (q.N + kTileN - 1) / kTileN;
-      sh.kb[i] = (K + kBK - 1) / kBK;
-      sh.first[i] = first;
-      first += sh.m_tiles[i] * sh.n_tiles[i] * q.k_parts;
+      x.first = first;
+      x.rows = M;
+      x.m_tiles = (M + kRows * CG - 1) / (kRows * CG);
+      x.n_tiles = (q.N + kTileN - 1) / kTileN;
+      x.kb = (K + kBK - 1) / kBK;
+      x.k_parts = q.k_parts;
+      x.group = q.group;
+      x.strip_inv = inverse(x.group * x.n_tiles);
+      x.group_inv = inverse(x.group);
+      x.last_inv = inverse(x.m_tiles % x.group);
+      first += x.m_tiles * x.n_tiles * x.k_parts;
     }
-    sh.first[p.count] = first;
+    sh.tiles = first;
     // The first product's tiles may be longer than the others': in rounds of the others, with the time of a read-out, which
-    // is about that of 12 blocks of K.
-    sh.long_tiles = p.count > 1 ? sh.first[1] : 0;
+    // is about that of 8 blocks of K.
+    sh.long_tiles = p.count > 1 ? sh.of[1].first : 0;
     sh.rest = sh.long_tiles % clusters;
-    sh.delta = p.count > 1 ? max(1, (sh.kb[0] / p.prod[0].k_parts + 12 + (sh.kb[1] + 12) / 2) / (sh.kb[1] + 12)) : 1;
-    for (int i = 0; i < p.count; ++i) {
-      const int G = p.prod[i].group;
-      sh.strip_inv[i] = inverse(G * sh.n_tiles[i]);
-      sh.group_inv[i] = inverse(G);
-      sh.last_inv[i] = inverse(sh.m_tiles[i] % G);
-    }
+    sh.delta = p.count > 1 ? max(1, (sh.of[0].kb / sh.of[0].k_parts + 8 + (sh.of[1].kb + 8) / 2) / (sh.of[1].kb + 8)) : 1;
     for (int i = 0; i < p.count; ++i) {
       tc::prefetch_tensormap(&p.prod[i].a);
       tc::prefetch_tensormap(&p.prod[i].b);
@@ -569,12 +579,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   tc::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
-  // blocks of K of a tile: its part, or what the cluster leaves to this CTA
-  auto k_range = [&](const Tile& t, int& k0, int& k1) {
-    const int kb = sh.kb[t.prod], parts = CG == 1 && split > 1 ? split : p.prod[t.prod].k_parts;
-    const int part = CG == 1 && split > 1 ? (int)rank : t.kpart;
-    k0 = parts == 1 ? 0 : kb * part / parts;
-    k1 = parts == 1 ? kb : kb * (part + 1) / parts;
+  // what the cluster leaves to this CTA of a tile's blocks of K
+  auto share = [&](Tile& t) {
+    if (CG == 1 && split > 1) t.k0 = t.k1 * (int)rank / split, t.k1 = t.k1 * ((int)rank + 1) / split;
   };
   if (warp == 0 || warp == 3) {
     // Warp 0 feeds A, warp 3 feeds B.  The whole warp runs the loop and one lane issues: operands then sit in uniform
@@ -593,15 +600,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       if (++slot == C::kStages) slot = 0, parity ^= 1, dst -= C::kStages * C::kStageBytes;
     };
     Tile t;
-    for (Walk walk(sh, cluster, clusters); ok && walk.get(p, sh, t); walk.next(sh)) {
+    for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
       const DevProduct& q = p.prod[t.prod];
-      int k0, k1;
-      k_range(t, k0, k1);
+      share(t);
       if (feeds_a) {
         const CUtensorMap* map = &q.a;
         const int m0 = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0);
         const bool mn = q.a_mn != 0;
-        for (int k = k0 * kBK; k < k1 * kBK; k += kBK) {
+        for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
           if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
           if (expects) expect_tx(mine + 8 * slot, bytes);
           if (leader) {
@@ -620,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           const int part = CG == 2 ? (int)rank : 0;
           const int r0 = q.b_row0 + (kPaired ? part * q.end.half + t.n * (BN / 2) : t.n * BN + part * (BN / 2));
           const int r1 = r0 + (kPaired ? q.end.half : BN / 2);      // (CG = 1: the other half of the columns)
-          for (int k = k0 * kBK; k < k1 * kBK; k += kBK) {
+          for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
             if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
             if (leader) {
               tma_2d<CG>(dst, map, full + 8 * slot, k, r0);
@@ -630,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           }
         } else {
           const int n0 = t.n * BN + (CG == 2 ? (int)rank * (BN / 2) : 0), base = q.b_row0;
-          for (int k = k0 * kBK; k < k1 * kBK; k += kBK) {
+          for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
             if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
             if (leader) {
 #pragma unroll
@@ -652,13 +658,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       uint32_t slot = 0, parity = 0, off = 0, set = 0, set_parity = 1;
       Tile t;
       bool ok = true;
-      for (Walk walk(sh, cluster, clusters); ok && walk.get(p, sh, t); walk.next(sh)) {
+      for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
         const bool a_mn = p.prod[t.prod].a_mn != 0;
         const uint64_t a_first = operand_desc(ring, a_mn);
         const uint32_t idesc = base_idesc | ((a_mn ? 1u : 0u) << 15);
         const uint32_t a_step = a_mn ? 128 : 2, b_step = BMN ? 128 : 2;    // 16 K further, in units of 16 bytes
-        int k0, k1;
-        k_range(t, k0, k1);
+        share(t);
+        const int k0 = t.k0, k1 = t.k1;
         const int parts = parts_of<END>(k1 - k0);
         for (int part = 0; ok && part < parts; ++part) {
           const uint32_t d = tmem + set * BN;
@@ -698,14 +704,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     uint32_t sets = 0;
     Tile t;
     bool ok = true;
-    for (Walk walk(sh, cluster, clusters); ok && walk.get(p, sh, t); walk.next(sh)) {
+    for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
       const End& e = p.prod[t.prod].end;
       const int N = p.prod[t.prod].N;
-      int k0, k1;
-      k_range(t, k0, k1);
+      share(t);
       const int row = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0) + in_tile;
-      const bool live = row < sh.rows[t.prod];
-      const bool warp_live = row - lane < sh.rows[t.prod];
+      const bool live = row < t.rows;
+      const bool warp_live = row - lane < t.rows;
       auto hand_back = [&](uint32_t set) {      // all loads from the accumulators have come back
         tc::tc_fence_before();
         __syncwarp();
@@ -718,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       row_begin<END>(e, row, live && split == 1, st);
       const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
       if constexpr (END == kCeStats) {
-        const int parts = parts_of<END>(k1 - k0);
+        const int parts = parts_of<END>(t.k1 - t.k0);
         float sum[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
@@ -772,18 +777,24 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
 #pragma unroll 1
         for (int c = wg * kMine; c < (wg + 1) * kMine; c += 32) {
           const int col = t.n * kTileN + c, n = N - col;
-          if (n <= 0 || (END != kCeGrad && !warp_live)) break;
+          const bool none = n <= 0 || (END != kCeGrad && !warp_live);
           float v[32], w[32];
-          tmem_ld32(from + c, v);
-          if constexpr (kPaired) tmem_ld32(from + BN / 2 + c, w);
-          tc::tmem_wait_ld();
-          if (k1 == k0) {
+          if (!none) {
+            tmem_ld32(from + c, v);
+            if constexpr (kPaired) tmem_ld32(from + BN / 2 + c, w);
+            tc::tmem_wait_ld();
+          }
+          if (none || c + 32 >= (wg + 1) * kMine || n <= 32) {     // the last piece: before it goes to memory
+            hand_back(set);
+            if (none) break;
+          }
+          if (t.k1 == t.k0) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = w[j] = 0.f;
           }
           row_piece<END, 32>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
+          if (n <= 32) break;
         }
-        hand_back(set);
       }
     }
   }
@@ -792,13 +803,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   if (split > 1) {
     cluster_sync();       // every CTA's part is in its shared memory
     Tile t;
-    if (warp >= 4 && Walk(sh, cluster, clusters).get(p, sh, t) && !guard.aborted()) {
+    if (warp >= 4 && Walk(sh, cluster, clusters).get(sh, t) && !guard.aborted()) {
       const End& e = p.prod[t.prod].end;
       const uint32_t buf = 0;      // (pieces of eight columns go to memory lane by lane)
       const int wg = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
       const int row = t.m * kRows + in_tile;
-      const bool live = row < sh.rows[t.prod];
-      if (t.m * kRows + (warp & 3) * 32 < sh.rows[t.prod]) {
+      const bool live = row < t.rows;
+      if (t.m * kRows + (warp & 3) * 32 < t.rows) {
         RowState st;
         row_begin<END>(e, row, live, st);
         const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
@@ -821,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           row_piece<END, 8>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
         }
         row_end<END>(e, row, live, (t.n * split + (int)rank) * 2 + wg, st);
-      } else if (END == kCeGrad && t.m * kRows < sh.rows[t.prod]) {
+      } else if (END == kCeGrad && t.m * kRows < t.rows) {
         // rows behind the last: zeros, they are K of the next product
         RowState st;
         row_begin<END>(e, row, false, st);

@@ -45,37 +45,49 @@ int status_word(int** out) {
 
 struct Shape { int cg, bn, split; };
 
-// Which tile.  The cost of a shape is its rounds of tiles times the time of a tile, which is K times the clocks of a
-// stage: 512 for 256 x 256 on a pair (MMA rate), 330 for 256 x 128 (operand traffic), 300 to 400 for 128 x 128 on one CTA.
-// A cluster that splits K pays for adding its parts up.
-Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, bool paired, bool may_split, int sms) {
+// How many clusters of `width` CTAs of 200 KB run at once: a cluster lies within one of the GPCs, which have 16 to 20 SMs.
+int64_t clusters_at_once(int width, int sms) {
+  const int gpcs = 8, each = sms / gpcs;      // 18
+  return width <= 2 ? sms / width : (int64_t)gpcs * (each / width);
+}
+
+// Which tile.  The cost of a shape is its rounds of tiles times the time of a tile: its blocks of K times the clocks of a
+// stage, and the read-out.  A stage takes its MMAs (512 clocks for 256 x 256 on a pair, 256 for the halves) or its operands'
+// bytes at 64 a clock and SM, whichever is more.  Sharing a tile costs a cluster the exchange of its parts.
+Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, int end, bool may_split, int sms) {
   Shape best{2, 256, 1};
   double best_cost = 1e300;
+  const bool paired = end == kSwiglu;
   auto consider = [&](Shape s, double cost) {
     if (cost < best_cost * 0.999) best_cost = cost, best = s;
   };
   for (int bn : {256, 128}) {
     const int64_t tile_n = paired ? bn / 2 : bn;
+    const double stage = bn == 256 ? 520 : 400, readout = bn == 256 ? 3500 : 2000;
     double work = 0;
-    int64_t tiles = 0, longest = 0;
+    int64_t tiles = 0;
     for (int i = 0; i < count; ++i) {
       const int64_t t = ceil_div(M[i], 256) * ceil_div(N[i], tile_n) * k_parts[i], kb = ceil_div(ceil_div(K[i], kBK), k_parts[i]);
       tiles += t;
-      work += (double)t * kb;
-      longest = kb > longest ? kb : longest;
+      // (a short tile takes its read-out's time)
+      work += (double)t * (kb * stage > readout ? kb * stage : readout);
     }
     const double mean = work / (double)(tiles > 0 ? tiles : 1);
-    const int64_t rounds = ceil_div(tiles, sms / 2);
-    consider({2, bn, 1}, (double)rounds * mean * (bn == 256 ? 512 : 330) + (bn == 256 ? 6000 : 3000));
+    consider({2, bn, 1}, (double)ceil_div(tiles, sms / 2) * mean + readout);
+    if (count == 1 && may_split)
+      for (int s = 2; s <= 4; ++s) {
+        const int64_t kb = ceil_div(K[0], kBK);
+        if (4 * s <= kb && tiles <= clusters_at_once(2 * s, sms)) consider({2, bn, s}, ceil_div(kb, s) * stage + readout + 4000);
+      }
   }
   if (count == 1 && may_split) {
     const int64_t tile_n = paired ? 64 : 128, tiles = ceil_div(M[0], kRows) * ceil_div(N[0], tile_n), kb = ceil_div(K[0], kBK);
     const int64_t rows = M[0] < kRows ? align_up(M[0], 8) : kRows;
-    const double stage = 256 + rows;
-    for (int s : {1, 2, 4, 8}) {
-      if (s > 1 && (s > kb || tiles * s > sms / s * s)) continue;
-      consider({1, 128, s}, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage + (s > 1 ? 4000 : 2000));
-    }
+    const double stage = 2 * (rows + 128) > 256 ? 2 * (rows + 128) : 256;
+    consider({1, 128, 1}, (double)ceil_div(tiles, sms) * kb * stage + 2000);
+    for (int s = 2; s <= 8; ++s)
+      if (2 * s <= kb && tiles <= (end == kCeStats ? 1 : 2) * clusters_at_once(s, sms))
+        consider({1, 128, s}, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage + 4000);
   }
   return best;
 }
@@ -103,8 +115,8 @@ int ce_parts(int64_t M, int64_t N, int64_t K) {
   int sms = 148;
   if (sm_count(&sms) != XKB_OK) sms = 148;
   const int one = 1;
-  const Shape s = shape_of(&M, &N, &K, &one, 1, false, true, sms);
-  return (int)(ceil_div(N, s.bn) * s.split * 2);
+  const Shape s = shape_of(&M, &N, &K, &one, 1, kCeStats, true, sms);
+  return (int)(ceil_div(N, s.bn) * (s.split > 1 ? s.bn / 8 : 2));
 }
 
 int launch(const Product* products, int count, int end, int dtype, bool chained, bool early_b, cudaStream_t stream) {
@@ -126,7 +138,7 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     XKB_REQUIRE(M[i] > 0 && N[i] > 0 && K[i] > 0 && M[i] < (1ll << 30) && N[i] < (1ll << 30) && K[i] < (1ll << 30),
                 "dense products: sizes out of range");
   }
-  const Shape s = shape_of(M, N, K, k_parts, count, end == kSwiglu, !any_a_mn && !parted, sms);
+  const Shape s = shape_of(M, N, K, k_parts, count, end, !any_a_mn && !parted, sms);
   const int a_rows = s.cg == 1 && !any_a_mn && M[0] < kRows ? (int)align_up(M[0], 8) : kRows;
   const CUtensorMapDataType dt = dtype == XKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   p.count = count;
@@ -134,6 +146,13 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   p.split = s.split;
   p.a_bytes = a_rows * 128;
   p.early_b = early_b ? 1 : 0;
+  const int read_warps = s.cg == 2 ? 8 : single_warps(end);
+  if (s.cg == 1) {      // a stage's place for A is as large as its rows
+    const int ring = read_warps == 4 ? Cfg<1, 128, 4>::kRing : Cfg<1, 128, 8>::kRing;
+    p.a_slot = (int)align_up(p.a_bytes, 1024);
+    p.stages = ring / (p.a_slot + Cfg<1, 128, 8>::kBBytes);
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+  }
   int64_t tiles = 0;
   const int tile_m = kRows * s.cg, tile_n = end == kSwiglu ? s.bn / 2 : s.bn;
   for (int i = 0; i < count; ++i) {
@@ -160,9 +179,9 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   l.cg = s.cg, l.bn = s.bn, l.split = s.split, l.chained = chained, l.stream = stream;
   const int margin = g_sm_margin.load(std::memory_order_relaxed);
   if (s.split > 1) {
-    l.grid = (int)tiles * s.split;     // one tile a cluster
+    l.grid = (int)tiles * s.split * s.cg;     // one tile a cluster
   } else {
-    int64_t most = (sms - margin) / s.cg;
+    int64_t most = (sms - margin) / s.cg * (read_warps == 4 ? 2 : 1);
     if (most < 1) most = 1;
     l.grid = (int)(tiles < most ? tiles : most) * s.cg;
   }

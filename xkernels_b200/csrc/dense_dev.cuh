@@ -18,8 +18,8 @@ namespace dense {
 
 constexpr int kBK = 64;             // K of a stage: 128 bytes, one swizzle row
 constexpr int kRows = 128;          // rows of D per CTA
-constexpr int kThreads = 384;       // warps 0: TMA, 1: MMA, 2: tensor memory, 4 to 11: read-out
-constexpr int kReadWarps = 8;
+constexpr int kControlWarps = 4;    // 0: TMA of A, 1: MMA, 2: tensor memory, 3: TMA of B; the read-out warps follow
+constexpr int kMaxStages = 12;
 constexpr int kABytes = kRows * 128;
 constexpr int kRowsOut = 32 * 64;   // a warp's 32 rows of 64 bytes on their way to or from memory
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
@@ -44,8 +44,9 @@ struct DevProduct {
 struct Params {
   DevProduct prod[kMaxProblems];
   int count, fmt;       // fmt: 1 bf16, 0 fp16
-  int split;            // CTAs that share a tile (CG = 1)
+  int split;            // CTAs (pairs) of a cluster that share a tile, a part of K each
   int a_bytes;          // bytes of A that a stage loads
+  int a_slot, stages;   // CG = 1: bytes that a stage has for A, stages
   int early_b;
   int* status;
 };
@@ -57,19 +58,23 @@ struct Extent {
 };
 
 struct Shared {
-  uint64_t full[8], empty[8], acc_full[2], acc_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   int abort_flag;
   uint32_t tmem;
   Extent of[kMaxProblems];
   int tiles, long_tiles, delta, rest;
 };
 
-template <int CG, int BN> struct Cfg {
+// CG: CTAs of a pair; BN: columns of a tile; RW: read-out warps.  RW = 4 leaves room for two CTAs on an SM.
+template <int CG, int BN, int RW> struct Cfg {
+  static constexpr int kThreads = 32 * (kControlWarps + RW);
+  static constexpr int kCtas = RW == 4 ? 2 : 1;
   static constexpr int kBBytes = BN / CG * 128;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = (209 * 1024 / kStageBytes) < 8 ? (209 * 1024 / kStageBytes) : 8;
-  static constexpr int kSmem = kStages * kStageBytes + kReadWarps * kRowsOut + 1024;
-  static_assert(kStages >= 4 && kStages <= 8, "");
+  static constexpr int kRing = (RW == 4 ? 102 : 209) * 1024;
+  static constexpr int kStageBytes = kABytes + kBBytes;                                           // CG = 2
+  static constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
+  static constexpr int kSmem = kRing + RW * kRowsOut + 1024;
+  static_assert(kRing >= BN * kRows * 4, "the parts of a sum lie where the stages were");
 };
 
 // ---- instructions that tc_common.cuh has no form of ----------------------------------------------------------
@@ -108,10 +113,10 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // Arrives on the barrier at this address (in both CTAs of a pair) once the MMAs issued so far are done.
-template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
+template <int CG> __device__ __forceinline__ void commit(uint32_t bar, uint16_t both) {
   if constexpr (CG == 2)
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"((uint16_t)3) : "memory");
+                 ::"r"(bar), "h"(both) : "memory");
   else
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -157,7 +162,8 @@ template <int CG> __device__ __forceinline__ void tmem_dealloc(uint32_t addr, ui
   else
     tc::tmem_dealloc(addr, cols);
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[16]) { tc::tmem_ld_32x16(addr, reinterpret_cast<uint32_t(&)[16]>(v)); }
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -509,47 +515,48 @@ struct Walk {
   }
 };
 
-template <int CG, int BN, bool BMN, int END>
-__global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<CG, BN>;
+template <int CG, int BN, int RW, bool BMN, int END>
+__global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kCtas) dense_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<CG, BN, RW>;
   constexpr bool kPaired = END == kSwiglu;
   constexpr int kTileN = kPaired ? BN / 2 : BN;    // columns of the result
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   const uint32_t ring = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int split = CG == 1 ? p.split : 1;
-  const int width = CG == 2 ? 2 : split;           // CTAs of a cluster
+  const int split = p.split, width = CG * split;   // width: CTAs of a cluster
   const uint32_t rank = width > 1 ? cluster_rank() : 0;
+  const int part = (int)rank / CG, half = (int)rank % CG, first_rank = (int)rank - half;   // of K; of the tile's rows
   const int cluster = blockIdx.x / width, clusters = gridDim.x / width;
+  const uint32_t stages = CG == 2 ? C::kStages : p.stages, a_slot = CG == 2 ? kABytes : p.a_slot, stage_bytes = a_slot + C::kBBytes;
   tc::Guard guard{&sh.abort_flag, p.status};
 
   if (!p.early_b) chain_wait();
   chain_trigger();
-  if (threadIdx.x == 0) {
-    sh.abort_flag = 0;
-    for (int s = 0; s < C::kStages; ++s) {
-      tc::mbar_init(&sh.full[s], 1);
-      tc::mbar_init(&sh.empty[s], 1);
+  if (warp == 0) {
+    if (lane == 0) {
+      sh.abort_flag = 0;
+      for (uint32_t s = 0; s < stages; ++s) {
+        tc::mbar_init(&sh.full[s], 1);
+        tc::mbar_init(&sh.empty[s], 1);
+      }
+      for (int a = 0; a < 2; ++a) {
+        tc::mbar_init(&sh.acc_full[a], 1);
+        tc::mbar_init(&sh.acc_empty[a], RW * CG);
+      }
+      tc::mbar_fence_init();
     }
-    for (int a = 0; a < 2; ++a) {
-      tc::mbar_init(&sh.acc_full[a], 1);
-      tc::mbar_init(&sh.acc_empty[a], kReadWarps * CG);
-    }
-    tc::mbar_fence_init();
-    int first = 0;
-    for (int i = 0; i < kMaxProblems; ++i) {
-      Extent& x = sh.of[i];
-      x.first = 0x7FFFFFFF;
-      if (i >= p.count) continue;
-      const DevProduct& q = p.prod[i];
+  } else if (warp == 1) {
+    int tiles = 0;
+    if (lane < p.count) {
+      const DevProduct& q = p.prod[lane];
+      Extent& x = sh.of[lane];
       int M = q.M, K = q.K;
       if (q.live != nullptr) {
         const int live = *q.live;
         if (q.live_is_k) K = min(live, K);
         else M = min(live, M);
       }
-      x.first = first;
       x.rows = M;
       x.m_tiles = (M + kRows * CG - 1) / (kRows * CG);
       x.n_tiles = (q.N + kTileN - 1) / kTileN;
@@ -559,29 +566,34 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       x.strip_inv = inverse(x.group * x.n_tiles);
       x.group_inv = inverse(x.group);
       x.last_inv = inverse(x.m_tiles % x.group);
-      first += x.m_tiles * x.n_tiles * x.k_parts;
+      tiles = x.m_tiles * x.n_tiles * x.k_parts;
     }
-    sh.tiles = first;
-    // The first product's tiles may be longer than the others': in rounds of the others, with the time of a read-out, which
-    // is about that of 8 blocks of K.
-    sh.long_tiles = p.count > 1 ? sh.of[1].first : 0;
-    sh.rest = sh.long_tiles % clusters;
-    sh.delta = p.count > 1 ? max(1, (sh.of[0].kb / sh.of[0].k_parts + 8 + (sh.of[1].kb + 8) / 2) / (sh.of[1].kb + 8)) : 1;
-    for (int i = 0; i < p.count; ++i) {
-      tc::prefetch_tensormap(&p.prod[i].a);
-      tc::prefetch_tensormap(&p.prod[i].b);
+    const int t0 = __shfl_sync(~0u, tiles, 0), t1 = __shfl_sync(~0u, tiles, 1), t2 = __shfl_sync(~0u, tiles, 2);
+    if (lane < kMaxProblems) sh.of[lane].first = lane >= p.count ? 0x7FFFFFFF : lane == 0 ? 0 : lane == 1 ? t0 : t0 + t1;
+    __syncwarp();
+    if (lane == 0) {
+      sh.tiles = t0 + t1 + t2;
+      // The first product's tiles may be longer than the others': in rounds of the others, with the time of a read-out,
+      // which is about that of 8 blocks of K.
+      sh.long_tiles = p.count > 1 ? t0 : 0;
+      sh.rest = sh.long_tiles % clusters;
+      sh.delta = p.count > 1 ? max(1, (sh.of[0].kb / sh.of[0].k_parts + 8 + (sh.of[1].kb + 8) / 2) / (sh.of[1].kb + 8)) : 1;
     }
+  } else if (warp == 2) {
+    tmem_alloc<CG>(&sh.tmem, 2 * BN);
+  } else if (warp == 3 && lane < p.count) {
+    tc::prefetch_tensormap(&p.prod[lane].a);
+    tc::prefetch_tensormap(&p.prod[lane].b);
   }
-  if (warp == 2) tmem_alloc<CG>(&sh.tmem, 2 * BN);
   tc::tc_fence_before();
   __syncthreads();
-  if (width > 1) cluster_sync();
+  if (CG == 2) cluster_sync();      // the other CTA's barriers are there
   tc::tc_fence_after();
   const uint32_t tmem = sh.tmem;
 
   // what the cluster leaves to this CTA of a tile's blocks of K
   auto share = [&](Tile& t) {
-    if (CG == 1 && split > 1) t.k0 = t.k1 * (int)rank / split, t.k1 = t.k1 * ((int)rank + 1) / split;
+    if (split > 1) t.k0 = t.k1 * part / split, t.k1 = t.k1 * (part + 1) / split;
   };
   if (warp == 0 || warp == 3) {
     // Warp 0 feeds A, warp 3 feeds B.  The whole warp runs the loop and one lane issues: operands then sit in uniform
@@ -590,14 +602,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
     const bool leader = tc::elect_one(), feeds_a = warp == 0;
     if (p.early_b && feeds_a) chain_wait();
     const uint32_t bytes = (uint32_t)(p.a_bytes + C::kBBytes) * CG;
-    const bool expects = leader && (CG == 1 || rank == 0);
+    const bool expects = leader && half == 0;
     const uint32_t empty = tc::smem_u32(sh.empty);
-    const uint32_t mine = tc::smem_u32(sh.full), full = CG == 2 ? map_to(mine, 0) : mine;   // the first CTA's count
-    uint32_t slot = 0, parity = 1, dst = ring + (feeds_a ? 0 : kABytes);
+    const uint32_t mine = tc::smem_u32(sh.full), full = CG == 2 ? map_to(mine, first_rank) : mine;   // the first CTA's count
+    uint32_t slot = 0, parity = 1, dst = ring + (feeds_a ? 0 : a_slot);
     bool ok = true;
     auto next = [&]() {
-      dst += C::kStageBytes;
-      if (++slot == C::kStages) slot = 0, parity ^= 1, dst -= C::kStages * C::kStageBytes;
+      dst += stage_bytes;
+      if (++slot == stages) slot = 0, parity ^= 1, dst -= stages * stage_bytes;
     };
     Tile t;
     for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
@@ -605,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       share(t);
       if (feeds_a) {
         const CUtensorMap* map = &q.a;
-        const int m0 = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0);
+        const int m0 = t.m * kRows * CG + half * kRows;
         const bool mn = q.a_mn != 0;
         for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
           if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
@@ -623,8 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       } else {
         const CUtensorMap* map = &q.b;
         if constexpr (!BMN) {
-          const int part = CG == 2 ? (int)rank : 0;
-          const int r0 = q.b_row0 + (kPaired ? part * q.end.half + t.n * (BN / 2) : t.n * BN + part * (BN / 2));
+          const int r0 = q.b_row0 + (kPaired ? half * q.end.half + t.n * (BN / 2) : t.n * BN + half * (BN / 2));
           const int r1 = r0 + (kPaired ? q.end.half : BN / 2);      // (CG = 1: the other half of the columns)
           for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
             if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
@@ -635,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
             next();
           }
         } else {
-          const int n0 = t.n * BN + (CG == 2 ? (int)rank * (BN / 2) : 0), base = q.b_row0;
+          const int n0 = t.n * BN + half * (BN / 2), base = q.b_row0;
           for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
             if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
             if (leader) {
@@ -648,13 +659,14 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       }
     }
   } else if (warp == 1) {
-    if (CG == 1 || rank == 0) {
+    if (half == 0) {
       const uint32_t base_idesc = (1u << 4) | ((uint32_t)p.fmt << 7) | ((uint32_t)p.fmt << 10) | ((BMN ? 1u : 0u) << 16) |
                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((kRows * CG) >> 4) << 24);
       const bool leader = tc::elect_one();
       const uint32_t full = tc::smem_u32(sh.full), empty = tc::smem_u32(sh.empty);
       const uint32_t acc_full = tc::smem_u32(sh.acc_full), acc_empty = tc::smem_u32(sh.acc_empty);
-      const uint64_t b_first = operand_desc(ring + kABytes, BMN);
+      const uint64_t b_first = operand_desc(ring + a_slot, BMN);
+      const uint16_t both = (uint16_t)(3u << first_rank);     // the CTAs of the pair
       uint32_t slot = 0, parity = 0, off = 0, set = 0, set_parity = 1;
       Tile t;
       bool ok = true;
@@ -666,11 +678,11 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         share(t);
         const int k0 = t.k0, k1 = t.k1;
         const int parts = parts_of<END>(k1 - k0);
-        for (int part = 0; ok && part < parts; ++part) {
+        for (int piece = 0; ok && piece < parts; ++piece) {
           const uint32_t d = tmem + set * BN;
           if (!wait(acc_empty + 8 * set, set_parity, guard, 2)) { ok = false; break; }
           tc::tc_fence_after();
-          const int b0 = END == kCeStats ? k0 + part * kPartBlocks : k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, k1) : k1;
+          const int b0 = END == kCeStats ? k0 + piece * kPartBlocks : k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, k1) : k1;
           uint32_t accumulate = 0;
           for (int k = b0; k < b1; ++k) {
             if (!wait(full + 8 * slot, parity, guard, 3)) { ok = false; break; }
@@ -682,24 +694,25 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
                 mma_ss<CG>(d, a + i * a_step, b + i * b_step, idesc, accumulate);
                 accumulate = 1;
               }
-              commit<CG>(empty + 8 * slot);
+              commit<CG>(empty + 8 * slot, both);
             }
             accumulate = 1;
-            off += C::kStageBytes >> 4;
-            if (++slot == C::kStages) slot = 0, parity ^= 1, off = 0;
+            off += stage_bytes >> 4;
+            if (++slot == stages) slot = 0, parity ^= 1, off = 0;
           }
-          if (ok && leader) commit<CG>(acc_full + 8 * set);
+          if (ok && leader) commit<CG>(acc_full + 8 * set, both);
           __syncwarp();
           set ^= 1;
           if (set == 0) set_parity ^= 1;
         }
       }
     }
-  } else if (warp >= 4) {
-    const uint32_t buf = ring + C::kStages * C::kStageBytes + (warp - 4) * kRowsOut;
+  } else if (warp >= kControlWarps) {
+    const uint32_t buf = ring + C::kRing + (warp - 4) * kRowsOut;
     const int wg = (warp - 4) >> 2, quad = warp & 3;
     const int in_tile = quad * 32 + lane;
-    constexpr int kMine = kTileN / 2;       // columns of a warpgroup
+    constexpr int kMine = kTileN * 4 / RW;  // columns of a warpgroup
+    constexpr int kPiece = RW == 4 && END == kDswiglu ? 16 : 32;    // (as many as registers allow)
     if (p.early_b) chain_wait();
     uint32_t sets = 0;
     Tile t;
@@ -708,13 +721,13 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
       const End& e = p.prod[t.prod].end;
       const int N = p.prod[t.prod].N;
       share(t);
-      const int row = t.m * kRows * CG + (CG == 2 ? (int)rank * kRows : 0) + in_tile;
+      const int row = t.m * kRows * CG + half * kRows + in_tile;
       const bool live = row < t.rows;
       const bool warp_live = row - lane < t.rows;
       auto hand_back = [&](uint32_t set) {      // all loads from the accumulators have come back
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) remote_arrive(map_to(tc::smem_u32(&sh.acc_empty[set]), CG == 2 ? 0 : rank));
+        if (lane == 0) remote_arrive(map_to(tc::smem_u32(&sh.acc_empty[set]), first_rank));
       };
       auto park = [&](int c, float x) {         // this CTA's part of a sum, columns of 128 rows, where the stages were
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (c * kRows + in_tile) * 4), "f"(x) : "memory");
@@ -727,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         float sum[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
-        for (int part = 0; part < parts; ++part, ++sets) {
+        for (int piece = 0; piece < parts; ++piece, ++sets) {
           const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16) + wg * kMine;
           if (!wait(tc::smem_u32(&sh.acc_full[set]), (sets >> 1) & 1, guard, 4)) { ok = false; break; }
           tc::tc_fence_after();
@@ -764,9 +777,9 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
         tc::tc_fence_after();
         if (split > 1) {
           if (warp_live) {
-            for (int c = wg * (BN / 2); c < (wg + 1) * (BN / 2); c += 32) {
+            for (int c = wg * (BN * 4 / RW); c < (wg + 1) * (BN * 4 / RW); c += 32) {
               float v[32];
-              tmem_ld32(from + c, v);
+              tmem_load(from + c, v);
               tc::tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; ++j) park(c + j, v[j]);
@@ -775,25 +788,25 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
           break;
         }
 #pragma unroll 1
-        for (int c = wg * kMine; c < (wg + 1) * kMine; c += 32) {
+        for (int c = wg * kMine; c < (wg + 1) * kMine; c += kPiece) {
           const int col = t.n * kTileN + c, n = N - col;
           const bool none = n <= 0 || (END != kCeGrad && !warp_live);
-          float v[32], w[32];
+          float v[kPiece], w[kPiece];
           if (!none) {
-            tmem_ld32(from + c, v);
-            if constexpr (kPaired) tmem_ld32(from + BN / 2 + c, w);
+            tmem_load(from + c, v);
+            if constexpr (kPaired) tmem_load(from + BN / 2 + c, w);
             tc::tmem_wait_ld();
           }
-          if (none || c + 32 >= (wg + 1) * kMine || n <= 32) {     // the last piece: before it goes to memory
+          if (none || c + kPiece >= (wg + 1) * kMine || n <= kPiece) {     // the last piece: before it goes to memory
             hand_back(set);
             if (none) break;
           }
           if (t.k1 == t.k0) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = w[j] = 0.f;
+            for (int j = 0; j < kPiece; ++j) v[j] = w[j] = 0.f;
           }
-          row_piece<END, 32>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
-          if (n <= 32) break;
+          row_piece<END, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
+          if (n <= kPiece) break;
         }
       }
     }
@@ -803,48 +816,37 @@ __global__ void __launch_bounds__(kThreads, 1) dense_kernel(const __grid_constan
   if (split > 1) {
     cluster_sync();       // every CTA's part is in its shared memory
     Tile t;
-    if (warp >= 4 && Walk(sh, cluster, clusters).get(sh, t) && !guard.aborted()) {
+    if (warp >= kControlWarps && Walk(sh, cluster, clusters).get(sh, t) && !guard.aborted()) {
+      // Pieces of eight columns, dealt out to the parts; a warp takes a piece of 32 rows.  Rows behind the last are nothing
+      // but for kCeGrad, whose zeros are K of the next product.
       const End& e = p.prod[t.prod].end;
-      const uint32_t buf = 0;      // (pieces of eight columns go to memory lane by lane)
-      const int wg = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
-      const int row = t.m * kRows + in_tile;
-      const bool live = row < t.rows;
-      if (t.m * kRows + (warp & 3) * 32 < t.rows) {
+      const int row0 = t.m * kRows * CG + half * kRows, rows = t.rows - row0;
+      const int quads = END == kCeGrad ? 4 : rows <= 0 ? 0 : min(4, (rows + 31) / 32);
+      const int pieces = (kTileN / 8 - part + split - 1) / split;
+      const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
+#pragma unroll 1
+      for (int i = warp - kControlWarps; i < pieces * quads; i += RW) {
+        const int quad = i % quads, piece = (i / quads) * split + part;
+        const int c = piece * 8, in_tile = quad * 32 + lane, row = row0 + in_tile;
+        const int col = t.n * kTileN + c, n = p.prod[t.prod].N - col;
+        const bool live = row < t.rows;
         RowState st;
         row_begin<END>(e, row, live, st);
-        const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
-        const int mine = kTileN / split;     // columns of this CTA
-#pragma unroll 1
-        for (int c = (int)rank * mine + wg * 8; c < ((int)rank + 1) * mine; c += 16) {
-          const int col = t.n * kTileN + c, n = p.prod[t.prod].N - col;
-          if (n <= 0) break;
-          float v[8], w[8];
+        float v[8], w[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
+        if (n > 0 && quad * 32 < rows) {
           for (int from = 0; from < split; ++from) {
-            const uint32_t base = map_to(ring + (c * kRows + in_tile) * 4, from);
+            const uint32_t base = map_to(ring + (c * kRows + in_tile) * 4, from * CG + half);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               v[j] += ld_cluster(base + j * kRows * 4);
               if constexpr (kPaired) w[j] += ld_cluster(base + (BN / 2 + j) * kRows * 4);
             }
           }
-          row_piece<END, 8>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
         }
-        row_end<END>(e, row, live, (t.n * split + (int)rank) * 2 + wg, st);
-      } else if (END == kCeGrad && t.m * kRows < t.rows) {
-        // rows behind the last: zeros, they are K of the next product
-        RowState st;
-        row_begin<END>(e, row, false, st);
-        const int mine = kTileN / split;
-        for (int c = (int)rank * mine + wg * 8; c < ((int)rank + 1) * mine; c += 16) {
-          const int col = t.n * kTileN + c, n = p.prod[t.prod].N - col;
-          if (n <= 0) break;
-          float v[8], w[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
-          row_piece<END, 8>(e, p.fmt, buf, row, false, t.kpart, col, n, 1.f, v, w, st);
-        }
+        if (n > 0) row_piece<END, 8>(e, p.fmt, 0, row, live, t.kpart, col, n, scale, v, w, st);
+        row_end<END>(e, row, live, t.n * (kTileN / 8) + piece, st);
       }
     }
   }
@@ -867,27 +869,28 @@ struct Launch {
   cudaStream_t stream;
 };
 
-template <int CG, int BN, bool BMN, int END>
+template <int CG, int BN, int RW, bool BMN, int END>
 int run_kernel(const Params& p, const Launch& l) {
-  using C = Cfg<CG, BN>;
+  using C = Cfg<CG, BN, RW>;
+  auto kernel = dense_kernel<CG, BN, RW, BMN, END>;
   static std::atomic<uint64_t> ready{0};      // devices on which this instance is set up
   int dev = 0;
   XKB_CHECK_CUDA(cudaGetDevice(&dev));
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit == 0 || !(ready.load(std::memory_order_acquire) & bit)) {
-    XKB_CHECK_CUDA(cudaFuncSetAttribute(dense_kernel<CG, BN, BMN, END>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    XKB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     ready.fetch_or(bit, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(l.grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = l.stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (CG == 2 || l.split > 1) {
+  if (CG * l.split > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = CG == 2 ? 2 : l.split;
+    attr[n].val.clusterDim.x = CG * l.split;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
@@ -898,15 +901,19 @@ int run_kernel(const Params& p, const Launch& l) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dense_kernel<CG, BN, BMN, END>, p));
+  XKB_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
   XKB_CHECK_LAUNCH("dense_kernel");
   return XKB_OK;
 }
 
+// Read-out warps of a single CTA: eight where the read-out adds up in registers, else four and two CTAs an SM, whose ends
+// (and the next kernel's first loads) overlap.
+constexpr int single_warps(int end) { return end == kCeStats ? 8 : 4; }
+
 template <bool BMN, int END>
 int run_variant(const Params& p, const Launch& l) {
-  if (l.cg == 2) return l.bn == 256 ? run_kernel<2, 256, BMN, END>(p, l) : run_kernel<2, 128, BMN, END>(p, l);
-  return run_kernel<1, 128, BMN, END>(p, l);
+  if (l.cg == 2) return l.bn == 256 ? run_kernel<2, 256, 8, BMN, END>(p, l) : run_kernel<2, 128, 8, BMN, END>(p, l);
+  return run_kernel<1, 128, single_warps(END), BMN, END>(p, l);
 }
 
 // one per translation unit

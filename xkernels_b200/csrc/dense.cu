@@ -45,21 +45,21 @@ int status_word(int** out) {
 
 struct Shape { int cg, bn, split; };
 
-// How many clusters of `width` CTAs of 200 KB run at once: a cluster lies within one of the GPCs, which have 16 to 20 SMs.
-int64_t clusters_at_once(int width, int sms) {
-  const int gpcs = 8, each = sms / gpcs;      // 18
-  return width <= 2 ? sms / width : (int64_t)gpcs * (each / width);
-}
-
 // Which tile.  The cost of a shape is its rounds of tiles times the time of a tile: its blocks of K times the clocks of a
 // stage, and the read-out.  A stage takes its MMAs (512 clocks for 256 x 256 on a pair, 256 for the halves) or its operands'
-// bytes at 64 a clock and SM, whichever is more.  Sharing a tile costs a cluster the exchange of its parts.
-Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, int end, bool may_split, int sms) {
-  Shape best{2, 256, 1};
+// bytes at 64 a clock and SM, whichever is more; and the operands have to come from memory once, at 3500 bytes a clock or 36
+// a clock and CTA.  Sharing a tile costs a cluster the exchange of its parts.
+int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, int end, bool may_split, int sms,
+             Shape* best) {
+  *best = {2, 256, 1};
   double best_cost = 1e300;
   const bool paired = end == kSwiglu;
-  auto consider = [&](Shape s, double cost) {
-    if (cost < best_cost * 0.999) best_cost = cost, best = s;
+  double bytes = 0;
+  for (int i = 0; i < count; ++i) bytes += 2.0 * K[i] * (M[i] + N[i] * (paired ? 2 : 1));
+  auto consider = [&](Shape s, int64_t ctas, double clocks, double tail) {
+    const double rate = ctas * 36.0 < 3500 ? ctas * 36.0 : 3500;
+    const double cost = (clocks > bytes / rate ? clocks : bytes / rate) + tail;
+    if (cost < best_cost * 0.999) best_cost = cost, *best = s;
   };
   for (int bn : {256, 128}) {
     const int64_t tile_n = paired ? bn / 2 : bn;
@@ -73,23 +73,35 @@ Shape shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* 
       work += (double)t * (kb * stage > readout ? kb * stage : readout);
     }
     const double mean = work / (double)(tiles > 0 ? tiles : 1);
-    consider({2, bn, 1}, (double)ceil_div(tiles, sms / 2) * mean + readout);
+    consider({2, bn, 1}, 2 * tiles, (double)ceil_div(tiles, sms / 2) * mean, readout);
     if (count == 1 && may_split)
       for (int s = 2; s <= 4; ++s) {
         const int64_t kb = ceil_div(K[0], kBK);
-        if (4 * s <= kb && tiles <= clusters_at_once(2 * s, sms)) consider({2, bn, s}, ceil_div(kb, s) * stage + readout + 4000);
+        if (4 * s > kb || tiles * 2 * s > sms) continue;
+        int most = 0;
+        const int rc = clusters_at_once(2, bn, 8, 2 * s, &most);
+        if (rc != XKB_OK) return rc;
+        if (tiles <= most) consider({2, bn, s}, 2 * tiles * s, ceil_div(kb, s) * stage, readout + 2500 + 500 * s);
       }
   }
   if (count == 1 && may_split) {
-    const int64_t tile_n = paired ? 64 : 128, tiles = ceil_div(M[0], kRows) * ceil_div(N[0], tile_n), kb = ceil_div(K[0], kBK);
-    const int64_t rows = M[0] < kRows ? align_up(M[0], 8) : kRows;
-    const double stage = 2 * (rows + 128) > 256 ? 2 * (rows + 128) : 256;
-    consider({1, 128, 1}, (double)ceil_div(tiles, sms) * kb * stage + 2000);
-    for (int s = 2; s <= 8; ++s)
-      if (2 * s <= kb && tiles <= (end == kCeStats ? 1 : 2) * clusters_at_once(s, sms))
-        consider({1, 128, s}, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage + 4000);
+    const int warps = single_warps(end);
+    const int64_t kb = ceil_div(K[0], kBK), rows = M[0] < kRows ? align_up(M[0], 8) : kRows;
+    for (int bn : {128, 64}) {
+      if (bn == 64 && end == kCeStats) continue;
+      const int64_t tiles = ceil_div(M[0], kRows) * ceil_div(N[0], paired ? bn / 2 : bn);
+      const double stage = 2 * (rows + bn) > 200 ? 2 * (rows + bn) : 200;
+      consider({1, bn, 1}, tiles, (double)ceil_div(tiles, sms) * kb * stage, 2000);
+      for (int s = 2; s <= 8; ++s) {
+        if (2 * s > kb || tiles * s > 2 * sms) continue;
+        int most = 0;
+        const int rc = clusters_at_once(1, bn, warps, s, &most);
+        if (rc != XKB_OK) return rc;
+        if (tiles <= most) consider({1, bn, s}, tiles * s, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage, 4000 + 500 * s);
+      }
+    }
   }
-  return best;
+  return XKB_OK;
 }
 
 int vec_of(const void* p, int64_t ld, int64_t extra = 0) {
@@ -111,12 +123,20 @@ int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64
   return parts;
 }
 
-int ce_parts(int64_t M, int64_t N, int64_t K) {
-  int sms = 148;
-  if (sm_count(&sms) != XKB_OK) sms = 148;
-  const int one = 1;
-  const Shape s = shape_of(&M, &N, &K, &one, 1, kCeStats, true, sms);
-  return (int)(ceil_div(N, s.bn) * (s.split > 1 ? s.bn / 8 : 2));
+int ce_parts(int64_t M, int64_t N, int64_t K, int* parts) {
+  int sms = 0, one = 1, rc = sm_count(&sms);
+  if (rc != XKB_OK) return rc;
+  Shape s;
+  rc = shape_of(&M, &N, &K, &one, 1, kCeStats, true, sms, &s);
+  if (rc != XKB_OK) return rc;
+  *parts = (int)(ceil_div(N, s.bn) * (s.split > 1 ? s.bn / 8 : 2));
+  return XKB_OK;
+}
+
+int64_t ce_most_parts(int64_t M, int64_t N) {
+  // shared tiles come in pieces of eight columns, and only tiles of which there are few are shared
+  const int64_t own = ceil_div(N, 128) * 2, shared = ceil_div(N, 256) * 32;
+  return ceil_div(M, 256) * ceil_div(N, 256) <= 148 ? shared : own;
 }
 
 int launch(const Product* products, int count, int end, int dtype, bool chained, bool early_b, cudaStream_t stream) {
@@ -138,7 +158,9 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     XKB_REQUIRE(M[i] > 0 && N[i] > 0 && K[i] > 0 && M[i] < (1ll << 30) && N[i] < (1ll << 30) && K[i] < (1ll << 30),
                 "dense products: sizes out of range");
   }
-  const Shape s = shape_of(M, N, K, k_parts, count, end, !any_a_mn && !parted, sms);
+  Shape s;
+  rc = shape_of(M, N, K, k_parts, count, end, !any_a_mn && !parted, sms, &s);
+  if (rc != XKB_OK) return rc;
   const int a_rows = s.cg == 1 && !any_a_mn && M[0] < kRows ? (int)align_up(M[0], 8) : kRows;
   const CUtensorMapDataType dt = dtype == XKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   p.count = count;
@@ -150,7 +172,7 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   if (s.cg == 1) {      // a stage's place for A is as large as its rows
     const int ring = read_warps == 4 ? Cfg<1, 128, 4>::kRing : Cfg<1, 128, 8>::kRing;
     p.a_slot = (int)align_up(p.a_bytes, 1024);
-    p.stages = ring / (p.a_slot + Cfg<1, 128, 8>::kBBytes);
+    p.stages = ring / (p.a_slot + s.bn * 128);
     if (p.stages > kMaxStages) p.stages = kMaxStages;
   }
   int64_t tiles = 0;

@@ -66,8 +66,9 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
 // In how many parts to take K of the first of two products [M0, N0, K0] (few long tiles) and [M1, N1, K1] (many short ones,
 // or none) that one launch deals out, so that the long ones do not outlast the rest.
 int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64_t K1);
-// How many pieces a row's statistics come in (kCeStats).
-int ce_parts(int64_t M, int64_t N, int64_t K);
+// How many pieces a row's statistics come in (kCeStats), and no more than how many.
+int ce_parts(int64_t M, int64_t N, int64_t K, int* parts);
+int64_t ce_most_parts(int64_t M, int64_t N);
 
 }  // namespace dense
 }  // namespace xkb

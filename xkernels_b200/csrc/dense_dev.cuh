@@ -9,6 +9,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "dense.h"
 #include "softmax_dev.cuh"
 #include "tc_common.cuh"
@@ -102,6 +104,10 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
   else
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -602,7 +608,6 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
     const bool leader = tc::elect_one(), feeds_a = warp == 0;
     if (p.early_b && feeds_a) chain_wait();
     const uint32_t bytes = (uint32_t)(p.a_bytes + C::kBBytes) * CG;
-    const bool expects = leader && half == 0;
     const uint32_t empty = tc::smem_u32(sh.empty);
     const uint32_t mine = tc::smem_u32(sh.full), full = CG == 2 ? map_to(mine, first_rank) : mine;   // the first CTA's count
     uint32_t slot = 0, parity = 1, dst = ring + (feeds_a ? 0 : a_slot);
@@ -612,25 +617,49 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       if (++slot == stages) slot = 0, parity ^= 1, dst -= stages * stage_bytes;
     };
     Tile t;
+    if (p.early_b && !feeds_a && Walk(sh, cluster, clusters).get(sh, t)) {
+      // While the predecessor runs: B of the first tile that the ring has no place for, as far as L2.  (An expert's second
+      // weights, 29 MB, come in beside its first ones: one row 27.6 -> 23 us a call.)
+      share(t);
+      const DevProduct& q = p.prod[t.prod];
+      if (leader)
+        for (int k = (t.k0 + (int)stages) * kBK; k < t.k1 * kBK; k += kBK) {
+          if constexpr (!BMN) {
+            const int r0 = q.b_row0 + (kPaired ? half * q.end.half + t.n * (BN / 2) : t.n * BN + half * (BN / 2));
+            prefetch_2d(&q.b, k, r0);
+            if constexpr (CG == 1) prefetch_2d(&q.b, k, r0 + (kPaired ? q.end.half : BN / 2));
+          } else {
+            for (int j = 0; j < BN / CG / 64; ++j) prefetch_2d(&q.b, t.n * BN + half * (BN / 2) + 64 * j, q.b_row0 + k);
+          }
+        }
+      __syncwarp();
+    }
     for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
       const DevProduct& q = p.prod[t.prod];
       share(t);
       if (feeds_a) {
         const CUtensorMap* map = &q.a;
         const int m0 = t.m * kRows * CG + half * kRows;
-        const bool mn = q.a_mn != 0;
-        for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
-          if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
-          if (expects) expect_tx(mine + 8 * slot, bytes);
-          if (leader) {
-            if (!mn) {
+        // (a loop for each orientation, one branch in it: with the choice inside an iteration took 250 clocks for 130)
+        if (q.a_mn == 0) {
+          for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
+            if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
+            if (leader) {
+              if (CG == 1 || half == 0) expect_tx(mine + 8 * slot, bytes);
               tma_2d<CG>(dst, map, full + 8 * slot, k, m0);
-            } else {
+            }
+            next();
+          }
+        } else {
+          for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
+            if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
+            if (leader) {
+              if (CG == 1 || half == 0) expect_tx(mine + 8 * slot, bytes);
               tma_2d<CG>(dst, map, full + 8 * slot, m0, k);
               tma_2d<CG>(dst + kBoxBytes, map, full + 8 * slot, m0 + 64, k);
             }
+            next();
           }
-          next();
         }
       } else {
         const CUtensorMap* map = &q.b;
@@ -670,36 +699,38 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       uint32_t slot = 0, parity = 0, off = 0, set = 0, set_parity = 1;
       Tile t;
       bool ok = true;
+      // the blocks b0 .. b1 of K into accumulator set `set`
+      auto multiply = [&](auto a_orientation, int b0, int b1) {
+        constexpr bool kAMn = decltype(a_orientation)::value;
+        constexpr uint32_t kAStep = kAMn ? 128 : 2, kBStep = BMN ? 128 : 2;    // 16 K further, in units of 16 bytes
+        const uint64_t a_first = operand_desc(ring, kAMn);
+        const uint32_t idesc = base_idesc | ((kAMn ? 1u : 0u) << 15), d = tmem + set * BN;
+        uint32_t accumulate = 0;
+        for (int k = b0; k < b1; ++k) {
+          if (!wait(full + 8 * slot, parity, guard, 3)) return false;
+          tc::tc_fence_after();
+          if (leader) {
+            const uint64_t a = a_first + off, b = b_first + off;
+            mma_ss<CG>(d, a, b, idesc, accumulate);
+#pragma unroll
+            for (int i = 1; i < kBK / 16; ++i) mma_ss<CG>(d, a + i * kAStep, b + i * kBStep, idesc, 1);
+            commit<CG>(empty + 8 * slot, both);
+          }
+          accumulate = 1;
+          off += stage_bytes >> 4;
+          if (++slot == stages) slot = 0, parity ^= 1, off = 0;
+        }
+        return true;
+      };
       for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
         const bool a_mn = p.prod[t.prod].a_mn != 0;
-        const uint64_t a_first = operand_desc(ring, a_mn);
-        const uint32_t idesc = base_idesc | ((a_mn ? 1u : 0u) << 15);
-        const uint32_t a_step = a_mn ? 128 : 2, b_step = BMN ? 128 : 2;    // 16 K further, in units of 16 bytes
         share(t);
-        const int k0 = t.k0, k1 = t.k1;
-        const int parts = parts_of<END>(k1 - k0);
+        const int parts = parts_of<END>(t.k1 - t.k0);
         for (int piece = 0; ok && piece < parts; ++piece) {
-          const uint32_t d = tmem + set * BN;
           if (!wait(acc_empty + 8 * set, set_parity, guard, 2)) { ok = false; break; }
           tc::tc_fence_after();
-          const int b0 = END == kCeStats ? k0 + piece * kPartBlocks : k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, k1) : k1;
-          uint32_t accumulate = 0;
-          for (int k = b0; k < b1; ++k) {
-            if (!wait(full + 8 * slot, parity, guard, 3)) { ok = false; break; }
-            tc::tc_fence_after();
-            if (leader) {
-              const uint64_t a = a_first + off, b = b_first + off;
-#pragma unroll
-              for (int i = 0; i < kBK / 16; ++i) {
-                mma_ss<CG>(d, a + i * a_step, b + i * b_step, idesc, accumulate);
-                accumulate = 1;
-              }
-              commit<CG>(empty + 8 * slot, both);
-            }
-            accumulate = 1;
-            off += stage_bytes >> 4;
-            if (++slot == stages) slot = 0, parity ^= 1, off = 0;
-          }
+          const int b0 = END == kCeStats ? t.k0 + piece * kPartBlocks : t.k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, t.k1) : t.k1;
+          ok = END == kStore && BMN && a_mn ? multiply(std::true_type{}, b0, b1) : multiply(std::false_type{}, b0, b1);
           if (ok && leader) commit<CG>(acc_full + 8 * set, both);
           __syncwarp();
           set ^= 1;
@@ -836,12 +867,29 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
         if (n > 0 && quad * 32 < rows) {
-          for (int from = 0; from < split; ++from) {
-            const uint32_t base = map_to(ring + (c * kRows + in_tile) * 4, from * CG + half);
+          // two parts' loads at a time: each is a round trip to another SM
+          const uint32_t at = ring + (c * kRows + in_tile) * 4;
+          for (int from = 0; from < split; from += 2) {
+            const uint32_t x = map_to(at, from * CG + half), y = map_to(at, min(from + 1, split - 1) * CG + half);
+            float a[2][8], b[2][8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              v[j] += ld_cluster(base + j * kRows * 4);
-              if constexpr (kPaired) w[j] += ld_cluster(base + (BN / 2 + j) * kRows * 4);
+              a[0][j] = ld_cluster(x + j * kRows * 4);
+              a[1][j] = ld_cluster(y + j * kRows * 4);
+              if constexpr (kPaired) {
+                b[0][j] = ld_cluster(x + (BN / 2 + j) * kRows * 4);
+                b[1][j] = ld_cluster(y + (BN / 2 + j) * kRows * 4);
+              }
+            }
+            const bool two = from + 1 < split;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              v[j] += a[0][j];
+              if (two) v[j] += a[1][j];
+              if constexpr (kPaired) {
+                w[j] += b[0][j];
+                if (two) w[j] += b[1][j];
+              }
             }
           }
         }
@@ -913,8 +961,13 @@ constexpr int single_warps(int end) { return end == kCeStats ? 8 : 4; }
 template <bool BMN, int END>
 int run_variant(const Params& p, const Launch& l) {
   if (l.cg == 2) return l.bn == 256 ? run_kernel<2, 256, 8, BMN, END>(p, l) : run_kernel<2, 128, 8, BMN, END>(p, l);
+  if constexpr (END != kCeStats)
+    if (l.bn == 64) return run_kernel<1, 64, 4, BMN, END>(p, l);
   return run_kernel<1, 128, single_warps(END), BMN, END>(p, l);
 }
+
+// How many clusters of so many CTAs of one of the kernels' sizes run at once on this device.
+int clusters_at_once(int cg, int bn, int read_warps, int width, int* out);
 
 // one per translation unit
 int run_ffn(int end, const Params& p, const Launch& l);

@@ -300,7 +300,7 @@ Work carve(void* ws, int64_t M, int64_t H, int64_t V, bool backward) {
     if (piece < V || w.k_parts > 1) w.acc = c.take<float>(w.k_parts * P * align_up(H, 32));
   } else {
     w.given = c.take<float>(P);
-    w.part = c.take<float2>(dense::ce_parts(M, V, H) * P);
+    w.part = c.take<float2>(dense::ce_most_parts(M, V) * P);
   }
   w.bytes = c.off;
   return w;
@@ -366,7 +366,8 @@ extern "C" int xkb_linear_cross_entropy(const void* hidden, int64_t ld_hidden, i
   dense::Product q = {};
   q.b = {weight, ld_weight, false, 0, V, H};
   q.M = M, q.N = V, q.K = H;
-  const int parts = dense::ce_parts(M, V, H);
+  int parts = 0;
+  XKB_TRY(dense::ce_parts(M, V, H, &parts));
   q.end.part = w.part, q.end.part_ld = parts;
   q.end.given = w.given;
   JoinArgs j = {};

@@ -81,7 +81,7 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
         int most = 0;
         const int rc = clusters_at_once(2, bn, 8, 2 * s, &most);
         if (rc != XKB_OK) return rc;
-        if (tiles <= most) consider({2, bn, s}, 2 * tiles * s, ceil_div(kb, s) * stage, readout + 2500 + 500 * s);
+        if (tiles <= most) consider({2, bn, s}, 2 * tiles * s, ceil_div(kb, s) * stage, readout + 8000);
       }
   }
   if (count == 1 && may_split) {
@@ -90,14 +90,14 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
     for (int bn : {128, 64}) {
       if (bn == 64 && end == kCeStats) continue;
       const int64_t tiles = ceil_div(M[0], kRows) * ceil_div(N[0], paired ? bn / 2 : bn);
-      const double stage = 2 * (rows + bn) > 200 ? 2 * (rows + bn) : 200;
+      const double mma = bn == 128 ? 275 : 260, stage = 2 * (rows + bn) > mma ? 2 * (rows + bn) : mma;
       consider({1, bn, 1}, tiles, (double)ceil_div(tiles, sms) * kb * stage, 2000);
       for (int s = 2; s <= 8; ++s) {
-        if (2 * s > kb || tiles * s > 2 * sms) continue;
+        if (4 * s > kb || tiles * s > 2 * sms) continue;
         int most = 0;
         const int rc = clusters_at_once(1, bn, warps, s, &most);
         if (rc != XKB_OK) return rc;
-        if (tiles <= most) consider({1, bn, s}, tiles * s, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage, 4000 + 500 * s);
+        if (tiles <= most) consider({1, bn, s}, tiles * s, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage, 4500 + 500 * s);
       }
     }
   }
@@ -172,8 +172,11 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   if (s.cg == 1) {      // a stage's place for A is as large as its rows
     const int ring = read_warps == 4 ? Cfg<1, 128, 4>::kRing : Cfg<1, 128, 8>::kRing;
     p.a_slot = (int)align_up(p.a_bytes, 1024);
-    p.stages = ring / (p.a_slot + s.bn * 128);
+    p.stages = ring / ((p.a_slot + s.bn * 128));
     if (p.stages > kMaxStages) p.stages = kMaxStages;
+    // An MMA reads 128 rows of A whatever its place holds (the rows behind the last make rows of D that nothing reads), and
+    // has to stay within the ring.
+    while (p.stages > 1 && (p.stages - 1) * (p.a_slot + s.bn * 128) + kABytes > ring) --p.stages;
   }
   int64_t tiles = 0;
   const int tile_m = kRows * s.cg, tile_n = end == kSwiglu ? s.bn / 2 : s.bn;
@@ -183,8 +186,12 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     rc = make_map_2d_pitched(&d.a, dt, q.a.base, q.a.rows, q.a.cols, (uint64_t)q.a.pitch * 2, q.a.k_rows ? 64 : a_rows, 64,
                              CU_TENSOR_MAP_SWIZZLE_128B, "left operand");
     if (rc != XKB_OK) return rc;
-    rc = make_map_2d_pitched(&d.b, dt, q.b.base, q.b.rows, q.b.cols, (uint64_t)q.b.pitch * 2, b_mn ? 64 : s.bn / 2, 64,
-                             CU_TENSOR_MAP_SWIZZLE_128B, "right operand");
+    if (end == kSwiglu)      // gate rows and up rows are planes
+      rc = make_map_3d_pitched(&d.b, dt, q.b.base, 2, q.N, q.b.cols, (uint64_t)q.N * q.b.pitch * 2, (uint64_t)q.b.pitch * 2, 2 / s.cg,
+                               s.bn / 2, 64, CU_TENSOR_MAP_SWIZZLE_128B, "right operand");
+    else
+      rc = make_map_2d_pitched(&d.b, dt, q.b.base, q.b.rows, q.b.cols, (uint64_t)q.b.pitch * 2, b_mn ? 64 : s.bn / s.cg, 64,
+                               CU_TENSOR_MAP_SWIZZLE_128B, "right operand");
     if (rc != XKB_OK) return rc;
     d.M = (int)q.M, d.N = (int)q.N, d.K = (int)q.K, d.b_row0 = (int)q.b.row0;
     d.live = q.live;

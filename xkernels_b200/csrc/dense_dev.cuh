@@ -28,7 +28,7 @@ constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
 // The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, so a long sum drifts towards 0
 // (2^-24 of it a step of 16 K: 5e-6 of the logits at K = 7168).  Where the result stays fp32 (kCeStats) an accumulator takes
 // 512 K, and the read-out adds them up in registers while the next is filled: 5e-7, as an fp32 sum on the ordinary cores.
-constexpr int kPartBlocks = 8;
+constexpr int kPartBlocks = 8;      // of 64 K
 template <int END> __device__ __forceinline__ int parts_of(int kb) {
   return END == kCeStats ? (kb + kPartBlocks - 1) / kPartBlocks : 1;
 }
@@ -55,7 +55,7 @@ struct Params {
 
 // A product in tiles, in shared memory: a role looks a tile up with a handful of loads side by side.
 struct Extent {
-  int first, m_tiles, n_tiles, kb, rows, k_parts, group;      // first: number of its first tile
+  int first, m_tiles, n_tiles, kb, rows, k_parts, group;      // first: number of its first tile; kb: stages of K
   uint32_t strip_inv, group_inv, last_inv;
 };
 
@@ -73,7 +73,7 @@ template <int CG, int BN, int RW> struct Cfg {
   static constexpr int kCtas = RW == 4 ? 2 : 1;
   static constexpr int kBBytes = BN / CG * 128;
   static constexpr int kRing = (RW == 4 ? 102 : 209) * 1024;
-  static constexpr int kStageBytes = kABytes + kBBytes;                                           // CG = 2
+  static constexpr int kStageBytes = kABytes + kBBytes;      // CG = 2
   static constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
   static constexpr int kSmem = kRing + RW * kRowsOut + 1024;
   static_assert(kRing >= BN * kRows * 4, "the parts of a sum lie where the stages were");
@@ -105,26 +105,44 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y) : "memory");
 }
+template <int CG>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if constexpr (CG == 2)
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z) : "memory");
+}
 __device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
 }
+// By the lane whose `leader` is not 0; all lanes of the warp call with the same operands.
 template <int CG>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   if constexpr (CG == 2)
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
   else
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
 // Arrives on the barrier at this address (in both CTAs of a pair) once the MMAs issued so far are done.
-template <int CG> __device__ __forceinline__ void commit(uint32_t bar, uint16_t both) {
+template <int CG> __device__ __forceinline__ void commit(uint32_t leader, uint32_t bar, uint16_t both) {
   if constexpr (CG == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(bar), "h"(both) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+                 ::"r"(bar), "h"(both), "r"(leader) : "memory");
   else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader) : "memory");
 }
 // Barriers by their address.  A wait is bounded (tc_common.cuh).
 __device__ __forceinline__ bool probe(uint32_t bar, uint32_t parity) {
@@ -526,6 +544,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   using C = Cfg<CG, BN, RW>;
   constexpr bool kPaired = END == kSwiglu;
   constexpr int kTileN = kPaired ? BN / 2 : BN;    // columns of the result
+  constexpr int kTmemCols = 2 * BN;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Shared sh;
   const uint32_t ring = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -534,7 +553,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   const uint32_t rank = width > 1 ? cluster_rank() : 0;
   const int part = (int)rank / CG, half = (int)rank % CG, first_rank = (int)rank - half;   // of K; of the tile's rows
   const int cluster = blockIdx.x / width, clusters = gridDim.x / width;
-  const uint32_t stages = CG == 2 ? C::kStages : p.stages, a_slot = CG == 2 ? kABytes : p.a_slot, stage_bytes = a_slot + C::kBBytes;
+  const uint32_t stages = CG == 2 ? C::kStages : p.stages, a_slot = CG == 2 ? kABytes : p.a_slot;
+  const uint32_t stage_bytes = a_slot + C::kBBytes;
   tc::Guard guard{&sh.abort_flag, p.status};
 
   if (!p.early_b) chain_wait();
@@ -586,17 +606,22 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       sh.delta = p.count > 1 ? max(1, (sh.of[0].kb / sh.of[0].k_parts + 8 + (sh.of[1].kb + 8) / 2) / (sh.of[1].kb + 8)) : 1;
     }
   } else if (warp == 2) {
-    tmem_alloc<CG>(&sh.tmem, 2 * BN);
+    tmem_alloc<CG>(&sh.tmem, kTmemCols);
   } else if (warp == 3 && lane < p.count) {
     tc::prefetch_tensormap(&p.prod[lane].a);
     tc::prefetch_tensormap(&p.prod[lane].b);
   }
-  tc::tc_fence_before();
-  __syncthreads();
-  if (CG == 2) cluster_sync();      // the other CTA's barriers are there
-  tc::tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  // Loads may start when the barriers and the plan are there (for a pair: the other CTA's barriers too); tensor memory can
+  // take longer.
+  if (CG == 2) cluster_sync();
+  else if (warp != 2) asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads - 32) : "memory");
 
+  auto wait_for_tmem = [&]() {      // warps 1, 2 and the read-out's
+    tc::tc_fence_before();
+    asm volatile("bar.sync 2, %0;" ::"n"(C::kThreads - 64) : "memory");
+    tc::tc_fence_after();
+    return sh.tmem;
+  };
   // what the cluster leaves to this CTA of a tile's blocks of K
   auto share = [&](Tile& t) {
     if (split > 1) t.k0 = t.k1 * part / split, t.k1 = t.k1 * (part + 1) / split;
@@ -624,10 +649,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       const DevProduct& q = p.prod[t.prod];
       if (leader)
         for (int k = (t.k0 + (int)stages) * kBK; k < t.k1 * kBK; k += kBK) {
-          if constexpr (!BMN) {
-            const int r0 = q.b_row0 + (kPaired ? half * q.end.half + t.n * (BN / 2) : t.n * BN + half * (BN / 2));
-            prefetch_2d(&q.b, k, r0);
-            if constexpr (CG == 1) prefetch_2d(&q.b, k, r0 + (kPaired ? q.end.half : BN / 2));
+          if constexpr (kPaired) {
+            prefetch_3d(&q.b, k, t.n * kTileN, half);
+          } else if constexpr (!BMN) {
+            prefetch_2d(&q.b, k, q.b_row0 + t.n * BN + half * (BN / 2));
           } else {
             for (int j = 0; j < BN / CG / 64; ++j) prefetch_2d(&q.b, t.n * BN + half * (BN / 2) + 64 * j, q.b_row0 + k);
           }
@@ -664,13 +689,13 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       } else {
         const CUtensorMap* map = &q.b;
         if constexpr (!BMN) {
-          const int r0 = q.b_row0 + (kPaired ? half * q.end.half + t.n * (BN / 2) : t.n * BN + half * (BN / 2));
-          const int r1 = r0 + (kPaired ? q.end.half : BN / 2);      // (CG = 1: the other half of the columns)
+          // gate and up rows of the same columns (planes of one map): both, or this CTA's half
+          const int r0 = kPaired ? t.n * kTileN : q.b_row0 + t.n * BN + half * (BN / 2);
           for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
             if (!wait(empty + 8 * slot, parity, guard, 5)) { ok = false; break; }
             if (leader) {
-              tma_2d<CG>(dst, map, full + 8 * slot, k, r0);
-              if constexpr (CG == 1) tma_2d<CG>(dst + (BN / 2) * 128, map, full + 8 * slot, k, r1);
+              if constexpr (kPaired) tma_3d<CG>(dst, map, full + 8 * slot, k, r0, half);
+              else tma_2d<CG>(dst, map, full + 8 * slot, k, r0);
             }
             next();
           }
@@ -687,11 +712,14 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
         }
       }
     }
+  } else if (warp == 2) {
+    wait_for_tmem();
   } else if (warp == 1) {
+    const uint32_t tmem = wait_for_tmem();
     if (half == 0) {
       const uint32_t base_idesc = (1u << 4) | ((uint32_t)p.fmt << 7) | ((uint32_t)p.fmt << 10) | ((BMN ? 1u : 0u) << 16) |
                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((kRows * CG) >> 4) << 24);
-      const bool leader = tc::elect_one();
+      const uint32_t leader = tc::elect_one() ? 1u : 0u;
       const uint32_t full = tc::smem_u32(sh.full), empty = tc::smem_u32(sh.empty);
       const uint32_t acc_full = tc::smem_u32(sh.acc_full), acc_empty = tc::smem_u32(sh.acc_empty);
       const uint64_t b_first = operand_desc(ring + a_slot, BMN);
@@ -709,13 +737,13 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
         for (int k = b0; k < b1; ++k) {
           if (!wait(full + 8 * slot, parity, guard, 3)) return false;
           tc::tc_fence_after();
-          if (leader) {
-            const uint64_t a = a_first + off, b = b_first + off;
-            mma_ss<CG>(d, a, b, idesc, accumulate);
+          // (Predicated, not in a branch: operands that change or are not constant stay in uniform registers.  Four MMAs of
+          // N = 128 take their issuer 270 clocks, in a branch 325; the MMAs themselves 256.)
+          const uint64_t a = a_first + off, b = b_first + off;
 #pragma unroll
-            for (int i = 1; i < kBK / 16; ++i) mma_ss<CG>(d, a + i * kAStep, b + i * kBStep, idesc, 1);
-            commit<CG>(empty + 8 * slot, both);
-          }
+          for (int i = 0; i < kBK / 16; ++i)
+            mma_ss<CG>(leader, d, a + i * kAStep, b + i * kBStep, idesc, i == 0 ? accumulate : 1u);
+          commit<CG>(leader, empty + 8 * slot, both);
           accumulate = 1;
           off += stage_bytes >> 4;
           if (++slot == stages) slot = 0, parity ^= 1, off = 0;
@@ -731,14 +759,14 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
           tc::tc_fence_after();
           const int b0 = END == kCeStats ? t.k0 + piece * kPartBlocks : t.k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, t.k1) : t.k1;
           ok = END == kStore && BMN && a_mn ? multiply(std::true_type{}, b0, b1) : multiply(std::false_type{}, b0, b1);
-          if (ok && leader) commit<CG>(acc_full + 8 * set, both);
-          __syncwarp();
+          commit<CG>(ok ? leader : 0u, acc_full + 8 * set, both);
           set ^= 1;
           if (set == 0) set_parity ^= 1;
         }
       }
     }
   } else if (warp >= kControlWarps) {
+    const uint32_t tmem = wait_for_tmem();
     const uint32_t buf = ring + C::kRing + (warp - 4) * kRowsOut;
     const int wg = (warp - 4) >> 2, quad = warp & 3;
     const int in_tile = quad * 32 + lane;
@@ -906,7 +934,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   if (width > 1) cluster_sync();
   if (warp == 2) {
     tc::tc_fence_after();
-    tmem_dealloc<CG>(tmem, 2 * BN);
+    tmem_dealloc<CG>(sh.tmem, kTmemCols);
   }
 }
 

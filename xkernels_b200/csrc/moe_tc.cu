@@ -1134,6 +1134,17 @@ int make_map_2d_pitched(CUtensorMap* map, CUtensorMapDataType dt, const void* ba
   return make_map(map, dt, 2, base, dims, strides, box, swz, what);
 }
 
+int make_map_3d_pitched(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t planes, uint64_t rows, uint64_t cols,
+                        uint64_t plane_bytes, uint64_t pitch_bytes, uint32_t box_planes, uint32_t box_rows, uint32_t box_cols,
+                        CUtensorMapSwizzle swz, const char* what) {
+  XKB_REQUIRE(pitch_bytes % 16 == 0 && pitch_bytes < (1ull << 40) && plane_bytes % 16 == 0 && plane_bytes < (1ull << 40),
+              "%s: row pitch %llu B or plane %llu B is not a multiple of 16", what, (unsigned long long)pitch_bytes,
+              (unsigned long long)plane_bytes);
+  const uint64_t dims[3] = {cols, rows, planes}, strides[2] = {pitch_bytes, plane_bytes};
+  const uint32_t box[3] = {box_cols, box_rows, box_planes};
+  return make_map(map, dt, 3, base, dims, strides, box, swz, what);
+}
+
 namespace {
 
 // Activations [rows, K] as (64 K, eight rows, K / 64, groups of eight rows); a box is some groups of one 256-K stage.

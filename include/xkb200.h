@@ -309,7 +309,7 @@ int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_grad_out, int dtype,
                            void* stream);
 
 /* Synchronises `stream` and reports (XKB_ERR_DEVICE) whether a kernel of the four calls
- * above ever gave up a bounded wait on the current device. */
+ * above gave up a bounded wait on the current device since the last report. */
 int xkb_dense_status(void* stream);
 
 

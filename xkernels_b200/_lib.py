@@ -185,6 +185,7 @@ class PythonCalls:
 
     topk_softmax = moe_align_block_size = moe_sum_reduce = _not_served
     token_logprobs = token_logprobs_backward = moe_balance_loss = moe_router_backward = moe_sum_reduce_backward = _not_served
+    linear_cross_entropy = linear_cross_entropy_backward = gated_ffn = gated_ffn_backward = _not_served
 
 
 def load_calls():
@@ -203,7 +204,10 @@ def load_calls():
     module.bind(*(ctypes.cast(fn, c_void_p).value for fn in (
         lib.xkb_topk_softmax, lib.xkb_moe_align_block_size, lib.xkb_moe_align_workspace_bytes, lib.xkb_moe_sum_reduce,
         lib.xkb_token_logprobs, lib.xkb_token_logprobs_backward, lib.xkb_moe_balance_loss,
-        lib.xkb_moe_balance_loss_workspace_bytes, lib.xkb_moe_router_backward, lib.xkb_moe_sum_reduce_backward)))
+        lib.xkb_moe_balance_loss_workspace_bytes, lib.xkb_moe_router_backward, lib.xkb_moe_sum_reduce_backward,
+        lib.xkb_linear_cross_entropy, lib.xkb_linear_cross_entropy_workspace_bytes, lib.xkb_linear_cross_entropy_backward,
+        lib.xkb_linear_cross_entropy_backward_workspace_bytes, lib.xkb_gated_ffn, lib.xkb_gated_ffn_workspace_bytes,
+        lib.xkb_gated_ffn_backward, lib.xkb_gated_ffn_backward_workspace_bytes)))
     _calls = module
     return module
 

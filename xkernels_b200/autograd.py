@@ -1,4 +1,5 @@
-"""Differentiable forms of the router, the combine, the balance loss and the token log-probabilities.
+"""Differentiable forms of the router, the combine, the balance loss, the token log-probabilities, the head's cross entropy and
+the gated feed-forward block.
 
 The functions have the arguments and results of their namesakes in :mod:`xkernels_b200.ops`; ``backward()`` runs the
 gradient ops there.  First derivatives only.
@@ -134,3 +135,60 @@ def token_logprobs(logits, token_ids, top_k=0):
     ``top_logprobs``."""
     _not_captured("token_logprobs", logits)
     return ops.TokenLogprobs(*_TokenLogprobs.apply(logits, token_ids, top_k))
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, labels):
+        r = ops.linear_cross_entropy(hidden, weight, labels)
+        ctx.save_for_backward(hidden, weight, labels, r.stats)
+        ctx.mark_non_differentiable(r.stats)
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss, grad_lse, _):
+        _not_capturing("linear_cross_entropy")
+        if grad_loss is None and grad_lse is None:
+            return None, None, None
+        hidden, weight, labels, stats = ctx.saved_tensors
+        gh, gw = ops.linear_cross_entropy_backward(hidden, weight, labels, stats, grad_loss=grad_loss, grad_lse=grad_lse,
+                                                   need_grad_hidden=ctx.needs_input_grad[0],
+                                                   need_grad_weight=ctx.needs_input_grad[1])
+        return gh, gw, None
+
+
+def linear_cross_entropy(hidden, weight, labels):
+    """:func:`xkernels_b200.linear_cross_entropy`, differentiable in ``hidden`` and ``weight`` through ``loss`` and ``lse``."""
+    _not_captured("linear_cross_entropy", hidden, weight)
+    return ops.LinearCrossEntropy(*_LinearCrossEntropy.apply(hidden, weight, labels))
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, w2, limit, recompute):
+        keep = not recompute and any(ctx.needs_input_grad[:3])
+        got = ops.gated_ffn(x, w13, w2, limit, keep)
+        out, gate_up = got if keep else (got, None)
+        ctx.save_for_backward(x, w13, w2, gate_up)
+        ctx.limit = limit
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        _not_capturing("gated_ffn")
+        if grad_out is None:
+            return None, None, None, None, None
+        x, w13, w2, gate_up = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*ops.gated_ffn_backward(grad_out, x, w13, w2, gate_up, ctx.limit, need[0], need[1], need[2]), None, None)
+
+
+def gated_ffn(x, w13, w2, swiglu_limit=None, recompute=False):
+    """:func:`xkernels_b200.gated_ffn`, differentiable in ``x``, ``w13`` and ``w2``.  ``recompute``: gate and up are not kept for
+    the backward pass, which multiplies them once more."""
+    _not_captured("gated_ffn", x, w13, w2)
+    return _GatedFfn.apply(x, w13, w2, swiglu_limit, recompute)

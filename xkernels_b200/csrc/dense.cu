@@ -231,7 +231,9 @@ extern "C" int xkb_dense_status(void* stream_) {
   int host = 0;
   XKB_CHECK_CUDA(cudaMemcpyAsync(&host, word, sizeof(int), cudaMemcpyDeviceToHost, stream));
   XKB_CHECK_CUDA(cudaStreamSynchronize(stream));
-  if (host != 0)
+  if (host != 0) {
+    XKB_CHECK_CUDA(cudaMemsetAsync(word, 0, sizeof(int), stream));     // reported once
     return fail(XKB_ERR_DEVICE, "a kernel of a dense product gave up a bounded wait: status 0x%x (wait site %d)", host, host >> 8);
+  }
   return XKB_OK;
 }

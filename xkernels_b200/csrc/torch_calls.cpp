@@ -1,4 +1,4 @@
-// The call path of the small ops (router, routing sort, top-k reduce, losses and gradients) from Python: checks, output
+// The call path of the small ops (router, routing sort, top-k reduce, losses and gradients) and the dense ones from Python: checks, output
 // tensors and the C-ABI call in one native function.
 //
 // These ops often take 3 to 10 us on the device and a call through Python and ctypes 9 to 18 us of host time, which therefore
@@ -32,6 +32,14 @@ decltype(&xkb_moe_balance_loss) g_balance;
 decltype(&xkb_moe_balance_loss_workspace_bytes) g_balance_bytes;
 decltype(&xkb_moe_router_backward) g_router_grad;
 decltype(&xkb_moe_sum_reduce_backward) g_sum_reduce_grad;
+decltype(&xkb_linear_cross_entropy) g_lce;
+decltype(&xkb_linear_cross_entropy_workspace_bytes) g_lce_bytes;
+decltype(&xkb_linear_cross_entropy_backward) g_lce_grad;
+decltype(&xkb_linear_cross_entropy_backward_workspace_bytes) g_lce_grad_bytes;
+decltype(&xkb_gated_ffn) g_ffn;
+decltype(&xkb_gated_ffn_workspace_bytes) g_ffn_bytes;
+decltype(&xkb_gated_ffn_backward) g_ffn_grad;
+decltype(&xkb_gated_ffn_backward_workspace_bytes) g_ffn_grad_bytes;
 
 bool modes_active() {
   return at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set();
@@ -392,8 +400,153 @@ PyObject* moe_sum_reduce_backward(PyObject*, PyObject* const* args, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
+// An operand of a dense product that is read in place: rows on 16 bytes that do not overlap, bf16 or fp16.
+const at::Tensor* operand(PyObject* obj, at::ScalarType type, int64_t rows, int64_t cols) {
+  const at::Tensor* t = plain(obj, false);
+  if (t == nullptr || t->dim() != 2 || t->scalar_type() != type || t->size(0) != rows || t->size(1) != cols || rows < 0 || cols < 1 ||
+      (cols > 1 && t->stride(1) != 1) || t->stride(0) % 8 != 0 || t->stride(0) < cols ||
+      reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 != 0)
+    return nullptr;
+  return t;
+}
+// The first operand, which says type and sizes.
+const at::Tensor* first_operand(PyObject* obj) {
+  const at::Tensor* t = plain(obj, false);
+  if (t == nullptr || t->dim() != 2 || (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kHalf)) return nullptr;
+  return operand(obj, t->scalar_type(), t->size(0), t->size(1));
+}
+bool limit_of(PyObject* obj, float* limit) {
+  *limit = 0.f;
+  if (obj == Py_None) return true;
+  if (!PyFloat_CheckExact(obj)) return false;
+  *limit = (float)PyFloat_AS_DOUBLE(obj);
+  return true;
+}
+at::Tensor workspace_of(int64_t bytes) { return fresh(at::kByte, {bytes > 0 ? bytes : 0}); }
+
+// linear_cross_entropy(hidden [M, H], weight [V, H], labels [M]) -> (loss, lse, stats)
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3 || modes_active() || args[2] == Py_None) Py_RETURN_NONE;
+  const at::Tensor *x = first_operand(args[0]), *w = plain(args[1], false), *labels;
+  if (x == nullptr || w == nullptr || w->dim() != 2 || w->size(0) < 1 ||
+      operand(args[1], x->scalar_type(), w->size(0), x->size(1)) == nullptr || !tokens_of(args[2], x->size(0), &labels))
+    Py_RETURN_NONE;
+  const int64_t M = x->size(0), H = x->size(1), V = w->size(0), ws_bytes = g_lce_bytes(M, H, V);
+  Pieces pieces(2 * Pieces::room(M) + Pieces::room(2 * M));
+  at::Tensor loss = pieces.take(at::kFloat, {M}), lse = pieces.take(at::kFloat, {M}), stats = pieces.take(at::kFloat, {M, 2}),
+             ws = workspace_of(ws_bytes);
+  const int code = code_of(x->scalar_type()), ids64 = labels->scalar_type() == at::kLong;
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_lce(x->const_data_ptr(), x->stride(0), code, w->const_data_ptr(), w->stride(0), labels->const_data_ptr(), ids64,
+                 static_cast<float*>(loss.mutable_data_ptr()), static_cast<float*>(lse.mutable_data_ptr()),
+                 static_cast<float*>(stats.mutable_data_ptr()), M, H, V, ws.mutable_data_ptr(), ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  return tuple_of(THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(lse)), THPVariable_Wrap(std::move(stats)));
+  END_HANDLE_TH_ERRORS
+}
+
+// linear_cross_entropy_backward(hidden, weight, labels, stats, grad_loss, grad_lse, need_grad_hidden, need_grad_weight)
+// -> (grad_hidden, grad_weight)
+PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8 || modes_active() || args[2] == Py_None || args[3] == Py_None || (args[4] == Py_None && args[5] == Py_None) ||
+      !PyBool_Check(args[6]) || !PyBool_Check(args[7]))
+    Py_RETURN_NONE;
+  const at::Tensor *x = first_operand(args[0]), *w = plain(args[1], false), *labels, *stats, *g_loss, *g_lse;
+  if (x == nullptr || w == nullptr || w->dim() != 2 || w->size(0) < 1 ||
+      operand(args[1], x->scalar_type(), w->size(0), x->size(1)) == nullptr || !tokens_of(args[2], x->size(0), &labels) ||
+      !optional(args[3], at::kFloat, x->size(0), 2, &stats) || !optional(args[4], at::kFloat, x->size(0), -1, &g_loss) ||
+      !optional(args[5], at::kFloat, x->size(0), -1, &g_lse))
+    Py_RETURN_NONE;
+  const int64_t M = x->size(0), H = x->size(1), V = w->size(0), ws_bytes = g_lce_grad_bytes(M, H, V);
+  const bool need_x = args[6] == Py_True, need_w = args[7] == Py_True;
+  at::Tensor gx, gw, ws = workspace_of(ws_bytes);
+  if (need_x) gx = fresh(x->scalar_type(), {M, H});
+  if (need_w) gw = fresh(x->scalar_type(), {V, H});
+  const int code = code_of(x->scalar_type()), ids64 = labels->scalar_type() == at::kLong;
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_lce_grad(x->const_data_ptr(), x->stride(0), code, w->const_data_ptr(), w->stride(0), labels->const_data_ptr(), ids64,
+                      data<float>(stats), data<float>(g_loss), data<float>(g_lse), need_x ? gx.mutable_data_ptr() : nullptr,
+                      need_w ? gw.mutable_data_ptr() : nullptr, M, H, V, ws.mutable_data_ptr(), ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  PyObject* a = need_x ? THPVariable_Wrap(std::move(gx)) : Py_NewRef(Py_None);
+  PyObject* b = need_w ? THPVariable_Wrap(std::move(gw)) : Py_NewRef(Py_None);
+  return tuple_of(a, b);
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_ffn(x [M, H], w13 [2 I, H], w2 [H, I], limit, save_gate_up) -> out, or (out, gate_up)
+PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  float limit;
+  if (n != 5 || modes_active() || !limit_of(args[3], &limit) || !PyBool_Check(args[4])) Py_RETURN_NONE;
+  const at::Tensor *x = first_operand(args[0]), *w2 = plain(args[2], false);
+  if (x == nullptr || w2 == nullptr || w2->dim() != 2) Py_RETURN_NONE;
+  const int64_t M = x->size(0), H = x->size(1), I = w2->size(1);
+  const at::Tensor* w13 = operand(args[1], x->scalar_type(), 2 * I, H);
+  if (w13 == nullptr || operand(args[2], x->scalar_type(), H, I) == nullptr) Py_RETURN_NONE;
+  const bool save = args[4] == Py_True;
+  const int64_t ws_bytes = g_ffn_bytes(M, H, I);
+  at::Tensor out = fresh(x->scalar_type(), {M, H}), gate_up, ws = workspace_of(ws_bytes);
+  if (save) gate_up = fresh(x->scalar_type(), {M, 2 * I});
+  const int code = code_of(x->scalar_type());
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_ffn(x->const_data_ptr(), x->stride(0), code, w13->const_data_ptr(), w13->stride(0), w2->const_data_ptr(), w2->stride(0), limit,
+                 out.mutable_data_ptr(), save ? gate_up.mutable_data_ptr() : nullptr, M, H, I, ws.mutable_data_ptr(), ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  if (!save) return THPVariable_Wrap(std::move(out));
+  return tuple_of(THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(gate_up)));
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_ffn_backward(grad_out, x, w13, w2, gate_up, limit, need_grad_x, need_grad_w13, need_grad_w2) -> (grad_x, grad_w13, grad_w2)
+PyObject* gated_ffn_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  float limit;
+  if (n != 9 || modes_active() || !limit_of(args[5], &limit) || !PyBool_Check(args[6]) || !PyBool_Check(args[7]) || !PyBool_Check(args[8]))
+    Py_RETURN_NONE;
+  const at::Tensor *x = first_operand(args[1]), *w2 = plain(args[3], false), *gate_up;
+  if (x == nullptr || w2 == nullptr || w2->dim() != 2) Py_RETURN_NONE;
+  const int64_t M = x->size(0), H = x->size(1), I = w2->size(1);
+  const at::Tensor *go = operand(args[0], x->scalar_type(), M, H), *w13 = operand(args[2], x->scalar_type(), 2 * I, H);
+  if (go == nullptr || w13 == nullptr || operand(args[3], x->scalar_type(), H, I) == nullptr ||
+      !optional(args[4], x->scalar_type(), M, 2 * I, &gate_up))
+    Py_RETURN_NONE;
+  const bool need[3] = {args[6] == Py_True, args[7] == Py_True, args[8] == Py_True};
+  const int64_t ws_bytes = g_ffn_grad_bytes(M, H, I, gate_up == nullptr);
+  at::Tensor g[3], ws = workspace_of(ws_bytes);
+  if (need[0]) g[0] = fresh(x->scalar_type(), {M, H});
+  if (need[1]) g[1] = fresh(x->scalar_type(), {2 * I, H});
+  if (need[2]) g[2] = fresh(x->scalar_type(), {H, I});
+  void* to[3];
+  for (int i = 0; i < 3; ++i) to[i] = need[i] ? g[i].mutable_data_ptr() : nullptr;
+  const int code = code_of(x->scalar_type());
+  void* const stream = stream_of(*x);
+  int status;
+  Py_BEGIN_ALLOW_THREADS
+  status = g_ffn_grad(go->const_data_ptr(), go->stride(0), code, x->const_data_ptr(), x->stride(0), w13->const_data_ptr(), w13->stride(0),
+                      w2->const_data_ptr(), w2->stride(0), data<void>(gate_up), limit, to[0], to[1], to[2], M, H, I, ws.mutable_data_ptr(),
+                      ws_bytes, stream);
+  Py_END_ALLOW_THREADS
+  if (status != 0) return PyLong_FromLong(status);
+  PyObject* out[3];
+  for (int i = 0; i < 3; ++i) out[i] = need[i] ? THPVariable_Wrap(std::move(g[i])) : Py_NewRef(Py_None);
+  return tuple_of(out[0], out[1], out[2]);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(...): the library's functions, as addresses, in the order of the pointers above
-constexpr Py_ssize_t kFunctions = 10;
+constexpr Py_ssize_t kFunctions = 18;
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != kFunctions) { PyErr_SetString(PyExc_TypeError, "bind: another number of addresses expected"); return nullptr; }
   void* p[kFunctions];
@@ -414,6 +567,14 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_balance_bytes = reinterpret_cast<decltype(g_balance_bytes)>(p[7]);
   g_router_grad = reinterpret_cast<decltype(g_router_grad)>(p[8]);
   g_sum_reduce_grad = reinterpret_cast<decltype(g_sum_reduce_grad)>(p[9]);
+  g_lce = reinterpret_cast<decltype(g_lce)>(p[10]);
+  g_lce_bytes = reinterpret_cast<decltype(g_lce_bytes)>(p[11]);
+  g_lce_grad = reinterpret_cast<decltype(g_lce_grad)>(p[12]);
+  g_lce_grad_bytes = reinterpret_cast<decltype(g_lce_grad_bytes)>(p[13]);
+  g_ffn = reinterpret_cast<decltype(g_ffn)>(p[14]);
+  g_ffn_bytes = reinterpret_cast<decltype(g_ffn_bytes)>(p[15]);
+  g_ffn_grad = reinterpret_cast<decltype(g_ffn_grad)>(p[16]);
+  g_ffn_grad_bytes = reinterpret_cast<decltype(g_ffn_grad_bytes)>(p[17]);
   Py_RETURN_NONE;
 }
 
@@ -425,7 +586,10 @@ PyMethodDef g_methods[] = {method<topk_softmax>("topk_softmax"), method<moe_alig
                            method<moe_sum_reduce>("moe_sum_reduce"), method<token_logprobs>("token_logprobs"),
                            method<token_logprobs_backward>("token_logprobs_backward"), method<moe_balance_loss>("moe_balance_loss"),
                            method<moe_router_backward>("moe_router_backward"),
-                           method<moe_sum_reduce_backward>("moe_sum_reduce_backward"), method<bind>("bind"), {nullptr, nullptr, 0, nullptr}};
+                           method<moe_sum_reduce_backward>("moe_sum_reduce_backward"),
+                           method<linear_cross_entropy>("linear_cross_entropy"),
+                           method<linear_cross_entropy_backward>("linear_cross_entropy_backward"), method<gated_ffn>("gated_ffn"),
+                           method<gated_ffn_backward>("gated_ffn_backward"), method<bind>("bind"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

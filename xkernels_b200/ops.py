@@ -135,15 +135,16 @@ def check_workspace_status(workspace) -> None:
 
 
 def check_status(dev=None, tag: int = 0) -> None:
-    """Synchronise and raise if a kernel of the last fused call on ``dev`` gave up a bounded
-    wait (the tcgen05 kernels never spin without a limit; they record a status word instead)."""
+    """Synchronise and raise if a kernel of the last fused call on ``dev``, or of any dense one there (:func:`gated_ffn`,
+    :func:`linear_cross_entropy` and their gradients), gave up a bounded wait (the tcgen05 kernels never spin without a
+    limit; they record a status word instead)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if dev is None else torch.device(dev)
     key = (dev.index if dev.index is not None else torch.cuda.current_device(), tag)
     buf = _workspaces.get(key)
-    if buf is None:
-        return
     with torch.cuda.device(dev):
-        _lib.check(_lib.load().xkb_workspace_status(buf.data_ptr(), _stream(dev)), "xkb_workspace_status")
+        _lib.check(_lib.load().xkb_dense_status(_stream(dev)), "xkb_dense_status")
+        if buf is not None:
+            _lib.check(_lib.load().xkb_workspace_status(buf.data_ptr(), _stream(dev)), "xkb_workspace_status")
 
 
 def release_workspaces() -> None:
@@ -652,6 +653,11 @@ def linear_cross_entropy(hidden, weight, labels):
     a loss of NaN, a row whose logits hold a NaN or +inf is NaN.  The same bits in every run.  Where :func:`token_logprobs` takes
     logits, this takes what they are made from; its gradient is :func:`linear_cross_entropy_backward`.  No reference counterpart.
     """
+    got = (_lib._calls or _lib.load_calls()).linear_cross_entropy(hidden, weight, labels)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_linear_cross_entropy")
+        return LinearCrossEntropy._make(got)
     lib = _lib.load()
     name = "linear_cross_entropy"
     dev = _require_cuda(name, hidden, weight, labels)
@@ -681,6 +687,12 @@ def linear_cross_entropy_backward(hidden, weight, labels, stats, grad_loss=None,
     vocabulary at a time, so no more than 256 MiB of their gradient are ever held.  Sums are fp32; the gradient of the logits is
     rounded to ``hidden``'s dtype as the operand of the next products.  The same bits in every run.
     """
+    got = (_lib._calls or _lib.load_calls()).linear_cross_entropy_backward(
+        hidden, weight, labels, stats, grad_loss, grad_lse, need_grad_hidden, need_grad_weight)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_linear_cross_entropy_backward")
+        return got
     lib = _lib.load()
     name = "linear_cross_entropy_backward"
     dev = _require_cuda(name, hidden, weight, labels, stats, grad_loss, grad_lse)
@@ -728,6 +740,11 @@ def gated_ffn(x, w13, w2, swiglu_limit=None, save_gate_up=False):
     Returns ``out`` ``[M, H]``, or ``(out, gate_up)`` with ``save_gate_up``: ``[M, 2*I]`` before the limit, for
     :func:`gated_ffn_backward`.  The same bits in every run.  No reference counterpart.
     """
+    got = (_lib._calls or _lib.load_calls()).gated_ffn(x, w13, w2, swiglu_limit, save_gate_up)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_gated_ffn")
+        return got
     lib = _lib.load()
     name = "gated_ffn"
     dev = _require_cuda(name, x, w13, w2)
@@ -757,6 +774,12 @@ def gated_ffn_backward(grad_out, x, w13, w2, gate_up=None, swiglu_limit=None, ne
     then decided on its result rounded to ``x``'s dtype, as with the saved one).  Gradients of gate and up and ``silu(gate) * up`` are
     rounded to ``x``'s dtype once, as operands of the next products; all sums are fp32.  The same bits in every run.
     """
+    got = (_lib._calls or _lib.load_calls()).gated_ffn_backward(
+        grad_out, x, w13, w2, gate_up, swiglu_limit, need_grad_x, need_grad_w13, need_grad_w2)
+    if got is not None:
+        if type(got) is int:
+            _lib.check(got, "xkb_gated_ffn_backward")
+        return got
     lib = _lib.load()
     name = "gated_ffn_backward"
     dev = _require_cuda(name, grad_out, x, w13, w2, gate_up)

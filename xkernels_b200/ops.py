@@ -606,6 +606,12 @@ def token_logprobs_backward(logits, token_ids, stats, entropy=None, grad_logprob
 _HALF_DT = {torch.bfloat16: _lib.XKB_BF16, torch.float16: _lib.XKB_F16}
 
 
+def _given(name, **tensors) -> None:
+    for what, t in tensors.items():
+        if t is None:
+            raise TypeError(f"{name}: {what} is missing")
+
+
 def _matrix(name, what, t, shape, dtype):
     """``t`` as an operand of a dense product: of ``dtype``, rows a multiple of 16 bytes apart, the first on 16 bytes.  Read in
     place where it is one already (a slice of wider rows too); else laid out once more."""
@@ -660,6 +666,7 @@ def linear_cross_entropy(hidden, weight, labels):
         return LinearCrossEntropy._make(got)
     lib = _lib.load()
     name = "linear_cross_entropy"
+    _given(name, hidden=hidden, weight=weight, labels=labels)
     dev = _require_cuda(name, hidden, weight, labels)
     hidden, labels, M, H, V = _linear_head(name, hidden, weight, labels)
     with _on(dev):
@@ -695,6 +702,7 @@ def linear_cross_entropy_backward(hidden, weight, labels, stats, grad_loss=None,
         return got
     lib = _lib.load()
     name = "linear_cross_entropy_backward"
+    _given(name, hidden=hidden, weight=weight, labels=labels, stats=stats)
     dev = _require_cuda(name, hidden, weight, labels, stats, grad_loss, grad_lse)
     if grad_loss is None and grad_lse is None:
         raise ValueError(f"{name}: no gradient is given")
@@ -747,6 +755,7 @@ def gated_ffn(x, w13, w2, swiglu_limit=None, save_gate_up=False):
         return got
     lib = _lib.load()
     name = "gated_ffn"
+    _given(name, x=x, w13=w13, w2=w2)
     dev = _require_cuda(name, x, w13, w2)
     M, H, I = _gated_sizes(name, x, w13, w2)
     limit = 0.0 if swiglu_limit is None else float(swiglu_limit)
@@ -782,6 +791,7 @@ def gated_ffn_backward(grad_out, x, w13, w2, gate_up=None, swiglu_limit=None, ne
         return got
     lib = _lib.load()
     name = "gated_ffn_backward"
+    _given(name, grad_out=grad_out, x=x, w13=w13, w2=w2)
     dev = _require_cuda(name, grad_out, x, w13, w2, gate_up)
     M, H, I = _gated_sizes(name, x, w13, w2)
     limit = 0.0 if swiglu_limit is None else float(swiglu_limit)

@@ -200,6 +200,14 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     d.k_parts = q.k_parts > 1 ? q.k_parts : 1;
     d.end = q.end;
     d.end.vec_out = vec_of(q.end.out, q.end.ld, end == kDswiglu ? q.end.half : 0);
+    // whole tiles of pairs, in the order of the rows
+    d.end.tma_out = s.split == 1 && s.cg == 2 && d.end.vec_out == 16 && q.end.row_map == nullptr && !q.end.acc_out && !q.end.acc_in &&
+                    (end == kStore || end == kCeGrad);
+    if (d.end.tma_out) {
+      rc = make_map_2d_pitched(&d.out, dt, q.end.out, end == kCeGrad ? align_up(q.M, 256) : q.M, q.N, (uint64_t)q.end.ld * 2, 32, 64,
+                               CU_TENSOR_MAP_SWIZZLE_128B, "result");
+      if (rc != XKB_OK) return rc;
+    }
     d.end.vec_h = vec_of(q.end.h, q.end.ld_h);
     d.end.vec_gu = vec_of(q.end.gate_up, q.end.ld_gu, q.end.half);
     tiles += ceil_div(q.M, tile_m) * ceil_div(q.N, tile_n) * d.k_parts;

@@ -50,6 +50,7 @@ struct End {
   int col0;                 // first column of the piece in the vocabulary
   // which vector accesses their rows allow (bytes: 16 or 2), set by the launcher
   int vec_out, vec_h, vec_gu;
+  int tma_out;          // rows of `out` leave by copies of 64 columns, set by the launcher
 };
 
 struct Product {

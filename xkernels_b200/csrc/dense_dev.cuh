@@ -23,7 +23,6 @@ constexpr int kRows = 128;          // rows of D per CTA
 constexpr int kControlWarps = 4;    // 0: TMA of A, 1: MMA, 2: tensor memory, 3: TMA of B; the read-out warps follow
 constexpr int kMaxStages = 12;
 constexpr int kABytes = kRows * 128;
-constexpr int kRowsOut = 32 * 64;   // a warp's 32 rows of 64 bytes on their way to or from memory
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
 // The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, so a long sum drifts towards 0
 // (2^-24 of it a step of 16 K: 5e-6 of the logits at K = 7168).  Where the result stays fp32 (kCeStats) an accumulator takes
@@ -34,7 +33,7 @@ template <int END> __device__ __forceinline__ int parts_of(int kb) {
 }
 
 struct DevProduct {
-  CUtensorMap a, b;
+  CUtensorMap a, b, out;      // out: where end.tma_out is set
   int M, N, K, b_row0;
   const int32_t* live;
   int live_is_k, a_mn;
@@ -72,10 +71,11 @@ template <int CG, int BN, int RW> struct Cfg {
   static constexpr int kThreads = 32 * (kControlWarps + RW);
   static constexpr int kCtas = RW == 4 ? 2 : 1;
   static constexpr int kBBytes = BN / CG * 128;
-  static constexpr int kRing = (RW == 4 ? 102 : 209) * 1024;
+  static constexpr int kRowBytes = CG == 2 ? 32 * 128 : 32 * 64;   // a warp's 32 rows of 128 or 64 bytes on their way
+  static constexpr int kRing = (RW == 4 ? 102 : CG == 2 ? 193 : 209) * 1024;
   static constexpr int kStageBytes = kABytes + kBBytes;      // CG = 2
   static constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
-  static constexpr int kSmem = kRing + RW * kRowsOut + 1024;
+  static constexpr int kSmem = kRing + RW * kRowBytes + 1024;
   static_assert(kRing >= BN * kRows * 4, "the parts of a sum lie where the stages were");
 };
 
@@ -296,6 +296,30 @@ __device__ __forceinline__ void rows_in(uint32_t buf, const void* from, uint32_t
   }
   __syncwarp();
 }
+// 16-bit results of 64 columns leave by a copy of their own: the lanes write their rows, halves of 32 columns, into 128-byte
+// rows (128-byte swizzle), and one lane starts the copy, which the warp does not wait for until the buffer's next use.
+// Full lines reach L2: the products of a head's gradient at 509 x 2048 x 50001, 168 -> 151 us.
+__device__ __forceinline__ void half_rows(uint32_t buf, int half, const uint32_t* w) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(buf + lane * 128 + (((half * 4 + u) ^ (lane & 7)) << 4)), "r"(w[4 * u]), "r"(w[4 * u + 1]), "r"(w[4 * u + 2]),
+                   "r"(w[4 * u + 3]) : "memory");
+}
+__device__ __forceinline__ void rows_copied() {      // what was started has left shared memory
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+__device__ __forceinline__ void copy_rows(uint32_t buf, const CUtensorMap* map, int x, int y) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(buf), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
 // CW columns of this lane's row: together where whole pieces of 32 are aligned, else each lane its own.
 template <int CW>
 __device__ __forceinline__ void put_row(uint32_t buf, void* base, int64_t at, bool live, const uint32_t (&w)[CW / 2], int n, int vec) {
@@ -316,6 +340,7 @@ struct RowState {
   int label;        // column of the label within the piece
   float4 coef;      // kCeGrad
   int64_t to;       // kStore: row of `out`
+  int half;         // of 64 columns that leave together
 };
 
 template <int END> __device__ __forceinline__ void row_begin(const End& e, int row, bool live, RowState& st) {
@@ -377,7 +402,12 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
     }
 #pragma unroll
     for (int j = 0; j < CW; j += 2) o[j / 2] = pack16(fmt, v[j], v[j + 1]);
-    put_row<CW>(buf, e.out, st.to * e.ld + col, live, o, n, e.vec_out);
+    if (CW == 32 && e.tma_out) {
+      if (st.half == 0) rows_copied();
+      half_rows(buf, st.half, o);
+    } else {
+      put_row<CW>(buf, e.out, st.to * e.ld + col, live, o, n, e.vec_out);
+    }
   } else if constexpr (END == kSwiglu) {
     if (e.gate_up != nullptr) {
 #pragma unroll
@@ -477,7 +507,12 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
       }
       o[j / 2] = pack16(fmt, d[0], d[1]);
     }
-    put_row<CW>(buf, e.out, (int64_t)row * e.ld + col, true, o, n, e.vec_out);
+    if (CW == 32 && e.tma_out) {
+      if (st.half == 0) rows_copied();
+      half_rows(buf, st.half, o);
+    } else {
+      put_row<CW>(buf, e.out, (int64_t)row * e.ld + col, true, o, n, e.vec_out);
+    }
   }
 }
 
@@ -599,11 +634,12 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
     __syncwarp();
     if (lane == 0) {
       sh.tiles = t0 + t1 + t2;
-      // The first product's tiles may be longer than the others': in rounds of the others, with the time of a read-out,
-      // which is about that of 8 blocks of K.
+      // The first product's tiles may be longer than the others': in rounds of the others, none of which takes less than a
+      // read-out, the time of 8 blocks of K (5 of a narrow tile).
       sh.long_tiles = p.count > 1 ? t0 : 0;
       sh.rest = sh.long_tiles % clusters;
-      sh.delta = p.count > 1 ? max(1, (sh.of[0].kb / sh.of[0].k_parts + 8 + (sh.of[1].kb + 8) / 2) / (sh.of[1].kb + 8)) : 1;
+      const int round = max(sh.of[1].kb, BN == 256 ? 8 : 5);
+      sh.delta = p.count > 1 ? max(1, (sh.of[0].kb / sh.of[0].k_parts + 4 + round / 2) / round) : 1;
     }
   } else if (warp == 2) {
     tmem_alloc<CG>(&sh.tmem, kTmemCols);
@@ -767,7 +803,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
     }
   } else if (warp >= kControlWarps) {
     const uint32_t tmem = wait_for_tmem();
-    const uint32_t buf = ring + C::kRing + (warp - 4) * kRowsOut;
+    const uint32_t buf = ring + C::kRing + (warp - kControlWarps) * C::kRowBytes;
     const int wg = (warp - 4) >> 2, quad = warp & 3;
     const int in_tile = quad * 32 + lane;
     constexpr int kMine = kTileN * 4 / RW;  // columns of a warpgroup
@@ -793,6 +829,16 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       };
       RowState st;
       row_begin<END>(e, row, live && split == 1, st);
+      if constexpr (END == kDswiglu) {      // gate and up of the tile come to L2 while it is multiplied
+        if (live) {
+          const int c0 = t.n * kTileN + wg * kMine, c1 = min(c0 + kMine, N);
+          const uint16_t* gu = static_cast<const uint16_t*>(e.gate_up) + (int64_t)row * e.ld_gu;
+          for (int c = c0; c < c1; c += 64) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + c));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + e.half + c));
+          }
+        }
+      }
       const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
       if constexpr (END == kCeStats) {
         const int parts = parts_of<END>(t.k1 - t.k0);
@@ -864,13 +910,17 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[j] = w[j] = 0.f;
           }
+          if constexpr (END == kStore || END == kCeGrad) st.half = ((c - wg * kMine) >> 5) & 1;
           row_piece<END, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
+          if constexpr (END == kStore || END == kCeGrad)
+            if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.prod[t.prod].out, col - 32 * st.half, row - lane);
           if (n <= kPiece) break;
         }
       }
     }
   }
   __syncwarp();
+  if (warp >= kControlWarps && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 
   if (split > 1) {
     cluster_sync();       // every CTA's part is in its shared memory

@@ -31,7 +31,7 @@ def make(M, H, I, dtype, dev, seed=0):
 
 # one row to a training batch; sizes below a tile, over a tile's edge, off every multiple; clusters that share a tile, pairs,
 # several rounds of tiles
-SIZES = [(1, 64, 64), (1, 7168, 2048), (2, 8, 8), (3, 65, 33), (1, 1, 1), (17, 200, 72), (64, 512, 256), (128, 1000, 136), (129, 264, 520), (200, 4096, 512),
+SIZES = [(1, 64, 64), (1, 7168, 2048), (3, 20000, 40), (16, 512, 136), (17, 512, 136), (2, 8, 8), (3, 65, 33), (1, 1, 1), (17, 200, 72), (64, 512, 256), (128, 1000, 136), (129, 264, 520), (200, 4096, 512),
          (257, 1024, 1416), (512, 4096, 1416), (1000, 2048, 264), (2048, 1024, 2048)]
 
 

@@ -15,10 +15,8 @@ __device__ int g_dense_status;
 
 namespace {
 
-int sm_count(int* out) {
+int sm_count(int dev, int* out) {
   static std::atomic<int> known[64];
-  int dev = 0;
-  XKB_CHECK_CUDA(cudaGetDevice(&dev));
   int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
   if (n == 0) {
     XKB_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
@@ -28,10 +26,8 @@ int sm_count(int* out) {
   return XKB_OK;
 }
 
-int status_word(int** out) {
+int status_word(int dev, int** out) {
   static std::atomic<int*> known[64];
-  int dev = 0;
-  XKB_CHECK_CUDA(cudaGetDevice(&dev));
   int* p = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
   if (p == nullptr) {
     void* at = nullptr;
@@ -49,8 +45,8 @@ struct Shape { int cg, bn, split; };
 // stage, and the read-out.  A stage takes its MMAs (512 clocks for 256 x 256 on a pair, 256 for the halves) or its operands'
 // bytes at 64 a clock and SM, whichever is more; and the operands have to come from memory once, at 3500 bytes a clock or 36
 // a clock and CTA.  Sharing a tile costs a cluster the exchange of its parts.
-int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, int end, bool may_split, int sms,
-             Shape* best) {
+int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, int end, bool may_split, bool two_terms,
+             int dev, int sms, Shape* best) {
   *best = {2, 256, 1};
   double best_cost = 1e300;
   const bool paired = end == kSwiglu;
@@ -62,6 +58,7 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
     if (cost < best_cost * 0.999) best_cost = cost, *best = s;
   };
   for (int bn : {256, 128}) {
+    if (two_terms) break;
     const int64_t tile_n = paired ? bn / 2 : bn;
     const double stage = bn == 256 ? 520 : 400, readout = bn == 256 ? 3500 : 2000;
     double work = 0;
@@ -79,14 +76,14 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
         const int64_t kb = ceil_div(K[0], kBK);
         if (4 * s > kb || tiles * 2 * s > sms) continue;
         int most = 0;
-        const int rc = clusters_at_once(2, bn, 8, 2 * s, &most);
+        const int rc = clusters_at_once(dev, 2, bn, 8, 2 * s, &most);
         if (rc != XKB_OK) return rc;
         if (tiles <= most) consider({2, bn, s}, 2 * tiles * s, ceil_div(kb, s) * stage, readout + 8000);
       }
   }
   if (count == 1 && may_split) {
     const int warps = single_warps(end);
-    const int64_t kb = ceil_div(K[0], kBK), rows = M[0] < kRows ? align_up(M[0], 8) : kRows;
+    const int64_t kb = ceil_div(K[0], kBK), rows = M[0] < kRows ? align_up(M[0], 8) * (two_terms ? 2 : 1) : kRows;
     for (int bn : {128, 64}) {
       if (bn == 64 && end == kCeStats) continue;
       const int64_t tiles = ceil_div(M[0], kRows) * ceil_div(N[0], paired ? bn / 2 : bn);
@@ -95,7 +92,7 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
       for (int s = 2; s <= 8; ++s) {
         if (4 * s > kb || tiles * s > 2 * sms) continue;
         int most = 0;
-        const int rc = clusters_at_once(1, bn, warps, s, &most);
+        const int rc = clusters_at_once(dev, 1, bn, warps, s, &most);
         if (rc != XKB_OK) return rc;
         if (tiles <= most) consider({1, bn, s}, tiles * s, (double)(ceil_div(tiles * s, sms) * ceil_div(kb, s)) * stage, 4500 + 500 * s);
       }
@@ -112,8 +109,8 @@ int vec_of(const void* p, int64_t ld, int64_t extra = 0) {
 }  // namespace
 
 int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64_t K1) {
-  int sms = 148;
-  if (sm_count(&sms) != XKB_OK) sms = 148;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || sm_count(dev, &sms) != XKB_OK) sms = 148;
   const int64_t pairs = sms / 2, tiles0 = ceil_div(M0, 256) * ceil_div(N0, 256), kb0 = ceil_div(K0, kBK);
   const int64_t tiles1 = M1 > 0 ? ceil_div(M1, 256) * ceil_div(N1, 256) : 0, kb1 = ceil_div(K1, kBK);
   // K blocks of a pair if all work is dealt out evenly, and of a pair with the most long tiles
@@ -124,10 +121,12 @@ int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64
 }
 
 int ce_parts(int64_t M, int64_t N, int64_t K, int* parts) {
-  int sms = 0, one = 1, rc = sm_count(&sms);
+  int dev = 0, sms = 0, one = 1;
+  XKB_CHECK_CUDA(cudaGetDevice(&dev));
+  int rc = sm_count(dev, &sms);
   if (rc != XKB_OK) return rc;
   Shape s;
-  rc = shape_of(&M, &N, &K, &one, 1, kCeStats, true, sms, &s);
+  rc = shape_of(&M, &N, &K, &one, 1, kCeStats, true, false, dev, sms, &s);
   if (rc != XKB_OK) return rc;
   *parts = (int)(ceil_div(N, s.bn) * (s.split > 1 ? s.bn / 8 : 2));
   return XKB_OK;
@@ -141,10 +140,12 @@ int64_t ce_most_parts(int64_t M, int64_t N) {
 
 int launch(const Product* products, int count, int end, int dtype, bool chained, bool early_b, cudaStream_t stream) {
   XKB_REQUIRE(count >= 1 && count <= kMaxProblems, "dense products: %d products", count);
-  int sms = 0, rc = sm_count(&sms);
+  int dev = 0, sms = 0;
+  XKB_CHECK_CUDA(cudaGetDevice(&dev));
+  int rc = sm_count(dev, &sms);
   if (rc != XKB_OK) return rc;
   Params p = {};
-  rc = status_word(&p.status);
+  rc = status_word(dev, &p.status);
   if (rc != XKB_OK) return rc;
   const bool b_mn = products[0].b.k_rows;
   int64_t M[kMaxProblems], N[kMaxProblems], K[kMaxProblems];
@@ -158,15 +159,18 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     XKB_REQUIRE(M[i] > 0 && N[i] > 0 && K[i] > 0 && M[i] < (1ll << 30) && N[i] < (1ll << 30) && K[i] < (1ll << 30),
                 "dense products: sizes out of range");
   }
+  const bool two_terms = products[0].a.rest != 0;
+  XKB_REQUIRE(!two_terms || (count == 1 && end == kStore && !b_mn && !any_a_mn && M[0] <= 64), "dense products: two terms of this product");
   Shape s;
-  rc = shape_of(M, N, K, k_parts, count, end, !any_a_mn && !parted, sms, &s);
+  rc = shape_of(M, N, K, k_parts, count, end, !any_a_mn && !parted, two_terms, dev, sms, &s);
   if (rc != XKB_OK) return rc;
   const int a_rows = s.cg == 1 && !any_a_mn && M[0] < kRows ? (int)align_up(M[0], 8) : kRows;
   const CUtensorMapDataType dt = dtype == XKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   p.count = count;
   p.fmt = dtype == XKB_BF16 ? 1 : 0;
   p.split = s.split;
-  p.a_bytes = a_rows * 128;
+  p.fold = two_terms ? a_rows : 0;
+  p.a_bytes = a_rows * 128 * (two_terms ? 2 : 1);
   p.early_b = early_b ? 1 : 0;
   const int read_warps = s.cg == 2 ? 8 : single_warps(end);
   if (s.cg == 1) {      // a stage's place for A is as large as its rows
@@ -183,7 +187,11 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   for (int i = 0; i < count; ++i) {
     const Product& q = products[i];
     DevProduct& d = p.prod[i];
-    rc = make_map_2d_pitched(&d.a, dt, q.a.base, q.a.rows, q.a.cols, (uint64_t)q.a.pitch * 2, q.a.k_rows ? 64 : a_rows, 64,
+    if (two_terms)
+      rc = make_map_3d_pitched(&d.a, dt, q.a.base, 2, q.a.rows, q.a.cols, (uint64_t)q.a.rest * 2, (uint64_t)q.a.pitch * 2, 2, a_rows, 64,
+                               CU_TENSOR_MAP_SWIZZLE_128B, "left operand");
+    else
+      rc = make_map_2d_pitched(&d.a, dt, q.a.base, q.a.rows, q.a.cols, (uint64_t)q.a.pitch * 2, q.a.k_rows ? 64 : a_rows, 64,
                              CU_TENSOR_MAP_SWIZZLE_128B, "left operand");
     if (rc != XKB_OK) return rc;
     if (end == kSwiglu)      // gate rows and up rows are planes
@@ -212,11 +220,13 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     d.end.vec_gu = vec_of(q.end.gate_up, q.end.ld_gu, q.end.half);
     tiles += ceil_div(q.M, tile_m) * ceil_div(q.N, tile_n) * d.k_parts;
   }
+  XKB_REQUIRE(tiles < (1ll << 31), "dense products: too many tiles");
   Launch l;
-  l.cg = s.cg, l.bn = s.bn, l.split = s.split, l.chained = chained, l.stream = stream;
+  l.dev = dev, l.cg = s.cg, l.bn = s.bn, l.split = s.split, l.chained = chained, l.stream = stream;
   const int margin = g_sm_margin.load(std::memory_order_relaxed);
-  if (s.split > 1) {
-    l.grid = (int)tiles * s.split * s.cg;     // one tile a cluster
+  if (s.split > 1 || two_terms) {
+    XKB_REQUIRE(tiles * s.split * s.cg < (1ll << 31), "dense products: too many tiles");
+    l.grid = (int)(tiles * s.split * s.cg);     // one tile a cluster
   } else {
     int64_t most = (sms - margin) / s.cg * (read_warps == 4 ? 2 : 1);
     if (most < 1) most = 1;
@@ -232,8 +242,10 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
 
 extern "C" int xkb_dense_status(void* stream_) {
   using namespace xkb;
+  int dev = 0;
+  XKB_CHECK_CUDA(cudaGetDevice(&dev));
   int* word = nullptr;
-  const int rc = dense::status_word(&word);
+  const int rc = dense::status_word(dev, &word);
   if (rc != XKB_OK) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   int host = 0;

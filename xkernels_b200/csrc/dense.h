@@ -23,6 +23,7 @@ struct Operand {
   bool k_rows;        // rows in memory are K
   int64_t row0;       // first row in memory (B of a piece of the vocabulary)
   int64_t rows, cols; // extents in memory; what lies outside reads as 0
+  int64_t rest;       // elements to a second term of the same form (left operand of kStore, up to 64 rows; 0: none)
 };
 
 struct End {
@@ -36,6 +37,7 @@ struct End {
   // kSwiglu, kDswiglu
   void* h;
   int64_t ld_h;
+  void* h_rest;             // kSwiglu: what the rounding left of h, rounded itself (nullptr: not wanted)
   void* gate_up;            // [M, 2 * half]
   int64_t ld_gu;
   int half;                 // columns of gate, which are in front of those of up

@@ -49,6 +49,7 @@ struct Params {
   int a_bytes;          // bytes of A that a stage loads
   int a_slot, stages;   // CG = 1: bytes that a stage has for A, stages
   int early_b;
+  int fold;             // CG = 1, kStore: A comes in two terms, row r of the second is row fold + r of the tile (0: one term)
   int* status;
 };
 
@@ -332,6 +333,8 @@ __device__ __forceinline__ void get_row(uint32_t buf, const void* base, int64_t 
   else if (live) load_row<CW>(base, at, w, n, vec);
 }
 
+// What a rounding to `hi` left of x; nothing of an infinity or a NaN (hi holds it).
+__device__ __forceinline__ float finite_rest(float x, float hi) { return fabsf(hi) < INFINITY ? x - hi : 0.f; }
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + exp2_fast(-kLog2e * x)); }
 
 // ---- what becomes of CW columns of a row ---------------------------------------------------------------------
@@ -430,9 +433,19 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
         }
         h[i] = g * sigmoid(g) * u;
       }
+      v[j] = h[0], v[j + 1] = h[1];
       o[j / 2] = pack16(fmt, h[0], h[1]);
     }
     put_row<CW>(buf, e.h, (int64_t)row * e.ld_h + col, live, o, n, e.vec_h);
+    if (e.h_rest != nullptr) {
+#pragma unroll
+      for (int j = 0; j < CW; j += 2) {
+        float hi[2];
+        unpack16(fmt, o[j / 2], hi[0], hi[1]);
+        o[j / 2] = pack16(fmt, finite_rest(v[j], hi[0]), finite_rest(v[j + 1], hi[1]));
+      }
+      put_row<CW>(buf, e.h_rest, (int64_t)row * e.ld_h + col, live, o, n, e.vec_h);
+    }
   } else if constexpr (END == kDswiglu) {
     uint32_t ug[CW / 2], uu[CW / 2];
     const int64_t half = e.half;
@@ -585,6 +598,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   const uint32_t ring = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = p.split, width = CG * split;   // width: CTAs of a cluster
+  const int fold = CG == 1 && END == kStore && !BMN ? p.fold : 0;
+  const bool parked = split > 1 || fold != 0;      // sums are put together in shared memory
   const uint32_t rank = width > 1 ? cluster_rank() : 0;
   const int part = (int)rank / CG, half = (int)rank % CG, first_rank = (int)rank - half;   // of K; of the tile's rows
   const int cluster = blockIdx.x / width, clusters = gridDim.x / width;
@@ -702,7 +717,16 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
         const CUtensorMap* map = &q.a;
         const int m0 = t.m * kRows * CG + half * kRows;
         // (a loop for each orientation, one branch in it: with the choice inside an iteration took 250 clocks for 130)
-        if (q.a_mn == 0) {
+        if (CG == 1 && END == kStore && !BMN && p.fold != 0) {
+          for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
+            if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
+            if (leader) {
+              expect_tx(mine + 8 * slot, bytes);
+              tma_3d<CG>(dst, map, full + 8 * slot, k, m0, 0);
+            }
+            next();
+          }
+        } else if (q.a_mn == 0) {
           for (int k = t.k0 * kBK; k < t.k1 * kBK; k += kBK) {
             if (!wait(empty + 8 * slot, parity, guard, 1)) { ok = false; break; }
             if (leader) {
@@ -828,7 +852,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (c * kRows + in_tile) * 4), "f"(x) : "memory");
       };
       RowState st;
-      row_begin<END>(e, row, live && split == 1, st);
+      row_begin<END>(e, row, live && !parked, st);
       if constexpr (END == kDswiglu) {      // gate and up of the tile come to L2 while it is multiplied
         if (live) {
           const int c0 = t.n * kTileN + wg * kMine, c1 = min(c0 + kMine, N);
@@ -880,8 +904,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
         ++sets;
         if (!wait(tc::smem_u32(&sh.acc_full[set]), ((sets - 1) >> 1) & 1, guard, 4)) break;
         tc::tc_fence_after();
-        if (split > 1) {
-          if (warp_live) {
+        if (parked) {
+          if (fold != 0 ? quad * 32 < 2 * fold : warp_live) {
             for (int c = wg * (BN * 4 / RW); c < (wg + 1) * (BN * 4 / RW); c += 32) {
               float v[32];
               tmem_load(from + c, v);
@@ -922,8 +946,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   __syncwarp();
   if (warp >= kControlWarps && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 
-  if (split > 1) {
-    cluster_sync();       // every CTA's part is in its shared memory
+  if (parked) {
+    if (split > 1) cluster_sync();       // every CTA's part is in its shared memory
+    else __syncthreads();
     Tile t;
     if (warp >= kControlWarps && Walk(sh, cluster, clusters).get(sh, t) && !guard.aborted()) {
       // Pieces of eight columns, dealt out to the parts; a warp takes a piece of 32 rows.  Rows behind the last are nothing
@@ -945,28 +970,29 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
         if (n > 0 && quad * 32 < rows) {
-          // two parts' loads at a time: each is a round trip to another SM
+          // some parts' loads at a time: each is a round trip to another SM
+          constexpr int kAtOnce = kPaired ? 2 : 4;
           const uint32_t at = ring + (c * kRows + in_tile) * 4;
-          for (int from = 0; from < split; from += 2) {
-            const uint32_t x = map_to(at, from * CG + half), y = map_to(at, min(from + 1, split - 1) * CG + half);
-            float a[2][8], b[2][8];
+          for (int from = 0; from < split; from += kAtOnce) {
+            float a[kAtOnce][8], b[kAtOnce][8];      // b: of up, or the second term's
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              a[0][j] = ld_cluster(x + j * kRows * 4);
-              a[1][j] = ld_cluster(y + j * kRows * 4);
-              if constexpr (kPaired) {
-                b[0][j] = ld_cluster(x + (BN / 2 + j) * kRows * 4);
-                b[1][j] = ld_cluster(y + (BN / 2 + j) * kRows * 4);
+            for (int i = 0; i < kAtOnce; ++i) {
+              const uint32_t x = map_to(at, min(from + i, split - 1) * CG + half);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                a[i][j] = ld_cluster(x + j * kRows * 4);
+                if constexpr (kPaired) b[i][j] = ld_cluster(x + (BN / 2 + j) * kRows * 4);
+                else if (fold != 0) b[i][j] = ld_cluster(x + (j * kRows + fold) * 4);
               }
             }
-            const bool two = from + 1 < split;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              v[j] += a[0][j];
-              if (two) v[j] += a[1][j];
-              if constexpr (kPaired) {
-                w[j] += b[0][j];
-                if (two) w[j] += b[1][j];
+            for (int i = 0; i < kAtOnce; ++i) {
+              if (from + i >= split) break;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                v[j] += a[i][j];
+                if constexpr (kPaired) w[j] += b[i][j];
+                else if (fold != 0) v[j] += b[i][j];
               }
             }
           }
@@ -990,7 +1016,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
 
 // ---- host ----------------------------------------------------------------------------------------------------
 struct Launch {
-  int cg, bn, split, grid;
+  int dev, cg, bn, split, grid;
   bool chained;
   cudaStream_t stream;
 };
@@ -1000,9 +1026,7 @@ int run_kernel(const Params& p, const Launch& l) {
   using C = Cfg<CG, BN, RW>;
   auto kernel = dense_kernel<CG, BN, RW, BMN, END>;
   static std::atomic<uint64_t> ready{0};      // devices on which this instance is set up
-  int dev = 0;
-  XKB_CHECK_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  const uint64_t bit = l.dev < 64 ? 1ull << l.dev : 0;
   if (bit == 0 || !(ready.load(std::memory_order_acquire) & bit)) {
     XKB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     ready.fetch_or(bit, std::memory_order_release);
@@ -1044,8 +1068,8 @@ int run_variant(const Params& p, const Launch& l) {
   return run_kernel<1, 128, single_warps(END), BMN, END>(p, l);
 }
 
-// How many clusters of so many CTAs of one of the kernels' sizes run at once on this device.
-int clusters_at_once(int cg, int bn, int read_warps, int width, int* out);
+// How many clusters of so many CTAs of one of the kernels' sizes run at once on a device, the current one.
+int clusters_at_once(int dev, int cg, int bn, int read_warps, int width, int* out);
 
 // one per translation unit
 int run_ffn(int end, const Params& p, const Launch& l);

@@ -27,11 +27,9 @@ template <int CG, int BN, int RW> int ask(int width, int* out) {
 }  // namespace
 
 // (The kernels differ in registers, but not in how many CTAs an SM holds.)
-int clusters_at_once(int cg, int bn, int read_warps, int width, int* out) {
+int clusters_at_once(int dev, int cg, int bn, int read_warps, int width, int* out) {
   static std::atomic<int> known[64][4][9];
   const int kind = cg == 2 ? (bn == 256 ? 0 : 1) : read_warps == 8 ? 2 : 3;     // (64 columns take the room of 128)
-  int dev = 0;
-  XKB_CHECK_CUDA(cudaGetDevice(&dev));
   int n = dev < 64 ? known[dev][kind][width].load(std::memory_order_relaxed) : 0;
   if (n == 0) {
     const int rc = kind == 0   ? ask<2, 256, 8>(width, &n)

@@ -21,6 +21,12 @@ namespace {
 
 int64_t pitch8(int64_t n) { return align_up(n, 8); }
 
+// Up to so many rows the activations go into the second product in two 16-bit terms, which leaves of their rounding 2^-16 (bf16)
+// or 2^-22 (fp16): a tile of the MMAs has 128 rows whatever they hold, so the second term's rows cost nothing but their copies
+// (one row of 7168 x 2048 28.5 -> 29.1 us).  With few rows the rounding errors of a row's few large activations do not average out: that row's
+// result was 2.5e-3 off in the norm with one term, and is 1.6e-3 off with two, which its own rounding is.
+constexpr int64_t kTwoTerms = 16;
+
 int check_sizes(const char* name, int dtype, int64_t M, int64_t H, int64_t I) {
   XKB_REQUIRE(dtype == XKB_BF16 || dtype == XKB_F16, "%s: dtype must be bf16 or fp16", name);
   XKB_REQUIRE(M >= 0 && H >= 1 && I >= 1 && M < (1ll << 28) && H < (1ll << 24) && I < (1ll << 24), "%s: M=%lld H=%lld I=%lld out of range",
@@ -49,7 +55,7 @@ using namespace xkb;
 
 extern "C" int64_t xkb_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I) {
   if (check_sizes("gated_ffn", XKB_BF16, M, H, I) != XKB_OK) return -1;
-  return align_up(M * pitch8(I) * 2, 256);
+  return (M <= kTwoTerms ? 2 : 1) * align_up(M * pitch8(I) * 2, 256);
 }
 
 extern "C" int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void* w13, int64_t ld_w13, const void* w2, int64_t ld_w2,
@@ -71,12 +77,14 @@ extern "C" int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void*
   up.a = {x, ld_x, false, 0, M, H};
   up.b = {w13, ld_w13, false, 0, 2 * I, H};
   up.M = M, up.N = I, up.K = H;
+  const int64_t rest = M <= kTwoTerms ? align_up(M * pitch8(I) * 2, 256) / 2 : 0;
   up.end.h = workspace, up.end.ld_h = pitch8(I);
+  if (rest != 0) up.end.h_rest = static_cast<uint16_t*>(workspace) + rest;
   up.end.gate_up = gate_up, up.end.ld_gu = 2 * I, up.end.half = (int)I;
   up.end.limit = limit;
   XKB_TRY(launch(&up, 1, kSwiglu, dtype, false, false, stream));
   Product down = {};
-  down.a = {workspace, pitch8(I), false, 0, M, I};
+  down.a = {workspace, pitch8(I), false, 0, M, I, rest};
   down.b = {w2, ld_w2, false, 0, H, I};
   down.M = M, down.N = H, down.K = I;
   down.end.out = out, down.end.ld = H;

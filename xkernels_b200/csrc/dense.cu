@@ -45,6 +45,10 @@ struct Shape { int cg, bn, split; };
 // stage, and the read-out.  A stage takes its MMAs (512 clocks for 256 x 256 on a pair, 256 for the halves) or its operands'
 // bytes at 64 a clock and SM, whichever is more; and the operands have to come from memory once, at 3500 bytes a clock or 36
 // a clock and CTA.  Sharing a tile costs a cluster the exchange of its parts.
+// Forced one by one, whole calls of gated_ffn: one row of 7168 x 2048, gate and up in single CTAs of 64 columns shared by
+// 2 / 1 / 3 / 4 27.1 / 33.7 / 29.5 / 28.5 us, of 128 by 4 27.4; the second product in 64 columns shared by 1 / 2 / 3 27.1 / 29.1 /
+// 33.3, in 128 by 2 29.0.  509 rows of 4096 x 1416: gate and up in pairs of 128 / 256 columns 31.3 / 40.8, 256 shared by 2 34.6,
+// single CTAs of 128 by 1 / 2 / 3 44.0 / 34.7 / 33.5.  (64 rows: by 4 28.8, by 2, which the rule takes, 30.1.)
 int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_parts, int count, int end, bool may_split, bool two_terms,
              int dev, int sms, Shape* best) {
   *best = {2, 256, 1};
@@ -188,17 +192,17 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     const Product& q = products[i];
     DevProduct& d = p.prod[i];
     if (two_terms)
-      rc = make_map_3d_pitched(&d.a, dt, q.a.base, 2, q.a.rows, q.a.cols, (uint64_t)q.a.rest * 2, (uint64_t)q.a.pitch * 2, 2, a_rows, 64,
+      rc = make_map_3d_pitched(&p.a[i], dt, q.a.base, 2, q.a.rows, q.a.cols, (uint64_t)q.a.rest * 2, (uint64_t)q.a.pitch * 2, 2, a_rows, 64,
                                CU_TENSOR_MAP_SWIZZLE_128B, "left operand");
     else
-      rc = make_map_2d_pitched(&d.a, dt, q.a.base, q.a.rows, q.a.cols, (uint64_t)q.a.pitch * 2, q.a.k_rows ? 64 : a_rows, 64,
+      rc = make_map_2d_pitched(&p.a[i], dt, q.a.base, q.a.rows, q.a.cols, (uint64_t)q.a.pitch * 2, q.a.k_rows ? 64 : a_rows, 64,
                              CU_TENSOR_MAP_SWIZZLE_128B, "left operand");
     if (rc != XKB_OK) return rc;
     if (end == kSwiglu)      // gate rows and up rows are planes
-      rc = make_map_3d_pitched(&d.b, dt, q.b.base, 2, q.N, q.b.cols, (uint64_t)q.N * q.b.pitch * 2, (uint64_t)q.b.pitch * 2, 2 / s.cg,
+      rc = make_map_3d_pitched(&p.b[i], dt, q.b.base, 2, q.N, q.b.cols, (uint64_t)q.N * q.b.pitch * 2, (uint64_t)q.b.pitch * 2, 2 / s.cg,
                                s.bn / 2, 64, CU_TENSOR_MAP_SWIZZLE_128B, "right operand");
     else
-      rc = make_map_2d_pitched(&d.b, dt, q.b.base, q.b.rows, q.b.cols, (uint64_t)q.b.pitch * 2, b_mn ? 64 : s.bn / s.cg, 64,
+      rc = make_map_2d_pitched(&p.b[i], dt, q.b.base, q.b.rows, q.b.cols, (uint64_t)q.b.pitch * 2, b_mn ? 64 : s.bn / s.cg, 64,
                                CU_TENSOR_MAP_SWIZZLE_128B, "right operand");
     if (rc != XKB_OK) return rc;
     d.M = (int)q.M, d.N = (int)q.N, d.K = (int)q.K, d.b_row0 = (int)q.b.row0;
@@ -212,7 +216,7 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     d.end.tma_out = s.split == 1 && s.cg == 2 && d.end.vec_out == 16 && q.end.row_map == nullptr && !q.end.acc_out && !q.end.acc_in &&
                     (end == kStore || end == kCeGrad);
     if (d.end.tma_out) {
-      rc = make_map_2d_pitched(&d.out, dt, q.end.out, end == kCeGrad ? align_up(q.M, 256) : q.M, q.N, (uint64_t)q.end.ld * 2, 32, 64,
+      rc = make_map_2d_pitched(&p.out[i], dt, q.end.out, end == kCeGrad ? align_up(q.M, 256) : q.M, q.N, (uint64_t)q.end.ld * 2, 32, 64,
                                CU_TENSOR_MAP_SWIZZLE_128B, "result");
       if (rc != XKB_OK) return rc;
     }

@@ -33,7 +33,6 @@ template <int END> __device__ __forceinline__ int parts_of(int kb) {
 }
 
 struct DevProduct {
-  CUtensorMap a, b, out;      // out: where end.tma_out is set
   int M, N, K, b_row0;
   const int32_t* live;
   int live_is_k, a_mn;
@@ -42,8 +41,8 @@ struct DevProduct {
   End end;
 };
 
+// (What a kernel needs first stands first: a line of parameters that nobody has touched yet is a trip to L2.)
 struct Params {
-  DevProduct prod[kMaxProblems];
   int count, fmt;       // fmt: 1 bf16, 0 fp16
   int split;            // CTAs (pairs) of a cluster that share a tile, a part of K each
   int a_bytes;          // bytes of A that a stage loads
@@ -51,6 +50,8 @@ struct Params {
   int early_b;
   int fold;             // CG = 1, kStore: A comes in two terms, row r of the second is row fold + r of the tile (0: one term)
   int* status;
+  DevProduct prod[kMaxProblems];
+  CUtensorMap a[kMaxProblems], b[kMaxProblems], out[kMaxProblems];      // out: where end.tma_out is set
 };
 
 // A product in tiles, in shared memory: a role looks a tile up with a handful of loads side by side.
@@ -114,14 +115,6 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, uin
   else
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
-  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void prefetch_2d(const CUtensorMap* map, int x, int y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
 }
 // By the lane whose `leader` is not 0; all lanes of the warp call with the same operands.
 template <int CG>
@@ -258,8 +251,8 @@ template <int CW> __device__ __forceinline__ void load_row(const void* base, int
 }
 
 // 64 bytes of 32 rows, lane = row, to memory: through shared memory, so that four lanes write a row's 64 bytes side by side
-// (a lane that writes its own row touches one sector of 32 lines an instruction: 3500 clocks a tile of 128 x 128 where this
-// takes 900).  to: this lane's row, 16-byte aligned; nullptr: not written.  All lanes of the warp call.
+// (a lane that writes its own row touches one sector of 32 lines an instruction).  to: this lane's row, 16-byte aligned;
+// nullptr: not written.  All lanes of the warp call.
 __device__ __forceinline__ uint32_t rows_at(uint32_t buf, int row, int unit) { return buf + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4); }
 __device__ __forceinline__ void rows_out(uint32_t buf, void* to, const uint32_t* w) {
   const int lane = threadIdx.x & 31;
@@ -659,8 +652,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   } else if (warp == 2) {
     tmem_alloc<CG>(&sh.tmem, kTmemCols);
   } else if (warp == 3 && lane < p.count) {
-    tc::prefetch_tensormap(&p.prod[lane].a);
-    tc::prefetch_tensormap(&p.prod[lane].b);
+    tc::prefetch_tensormap(&p.a[lane]);
+    tc::prefetch_tensormap(&p.b[lane]);
   }
   // Loads may start when the barriers and the plan are there (for a pair: the other CTA's barriers too); tensor memory can
   // take longer.
@@ -679,8 +672,8 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
   };
   if (warp == 0 || warp == 3) {
     // Warp 0 feeds A, warp 3 feeds B.  The whole warp runs the loop and one lane issues: operands then sit in uniform
-    // registers (in a loop of one lane a copy took its issuer 200 clocks, and both operands' 600 a stage where the MMAs
-    // take 512).
+    // registers (a stage took its issuer 312 clocks in a loop of one lane, 136 so; one warp for both operands was slower
+    // than the MMAs, 600 against 512).
     const bool leader = tc::elect_one(), feeds_a = warp == 0;
     if (p.early_b && feeds_a) chain_wait();
     const uint32_t bytes = (uint32_t)(p.a_bytes + C::kBBytes) * CG;
@@ -688,33 +681,23 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
     const uint32_t mine = tc::smem_u32(sh.full), full = CG == 2 ? map_to(mine, first_rank) : mine;   // the first CTA's count
     uint32_t slot = 0, parity = 1, dst = ring + (feeds_a ? 0 : a_slot);
     bool ok = true;
+    // The bounded waits count this kernel's own time: a role waits for the predecessor before the first that could last, which
+    // for B is when the ring is full.
+    bool ahead = p.early_b && !feeds_a;
     auto next = [&]() {
       dst += stage_bytes;
-      if (++slot == stages) slot = 0, parity ^= 1, dst -= stages * stage_bytes;
+      if (++slot == stages) {
+        slot = 0, parity ^= 1, dst -= stages * stage_bytes;
+        if (ahead) chain_wait();
+        ahead = false;
+      }
     };
     Tile t;
-    if (p.early_b && !feeds_a && Walk(sh, cluster, clusters).get(sh, t)) {
-      // While the predecessor runs: B of the first tile that the ring has no place for, as far as L2.  (An expert's second
-      // weights, 29 MB, come in beside its first ones: one row 27.6 -> 23 us a call.)
-      share(t);
-      const DevProduct& q = p.prod[t.prod];
-      if (leader)
-        for (int k = (t.k0 + (int)stages) * kBK; k < t.k1 * kBK; k += kBK) {
-          if constexpr (kPaired) {
-            prefetch_3d(&q.b, k, t.n * kTileN, half);
-          } else if constexpr (!BMN) {
-            prefetch_2d(&q.b, k, q.b_row0 + t.n * BN + half * (BN / 2));
-          } else {
-            for (int j = 0; j < BN / CG / 64; ++j) prefetch_2d(&q.b, t.n * BN + half * (BN / 2) + 64 * j, q.b_row0 + k);
-          }
-        }
-      __syncwarp();
-    }
     for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
       const DevProduct& q = p.prod[t.prod];
       share(t);
       if (feeds_a) {
-        const CUtensorMap* map = &q.a;
+        const CUtensorMap* map = &p.a[t.prod];
         const int m0 = t.m * kRows * CG + half * kRows;
         // (a loop for each orientation, one branch in it: with the choice inside an iteration took 250 clocks for 130)
         if (CG == 1 && END == kStore && !BMN && p.fold != 0) {
@@ -747,7 +730,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
           }
         }
       } else {
-        const CUtensorMap* map = &q.b;
+        const CUtensorMap* map = &p.b[t.prod];
         if constexpr (!BMN) {
           // gate and up rows of the same columns (planes of one map): both, or this CTA's half
           const int r0 = kPaired ? t.n * kTileN : q.b_row0 + t.n * BN + half * (BN / 2);
@@ -776,6 +759,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
     wait_for_tmem();
   } else if (warp == 1) {
     const uint32_t tmem = wait_for_tmem();
+    if (p.early_b) chain_wait();
     if (half == 0) {
       const uint32_t base_idesc = (1u << 4) | ((uint32_t)p.fmt << 7) | ((uint32_t)p.fmt << 10) | ((BMN ? 1u : 0u) << 16) |
                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)((kRows * CG) >> 4) << 24);
@@ -832,6 +816,11 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
     const int in_tile = quad * 32 + lane;
     constexpr int kMine = kTileN * 4 / RW;  // columns of a warpgroup
     constexpr int kPiece = RW == 4 && END == kDswiglu ? 16 : 32;    // (as many as registers allow)
+    {      // the parameters of the end come to the SM while the first tile is multiplied (77 x 2056 x 32001 35.1 -> 34.4 us)
+      const End& e = p.prod[0].end;
+      asm volatile("" ::"l"(e.out), "l"(e.ld), "l"(e.h), "l"(e.h_rest), "l"(e.gate_up), "l"(e.ld_gu), "r"(e.half), "f"(e.limit), "r"(e.vec_out),
+                   "r"(e.vec_h), "r"(e.vec_gu), "r"(e.tma_out), "l"(e.acc), "l"(e.part), "l"(e.given));
+    }
     if (p.early_b) chain_wait();
     uint32_t sets = 0;
     Tile t;
@@ -937,7 +926,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
           if constexpr (END == kStore || END == kCeGrad) st.half = ((c - wg * kMine) >> 5) & 1;
           row_piece<END, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
           if constexpr (END == kStore || END == kCeGrad)
-            if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.prod[t.prod].out, col - 32 * st.half, row - lane);
+            if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.out[t.prod], col - 32 * st.half, row - lane);
           if (n <= kPiece) break;
         }
       }

@@ -178,7 +178,7 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   p.early_b = early_b ? 1 : 0;
   const int read_warps = s.cg == 2 ? 8 : single_warps(end);
   if (s.cg == 1) {      // a stage's place for A is as large as its rows
-    const int ring = read_warps == 4 ? Cfg<1, 128, 4>::kRing : Cfg<1, 128, 8>::kRing;
+    const int ring = read_warps == 4 ? Cfg<1, 128, 4, kStore>::kRing : Cfg<1, 128, 8, kCeStats>::kRing;
     p.a_slot = (int)align_up(p.a_bytes, 1024);
     p.stages = ring / ((p.a_slot + s.bn * 128));
     if (p.stages > kMaxStages) p.stages = kMaxStages;

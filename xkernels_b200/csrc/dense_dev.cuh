@@ -69,12 +69,13 @@ struct Shared {
 };
 
 // CG: CTAs of a pair; BN: columns of a tile; RW: read-out warps.  RW = 4 leaves room for two CTAs on an SM.
-template <int CG, int BN, int RW> struct Cfg {
+template <int CG, int BN, int RW, int END> struct Cfg {
   static constexpr int kThreads = 32 * (kControlWarps + RW);
   static constexpr int kCtas = RW == 4 ? 2 : 1;
   static constexpr int kBBytes = BN / CG * 128;
-  static constexpr int kRowBytes = CG == 2 ? 32 * 128 : 32 * 64;   // a warp's 32 rows of 128 or 64 bytes on their way
-  static constexpr int kRing = (RW == 4 ? 102 : CG == 2 ? 193 : 209) * 1024;
+  // a warp's 32 rows of 64 or 128 bytes on their way; kDswiglu: of its result, of gate and of up
+  static constexpr int kRowBytes = 32 * 64 * (CG == 1 ? 1 : END == kDswiglu ? 3 : 2);
+  static constexpr int kRing = (RW == 4 ? 102 : CG == 1 ? 209 : END == kDswiglu ? 177 : 193) * 1024;
   static constexpr int kStageBytes = kABytes + kBBytes;      // CG = 2
   static constexpr int kStages = kRing / kStageBytes < 8 ? kRing / kStageBytes : 8;
   static constexpr int kSmem = kRing + RW * kRowBytes + 1024;
@@ -270,6 +271,25 @@ __device__ __forceinline__ void rows_out(uint32_t buf, void* to, const uint32_t*
   }
   __syncwarp();
 }
+// The first half of rows_in: starts copies of the rows into the buffer that nothing waits for yet.
+__device__ __forceinline__ void rows_start(uint32_t buf, const void* from) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + (lane >> 2);
+    const char* p = reinterpret_cast<const char*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(from), row));
+    if (p != nullptr)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(rows_at(buf, row, lane & 3)), "l"(p + (lane & 3) * 16) : "memory");
+  }
+}
+__device__ __forceinline__ void rows_take(uint32_t buf, uint32_t* w) {      // of rows that have arrived
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint4 x = tc::lds128(rows_at(buf, lane, u));
+    w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
+  }
+}
 __device__ __forceinline__ void rows_in(uint32_t buf, const void* from, uint32_t* w) {
   const int lane = threadIdx.x & 31;
   uint4 v[4];
@@ -337,6 +357,8 @@ struct RowState {
   float4 coef;      // kCeGrad
   int64_t to;       // kStore: row of `out`
   int half;         // of 64 columns that leave together
+  bool here;        // kDswiglu: gate and up of the piece are in the buffers behind `buf`
+  const uint16_t* next;   // gate of the next piece (nullptr: none that is copied ahead)
 };
 
 template <int END> __device__ __forceinline__ void row_begin(const End& e, int row, bool live, RowState& st) {
@@ -442,8 +464,20 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
   } else if constexpr (END == kDswiglu) {
     uint32_t ug[CW / 2], uu[CW / 2];
     const int64_t half = e.half;
-    get_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + col, live, ug, n, e.vec_gu);
-    get_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + half + col, live, uu, n, e.vec_gu);
+    if (CW == 32 && st.here) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      rows_take(buf + 2048, ug);
+      rows_take(buf + 4096, uu);
+      __syncwarp();
+      if (st.next != nullptr) {      // (the same in all lanes but for rows that are none)
+        rows_start(buf + 2048, live ? st.next : nullptr);
+        rows_start(buf + 4096, live ? st.next + half : nullptr);
+      }
+    } else {
+      get_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + col, live, ug, n, e.vec_gu);
+      get_row<CW>(buf, e.gate_up, (int64_t)row * e.ld_gu + half + col, live, uu, n, e.vec_gu);
+    }
 #pragma unroll
     for (int j = 0; j < CW; j += 2) {
       float g[2], u[2], dg[2], du[2], h[2];
@@ -581,8 +615,8 @@ struct Walk {
 };
 
 template <int CG, int BN, int RW, bool BMN, int END>
-__global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kCtas) dense_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<CG, BN, RW>;
+__global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW, END>::kCtas) dense_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<CG, BN, RW, END>;
   constexpr bool kPaired = END == kSwiglu;
   constexpr int kTileN = kPaired ? BN / 2 : BN;    // columns of the result
   constexpr int kTmemCols = 2 * BN;
@@ -842,14 +876,14 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
       };
       RowState st;
       row_begin<END>(e, row, live && !parked, st);
-      if constexpr (END == kDswiglu) {      // gate and up of the tile come to L2 while it is multiplied
-        if (live) {
-          const int c0 = t.n * kTileN + wg * kMine, c1 = min(c0 + kMine, N);
-          const uint16_t* gu = static_cast<const uint16_t*>(e.gate_up) + (int64_t)row * e.ld_gu;
-          for (int c = c0; c < c1; c += 64) {
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + c));
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(gu + e.half + c));
-          }
+      // Gate and up of a piece are copied ahead while the one before it, or the tile, is computed.  (Loaded when they were
+      // needed, a piece of 32 columns took 6 us, and the read-out of a tile 21 to 32 beside 41 of its MMAs.)
+      const uint16_t* gate_row = nullptr;
+      if constexpr (END == kDswiglu && CG == 2) {
+        gate_row = static_cast<const uint16_t*>(e.gate_up) + (int64_t)row * e.ld_gu + t.n * kTileN;
+        if (!parked && warp_live && e.vec_gu == 16 && t.n * kTileN + wg * kMine + 32 <= N) {
+          rows_start(buf + 2048, live ? gate_row + wg * kMine : nullptr);
+          rows_start(buf + 4096, live ? gate_row + wg * kMine + e.half : nullptr);
         }
       }
       const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
@@ -924,6 +958,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
             for (int j = 0; j < kPiece; ++j) v[j] = w[j] = 0.f;
           }
           if constexpr (END == kStore || END == kCeGrad) st.half = ((c - wg * kMine) >> 5) & 1;
+          if constexpr (END == kDswiglu) {
+            st.here = CG == 2 && e.vec_gu == 16 && n >= 32;
+            st.next = CG == 2 && e.vec_gu == 16 && n >= 64 && c + 32 < (wg + 1) * kMine ? gate_row + c + 32 : nullptr;
+          }
           row_piece<END, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
           if constexpr (END == kStore || END == kCeGrad)
             if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.out[t.prod], col - 32 * st.half, row - lane);
@@ -955,6 +993,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW>::kThreads, Cfg<CG, BN, RW>::kC
         const bool live = row < t.rows;
         RowState st;
         row_begin<END>(e, row, live, st);
+        if constexpr (END == kDswiglu) st.here = false, st.next = nullptr;
         float v[8], w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = w[j] = 0.f;
@@ -1012,7 +1051,7 @@ struct Launch {
 
 template <int CG, int BN, int RW, bool BMN, int END>
 int run_kernel(const Params& p, const Launch& l) {
-  using C = Cfg<CG, BN, RW>;
+  using C = Cfg<CG, BN, RW, END>;
   auto kernel = dense_kernel<CG, BN, RW, BMN, END>;
   static std::atomic<uint64_t> ready{0};      // devices on which this instance is set up
   const uint64_t bit = l.dev < 64 ? 1ull << l.dev : 0;

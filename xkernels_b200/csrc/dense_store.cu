@@ -7,7 +7,7 @@ namespace dense {
 namespace {
 
 template <int CG, int BN, int RW> int ask(int width, int* out) {
-  using C = Cfg<CG, BN, RW>;
+  using C = Cfg<CG, BN, RW, kStore>;
   auto kernel = dense_kernel<CG, BN, RW, false, kStore>;
   XKB_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
   cudaLaunchConfig_t cfg = {};

@@ -308,6 +308,14 @@ int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_grad_out, int dtype,
                            int64_t I, void* workspace, int64_t workspace_bytes,
                            void* stream);
 
+/* Up to XKB_LAY_OUT_MOST matrices of 16-bit elements [rows, cols] (row stride ld, any
+ * alignment of 2 bytes) copied to rows of cols rounded up to 8 elements, as the four calls
+ * above want their operands.  The arrays are in host memory.  One launch. */
+#define XKB_LAY_OUT_MOST 4
+int xkb_lay_out_rows(const void* const* from_host, const int64_t* ld_host,
+                     const int64_t* rows_host, const int64_t* cols_host,
+                     void* const* to_host, int count, void* stream);
+
 /* Synchronises `stream` and reports (XKB_ERR_DEVICE) whether a kernel of the four calls
  * above gave up a bounded wait on the current device since the last report. */
 int xkb_dense_status(void* stream);

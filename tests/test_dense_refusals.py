@@ -86,6 +86,23 @@ def test_linear_cross_entropy_backward(lib):
     assert size(-1, 8, 8) == -1 and size(0, 8, 8) == 0
 
 
+def test_lay_out_rows(lib):
+    arrays = lambda t, *v: (t * 4)(*v)  # noqa: E731
+    ok = dict(f=arrays(ctypes.c_void_p, P, P), ld=arrays(ctypes.c_int64, 9, 9), rows=arrays(ctypes.c_int64, 0, 0), cols=arrays(ctypes.c_int64, 9, 3),
+              to=arrays(ctypes.c_void_p, P, P), count=2)
+
+    def call(**kw):
+        a = {**ok, **kw}
+        return lib.xkb_lay_out_rows(a["f"], a["ld"], a["rows"], a["cols"], a["to"], a["count"], None)
+
+    assert call() == 0 and call(count=0, f=None) == 0
+    for bad in (dict(count=5), dict(count=-1), dict(f=None), dict(to=None), dict(rows=arrays(ctypes.c_int64, 0, -1)), dict(cols=arrays(ctypes.c_int64, 0, 3)),
+                dict(ld=arrays(ctypes.c_int64, -1, 9)), dict(rows=arrays(ctypes.c_int64, 0, 1), f=arrays(ctypes.c_void_p, P, None)),
+                dict(rows=arrays(ctypes.c_int64, 1, 0), to=arrays(ctypes.c_void_p, P + 1, P))):
+        assert call(**bad) == -1, bad
+        assert b"lay_out_rows" in lib.xkb_last_error()
+
+
 def test_there_is_no_cpu_path(lib):
     x, w, labels = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(9, 8, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
     w13, w2, st, g = torch.zeros(12, 8, dtype=torch.bfloat16), torch.zeros(8, 6, dtype=torch.bfloat16), torch.zeros(4, 2), torch.zeros(4)

@@ -46,6 +46,19 @@ def test_calls_of_the_python_form(served, cuda_device):  # noqa: F811
     assert served == ["gated_ffn"]
     got = xkb.gated_ffn(x, w13, w2, 2), xkb.gated_ffn(x, w13.t().contiguous().t(), w2, 2.0)       # a whole number, turned weights
     assert served == ["gated_ffn"] and all(torch.equal(a, want) for a in got)
-    xkb.linear_cross_entropy(n(5, 23), n(30, 23), labels)                                         # rows of no whole 16 bytes
+    xkb.linear_cross_entropy(n(5, 23), n(23, 30).t(), labels)                                     # turned weights
+    assert served == ["gated_ffn"]
     xkb.linear_cross_entropy(x, w.requires_grad_(), labels)                                       # (a leaf is served: nothing is recorded here)
     assert served == ["gated_ffn", "linear_cross_entropy"]
+
+
+@pytest.mark.parametrize("H,I", [(23, 9), (24, 9), (23, 16), (257, 130)])
+def test_rows_of_no_whole_16_bytes(H, I, served, cuda_device):  # noqa: F811
+    g = torch.Generator(device=cuda_device).manual_seed(H + I)
+    x, w13, w2, w = (torch.randn(s, generator=g, device=cuda_device).to(torch.bfloat16) / 8 for s in ((37, H), (2 * I, H), (H, I), (60, H)))
+    labels = torch.randint(-1, 60, (37,), generator=g, device=cuda_device)
+    out, gate_up = _both(lambda: xkb.gated_ffn(x, w13, w2, None, True))
+    _both(lambda: xkb.gated_ffn_backward(out, x, w13, w2, gate_up))
+    r = xkb.LinearCrossEntropy(*_both(lambda: xkb.linear_cross_entropy(x, w, labels)))
+    _both(lambda: xkb.linear_cross_entropy_backward(x, w, labels, r.stats, r.loss))
+    assert len(served) == 4

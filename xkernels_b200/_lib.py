@@ -97,6 +97,7 @@ SIGNATURES = {
         [c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_void_p,
          c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p],
     ),
+    "xkb_lay_out_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "xkb_dense_status": (c_int, [c_void_p]),
     "xkb_fused_moe_int4_w4a16_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
     "xkb_fused_moe_int4_w4a16": (
@@ -207,7 +208,7 @@ def load_calls():
         lib.xkb_moe_balance_loss_workspace_bytes, lib.xkb_moe_router_backward, lib.xkb_moe_sum_reduce_backward,
         lib.xkb_linear_cross_entropy, lib.xkb_linear_cross_entropy_workspace_bytes, lib.xkb_linear_cross_entropy_backward,
         lib.xkb_linear_cross_entropy_backward_workspace_bytes, lib.xkb_gated_ffn, lib.xkb_gated_ffn_workspace_bytes,
-        lib.xkb_gated_ffn_backward, lib.xkb_gated_ffn_backward_workspace_bytes)))
+        lib.xkb_gated_ffn_backward, lib.xkb_gated_ffn_backward_workspace_bytes, lib.xkb_lay_out_rows)))
     _calls = module
     return module
 

@@ -244,6 +244,73 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
 }  // namespace dense
 }  // namespace xkb
 
+namespace xkb {
+namespace {
+
+// Matrices laid out once more with rows of whole 16 bytes: a warp copies 256 elements of a row at a time, lane = column, since
+// rows start anywhere.  Bound by latency where they are small (why all operands of a call go in one launch), else by memory.
+struct LayOut {
+  const uint16_t* from[XKB_LAY_OUT_MOST];
+  uint16_t* to[XKB_LAY_OUT_MOST];
+  int64_t ld[XKB_LAY_OUT_MOST], cols[XKB_LAY_OUT_MOST], first[XKB_LAY_OUT_MOST + 1];      // first: number of its first piece
+  int count;
+};
+constexpr int kPiece = 256;
+
+__global__ void __launch_bounds__(256) lay_out_kernel(const LayOut a) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < a.first[a.count]; u += (int64_t)gridDim.x * 8) {
+    int i = 0;
+    while (i + 1 < a.count && u >= a.first[i + 1]) ++i;
+    const int64_t cols = a.cols[i], pieces = (cols + kPiece - 1) / kPiece, v = u - a.first[i];
+    const int64_t row = v / pieces, c0 = (v - row * pieces) * kPiece, ld_to = (cols + 7) / 8 * 8;
+    const uint16_t* from = a.from[i] + row * a.ld[i];
+    uint16_t* to = a.to[i] + row * ld_to;
+    uint16_t x[kPiece / 32];
+#pragma unroll
+    for (int j = 0; j < kPiece / 32; ++j) {
+      const int64_t c = c0 + j * 32 + lane;
+      x[j] = c < cols ? from[c] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int j = 0; j < kPiece / 32; ++j) {
+      const int64_t c = c0 + j * 32 + lane;
+      if (c < cols) to[c] = x[j];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace xkb
+
+extern "C" int xkb_lay_out_rows(const void* const* from_host, const int64_t* ld_host, const int64_t* rows_host, const int64_t* cols_host,
+                                void* const* to_host, int count, void* stream_) {
+  using namespace xkb;
+  XKB_REQUIRE(count >= 0 && count <= XKB_LAY_OUT_MOST, "lay_out_rows: %d matrices", count);
+  XKB_REQUIRE(count == 0 || (from_host != nullptr && ld_host != nullptr && rows_host != nullptr && cols_host != nullptr && to_host != nullptr),
+              "lay_out_rows: null array");
+  LayOut a = {};
+  int64_t pieces = 0;
+  for (int i = 0; i < count; ++i) {
+    XKB_REQUIRE(rows_host[i] >= 0 && rows_host[i] < (1ll << 28) && cols_host[i] >= 1 && cols_host[i] < (1ll << 24) && ld_host[i] >= 0 &&
+                    ld_host[i] < (1ll << 32), "lay_out_rows: sizes out of range");
+    XKB_REQUIRE(rows_host[i] == 0 || (from_host[i] != nullptr && to_host[i] != nullptr && address_bits(from_host[i], to_host[i]) % 2 == 0),
+                "lay_out_rows: null or misaligned matrix");
+    a.from[i] = static_cast<const uint16_t*>(from_host[i]);
+    a.to[i] = static_cast<uint16_t*>(to_host[i]);
+    a.ld[i] = ld_host[i], a.cols[i] = cols_host[i];
+    a.first[i] = pieces;
+    pieces += rows_host[i] * ceil_div(cols_host[i], kPiece);
+  }
+  a.first[count] = pieces;
+  a.count = count;
+  if (pieces == 0) return XKB_OK;
+  const int64_t blocks = ceil_div(pieces, 8);
+  lay_out_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, static_cast<cudaStream_t>(stream_)>>>(a);
+  XKB_CHECK_LAUNCH("lay_out_kernel");
+  return XKB_OK;
+}
+
 extern "C" int xkb_dense_status(void* stream_) {
   using namespace xkb;
   int dev = 0;

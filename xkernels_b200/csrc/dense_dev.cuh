@@ -310,6 +310,38 @@ __device__ __forceinline__ void rows_in(uint32_t buf, const void* from, uint32_t
   }
   __syncwarp();
 }
+// The same for rows that start anywhere and for the last n columns: a row at a time, lane = column.
+__device__ __forceinline__ void rows_out_any(uint32_t buf, uint16_t* to, const uint32_t* w, int n) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(rows_at(buf, lane, u)), "r"(w[4 * u]), "r"(w[4 * u + 1]), "r"(w[4 * u + 2]), "r"(w[4 * u + 3]) : "memory");
+  __syncwarp();
+#pragma unroll 8
+  for (int row = 0; row < 32; ++row) {
+    uint16_t* p = reinterpret_cast<uint16_t*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(to), row));
+    const uint32_t v = tc::lds16(rows_at(buf, row, lane >> 3) + (lane & 7) * 2);
+    if (p != nullptr && lane < n) p[lane] = (uint16_t)v;
+  }
+  __syncwarp();
+}
+__device__ __forceinline__ void rows_in_any(uint32_t buf, const uint16_t* from, uint32_t* w, int n) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 8
+  for (int row = 0; row < 32; ++row) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(from), row));
+    const uint16_t v = p != nullptr && lane < n ? p[lane] : (uint16_t)0;
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(rows_at(buf, row, lane >> 3) + (lane & 7) * 2), "h"(v) : "memory");
+  }
+  __syncwarp();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint4 x = tc::lds128(rows_at(buf, lane, u));
+    w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
+  }
+  __syncwarp();
+}
 // 16-bit results of 64 columns leave by a copy of their own: the lanes write their rows, halves of 32 columns, into 128-byte
 // rows (128-byte swizzle), and one lane starts the copy, which the warp does not wait for until the buffer's next use.
 // Full lines reach L2: the products of a head's gradient at 509 x 2048 x 50001, 168 -> 151 us.
@@ -334,15 +366,19 @@ __device__ __forceinline__ void copy_rows(uint32_t buf, const CUtensorMap* map, 
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   }
 }
-// CW columns of this lane's row: together where whole pieces of 32 are aligned, else each lane its own.
+// CW columns of this lane's row: pieces of 32 together, smaller ones each lane its own.
 template <int CW>
 __device__ __forceinline__ void put_row(uint32_t buf, void* base, int64_t at, bool live, const uint32_t (&w)[CW / 2], int n, int vec) {
-  if (CW == 32 && n >= CW && vec >= 16) rows_out(buf, live ? static_cast<uint16_t*>(base) + at : nullptr, w);
+  uint16_t* to = live ? static_cast<uint16_t*>(base) + at : nullptr;
+  if (CW == 32 && n >= CW && vec >= 16) rows_out(buf, to, w);
+  else if (CW == 32) rows_out_any(buf, to, w, n);
   else if (live) store_row<CW>(base, at, w, n, vec);
 }
 template <int CW>
 __device__ __forceinline__ void get_row(uint32_t buf, const void* base, int64_t at, bool live, uint32_t (&w)[CW / 2], int n, int vec) {
-  if (CW == 32 && n >= CW && vec >= 16) rows_in(buf, live ? static_cast<const uint16_t*>(base) + at : nullptr, w);
+  const uint16_t* from = live ? static_cast<const uint16_t*>(base) + at : nullptr;
+  if (CW == 32 && n >= CW && vec >= 16) rows_in(buf, from, w);
+  else if (CW == 32) rows_in_any(buf, from, w, n);
   else if (live) load_row<CW>(base, at, w, n, vec);
 }
 

@@ -40,6 +40,7 @@ decltype(&xkb_gated_ffn) g_ffn;
 decltype(&xkb_gated_ffn_workspace_bytes) g_ffn_bytes;
 decltype(&xkb_gated_ffn_backward) g_ffn_grad;
 decltype(&xkb_gated_ffn_backward_workspace_bytes) g_ffn_grad_bytes;
+decltype(&xkb_lay_out_rows) g_lay_out;
 
 bool modes_active() {
   return at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set();
@@ -400,20 +401,55 @@ PyObject* moe_sum_reduce_backward(PyObject*, PyObject* const* args, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
-// An operand of a dense product that is read in place: rows on 16 bytes that do not overlap, bf16 or fp16.
-const at::Tensor* operand(PyObject* obj, at::ScalarType type, int64_t rows, int64_t cols) {
-  const at::Tensor* t = plain(obj, false);
-  if (t == nullptr || t->dim() != 2 || t->scalar_type() != type || t->size(0) != rows || t->size(1) != cols || rows < 0 || cols < 1 ||
-      (cols > 1 && t->stride(1) != 1) || t->stride(0) % 8 != 0 || t->stride(0) < cols ||
-      reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 != 0)
-    return nullptr;
-  return t;
-}
+// Operands of a dense product, bf16 or fp16: read in place where rows start on 16 bytes and do not overlap, else laid out once
+// more, all of a call in one launch.
+struct Operands {
+  const void* at[XKB_LAY_OUT_MOST];
+  int64_t ld[XKB_LAY_OUT_MOST];
+  int count = 0, copies = 0;
+  const void* from[XKB_LAY_OUT_MOST];
+  int64_t from_ld[XKB_LAY_OUT_MOST], rows[XKB_LAY_OUT_MOST], cols[XKB_LAY_OUT_MOST], offset[XKB_LAY_OUT_MOST], bytes = 0;
+  int which[XKB_LAY_OUT_MOST];
+  at::Tensor room;
+
+  static const at::Tensor* matrix(PyObject* obj, at::ScalarType type) {
+    const at::Tensor* t = plain(obj, false);
+    return t != nullptr && t->dim() == 2 && t->scalar_type() == type && t->size(1) >= 1 && (t->size(1) == 1 || t->stride(1) == 1) ? t : nullptr;
+  }
+  // false: not this path's
+  bool add(PyObject* obj, at::ScalarType type, int64_t n, int64_t m) {
+    const at::Tensor* t = matrix(obj, type);
+    if (t == nullptr || t->size(0) != n || t->size(1) != m) return false;
+    at[count] = t->const_data_ptr();
+    ld[count] = t->stride(0);
+    if (t->stride(0) % 8 != 0 || t->stride(0) < m || reinterpret_cast<uintptr_t>(at[count]) % 16 != 0) {
+      from[copies] = at[count], from_ld[copies] = t->stride(0), rows[copies] = n, cols[copies] = m;
+      which[copies] = count, offset[copies] = bytes;
+      ld[count] = (m + 7) / 8 * 8;
+      bytes += (n * ld[count] * 2 + 255) / 256 * 256;
+      ++copies;
+    }
+    ++count;
+    return true;
+  }
+  void allocate() {
+    if (copies == 0) return;
+    room = fresh(at::kByte, {bytes});
+    char* base = static_cast<char*>(room.mutable_data_ptr());
+    for (int i = 0; i < copies; ++i) at[which[i]] = base + offset[i];
+  }
+  int lay_out(void* stream) const {
+    if (copies == 0) return 0;
+    void* to[XKB_LAY_OUT_MOST];
+    for (int i = 0; i < copies; ++i) to[i] = const_cast<void*>(at[which[i]]);
+    return g_lay_out(from, from_ld, rows, cols, to, copies, stream);
+  }
+};
 // The first operand, which says type and sizes.
 const at::Tensor* first_operand(PyObject* obj) {
   const at::Tensor* t = plain(obj, false);
-  if (t == nullptr || t->dim() != 2 || (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kHalf)) return nullptr;
-  return operand(obj, t->scalar_type(), t->size(0), t->size(1));
+  if (t == nullptr || (t->scalar_type() != at::kBFloat16 && t->scalar_type() != at::kHalf)) return nullptr;
+  return Operands::matrix(obj, t->scalar_type());
 }
 bool limit_of(PyObject* obj, float* limit) {
   *limit = 0.f;
@@ -429,18 +465,21 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 3 || modes_active() || args[2] == Py_None) Py_RETURN_NONE;
   const at::Tensor *x = first_operand(args[0]), *w = plain(args[1], false), *labels;
-  if (x == nullptr || w == nullptr || w->dim() != 2 || w->size(0) < 1 ||
-      operand(args[1], x->scalar_type(), w->size(0), x->size(1)) == nullptr || !tokens_of(args[2], x->size(0), &labels))
+  Operands o;      // (hidden states are read wherever they start)
+  if (x == nullptr || w == nullptr || w->dim() != 2 || w->size(0) < 1 || x->stride(0) < 0 ||
+      !o.add(args[1], x->scalar_type(), w->size(0), x->size(1)) || !tokens_of(args[2], x->size(0), &labels))
     Py_RETURN_NONE;
   const int64_t M = x->size(0), H = x->size(1), V = w->size(0), ws_bytes = g_lce_bytes(M, H, V);
   Pieces pieces(2 * Pieces::room(M) + Pieces::room(2 * M));
   at::Tensor loss = pieces.take(at::kFloat, {M}), lse = pieces.take(at::kFloat, {M}), stats = pieces.take(at::kFloat, {M, 2}),
              ws = workspace_of(ws_bytes);
+  o.allocate();
   const int code = code_of(x->scalar_type()), ids64 = labels->scalar_type() == at::kLong;
   void* const stream = stream_of(*x);
   int status;
   Py_BEGIN_ALLOW_THREADS
-  status = g_lce(x->const_data_ptr(), x->stride(0), code, w->const_data_ptr(), w->stride(0), labels->const_data_ptr(), ids64,
+  status = o.lay_out(stream);
+  if (status == 0) status = g_lce(x->const_data_ptr(), x->stride(0), code, o.at[0], o.ld[0], labels->const_data_ptr(), ids64,
                  static_cast<float*>(loss.mutable_data_ptr()), static_cast<float*>(lse.mutable_data_ptr()),
                  static_cast<float*>(stats.mutable_data_ptr()), M, H, V, ws.mutable_data_ptr(), ws_bytes, stream);
   Py_END_ALLOW_THREADS
@@ -457,8 +496,9 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
       !PyBool_Check(args[6]) || !PyBool_Check(args[7]))
     Py_RETURN_NONE;
   const at::Tensor *x = first_operand(args[0]), *w = plain(args[1], false), *labels, *stats, *g_loss, *g_lse;
-  if (x == nullptr || w == nullptr || w->dim() != 2 || w->size(0) < 1 ||
-      operand(args[1], x->scalar_type(), w->size(0), x->size(1)) == nullptr || !tokens_of(args[2], x->size(0), &labels) ||
+  Operands o;
+  if (x == nullptr || w == nullptr || w->dim() != 2 || w->size(0) < 1 || x->stride(0) < 0 ||
+      !o.add(args[1], x->scalar_type(), w->size(0), x->size(1)) || !tokens_of(args[2], x->size(0), &labels) ||
       !optional(args[3], at::kFloat, x->size(0), 2, &stats) || !optional(args[4], at::kFloat, x->size(0), -1, &g_loss) ||
       !optional(args[5], at::kFloat, x->size(0), -1, &g_lse))
     Py_RETURN_NONE;
@@ -467,11 +507,13 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
   at::Tensor gx, gw, ws = workspace_of(ws_bytes);
   if (need_x) gx = fresh(x->scalar_type(), {M, H});
   if (need_w) gw = fresh(x->scalar_type(), {V, H});
+  o.allocate();
   const int code = code_of(x->scalar_type()), ids64 = labels->scalar_type() == at::kLong;
   void* const stream = stream_of(*x);
   int status;
   Py_BEGIN_ALLOW_THREADS
-  status = g_lce_grad(x->const_data_ptr(), x->stride(0), code, w->const_data_ptr(), w->stride(0), labels->const_data_ptr(), ids64,
+  status = o.lay_out(stream);
+  if (status == 0) status = g_lce_grad(x->const_data_ptr(), x->stride(0), code, o.at[0], o.ld[0], labels->const_data_ptr(), ids64,
                       data<float>(stats), data<float>(g_loss), data<float>(g_lse), need_x ? gx.mutable_data_ptr() : nullptr,
                       need_w ? gw.mutable_data_ptr() : nullptr, M, H, V, ws.mutable_data_ptr(), ws_bytes, stream);
   Py_END_ALLOW_THREADS
@@ -490,18 +532,21 @@ PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor *x = first_operand(args[0]), *w2 = plain(args[2], false);
   if (x == nullptr || w2 == nullptr || w2->dim() != 2) Py_RETURN_NONE;
   const int64_t M = x->size(0), H = x->size(1), I = w2->size(1);
-  const at::Tensor* w13 = operand(args[1], x->scalar_type(), 2 * I, H);
-  if (w13 == nullptr || operand(args[2], x->scalar_type(), H, I) == nullptr) Py_RETURN_NONE;
+  Operands o;
+  if (!o.add(args[0], x->scalar_type(), M, H) || !o.add(args[1], x->scalar_type(), 2 * I, H) || !o.add(args[2], x->scalar_type(), H, I))
+    Py_RETURN_NONE;
   const bool save = args[4] == Py_True;
   const int64_t ws_bytes = g_ffn_bytes(M, H, I);
   at::Tensor out = fresh(x->scalar_type(), {M, H}), gate_up, ws = workspace_of(ws_bytes);
   if (save) gate_up = fresh(x->scalar_type(), {M, 2 * I});
+  o.allocate();
   const int code = code_of(x->scalar_type());
   void* const stream = stream_of(*x);
   int status;
   Py_BEGIN_ALLOW_THREADS
-  status = g_ffn(x->const_data_ptr(), x->stride(0), code, w13->const_data_ptr(), w13->stride(0), w2->const_data_ptr(), w2->stride(0), limit,
-                 out.mutable_data_ptr(), save ? gate_up.mutable_data_ptr() : nullptr, M, H, I, ws.mutable_data_ptr(), ws_bytes, stream);
+  status = o.lay_out(stream);
+  if (status == 0)
+    status = g_ffn(o.at[0], o.ld[0], code, o.at[1], o.ld[1], o.at[2], o.ld[2], limit, out.mutable_data_ptr(), save ? gate_up.mutable_data_ptr() : nullptr, M, H, I, ws.mutable_data_ptr(), ws_bytes, stream);
   Py_END_ALLOW_THREADS
   if (status != 0) return PyLong_FromLong(status);
   if (!save) return THPVariable_Wrap(std::move(out));
@@ -518,9 +563,9 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor *x = first_operand(args[1]), *w2 = plain(args[3], false), *gate_up;
   if (x == nullptr || w2 == nullptr || w2->dim() != 2) Py_RETURN_NONE;
   const int64_t M = x->size(0), H = x->size(1), I = w2->size(1);
-  const at::Tensor *go = operand(args[0], x->scalar_type(), M, H), *w13 = operand(args[2], x->scalar_type(), 2 * I, H);
-  if (go == nullptr || w13 == nullptr || operand(args[3], x->scalar_type(), H, I) == nullptr ||
-      !optional(args[4], x->scalar_type(), M, 2 * I, &gate_up))
+  Operands o;
+  if (!o.add(args[0], x->scalar_type(), M, H) || !o.add(args[1], x->scalar_type(), M, H) || !o.add(args[2], x->scalar_type(), 2 * I, H) ||
+      !o.add(args[3], x->scalar_type(), H, I) || !optional(args[4], x->scalar_type(), M, 2 * I, &gate_up))
     Py_RETURN_NONE;
   const bool need[3] = {args[6] == Py_True, args[7] == Py_True, args[8] == Py_True};
   const int64_t ws_bytes = g_ffn_grad_bytes(M, H, I, gate_up == nullptr);
@@ -528,15 +573,17 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (need[0]) g[0] = fresh(x->scalar_type(), {M, H});
   if (need[1]) g[1] = fresh(x->scalar_type(), {2 * I, H});
   if (need[2]) g[2] = fresh(x->scalar_type(), {H, I});
+  o.allocate();
   void* to[3];
   for (int i = 0; i < 3; ++i) to[i] = need[i] ? g[i].mutable_data_ptr() : nullptr;
   const int code = code_of(x->scalar_type());
   void* const stream = stream_of(*x);
   int status;
   Py_BEGIN_ALLOW_THREADS
-  status = g_ffn_grad(go->const_data_ptr(), go->stride(0), code, x->const_data_ptr(), x->stride(0), w13->const_data_ptr(), w13->stride(0),
-                      w2->const_data_ptr(), w2->stride(0), data<void>(gate_up), limit, to[0], to[1], to[2], M, H, I, ws.mutable_data_ptr(),
-                      ws_bytes, stream);
+  status = o.lay_out(stream);
+  if (status == 0)
+    status = g_ffn_grad(o.at[0], o.ld[0], code, o.at[1], o.ld[1], o.at[2], o.ld[2], o.at[3], o.ld[3], data<void>(gate_up), limit, to[0], to[1],
+                        to[2], M, H, I, ws.mutable_data_ptr(), ws_bytes, stream);
   Py_END_ALLOW_THREADS
   if (status != 0) return PyLong_FromLong(status);
   PyObject* out[3];
@@ -546,7 +593,7 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // bind(...): the library's functions, as addresses, in the order of the pointers above
-constexpr Py_ssize_t kFunctions = 18;
+constexpr Py_ssize_t kFunctions = 19;
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != kFunctions) { PyErr_SetString(PyExc_TypeError, "bind: another number of addresses expected"); return nullptr; }
   void* p[kFunctions];
@@ -575,6 +622,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_ffn_bytes = reinterpret_cast<decltype(g_ffn_bytes)>(p[15]);
   g_ffn_grad = reinterpret_cast<decltype(g_ffn_grad)>(p[16]);
   g_ffn_grad_bytes = reinterpret_cast<decltype(g_ffn_grad_bytes)>(p[17]);
+  g_lay_out = reinterpret_cast<decltype(g_lay_out)>(p[18]);
   Py_RETURN_NONE;
 }
 

@@ -193,3 +193,26 @@ def test_inputs_are_left_alone_and_sms_may_be_kept_free(cuda_device):
     finally:
         _lib.set_sm_margin(0)
     assert all(torch.equal(a, b) for a, b in zip(t, before))
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """2.5e9 elements of gate and up: the last rows are those of a short call with the same weights, bit for bit where the tile is
+    the same and to a rounding's error where not."""
+    M, H, I, tail = 1_200_000, 64, 1040, 700
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    x = torch.randn(M, H, generator=g, device=cuda_device, dtype=torch.float32).to(BF)
+    w13, w2 = (torch.randn(2 * I, H, generator=g, device=cuda_device) / 8).to(BF), (torch.randn(H, I, generator=g, device=cuda_device) / 32).to(BF)
+    out, raw = xkb.gated_ffn(x, w13, w2, save_gate_up=True)
+    assert raw.numel() > 2 ** 31
+    (want, err), (wraw, eraw) = du.gated_ffn(x[-tail:], w13, w2)
+    assert_near(out[-tail:], want, err, "out")
+    assert_near(raw[-tail:], wraw, eraw, "gate_up")
+    go = torch.zeros_like(x)
+    go[-tail:] = torch.randn(tail, H, generator=g, device=cuda_device).to(BF)        # the weights' gradients are the last rows'
+    gx, g13, g2 = xkb.gated_ffn_backward(go, x, w13, w2, raw)
+    del out
+    (vx, ex), (v13, e13), (v2, e2) = du.gated_ffn_grad(go[-tail:], x[-tail:], w13, w2, raw[-tail:])
+    assert_near(gx[-tail:], vx, ex, "grad x")
+    assert_near(g13, v13, e13, "grad w13")
+    assert_near(g2, v2, e2, "grad w2")
+    assert not gx[:-tail].any()

@@ -244,3 +244,24 @@ def test_two_streams_and_captured_calls(cuda_device):
     graphs[2].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(outs[2], step(*sets[2])))
+
+
+def test_many_rows(cuda_device):
+    """Far more rows than blocks, most of them padding, and a piece of the least width."""
+    M, H, V = 700_001, 64, 700
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    x = torch.randn(M, H, generator=g, device=cuda_device).to(BF)
+    w = (torch.randn(V, H, generator=g, device=cuda_device) / 6).to(BF)
+    labels = torch.randint(0, V, (M,), generator=g, device=cuda_device)
+    labels[torch.rand(M, generator=g, device=cuda_device) < 0.99] = -1
+    on = labels >= 0
+    r = xkb.linear_cross_entropy(x, w, labels)
+    few = xkb.LinearCrossEntropy(*(t[on] for t in r))
+    stats_near(few, x[on], w, labels[on])
+    assert not r.loss[~on].any() and not r.stats[~on].any()
+    gl = torch.rand(M, generator=g, device=cuda_device)
+    gx, gw = xkb.linear_cross_entropy_backward(x, w, labels, r.stats, grad_loss=gl)
+    (vx, ex), (vw, ew) = du.cross_entropy_grad(x[on], w, labels[on], few.stats, gl[on], None)
+    assert_near(gx[on], vx, ex, "grad hidden")
+    assert_near(gw, vw, ew, "grad weight")
+    assert not gx[~on].any()

@@ -282,7 +282,8 @@ int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_hidden, int
  * x [M, H], w13 [2 I, H] (gate rows first, as in the fused calls), w2 [H, I], all
  * bf16 or fp16, row strides multiples of 8 elements and first rows on 16 bytes.
  * limit > 0: gate is cut off at limit, up at +-limit (as in fused_moe_mxfp4).
- * Products are added up in fp32; silu(gate) * up is rounded to dtype once.
+ * Products are added up in fp32; silu(gate) * up is rounded to dtype (up to 16
+ * rows: held in two terms of dtype) as the operand of the second product.
  * out [M, H] and, if not NULL, gate_up [M, 2 I] (before the limit), contiguous.
  * No reference counterpart.  Two launches.
  * ---------------------------------------------------------------------- */

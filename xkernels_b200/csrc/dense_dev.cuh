@@ -25,8 +25,8 @@ constexpr int kMaxStages = 12;
 constexpr int kABytes = kRows * 128;
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
 // The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, so a long sum drifts towards 0
-// (2^-24 of it a step of 16 K: 5e-6 of the logits at K = 7168).  Where the result stays fp32 (kCeStats) an accumulator takes
-// 512 K, and the read-out adds them up in registers while the next is filled: 5e-7, as an fp32 sum on the ordinary cores.
+// (in proportion to K: losses were 1.4e-6 off at K = 2048).  Where the result stays fp32 (kCeStats) an accumulator takes 512 K,
+// and the read-out adds them up in registers while the next is filled: 3.6e-7, as an fp32 product on the ordinary cores.
 constexpr int kPartBlocks = 8;      // of 64 K
 template <int END> __device__ __forceinline__ int parts_of(int kb) {
   return END == kCeStats ? (kb + kPartBlocks - 1) / kPartBlocks : 1;

@@ -744,7 +744,8 @@ def gated_ffn(x, w13, w2, swiglu_limit=None, save_gate_up=False):
 
     ``x`` ``[M, H]``, ``w13`` ``[2*I, H]`` (gate rows first, as in :func:`fused_moe_mxfp4`), ``w2`` ``[H, I]``, all bf16 or all fp16;
     rows may lie apart.  ``swiglu_limit`` (None or 0: none) cuts gate off at the limit and up at plus and minus it, as there.
-    Products are added up in fp32, and ``silu(gate) * up`` is rounded to ``x``'s dtype once, as the operand of the second product.
+    Products are added up in fp32, and ``silu(gate) * up`` is rounded to ``x``'s dtype once, as the operand of the second product (up to
+    16 rows: held in two terms of it).
     Returns ``out`` ``[M, H]``, or ``(out, gate_up)`` with ``save_gate_up``: ``[M, 2*I]`` before the limit, for
     :func:`gated_ffn_backward`.  The same bits in every run.  No reference counterpart.
     """

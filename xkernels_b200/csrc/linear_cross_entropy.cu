@@ -26,7 +26,9 @@ constexpr int kListBlocks = 296;                    // two on every SM
 constexpr int kSegment = 2048;                      // elements of a row that a warp copies at a time: eight loads a lane in flight
 constexpr int kJoinThreads = 128;
 constexpr int kRowPad = 256;                       // rows of the row arrays are a multiple of this
-constexpr int64_t kPieceBytes = 256ll << 20;       // of the logits' gradient that is held at a time
+// Of the logits' gradient that is held at a time.  4096 x 7168 x 128000, pieces of 64 / 128 / 256 / 512 / 1100 MiB (all of it):
+// 15.4 / 14.8 / 15.0 / 14.9 / 15.3 ms, spread of runs 0.3.
+constexpr int64_t kPieceBytes = 256ll << 20;
 
 struct Rows {
   int32_t* count;      // rows with a label

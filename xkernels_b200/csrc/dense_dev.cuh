@@ -975,6 +975,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
           }
           break;
         }
+        // The tile before may have been another product's, whose last rows a copy still reads from the buffer.
+        if constexpr (END == kStore)
+          if (!e.tma_out) rows_copied();
 #pragma unroll 1
         for (int c = wg * kMine; c < (wg + 1) * kMine; c += kPiece) {
           const int col = t.n * kTileN + c, n = N - col;

@@ -62,7 +62,8 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
     if (cost < best_cost * 0.999) best_cost = cost, *best = s;
   };
   for (int bn : {256, 128}) {
-    if (two_terms) break;
+    // (two terms are single CTAs' alone; statistics of one row tile have their shorter sums there: part_blocks)
+    if (two_terms || (end == kCeStats && M[0] <= kRows)) break;
     const int64_t tile_n = paired ? bn / 2 : bn;
     const double stage = bn == 256 ? 520 : 400, readout = bn == 256 ? 3500 : 2000;
     double work = 0;

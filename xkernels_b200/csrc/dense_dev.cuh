@@ -24,12 +24,17 @@ constexpr int kControlWarps = 4;    // 0: TMA of A, 1: MMA, 2: tensor memory, 3:
 constexpr int kMaxStages = 12;
 constexpr int kABytes = kRows * 128;
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
-// The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, so a long sum drifts towards 0
-// (in proportion to K: losses were 1.4e-6 off at K = 2048).  Where the result stays fp32 (kCeStats) an accumulator takes 512 K,
-// and the read-out adds them up in registers while the next is filled: 3.6e-7, as an fp32 product on the ordinary cores.
-constexpr int kPartBlocks = 8;      // of 64 K
-template <int END> __device__ __forceinline__ int parts_of(int kb) {
-  return END == kCeStats ? (kb + kPartBlocks - 1) / kPartBlocks : 1;
+// The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, at each step of 16 K, so a long sum
+// drifts towards 0 in proportion to K (losses of many rows were 1.4e-6 off at K = 2048).  Where the result stays fp32 (kCeStats) an
+// accumulator takes part_blocks() of 64 K, and the read-out adds them up in registers while the next is filled.  Error of losses in
+// the norm, 4096 x 7168 x 128000 in pairs by 512 / 256 K: 4.0e-7 / 2.1e-7 (an fp32 product on the ordinary cores: 1.1e-6), but 3 to
+// 20 % more time, for the read-out of short parts outlasts their MMAs.  Single CTAs, which take up to 128 rows, wait for the
+// weight's bytes, and a single row's small loss takes the drift of its largest logit whole: 1 x 4096 x 50001 by 512 / 128 / 64 K
+// 2.7e-6 / 8.6e-8 / 1.1e-6 (one number; the ordinary cores' 9.2e-8) in 91 / 92 / 99 us, 128 x 7168 x 32001 4.5e-7 / 1.8e-7 / 2.0e-7 in
+// 99 / 99 / 103.
+template <int CG> __device__ __forceinline__ constexpr int part_blocks() { return CG == 1 ? 2 : 8; }
+template <int END, int CG> __device__ __forceinline__ int parts_of(int kb) {
+  return END == kCeStats ? (kb + part_blocks<CG>() - 1) / part_blocks<CG>() : 1;
 }
 
 struct DevProduct {
@@ -867,11 +872,12 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
       for (Walk walk(sh, cluster, clusters); ok && walk.get(sh, t); walk.next(sh)) {
         const bool a_mn = p.prod[t.prod].a_mn != 0;
         share(t);
-        const int parts = parts_of<END>(t.k1 - t.k0);
+        const int parts = parts_of<END, CG>(t.k1 - t.k0);
         for (int piece = 0; ok && piece < parts; ++piece) {
           if (!wait(acc_empty + 8 * set, set_parity, guard, 2)) { ok = false; break; }
           tc::tc_fence_after();
-          const int b0 = END == kCeStats ? t.k0 + piece * kPartBlocks : t.k0, b1 = END == kCeStats ? min(b0 + kPartBlocks, t.k1) : t.k1;
+          const int b0 = END == kCeStats ? t.k0 + piece * part_blocks<CG>() : t.k0;
+          const int b1 = END == kCeStats ? min(b0 + part_blocks<CG>(), t.k1) : t.k1;
           ok = END == kStore && BMN && a_mn ? multiply(std::true_type{}, b0, b1) : multiply(std::false_type{}, b0, b1);
           commit<CG>(ok ? leader : 0u, acc_full + 8 * set, both);
           set ^= 1;
@@ -924,7 +930,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
       }
       const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
       if constexpr (END == kCeStats) {
-        const int parts = parts_of<END>(t.k1 - t.k0);
+        const int parts = parts_of<END, CG>(t.k1 - t.k0);
         float sum[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) sum[j] = 0.f;

@@ -167,8 +167,7 @@ def linear_cross_entropy(hidden, weight, labels):
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w13, w2, limit, recompute):
-        keep = not recompute and any(ctx.needs_input_grad[:3])
+    def forward(ctx, x, w13, w2, limit, keep):
         got = ops.gated_ffn(x, w13, w2, limit, keep)
         out, gate_up = got if keep else (got, None)
         ctx.save_for_backward(x, w13, w2, gate_up)
@@ -191,4 +190,6 @@ def gated_ffn(x, w13, w2, swiglu_limit=None, recompute=False):
     """:func:`xkernels_b200.gated_ffn`, differentiable in ``x``, ``w13`` and ``w2``.  ``recompute``: gate and up are not kept for
     the backward pass, which multiplies them once more."""
     _not_captured("gated_ffn", x, w13, w2)
-    return _GatedFfn.apply(x, w13, w2, swiglu_limit, recompute)
+    # (asked here: within forward() gradients are off, and ctx.needs_input_grad is true of a leaf under no_grad as well)
+    records = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, w13, w2))
+    return _GatedFfn.apply(x, w13, w2, swiglu_limit, records and not recompute)

@@ -61,6 +61,9 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
     const double cost = (clocks > bytes / rate ? clocks : bytes / rate) + tail;
     if (cost < best_cost * 0.999) best_cost = cost, *best = s;
   };
+  // More of K than one accumulator is to take: pairs whose tile is their own have a way for it.  (Two terms have single CTAs only, and
+  // no such K.)
+  auto long_sum = [&](int64_t kb, int s) { return end == kStore && !two_terms && ceil_div(kb, s) > kLongBlocks; };
   for (int bn : {256, 128}) {
     // (two terms are single CTAs' alone; statistics of one row tile have their shorter sums there: part_blocks)
     if (two_terms || (end == kCeStats && M[0] <= kRows)) break;
@@ -79,7 +82,7 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
     if (count == 1 && may_split)
       for (int s = 2; s <= 4; ++s) {
         const int64_t kb = ceil_div(K[0], kBK);
-        if (4 * s > kb || tiles * 2 * s > sms) continue;
+        if (4 * s > kb || tiles * 2 * s > sms || long_sum(kb, s)) continue;
         int most = 0;
         const int rc = clusters_at_once(dev, 2, bn, 8, 2 * s, &most);
         if (rc != XKB_OK) return rc;
@@ -93,9 +96,9 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
       if (bn == 64 && end == kCeStats) continue;
       const int64_t tiles = ceil_div(M[0], kRows) * ceil_div(N[0], paired ? bn / 2 : bn);
       const double mma = bn == 128 ? 275 : 260, stage = 2 * (rows + bn) > mma ? 2 * (rows + bn) : mma;
-      consider({1, bn, 1}, tiles, (double)ceil_div(tiles, sms) * kb * stage, 2000);
+      if (!long_sum(kb, 1)) consider({1, bn, 1}, tiles, (double)ceil_div(tiles, sms) * kb * stage, 2000);
       for (int s = 2; s <= 8; ++s) {
-        if (4 * s > kb || tiles * s > 2 * sms) continue;
+        if (4 * s > kb || tiles * s > 2 * sms || long_sum(kb, s)) continue;
         int most = 0;
         const int rc = clusters_at_once(dev, 1, bn, warps, s, &most);
         if (rc != XKB_OK) return rc;
@@ -237,7 +240,12 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     if (most < 1) most = 1;
     l.grid = (int)(tiles < most ? tiles : most) * s.cg;
   }
-  if (end == kStore) return run_store(b_mn, p, l);
+  if (end == kStore) {
+    bool long_sums = false;
+    for (int i = 0; i < count; ++i) long_sums |= ceil_div(ceil_div(K[i], kBK), k_parts[i]) > kLongBlocks;
+    // (a kernel of its own: with its registers the ordinary one took 5 % longer, 509 x 4096 x 1416 backward 51.7 -> 54.7 us)
+    return long_sums && s.cg == 2 && s.split == 1 ? run_store_long(b_mn, p, l) : run_store(b_mn, p, l);
+  }
   if (end == kSwiglu || end == kDswiglu) return run_ffn(end, p, l);
   return run_ce(end, p, l);
 }

@@ -12,6 +12,7 @@ constexpr int kSwiglu = 1;    // gate and up of the same column side by side: si
 constexpr int kDswiglu = 2;   // D is the gradient of silu(gate) * up: the gradients of both, and the product itself
 constexpr int kCeStats = 3;   // D are logits: maximum and sum of exponentials of a row's piece, the label's logit
 constexpr int kCeGrad = 4;    // D are logits: their gradient, rounded to 16 bits
+constexpr int kStoreLong = 5; // kStore of sums so long that they are added up in parts (the launcher's choice)
 
 constexpr int kMaxProblems = 3;
 

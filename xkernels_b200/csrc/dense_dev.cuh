@@ -26,15 +26,22 @@ constexpr int kABytes = kRows * 128;
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
 // The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, at each step of 16 K, so a long sum
 // drifts towards 0 in proportion to K (losses of many rows were 1.4e-6 off at K = 2048).  Where the result stays fp32 (kCeStats) an
-// accumulator takes part_blocks() of 64 K, and the read-out adds them up in registers while the next is filled.  Error of losses in
+// accumulator takes kPartBlocks of 64 K, and the read-out adds them up in registers while the next is filled.  Error of losses in
 // the norm, 4096 x 7168 x 128000 in pairs by 512 / 256 K: 4.0e-7 / 2.1e-7 (an fp32 product on the ordinary cores: 1.1e-6), but 3 to
 // 20 % more time, for the read-out of short parts outlasts their MMAs.  Single CTAs, which take up to 128 rows, wait for the
 // weight's bytes, and a single row's small loss takes the drift of its largest logit whole: 1 x 4096 x 50001 by 512 / 128 / 64 K
 // 2.7e-6 / 8.6e-8 / 1.1e-6 (one number; the ordinary cores' 9.2e-8) in 91 / 92 / 99 us, 128 x 7168 x 32001 4.5e-7 / 1.8e-7 / 2.0e-7 in
 // 99 / 99 / 103.
-template <int CG> __device__ __forceinline__ constexpr int part_blocks() { return CG == 1 ? 2 : 8; }
-template <int END, int CG> __device__ __forceinline__ int parts_of(int kb) {
-  return END == kCeStats ? (kb + part_blocks<CG>() - 1) / part_blocks<CG>() : 1;
+// Stored results are rounded to 16 bits, and only sums far longer than a layer is wide drift as far as that: sums over rows of
+// one sign lost 6e-9 of themselves a row (1.6e-3 of 2^18 rows in fp16, whose half step is 4.9e-4).  Pairs add sums of more than 16384 K
+// up in parts of that the same way (kStoreLong), and single CTAs are not given them.  Other ends contract over a layer's width H,
+// in one accumulator.
+constexpr int kLongBlocks = 256;
+template <int END> constexpr bool kStores = END == kStore || END == kStoreLong;
+template <int END> constexpr bool kInParts = END == kCeStats || END == kStoreLong;
+template <int END, int CG> constexpr int kPartBlocks = END == kStoreLong ? kLongBlocks : CG == 1 ? 2 : 8;
+template <int END, int CG> __device__ __forceinline__ int parts_of(int kb) {      // no blocks are one part too
+  return kInParts<END> && kb > 0 ? (kb + kPartBlocks<END, CG> - 1) / kPartBlocks<END, CG> : 1;
 }
 
 struct DevProduct {
@@ -417,7 +424,7 @@ template <int END> __device__ __forceinline__ void row_begin(const End& e, int r
     }
     if constexpr (END == kCeGrad) st.coef = live ? e.coef[row] : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  if constexpr (END == kStore) st.to = live && e.row_map != nullptr ? e.row_map[row] : row;
+  if constexpr (kStores<END>) st.to = live && e.row_map != nullptr ? e.row_map[row] : row;
 }
 template <int END> __device__ __forceinline__ void row_end(const End& e, int row, bool live, int part, const RowState& st) {
   if constexpr (END == kCeStats)
@@ -429,7 +436,7 @@ template <int END, int CW>
 __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, int row, bool live, int kpart, int col, int n, float scale, float (&v)[CW],
                                           float (&w)[CW], RowState& st) {
   uint32_t o[CW / 2];
-  if constexpr (END == kStore) {
+  if constexpr (kStores<END>) {
     if (e.acc_in || e.acc_out) {
       float* acc = e.acc + kpart * e.acc_part + (int64_t)row * e.acc_ld + col;
       constexpr int kHalf = CW == 32 ? 16 : CW;
@@ -876,9 +883,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
         for (int piece = 0; ok && piece < parts; ++piece) {
           if (!wait(acc_empty + 8 * set, set_parity, guard, 2)) { ok = false; break; }
           tc::tc_fence_after();
-          const int b0 = END == kCeStats ? t.k0 + piece * part_blocks<CG>() : t.k0;
-          const int b1 = END == kCeStats ? min(b0 + part_blocks<CG>(), t.k1) : t.k1;
-          ok = END == kStore && BMN && a_mn ? multiply(std::true_type{}, b0, b1) : multiply(std::false_type{}, b0, b1);
+          constexpr int kPart = kPartBlocks<END, CG>;
+          const int b0 = t.k0 + piece * kPart, b1 = kInParts<END> ? min(b0 + kPart, t.k1) : t.k1;
+          ok = kStores<END> && BMN && a_mn ? multiply(std::true_type{}, b0, b1) : multiply(std::false_type{}, b0, b1);
           commit<CG>(ok ? leader : 0u, acc_full + 8 * set, both);
           set ^= 1;
           if (set == 0) set_parity ^= 1;
@@ -913,6 +920,21 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
         __syncwarp();
         if (lane == 0) remote_arrive(map_to(tc::smem_u32(&sh.acc_empty[set]), first_rank));
       };
+      auto add_part = [&](uint32_t n, float (&sum)[kMine]) {      // the n-th accumulators in turn, this warp's lanes and columns
+        const uint32_t set = n & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16) + wg * kMine;
+        if (!wait(tc::smem_u32(&sh.acc_full[set]), (n >> 1) & 1, guard, 4)) return false;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kMine; c += 16) {
+          uint32_t v[16];
+          tc::tmem_ld_32x16(from + c, v);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(v[j]);
+        }
+        hand_back(set);
+        return true;
+      };
       auto park = [&](int c, float x) {         // this CTA's part of a sum, columns of 128 rows, where the stages were
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + (c * kRows + in_tile) * 4), "f"(x) : "memory");
       };
@@ -928,26 +950,14 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
           rows_start(buf + 4096, live ? gate_row + wg * kMine + e.half : nullptr);
         }
       }
-      const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
+      const float scale = kStores<END> && e.scale != nullptr ? *e.scale : 1.f;
       if constexpr (END == kCeStats) {
         const int parts = parts_of<END, CG>(t.k1 - t.k0);
         float sum[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
-        for (int piece = 0; piece < parts; ++piece, ++sets) {
-          const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16) + wg * kMine;
-          if (!wait(tc::smem_u32(&sh.acc_full[set]), (sets >> 1) & 1, guard, 4)) { ok = false; break; }
-          tc::tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < kMine; c += 16) {
-            uint32_t v[16];
-            tc::tmem_ld_32x16(from + c, v);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum[c + j] += __uint_as_float(v[j]);
-          }
-          hand_back(set);
-        }
+        for (int piece = 0; piece < parts; ++piece, ++sets)
+          if (!add_part(sets, sum)) { ok = false; break; }
         if (!ok) break;
         if (split > 1) {
           if (warp_live)
@@ -965,6 +975,30 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
         }
         row_end<END>(e, row, live, t.n * 2 + wg, st);
       } else {
+        if constexpr (END == kStoreLong) {
+          int left = parts_of<END, CG>(t.k1 - t.k0) - 1;
+          if (left > 0) {      // the parts before the last go to its accumulators
+            float sum[kMine];
+#pragma unroll
+            for (int j = 0; j < kMine; ++j) sum[j] = 0.f;
+            for (; left > 0; --left, ++sets)
+              if (!add_part(sets, sum)) { ok = false; break; }
+            const uint32_t set = sets & 1, to = tmem + set * BN + ((uint32_t)(quad * 32) << 16) + wg * kMine;
+            if (!ok || !wait(tc::smem_u32(&sh.acc_full[set]), (sets >> 1) & 1, guard, 4)) break;
+            tc::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < kMine; c += 16) {
+              uint32_t v[16];
+              tc::tmem_ld_32x16(to + c, v);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(sum[c + j] + __uint_as_float(v[j]));
+              tc::tmem_st_32x8(to + c, v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+              tc::tmem_st_32x8(to + c + 8, v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]);
+            }
+            tc::tmem_wait_st();
+          }
+        }
         const uint32_t set = sets & 1, from = tmem + set * BN + ((uint32_t)(quad * 32) << 16);
         ++sets;
         if (!wait(tc::smem_u32(&sh.acc_full[set]), ((sets - 1) >> 1) & 1, guard, 4)) break;
@@ -982,7 +1016,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
           break;
         }
         // The tile before may have been another product's, whose last rows a copy still reads from the buffer.
-        if constexpr (END == kStore)
+        if constexpr (kStores<END>)
           if (!e.tma_out) rows_copied();
 #pragma unroll 1
         for (int c = wg * kMine; c < (wg + 1) * kMine; c += kPiece) {
@@ -1002,13 +1036,13 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[j] = w[j] = 0.f;
           }
-          if constexpr (END == kStore || END == kCeGrad) st.half = ((c - wg * kMine) >> 5) & 1;
+          if constexpr (kStores<END> || END == kCeGrad) st.half = ((c - wg * kMine) >> 5) & 1;
           if constexpr (END == kDswiglu) {
             st.here = CG == 2 && e.vec_gu == 16 && n >= 32;
             st.next = CG == 2 && e.vec_gu == 16 && n >= 64 && c + 32 < (wg + 1) * kMine ? gate_row + c + 32 : nullptr;
           }
           row_piece<END, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
-          if constexpr (END == kStore || END == kCeGrad)
+          if constexpr (kStores<END> || END == kCeGrad)
             if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.out[t.prod], col - 32 * st.half, row - lane);
           if (n <= kPiece) break;
         }
@@ -1029,7 +1063,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
       const int row0 = t.m * kRows * CG + half * kRows, rows = t.rows - row0;
       const int quads = END == kCeGrad ? 4 : rows <= 0 ? 0 : min(4, (rows + 31) / 32);
       const int pieces = (kTileN / 8 - part + split - 1) / split;
-      const float scale = END == kStore && e.scale != nullptr ? *e.scale : 1.f;
+      const float scale = kStores<END> && e.scale != nullptr ? *e.scale : 1.f;
 #pragma unroll 1
       for (int i = warp - kControlWarps; i < pieces * quads; i += RW) {
         const int quad = i % quads, piece = (i / quads) * split + part;
@@ -1147,6 +1181,7 @@ int clusters_at_once(int dev, int cg, int bn, int read_warps, int width, int* ou
 // one per translation unit
 int run_ffn(int end, const Params& p, const Launch& l);
 int run_store(bool b_mn, const Params& p, const Launch& l);
+int run_store_long(bool b_mn, const Params& p, const Launch& l);      // of whole tiles of pairs
 int run_ce(int end, const Params& p, const Launch& l);
 
 }  // namespace dense

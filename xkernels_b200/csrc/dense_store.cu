@@ -46,6 +46,10 @@ int clusters_at_once(int dev, int cg, int bn, int read_warps, int width, int* ou
 int run_store(bool b_mn, const Params& p, const Launch& l) {
   return b_mn ? run_variant<true, kStore>(p, l) : run_variant<false, kStore>(p, l);
 }
+int run_store_long(bool b_mn, const Params& p, const Launch& l) {
+  if (l.bn == 256) return b_mn ? run_kernel<2, 256, 8, true, kStoreLong>(p, l) : run_kernel<2, 256, 8, false, kStoreLong>(p, l);
+  return b_mn ? run_kernel<2, 128, 8, true, kStoreLong>(p, l) : run_kernel<2, 128, 8, false, kStoreLong>(p, l);
+}
 
 }  // namespace dense
 }  // namespace xkb

@@ -29,6 +29,7 @@ int64_t pitch8(int64_t n) { return align_up(n, 8); }
 // average out: that row's result was 2.5e-3 off in the norm with one term, and is 1.6e-3 off with two, which its own
 // rounding is.
 constexpr int64_t kTwoTerms = 16;
+bool two_terms(int64_t M, int64_t I) { return M <= kTwoTerms && I <= 65536; }     // I: what one accumulator may take, a part of it as a rule
 
 int check_sizes(const char* name, int dtype, int64_t M, int64_t H, int64_t I) {
   XKB_REQUIRE(dtype == XKB_BF16 || dtype == XKB_F16, "%s: dtype must be bf16 or fp16", name);
@@ -58,7 +59,7 @@ using namespace xkb;
 
 extern "C" int64_t xkb_gated_ffn_workspace_bytes(int64_t M, int64_t H, int64_t I) {
   if (check_sizes("gated_ffn", XKB_BF16, M, H, I) != XKB_OK) return -1;
-  return (M <= kTwoTerms ? 2 : 1) * align_up(M * pitch8(I) * 2, 256);
+  return (two_terms(M, I) ? 2 : 1) * align_up(M * pitch8(I) * 2, 256);
 }
 
 extern "C" int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void* w13, int64_t ld_w13, const void* w2, int64_t ld_w2,
@@ -80,7 +81,7 @@ extern "C" int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void*
   up.a = {x, ld_x, false, 0, M, H};
   up.b = {w13, ld_w13, false, 0, 2 * I, H};
   up.M = M, up.N = I, up.K = H;
-  const int64_t rest = M <= kTwoTerms ? align_up(M * pitch8(I) * 2, 256) / 2 : 0;
+  const int64_t rest = two_terms(M, I) ? align_up(M * pitch8(I) * 2, 256) / 2 : 0;
   up.end.h = workspace, up.end.ld_h = pitch8(I);
   if (rest != 0) up.end.h_rest = static_cast<uint16_t*>(workspace) + rest;
   up.end.gate_up = gate_up, up.end.ld_gu = 2 * I, up.end.half = (int)I;

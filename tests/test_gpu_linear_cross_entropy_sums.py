@@ -52,3 +52,15 @@ def test_sums_of_one_sign_do_not_drift(cuda_device):
         r = xkb.linear_cross_entropy(x, w, z.argmax()[None])
         off.append(float((r.stats[0, 0].double() - z.max()) / z.max()))
     assert abs(sum(off)) / len(off) <= 3 * ULP, off
+
+
+@pytest.mark.parametrize("M", [129, 300, 1000])
+@pytest.mark.parametrize("H", [512, 2048, 4096])
+def test_terms_below_the_last_place_of_many_rows(H, M, cuda_device):
+    """The same with parts of 512 K: 32 steps of less than an ulp; the other parts hold 24 ulp each, and add up exactly."""
+    x, w = torch.zeros(M, H, device=cuda_device), torch.zeros(1000, H, device=cuda_device)
+    x[:, 0] = w[7, 0] = 1
+    x[:, 16::16], w[7, 16::16] = 2.0 ** -12, 0.75 * 2.0 ** -11
+    z = 1 + 0.75 * ULP * (H // 16 - 1)
+    r = xkb.linear_cross_entropy(x.to(torch.bfloat16), w.to(torch.bfloat16), torch.full((M,), 8, device=cuda_device))
+    assert float((r.stats[:, 0].double() - z).abs().max()) <= 32 * ULP

@@ -27,9 +27,11 @@ int64_t pitch8(int64_t n) { return align_up(n, 8); }
 // or 2^-22 (fp16): a tile of the MMAs has 128 rows whatever they hold, so the second term's rows cost nothing but their copies
 // (one row of 7168 x 2048 28.5 -> 29.1 us).  With few rows the rounding errors of a row's few large activations do not
 // average out: that row's result was 2.5e-3 off in the norm with one term, and is 1.6e-3 off with two, which its own
-// rounding is.
+// rounding is.  16: the rows of both terms then belong to one read-out warp.
 constexpr int64_t kTwoTerms = 16;
-bool two_terms(int64_t M, int64_t I) { return M <= kTwoTerms && I <= 65536; }     // I: what one accumulator may take, a part of it as a rule
+// I: as much as single CTAs, which alone take two terms, may add up in one accumulator (a part of it as a rule): 4e-4 lost at most
+// where all terms are of one sign.
+bool two_terms(int64_t M, int64_t I) { return M <= kTwoTerms && I <= 65536; }
 
 int check_sizes(const char* name, int dtype, int64_t M, int64_t H, int64_t I) {
   XKB_REQUIRE(dtype == XKB_BF16 || dtype == XKB_F16, "%s: dtype must be bf16 or fp16", name);

@@ -172,7 +172,8 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
   Shape s;
   rc = shape_of(M, N, K, k_parts, count, end, !any_a_mn && !parted, two_terms, dev, sms, &s);
   if (rc != XKB_OK) return rc;
-  const int a_rows = s.cg == 1 && !any_a_mn && M[0] < kRows ? (int)align_up(M[0], 8) : kRows;
+  const int64_t a_last = M[0] + (end == kStore ? products[0].end.second : 0);      // rows of A that count
+  const int a_rows = s.cg == 1 && !any_a_mn && a_last < kRows ? (int)align_up(a_last, 8) : kRows;
   const CUtensorMapDataType dt = dtype == XKB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   p.count = count;
   p.fmt = dtype == XKB_BF16 ? 1 : 0;
@@ -244,7 +245,7 @@ int launch(const Product* products, int count, int end, int dtype, bool chained,
     bool long_sums = false;
     for (int i = 0; i < count; ++i) long_sums |= ceil_div(ceil_div(K[i], kBK), k_parts[i]) > kLongBlocks;
     // (a kernel of its own: with its registers the ordinary one took 5 % longer, 509 x 4096 x 1416 backward 51.7 -> 54.7 us)
-    return long_sums && s.cg == 2 && s.split == 1 ? run_store_long(b_mn, p, l) : run_store(b_mn, p, l);
+    return long_sums && s.cg == 2 && s.split == 1 && products[0].end.second == 0 ? run_store_long(b_mn, p, l) : run_store(b_mn, p, l);
   }
   if (end == kSwiglu || end == kDswiglu) return run_ffn(end, p, l);
   return run_ce(end, p, l);

@@ -12,7 +12,8 @@ constexpr int kSwiglu = 1;    // gate and up of the same column side by side: si
 constexpr int kDswiglu = 2;   // D is the gradient of silu(gate) * up: the gradients of both, and the product itself
 constexpr int kCeStats = 3;   // D are logits: maximum and sum of exponentials of a row's piece, the label's logit
 constexpr int kCeGrad = 4;    // D are logits: their gradient, rounded to 16 bits
-constexpr int kStoreLong = 5; // kStore of sums so long that they are added up in parts (the launcher's choice)
+// The launcher's choices: kStore of sums so long that they are added up in parts; the two gradients with second terms (End::second).
+constexpr int kStoreLong = 5, kDswigluTwo = 6, kCeGradTwo = 7;
 
 constexpr int kMaxProblems = 3;
 
@@ -51,6 +52,9 @@ struct End {
   float* given;
   const float4* coef;       // m, l, factor of p, what is taken off at the label
   int col0;                 // first column of the piece in the vocabulary
+  // kDswiglu, kCeGrad: what the rounding of row r left, itself rounded, is written to row second + r.  kStore: row second + r of D
+  // is added to row r.  (0: one term.  16 at most, and no more rows.)
+  int second;
   // which vector accesses their rows allow (bytes: 16 or 2), set by the launcher
   int vec_out, vec_h, vec_gu;
   int tma_out;          // rows of `out` leave by copies of 64 columns, set by the launcher

@@ -81,7 +81,10 @@ struct Shared {
 };
 
 // CG: CTAs of a pair; BN: columns of a tile; RW: read-out warps.  RW = 4 leaves room for two CTAs on an SM.
-template <int CG, int BN, int RW, int END> struct Cfg {
+// (Ends with second terms are instances of their own: as a choice within, they cost calls without 1 to 7 %.)
+constexpr int end_of(int way) { return way == kDswigluTwo ? kDswiglu : way == kCeGradTwo ? kCeGrad : way; }
+template <int CG, int BN, int RW, int WAY> struct Cfg {
+  static constexpr int END = end_of(WAY);
   static constexpr int kThreads = 32 * (kControlWarps + RW);
   static constexpr int kCtas = RW == 4 ? 2 : 1;
   static constexpr int kBBytes = BN / CG * 128;
@@ -396,6 +399,17 @@ __device__ __forceinline__ void get_row(uint32_t buf, const void* base, int64_t 
 
 // What a rounding to `hi` left of x; nothing of an infinity or a NaN (hi holds it).
 __device__ __forceinline__ float finite_rest(float x, float hi) { return fabsf(hi) < INFINITY ? x - hi : 0.f; }
+// Two values rounded.  TWO: rows second .. 2 second of a warp's 32 become what the rounding of the rows `second` before them left.
+template <bool TWO> __device__ __forceinline__ uint32_t pack_terms(int fmt, int second, int row, float x0, float x1) {
+  const uint32_t o = pack16(fmt, x0, x1);
+  if constexpr (TWO) {
+    float h0, h1;
+    unpack16(fmt, o, h0, h1);
+    const uint32_t rest = __shfl_sync(~0u, pack16(fmt, finite_rest(x0, h0), finite_rest(x1, h1)), (threadIdx.x & 31) - second);
+    return row >= second && row < 2 * second ? rest : o;
+  }
+  return o;
+}
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + exp2_fast(-kLog2e * x)); }
 
 // ---- what becomes of CW columns of a row ---------------------------------------------------------------------
@@ -432,11 +446,15 @@ template <int END> __device__ __forceinline__ void row_end(const End& e, int row
 }
 
 // v: columns col .. col + CW of D (kSwiglu: of gate, w: of up), n of which exist
-template <int END, int CW>
+template <int END, bool TWO, int CW>
 __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, int row, bool live, int kpart, int col, int n, float scale, float (&v)[CW],
                                           float (&w)[CW], RowState& st) {
   uint32_t o[CW / 2];
   if constexpr (kStores<END>) {
+    if (END == kStore && e.second != 0) {
+#pragma unroll
+      for (int j = 0; j < CW; ++j) v[j] += __shfl_down_sync(~0u, v[j], e.second);
+    }
     if (e.acc_in || e.acc_out) {
       float* acc = e.acc + kpart * e.acc_part + (int64_t)row * e.acc_ld + col;
       constexpr int kHalf = CW == 32 ? 16 : CW;
@@ -547,13 +565,14 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
           if (fabsf(u[i]) > e.limit) du[i] = 0.f;
         }
       }
-      o[j / 2] = pack16(fmt, h[0], h[1]);
-      ug[j / 2] = pack16(fmt, dg[0], dg[1]);
-      uu[j / 2] = pack16(fmt, du[0], du[1]);
+      o[j / 2] = pack_terms<TWO>(fmt, e.second, row, h[0], h[1]);
+      ug[j / 2] = pack_terms<TWO>(fmt, e.second, row, dg[0], dg[1]);
+      uu[j / 2] = pack_terms<TWO>(fmt, e.second, row, du[0], du[1]);
     }
-    put_row<CW>(buf, e.out, (int64_t)row * e.ld + col, live, ug, n, e.vec_out);
-    put_row<CW>(buf, e.out, (int64_t)row * e.ld + half + col, live, uu, n, e.vec_out);
-    if (e.h != nullptr) put_row<CW>(buf, e.h, (int64_t)row * e.ld_h + col, live, o, n, e.vec_h);
+    const bool kept = live || (TWO && row < 2 * e.second);
+    put_row<CW>(buf, e.out, (int64_t)row * e.ld + col, kept, ug, n, e.vec_out);
+    put_row<CW>(buf, e.out, (int64_t)row * e.ld + half + col, kept, uu, n, e.vec_out);
+    if (e.h != nullptr) put_row<CW>(buf, e.h, (int64_t)row * e.ld_h + col, kept, o, n, e.vec_h);
   } else if constexpr (END == kCeStats) {
     float top = -INFINITY;
 #pragma unroll
@@ -593,7 +612,7 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
         if (j + i == at) d[i] -= c.w;
         if (!live) d[i] = 0.f;
       }
-      o[j / 2] = pack16(fmt, d[0], d[1]);
+      o[j / 2] = pack_terms<TWO>(fmt, e.second, row, d[0], d[1]);
     }
     if (CW == 32 && e.tma_out) {
       if (st.half == 0) rows_copied();
@@ -662,9 +681,11 @@ struct Walk {
   }
 };
 
-template <int CG, int BN, int RW, bool BMN, int END>
-__global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW, END>::kCtas) dense_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<CG, BN, RW, END>;
+template <int CG, int BN, int RW, bool BMN, int WAY>
+__global__ void __launch_bounds__(Cfg<CG, BN, RW, WAY>::kThreads, Cfg<CG, BN, RW, WAY>::kCtas) dense_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<CG, BN, RW, WAY>;
+  constexpr int END = C::END;
+  constexpr bool kTwo = WAY != END;
   constexpr bool kPaired = END == kSwiglu;
   constexpr int kTileN = kPaired ? BN / 2 : BN;    // columns of the result
   constexpr int kTmemCols = 2 * BN;
@@ -971,7 +992,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-          if (N - col > 0) row_piece<END, 32>(e, p.fmt, buf, row, live, t.kpart, col, N - col, scale, v, v, st);
+          if (N - col > 0) row_piece<END, kTwo, 32>(e, p.fmt, buf, row, live, t.kpart, col, N - col, scale, v, v, st);
         }
         row_end<END>(e, row, live, t.n * 2 + wg, st);
       } else {
@@ -1041,7 +1062,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
             st.here = CG == 2 && e.vec_gu == 16 && n >= 32;
             st.next = CG == 2 && e.vec_gu == 16 && n >= 64 && c + 32 < (wg + 1) * kMine ? gate_row + c + 32 : nullptr;
           }
-          row_piece<END, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
+          row_piece<END, kTwo, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
           if constexpr (kStores<END> || END == kCeGrad)
             if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.out[t.prod], col - 32 * st.half, row - lane);
           if (n <= kPiece) break;
@@ -1104,7 +1125,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, END>::kThreads, Cfg<CG, BN, RW
             }
           }
         }
-        if (n > 0) row_piece<END, 8>(e, p.fmt, 0, row, live, t.kpart, col, n, scale, v, w, st);
+        if (n > 0) row_piece<END, kTwo, 8>(e, p.fmt, 0, row, live, t.kpart, col, n, scale, v, w, st);
         row_end<END>(e, row, live, t.n * (kTileN / 8) + piece, st);
       }
     }
@@ -1128,10 +1149,10 @@ struct Launch {
   cudaStream_t stream;
 };
 
-template <int CG, int BN, int RW, bool BMN, int END>
+template <int CG, int BN, int RW, bool BMN, int WAY>
 int run_kernel(const Params& p, const Launch& l) {
-  using C = Cfg<CG, BN, RW, END>;
-  auto kernel = dense_kernel<CG, BN, RW, BMN, END>;
+  using C = Cfg<CG, BN, RW, WAY>;
+  auto kernel = dense_kernel<CG, BN, RW, BMN, WAY>;
   static std::atomic<uint64_t> ready{0};      // devices on which this instance is set up
   const uint64_t bit = l.dev < 64 ? 1ull << l.dev : 0;
   if (bit == 0 || !(ready.load(std::memory_order_acquire) & bit)) {

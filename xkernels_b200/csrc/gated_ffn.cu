@@ -14,7 +14,8 @@ namespace xkb {
 namespace dense {
 
 int run_ffn(int end, const Params& p, const Launch& l) {
-  return end == kSwiglu ? run_variant<false, kSwiglu>(p, l) : run_variant<true, kDswiglu>(p, l);
+  if (end == kSwiglu) return run_variant<false, kSwiglu>(p, l);
+  return p.prod[0].end.second != 0 ? run_variant<true, kDswigluTwo>(p, l) : run_variant<true, kDswiglu>(p, l);
 }
 
 }  // namespace dense
@@ -32,6 +33,9 @@ constexpr int64_t kTwoTerms = 16;
 // I: as much as single CTAs, which alone take two terms, may add up in one accumulator (a part of it as a rule): 4e-4 lost at most
 // where all terms are of one sign.
 bool two_terms(int64_t M, int64_t I) { return M <= kTwoTerms && I <= 65536; }
+// The gradients' operands too (1 x 7168 x 2048 bf16 2.4e-3 off with one term, 1.7e-3 with two, 58 and 60 us); grad_x contracts over 2 I,
+// in one accumulator.
+bool two_terms_back(int64_t M, int64_t I) { return two_terms(M, 2 * I); }
 
 int check_sizes(const char* name, int dtype, int64_t M, int64_t H, int64_t I) {
   XKB_REQUIRE(dtype == XKB_BF16 || dtype == XKB_F16, "%s: dtype must be bf16 or fp16", name);
@@ -99,7 +103,10 @@ extern "C" int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void*
 
 extern "C" int64_t xkb_gated_ffn_backward_workspace_bytes(int64_t M, int64_t H, int64_t I, int recompute) {
   if (check_sizes("gated_ffn_backward", XKB_BF16, M, H, I) != XKB_OK) return -1;
-  return align_up(M * pitch8(I) * 2, 256) + (recompute ? 2 : 1) * align_up(M * pitch8(2 * I) * 2, 256);
+  const bool few = two_terms_back(M, I);
+  const int64_t rows = few ? 2 * M : M;
+  return align_up(rows * pitch8(I) * 2, 256) + align_up(rows * pitch8(2 * I) * 2, 256) + (few ? 2 * align_up(rows * pitch8(H) * 2, 256) : 0) +
+         (recompute ? align_up(M * pitch8(2 * I) * 2, 256) : 0);
 }
 
 extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int dtype, const void* x, int64_t ld_x, const void* w13,
@@ -125,10 +132,23 @@ extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int d
     return fail(XKB_ERR_WORKSPACE, "%s: needs a workspace of %lld bytes on 256 bytes", name, (long long)need);
   using namespace dense;
   Carver ws(workspace);
-  void* h = ws.take<uint16_t>(M * pitch8(I));
-  void* d13 = ws.take<uint16_t>(M * pitch8(2 * I));
+  // Up to 16 rows the operands that the activation's gradient leaves have two terms, M rows apart: grad_x adds its rows of both, and
+  // the weights' gradients take the second term's rows as further K, beside x and grad_out once more.
+  const bool few = two_terms_back(M, I);
+  const int64_t rows = few ? 2 * M : M;
+  void* h = ws.take<uint16_t>(rows * pitch8(I));
+  void* d13 = ws.take<uint16_t>(rows * pitch8(2 * I));
   int64_t ld_gu = 2 * I;
-  bool chained = false;
+  bool chained = false, early = false;      // early: w2 is no output of the predecessor
+  if (few) {
+    uint16_t *x2 = ws.take<uint16_t>(rows * pitch8(H)), *go2 = ws.take<uint16_t>(rows * pitch8(H));
+    const void* from[4] = {x, x, grad_out, grad_out};
+    const int64_t ld[4] = {ld_x, ld_x, ld_go, ld_go}, each[4] = {M, M, M, M}, cols[4] = {H, H, H, H};
+    void* to[4] = {x2, x2 + M * pitch8(H), go2, go2 + M * pitch8(H)};
+    XKB_TRY(xkb_lay_out_rows(from, ld, each, cols, to, 4, stream));
+    x = x2, grad_out = go2, ld_x = ld_go = pitch8(H);
+    chained = true;
+  }
   if (gate_up == nullptr) {
     ld_gu = pitch8(2 * I);
     void* again = ws.take<uint16_t>(M * ld_gu);
@@ -137,9 +157,9 @@ extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int d
     up.b = {w13, ld_w13, false, 0, 2 * I, H};
     up.M = M, up.N = I, up.K = H;
     up.end.gate_up = again, up.end.ld_gu = ld_gu, up.end.half = (int)I;
-    XKB_TRY(launch(&up, 1, kSwiglu, dtype, false, false, stream));
+    XKB_TRY(launch(&up, 1, kSwiglu, dtype, chained, false, stream));
     gate_up = again;
-    chained = true;
+    chained = early = true;
   }
   Product open = {};
   open.a = {grad_out, ld_go, false, 0, M, H};
@@ -149,27 +169,29 @@ extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int d
   open.end.h = grad_w2 != nullptr ? h : nullptr, open.end.ld_h = pitch8(I);
   open.end.gate_up = const_cast<void*>(gate_up), open.end.ld_gu = ld_gu, open.end.half = (int)I;
   open.end.limit = limit;
-  XKB_TRY(launch(&open, 1, kDswiglu, dtype, chained, chained, stream));
+  open.end.second = few ? (int)M : 0;
+  XKB_TRY(launch(&open, 1, kDswiglu, dtype, chained, early, stream));
   Product q[3] = {};
   int n = 0;
   if (grad_x != nullptr) {
-    q[n].a = {d13, pitch8(2 * I), false, 0, M, 2 * I};
+    q[n].a = {d13, pitch8(2 * I), false, 0, rows, 2 * I};
     q[n].b = {w13, ld_w13, true, 0, 2 * I, H};
     q[n].M = M, q[n].N = H, q[n].K = 2 * I;
     q[n].end.out = grad_x, q[n].end.ld = H;
+    q[n].end.second = open.end.second;
     ++n;
   }
   if (grad_w13 != nullptr) {
-    q[n].a = {d13, pitch8(2 * I), true, 0, M, 2 * I};
-    q[n].b = {x, ld_x, true, 0, M, H};
-    q[n].M = 2 * I, q[n].N = H, q[n].K = M;
+    q[n].a = {d13, pitch8(2 * I), true, 0, rows, 2 * I};
+    q[n].b = {x, ld_x, true, 0, rows, H};
+    q[n].M = 2 * I, q[n].N = H, q[n].K = rows;
     q[n].end.out = grad_w13, q[n].end.ld = H;
     ++n;
   }
   if (grad_w2 != nullptr) {
-    q[n].a = {grad_out, ld_go, true, 0, M, H};
-    q[n].b = {h, pitch8(I), true, 0, M, I};
-    q[n].M = H, q[n].N = I, q[n].K = M;
+    q[n].a = {grad_out, ld_go, true, 0, rows, H};
+    q[n].b = {h, pitch8(I), true, 0, rows, I};
+    q[n].M = H, q[n].N = I, q[n].K = rows;
     q[n].end.out = grad_w2, q[n].end.ld = I;
     ++n;
   }

@@ -65,8 +65,8 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
   // no such K.)
   auto long_sum = [&](int64_t kb, int s) { return end == kStore && !two_terms && ceil_div(kb, s) > kLongBlocks; };
   for (int bn : {256, 128}) {
-    // (two terms are single CTAs' alone; statistics of one row tile have their shorter sums there: part_blocks)
-    if (two_terms || (end == kCeStats && M[0] <= kRows)) break;
+    // (two terms are single CTAs' alone; logits of one row tile have their shorter sums there: kPartBlocks)
+    if (two_terms || ((end == kCeStats || end == kCeGrad) && M[0] <= kRows)) break;
     const int64_t tile_n = paired ? bn / 2 : bn;
     const double stage = bn == 256 ? 520 : 400, readout = bn == 256 ? 3500 : 2000;
     double work = 0;
@@ -93,7 +93,7 @@ int shape_of(const int64_t* M, const int64_t* N, const int64_t* K, const int* k_
     const int warps = single_warps(end);
     const int64_t kb = ceil_div(K[0], kBK), rows = M[0] < kRows ? align_up(M[0], 8) * (two_terms ? 2 : 1) : kRows;
     for (int bn : {128, 64}) {
-      if (bn == 64 && end == kCeStats) continue;
+      if (bn == 64 && warps == 8) continue;
       const int64_t tiles = ceil_div(M[0], kRows) * ceil_div(N[0], paired ? bn / 2 : bn);
       const double mma = bn == 128 ? 275 : 260, stage = 2 * (rows + bn) > mma ? 2 * (rows + bn) : mma;
       if (!long_sum(kb, 1)) consider({1, bn, 1}, tiles, (double)ceil_div(tiles, sms) * kb * stage, 2000);

@@ -25,20 +25,22 @@ constexpr int kMaxStages = 12;
 constexpr int kABytes = kRows * 128;
 constexpr int kBoxBytes = 64 * 128;  // a box of 64 K rows by 64 elements
 // The tensor cores cut off what an fp32 accumulator cannot hold instead of rounding it, at each step of 16 K, so a long sum
-// drifts towards 0 in proportion to K (losses of many rows were 1.4e-6 off at K = 2048).  Where the result stays fp32 (kCeStats) an
-// accumulator takes kPartBlocks of 64 K, and the read-out adds them up in registers while the next is filled.  Error of losses in
-// the norm, 4096 x 7168 x 128000 in pairs by 512 / 256 K: 4.0e-7 / 2.1e-7 (an fp32 product on the ordinary cores: 1.1e-6), but 3 to
+// drifts towards 0 in proportion to K (losses of many rows were 1.4e-6 off at K = 2048).  Logits stay fp32, in the statistics
+// (kCeStats) as in their gradient (kCeGrad: d of a token that the head is sure of is a difference of numbers close to 1), so an
+// accumulator of theirs takes kPartBlocks of 64 K, and the read-out adds them up in registers while the next is filled.  Error of losses
+// in the norm, 4096 x 7168 x 128000 in pairs by 512 / 256 K: 4.0e-7 / 2.1e-7 (an fp32 product on the ordinary cores: 1.1e-6), but 3 to
 // 20 % more time, for the read-out of short parts outlasts their MMAs.  Single CTAs, which take up to 128 rows, wait for the
 // weight's bytes, and a single row's small loss takes the drift of its largest logit whole: 1 x 4096 x 50001 by 512 / 128 / 64 K
 // 2.7e-6 / 8.6e-8 / 1.1e-6 (one number; the ordinary cores' 9.2e-8) in 91 / 92 / 99 us, 128 x 7168 x 32001 4.5e-7 / 1.8e-7 / 2.0e-7 in
-// 99 / 99 / 103.
+// 99 / 99 / 103.  Logits of terms of one sign in the gradient, fp16, in 2^-23 of them: one accumulator of 1024 / 4096 K 44 / 194 off, in
+// parts of 512 K 20, of 128 K 3; 4096 x 7168 x 16384 backward 1850 -> 1860 us, 509 x 2048 x 50001 255 -> 262, 77 x 2056 x 32001 130.
 // Stored results are rounded to 16 bits, and only sums far longer than a layer is wide drift as far as that: sums over rows of
 // one sign lost 6e-9 of themselves a row (1.6e-3 of 2^18 rows in fp16, whose half step is 4.9e-4).  Pairs add sums of more than 16384 K
 // up in parts of that the same way (kStoreLong), and single CTAs are not given them.  Other ends contract over a layer's width H,
 // in one accumulator.
 constexpr int kLongBlocks = 256;
 template <int END> constexpr bool kStores = END == kStore || END == kStoreLong;
-template <int END> constexpr bool kInParts = END == kCeStats || END == kStoreLong;
+template <int END> constexpr bool kInParts = END == kCeStats || END == kCeGrad || END == kStoreLong;
 template <int END, int CG> constexpr int kPartBlocks = END == kStoreLong ? kLongBlocks : CG == 1 ? 2 : 8;
 template <int END, int CG> __device__ __forceinline__ int parts_of(int kb) {      // no blocks are one part too
   return kInParts<END> && kb > 0 ? (kb + kPartBlocks<END, CG> - 1) / kPartBlocks<END, CG> : 1;
@@ -972,7 +974,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, WAY>::kThreads, Cfg<CG, BN, RW
         }
       }
       const float scale = kStores<END> && e.scale != nullptr ? *e.scale : 1.f;
-      if constexpr (END == kCeStats) {
+      if constexpr (END == kCeStats || END == kCeGrad) {
         const int parts = parts_of<END, CG>(t.k1 - t.k0);
         float sum[kMine];
 #pragma unroll
@@ -988,11 +990,15 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, WAY>::kThreads, Cfg<CG, BN, RW
         }
 #pragma unroll
         for (int c = 0; c < kMine; c += 32) {
-          const int col = t.n * kTileN + wg * kMine + c;
+          const int col = t.n * kTileN + wg * kMine + c, n = N - col;
+          if (n <= 0) break;
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-          if (N - col > 0) row_piece<END, kTwo, 32>(e, p.fmt, buf, row, live, t.kpart, col, N - col, scale, v, v, st);
+          if constexpr (END == kCeGrad) st.half = (c >> 5) & 1;
+          row_piece<END, kTwo, 32>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, v, st);
+          if constexpr (END == kCeGrad)
+            if (e.tma_out && (st.half == 1 || n <= 32)) copy_rows(buf, &p.out[t.prod], col - 32 * st.half, row - lane);
         }
         row_end<END>(e, row, live, t.n * 2 + wg, st);
       } else {
@@ -1042,7 +1048,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, WAY>::kThreads, Cfg<CG, BN, RW
 #pragma unroll 1
         for (int c = wg * kMine; c < (wg + 1) * kMine; c += kPiece) {
           const int col = t.n * kTileN + c, n = N - col;
-          const bool none = n <= 0 || (END != kCeGrad && !warp_live);
+          const bool none = n <= 0 || !warp_live;
           float v[kPiece], w[kPiece];
           if (!none) {
             tmem_load(from + c, v);
@@ -1057,13 +1063,13 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, WAY>::kThreads, Cfg<CG, BN, RW
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[j] = w[j] = 0.f;
           }
-          if constexpr (kStores<END> || END == kCeGrad) st.half = ((c - wg * kMine) >> 5) & 1;
+          if constexpr (kStores<END>) st.half = ((c - wg * kMine) >> 5) & 1;
           if constexpr (END == kDswiglu) {
             st.here = CG == 2 && e.vec_gu == 16 && n >= 32;
             st.next = CG == 2 && e.vec_gu == 16 && n >= 64 && c + 32 < (wg + 1) * kMine ? gate_row + c + 32 : nullptr;
           }
           row_piece<END, kTwo, kPiece>(e, p.fmt, buf, row, live, t.kpart, col, n, scale, v, w, st);
-          if constexpr (kStores<END> || END == kCeGrad)
+          if constexpr (kStores<END>)
             if (e.tma_out && (st.half == 1 || n <= kPiece)) copy_rows(buf, &p.out[t.prod], col - 32 * st.half, row - lane);
           if (n <= kPiece) break;
         }
@@ -1186,14 +1192,14 @@ int run_kernel(const Params& p, const Launch& l) {
 
 // Read-out warps of a single CTA: eight where the read-out adds up in registers, else four and two CTAs an SM, whose ends
 // (and the next kernel's first loads) overlap.
-constexpr int single_warps(int end) { return end == kCeStats ? 8 : 4; }
+constexpr int single_warps(int end) { return end == kCeStats || end == kCeGrad ? 8 : 4; }
 
-template <bool BMN, int END>
+template <bool BMN, int WAY>
 int run_variant(const Params& p, const Launch& l) {
-  if (l.cg == 2) return l.bn == 256 ? run_kernel<2, 256, 8, BMN, END>(p, l) : run_kernel<2, 128, 8, BMN, END>(p, l);
-  if constexpr (END != kCeStats)
-    if (l.bn == 64) return run_kernel<1, 64, 4, BMN, END>(p, l);
-  return run_kernel<1, 128, single_warps(END), BMN, END>(p, l);
+  if (l.cg == 2) return l.bn == 256 ? run_kernel<2, 256, 8, BMN, WAY>(p, l) : run_kernel<2, 128, 8, BMN, WAY>(p, l);
+  if constexpr (single_warps(end_of(WAY)) == 4)
+    if (l.bn == 64) return run_kernel<1, 64, 4, BMN, WAY>(p, l);
+  return run_kernel<1, 128, single_warps(end_of(WAY)), BMN, WAY>(p, l);
 }
 
 // How many clusters of so many CTAs of one of the kernels' sizes run at once on a device, the current one.

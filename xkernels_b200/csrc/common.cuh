@@ -41,6 +41,13 @@ inline void count_launch(int n = 1) { g_launches.fetch_add(n, std::memory_order_
     if (!(cond)) return ::xkb::fail(XKB_ERR_ARG, __VA_ARGS__);                      \
   } while (0)
 
+// For calls that return a status.
+#define XKB_TRY(expr)              \
+  do {                             \
+    const int _rc = (expr);        \
+    if (_rc != XKB_OK) return _rc; \
+  } while (0)
+
 inline int64_t align_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

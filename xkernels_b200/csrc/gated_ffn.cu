@@ -52,12 +52,6 @@ int check_operand(const char* name, const char* what, const void* p, int64_t ld,
   return XKB_OK;
 }
 
-#define XKB_TRY(expr)              \
-  do {                             \
-    const int _rc = (expr);        \
-    if (_rc != XKB_OK) return _rc; \
-  } while (0)
-
 }  // namespace
 }  // namespace xkb
 

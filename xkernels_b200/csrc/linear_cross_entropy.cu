@@ -349,12 +349,6 @@ int launch_list(const ListArgs& a, cudaStream_t stream) {
   return XKB_OK;
 }
 
-#define XKB_TRY(expr)              \
-  do {                             \
-    const int _rc = (expr);        \
-    if (_rc != XKB_OK) return _rc; \
-  } while (0)
-
 }  // namespace
 }  // namespace xkb
 

@@ -135,13 +135,21 @@ extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int d
   int64_t ld_gu = 2 * I;
   bool chained = false, early = false;      // early: w2 is no output of the predecessor
   if (few) {
-    uint16_t *x2 = ws.take<uint16_t>(rows * pitch8(H)), *go2 = ws.take<uint16_t>(rows * pitch8(H));
-    const void* from[4] = {x, x, grad_out, grad_out};
-    const int64_t ld[4] = {ld_x, ld_x, ld_go, ld_go}, each[4] = {M, M, M, M}, cols[4] = {H, H, H, H};
-    void* to[4] = {x2, x2 + M * pitch8(H), go2, go2 + M * pitch8(H)};
-    XKB_TRY(xkb_lay_out_rows(from, ld, each, cols, to, 4, stream));
-    x = x2, grad_out = go2, ld_x = ld_go = pitch8(H);
-    chained = true;
+    const void* from[4];
+    void* to[4];
+    int64_t ld[4], each[4], cols[4];
+    int copies = 0;
+    auto twice = [&](const void*& p, int64_t& pitch) {
+      uint16_t* at = ws.take<uint16_t>(rows * pitch8(H));
+      for (int i = 0; i < 2; ++i, ++copies) from[copies] = p, ld[copies] = pitch, each[copies] = M, cols[copies] = H, to[copies] = at + i * M * pitch8(H);
+      p = at, pitch = pitch8(H);
+    };
+    if (grad_w13 != nullptr) twice(x, ld_x);
+    if (grad_w2 != nullptr) twice(grad_out, ld_go);
+    if (copies > 0) {
+      XKB_TRY(xkb_lay_out_rows(from, ld, each, cols, to, copies, stream));
+      chained = true;
+    }
   }
   if (gate_up == nullptr) {
     ld_gu = pitch8(2 * I);

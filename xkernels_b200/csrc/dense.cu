@@ -263,6 +263,7 @@ struct LayOut {
   const uint16_t* from[XKB_LAY_OUT_MOST];
   uint16_t* to[XKB_LAY_OUT_MOST];
   int64_t ld[XKB_LAY_OUT_MOST], cols[XKB_LAY_OUT_MOST], first[XKB_LAY_OUT_MOST + 1];      // first: number of its first piece
+  int exponent[XKB_LAY_OUT_MOST];      // bits of it: infinities and NaN, which have them all, become 0 (0: they stay)
   int count;
 };
 constexpr int kPiece = 256;
@@ -273,6 +274,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const LayOut a) {
     int i = 0;
     while (i + 1 < a.count && u >= a.first[i + 1]) ++i;
     const int64_t cols = a.cols[i], pieces = (cols + kPiece - 1) / kPiece, v = u - a.first[i];
+    const int all = a.exponent[i];
     const int64_t row = v / pieces, c0 = (v - row * pieces) * kPiece, ld_to = (cols + 7) / 8 * 8;
     const uint16_t* from = a.from[i] + row * a.ld[i];
     uint16_t* to = a.to[i] + row * ld_to;
@@ -285,17 +287,15 @@ __global__ void __launch_bounds__(256) lay_out_kernel(const LayOut a) {
 #pragma unroll
     for (int j = 0; j < kPiece / 32; ++j) {
       const int64_t c = c0 + j * 32 + lane;
-      if (c < cols) to[c] = x[j];
+      if (c < cols) to[c] = all != 0 && (x[j] & all) == all ? (uint16_t)0 : x[j];
     }
   }
 }
 
 }  // namespace
-}  // namespace xkb
 
-extern "C" int xkb_lay_out_rows(const void* const* from_host, const int64_t* ld_host, const int64_t* rows_host, const int64_t* cols_host,
-                                void* const* to_host, int count, void* stream_) {
-  using namespace xkb;
+int dense::lay_out(const void* const* from_host, const int64_t* ld_host, const int64_t* rows_host, const int64_t* cols_host,
+                   void* const* to_host, const int* exponent_host, int count, cudaStream_t stream) {
   XKB_REQUIRE(count >= 0 && count <= XKB_LAY_OUT_MOST, "lay_out_rows: %d matrices", count);
   XKB_REQUIRE(count == 0 || (from_host != nullptr && ld_host != nullptr && rows_host != nullptr && cols_host != nullptr && to_host != nullptr),
               "lay_out_rows: null array");
@@ -309,6 +309,7 @@ extern "C" int xkb_lay_out_rows(const void* const* from_host, const int64_t* ld_
     a.from[i] = static_cast<const uint16_t*>(from_host[i]);
     a.to[i] = static_cast<uint16_t*>(to_host[i]);
     a.ld[i] = ld_host[i], a.cols[i] = cols_host[i];
+    a.exponent[i] = exponent_host != nullptr ? exponent_host[i] : 0;
     a.first[i] = pieces;
     pieces += rows_host[i] * ceil_div(cols_host[i], kPiece);
   }
@@ -316,9 +317,16 @@ extern "C" int xkb_lay_out_rows(const void* const* from_host, const int64_t* ld_
   a.count = count;
   if (pieces == 0) return XKB_OK;
   const int64_t blocks = ceil_div(pieces, 8);
-  lay_out_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, static_cast<cudaStream_t>(stream_)>>>(a);
+  lay_out_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, stream>>>(a);
   XKB_CHECK_LAUNCH("lay_out_kernel");
   return XKB_OK;
+}
+
+}  // namespace xkb
+
+extern "C" int xkb_lay_out_rows(const void* const* from_host, const int64_t* ld_host, const int64_t* rows_host, const int64_t* cols_host,
+                                void* const* to_host, int count, void* stream_) {
+  return xkb::dense::lay_out(from_host, ld_host, rows_host, cols_host, to_host, nullptr, count, static_cast<cudaStream_t>(stream_));
 }
 
 extern "C" int xkb_dense_status(void* stream_) {

@@ -77,6 +77,9 @@ int k_parts_of(int64_t M0, int64_t N0, int64_t K0, int64_t M1, int64_t N1, int64
 // How many pieces a row's statistics come in (kCeStats), and no more than how many.
 int ce_parts(int64_t M, int64_t N, int64_t K, int* parts);
 int64_t ce_most_parts(int64_t M, int64_t N);
+// xkb_lay_out_rows; exponent_host, if not null: bits of a type's exponent, for copies in which infinities and NaN become 0 (0: they stay).
+int lay_out(const void* const* from_host, const int64_t* ld_host, const int64_t* rows_host, const int64_t* cols_host, void* const* to_host,
+            const int* exponent_host, int count, cudaStream_t stream);
 
 }  // namespace dense
 }  // namespace xkb

@@ -401,6 +401,9 @@ __device__ __forceinline__ void get_row(uint32_t buf, const void* base, int64_t 
 
 // What a rounding to `hi` left of x; nothing of an infinity or a NaN (hi holds it).
 __device__ __forceinline__ float finite_rest(float x, float hi) { return fabsf(hi) < INFINITY ? x - hi : 0.f; }
+// The sum of first terms and that of second ones; not beside an infinity, for an infinite factor has made them infinite too, of either sign,
+// or a NaN.
+__device__ __forceinline__ float add_second(float first, float second) { return fabsf(first) < INFINITY ? first + second : first; }
 // Two values rounded.  TWO: rows second .. 2 second of a warp's 32 become what the rounding of the rows `second` before them left.
 template <bool TWO> __device__ __forceinline__ uint32_t pack_terms(int fmt, int second, int row, float x0, float x1) {
   const uint32_t o = pack16(fmt, x0, x1);
@@ -455,7 +458,7 @@ __device__ __forceinline__ void row_piece(const End& e, int fmt, uint32_t buf, i
   if constexpr (kStores<END>) {
     if (END == kStore && e.second != 0) {
 #pragma unroll
-      for (int j = 0; j < CW; ++j) v[j] += __shfl_down_sync(~0u, v[j], e.second);
+      for (int j = 0; j < CW; ++j) v[j] = add_second(v[j], __shfl_down_sync(~0u, v[j], e.second));
     }
     if (e.acc_in || e.acc_out) {
       float* acc = e.acc + kpart * e.acc_part + (int64_t)row * e.acc_ld + col;
@@ -1126,7 +1129,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, RW, WAY>::kThreads, Cfg<CG, BN, RW
               for (int j = 0; j < 8; ++j) {
                 v[j] += a[i][j];
                 if constexpr (kPaired) w[j] += b[i][j];
-                else if (fold != 0) v[j] += b[i][j];
+                else if (fold != 0) v[j] = add_second(v[j], b[i][j]);
               }
             }
           }

@@ -33,7 +33,7 @@ constexpr int64_t kTwoTerms = 16;
 // I: as much as single CTAs, which alone take two terms, may add up in one accumulator (a part of it as a rule): 4e-4 lost at most
 // where all terms are of one sign.
 bool two_terms(int64_t M, int64_t I) { return M <= kTwoTerms && I <= 65536; }
-// The gradients' operands too (1 x 7168 x 2048 bf16 2.4e-3 off with one term, 1.7e-3 with two, 58 and 60 us); grad_x contracts over 2 I,
+// The gradients' operands too (1 x 7168 x 2048 bf16 2.4e-3 off with one term, 1.7e-3 with two, 58 and 62 us); grad_x contracts over 2 I,
 // in one accumulator.
 bool two_terms_back(int64_t M, int64_t I) { return two_terms(M, 2 * I); }
 
@@ -127,7 +127,8 @@ extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int d
   using namespace dense;
   Carver ws(workspace);
   // Up to 16 rows the operands that the activation's gradient leaves have two terms, M rows apart: grad_x adds its rows of both, and
-  // the weights' gradients take the second term's rows as further K, beside x and grad_out once more.
+  // the weights' gradients take the second term's rows as further K, beside x and grad_out once more (but for what is infinite there or
+  // a NaN, which the first terms' rows have: a term of the other sign, or of 0, would make a NaN of an infinity).
   const bool few = two_terms_back(M, I);
   const int64_t rows = few ? 2 * M : M;
   void* h = ws.take<uint16_t>(rows * pitch8(I));
@@ -138,16 +139,19 @@ extern "C" int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_go, int d
     const void* from[4];
     void* to[4];
     int64_t ld[4], each[4], cols[4];
-    int copies = 0;
+    int exponent[4], copies = 0;
     auto twice = [&](const void*& p, int64_t& pitch) {
       uint16_t* at = ws.take<uint16_t>(rows * pitch8(H));
-      for (int i = 0; i < 2; ++i, ++copies) from[copies] = p, ld[copies] = pitch, each[copies] = M, cols[copies] = H, to[copies] = at + i * M * pitch8(H);
+      for (int i = 0; i < 2; ++i, ++copies) {
+        from[copies] = p, ld[copies] = pitch, each[copies] = M, cols[copies] = H, to[copies] = at + i * M * pitch8(H);
+        exponent[copies] = i == 0 ? 0 : dtype == XKB_BF16 ? 0x7F80 : 0x7C00;
+      }
       p = at, pitch = pitch8(H);
     };
     if (grad_w13 != nullptr) twice(x, ld_x);
     if (grad_w2 != nullptr) twice(grad_out, ld_go);
     if (copies > 0) {
-      XKB_TRY(xkb_lay_out_rows(from, ld, each, cols, to, copies, stream));
+      XKB_TRY(lay_out(from, ld, each, cols, to, exponent, copies, stream));
       chained = true;
     }
   }

@@ -30,7 +30,7 @@ extern "C" {
 /* dtype codes used by the `*_dtype` parameters */
 #define XKB_BF16 0
 #define XKB_F32 1
-#define XKB_F16 2 /* accepted for logits (router, head) only */
+#define XKB_F16 2 /* accepted for logits (router, head) and by the dense operators only */
 
 /* kernel-path selectors for the `path` parameters */
 #define XKB_PATH_AUTO 0  /* tensor-core kernel when the shape allows, else SIMT */
@@ -243,9 +243,11 @@ int xkb_token_logprobs_backward(const void* logits, int dtype, int64_t ld,
  * hidden [M, H] (row stride ld_hidden, any alignment of 2 bytes), weight [V, H]
  * (row stride ld_weight a multiple of 8, first row on 16 bytes), both bf16 or fp16;
  * labels [M] int32, or int64 with ids64 = 1; loss, lse [M] and stats [M, 2] = (m, l)
- * fp32.  A row with a negative label is padding: it is not read, and its results are
- * 0; a label >= V gives a loss of NaN; a row whose logits hold a NaN or +inf is NaN.
- * M, V < 2^28.  Three launches; the same bits in every run.
+ * fp32.  A row with a negative label is padding: its results are 0, and what it holds
+ * has no influence on any other (up to 128 rows that start on 16 bytes are multiplied
+ * where they are, padding too; else padding rows are not read); a label >= V gives a
+ * loss of NaN; a row whose logits hold a NaN or +inf is NaN.  M, V < 2^28.  Three
+ * launches, two for rows multiplied in place; the same bits in every run.
  * ---------------------------------------------------------------------- */
 int64_t xkb_linear_cross_entropy_workspace_bytes(int64_t M, int64_t H, int64_t V);
 int xkb_linear_cross_entropy(const void* hidden, int64_t ld_hidden, int dtype,
@@ -262,9 +264,13 @@ int xkb_linear_cross_entropy(const void* hidden, int64_t ld_hidden, int dtype,
  *   d = p (grad_loss + grad_lse) - grad_loss onehot(label),  p = exp(z - m - l),
  *   grad_hidden = d weight,  grad_weight = d^T hidden.
  * z is multiplied again, a piece of the vocabulary at a time; d is rounded to dtype
- * (fp16: times a power of two that keeps small probabilities).  Padding rows are not
- * read and have a gradient of 0; a label >= V makes its row of d NaN.  The workspace
- * holds one piece of d, 256 MiB at most (or 256 columns of it).
+ * (fp16: times a power of two that keeps small probabilities; up to 16 rows: held in
+ * two terms of dtype).  Padding rows are not read and have a gradient of 0; a label
+ * >= V makes its row of d NaN.
+ * The workspace holds one piece of d (256 MiB, or 256 columns where they take more:
+ * beyond 2^19 rows), a copy of the rows (M up to a multiple of 256, times H) and, where
+ * the vocabulary goes by in pieces or its sums in parts, fp32 sums of grad_hidden, one
+ * to 32 times 4 bytes an element, wanted or not.
  * ---------------------------------------------------------------------- */
 int64_t xkb_linear_cross_entropy_backward_workspace_bytes(int64_t M, int64_t H, int64_t V);
 int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_hidden, int dtype,
@@ -283,7 +289,8 @@ int xkb_linear_cross_entropy_backward(const void* hidden, int64_t ld_hidden, int
  * bf16 or fp16, row strides multiples of 8 elements and first rows on 16 bytes.
  * limit > 0: gate is cut off at limit, up at +-limit (as in fused_moe_mxfp4).
  * Products are added up in fp32; silu(gate) * up is rounded to dtype (up to 16
- * rows: held in two terms of dtype) as the operand of the second product.
+ * rows, I <= 65536: held in two terms of dtype) as the operand of the second
+ * product.  It is not scaled: beyond fp16's 65504 it is infinite, as a cast makes it.
  * out [M, H] and, if not NULL, gate_up [M, 2 I] (before the limit), contiguous.
  * No reference counterpart.  Two launches.
  * ---------------------------------------------------------------------- */
@@ -298,7 +305,9 @@ int xkb_gated_ffn(const void* x, int64_t ld_x, int dtype, const void* w13,
  * (contiguous; NULL: not wanted) from grad_out [M, H].  gate_up [M, 2 I] contiguous
  * as gated_ffn left it, or NULL: multiplied again (recompute = 1 in the query).
  * A gate above the limit, an up beyond +-limit has a gradient of 0.
- * The gradients of gate and up, and silu(gate) * up, are rounded to dtype once.
+ * The gradients of gate and up, and silu(gate) * up, are rounded to dtype once (up to
+ * 16 rows, I <= 32768: held in two terms of dtype) and not scaled: in fp16 they are
+ * infinite beyond 65504 and lose bits below 6e-5 (a caller scales the loss).
  * ---------------------------------------------------------------------- */
 int64_t xkb_gated_ffn_backward_workspace_bytes(int64_t M, int64_t H, int64_t I, int recompute);
 int xkb_gated_ffn_backward(const void* grad_out, int64_t ld_grad_out, int dtype,

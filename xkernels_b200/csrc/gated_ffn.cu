@@ -2,12 +2,12 @@
 //
 // Forward, two products: gate and up columns of one tile lie side by side in tensor memory, so the read-out has both and
 // writes their silu(gate) * up, rounded to 16 bits as the operand of the second product has to be (and gate and up, for
-// the backward pass, if they are wanted).  8192 rows of 7168 x 2048: 302 + 155 us, tensor pipe 90 and 83 % busy (1500
-// TFLOP/s); one row: 27 us, of which 15 stream the weights at 5.7 TB/s.
+// the backward pass, if they are wanted).  8192 rows of 7168 x 2048: 309 + 157 us one at a time, tensor pipe 90 and 82 % busy (1550
+// TFLOP/s), 574 us in a loop, where the power limit holds (1260); one row: 30 us a call among others, 24 with the weights in L2.
 // Backward, two launches: dh = dout W2 with the derivative of the activation in the read-out, which leaves [dgate dup] and
-// the activations once more, each rounded once; then dx = [dgate dup] W13, dW13 = [dgate dup]^T x and dW2 = dout^T h as one
-// launch whose tiles are dealt out over all SMs together.  4096 rows: 102 + 377 us, 59 and 89 % (the first is 128 tiles on 74
-// pairs, two rounds).
+// the activations once more, each rounded once (up to 16 rows: in two terms); then dx = [dgate dup] W13, dW13 = [dgate dup]^T x and dW2 = dout^T h as one
+// launch whose tiles are dealt out over all SMs together.  4096 rows: 105 + 385 us, 58 and 88 % (the first is 128 tiles on 74
+// pairs, two rounds), 580 in a loop.
 #include "dense_dev.cuh"
 
 namespace xkb {

@@ -4,10 +4,10 @@
 // many there are stays on the device.  Forward: the dense product's read-out keeps maximum and sum of exponentials of a
 // row's piece of the vocabulary, and one kernel joins the pieces in a fixed order.  Backward: the vocabulary goes by in
 // pieces; a piece's logits are multiplied once more and leave the read-out as their gradient d = p (a + b) - a onehot, rounded
-// once to 16 bits as the operand of the next products has to be; d W, added up over the pieces in fp32, and d^T x follow as one
+// once to 16 bits as the operand of the next products has to be (up to 16 rows in two terms of them); d W, added up over the pieces in fp32, and d^T x follow as one
 // launch.  Three products a piece, 2 M H V each: bound by the tensor cores, and by the weight's bytes where rows are few.
-// 4096 x 7168 x 128000: 4.5 ms and 15.1 ms (1490 and 1340 TFLOP/s, tensor pipe 93 % busy, power); one row of 4096 x 50001: 72 us,
-// 5.7 TB/s.
+// 4096 x 7168 x 128000, tensor pipe 93 % busy: 4.6 and 13.9 ms between pauses (1470 and 1460 TFLOP/s), 5.5 and 16.2 in a loop, where
+// the power limit holds (1230 and 1250).  One row of 4096 x 50001: 76 us in a graph (5.4 TB/s), 84 a call among others.
 #include "dense_dev.cuh"
 
 namespace xkb {

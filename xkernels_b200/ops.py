@@ -655,8 +655,9 @@ def linear_cross_entropy(hidden, weight, labels):
     """Cross entropy of a head: ``loss[i] = lse(z[i]) - z[i, labels[i]]`` with ``z = hidden @ weight.T``, which is never stored.
 
     ``hidden`` ``[M, H]`` and ``weight`` ``[V, H]`` bf16 or fp16 (products are added up in fp32), ``labels`` ``[M]`` int32 or int64.
-    A negative label is padding: the row is not read, its results are 0, and it costs next to nothing.  A label of V or more gives
-    a loss of NaN, a row whose logits hold a NaN or +inf is NaN.  The same bits in every run.  Where :func:`token_logprobs` takes
+    A negative label is padding: its results are 0, and what the row holds has no influence on any other.  Among more than 128 rows it
+    is not read and costs next to nothing; up to 128 are multiplied together, which takes as long whatever they are.  A label of V or
+    more gives a loss of NaN, a row whose logits hold a NaN or +inf is NaN.  The same bits in every run.  Where :func:`token_logprobs` takes
     logits, this takes what they are made from; its gradient is :func:`linear_cross_entropy_backward`.  No reference counterpart.
     """
     got = (_lib._calls or _lib.load_calls()).linear_cross_entropy(hidden, weight, labels)
@@ -691,8 +692,10 @@ def linear_cross_entropy_backward(hidden, weight, labels, stats, grad_loss=None,
 
     ``stats`` is what the forward call returned; ``grad_loss`` and ``grad_lse`` ``[M]`` are the gradients of its outputs (one at
     least is needed; the other counts as 0; of padding rows they are not read).  The logits are multiplied once more, a piece of the
-    vocabulary at a time, so no more than 256 MiB of their gradient are ever held.  Sums are fp32; the gradient of the logits is
-    rounded to ``hidden``'s dtype as the operand of the next products.  The same bits in every run.
+    vocabulary at a time, so 256 MiB of their gradient are held at most (or 256 columns of it, which is more beyond 2^19 rows), besides
+    a copy of the rows and, where there are several pieces or sums go in parts, fp32 sums of ``grad_hidden``.  Sums are fp32; the
+    gradient of the logits is rounded to ``hidden``'s dtype (up to 16 rows: held in two terms of it) as the operand of the next
+    products.  The same bits in every run.
     """
     got = (_lib._calls or _lib.load_calls()).linear_cross_entropy_backward(
         hidden, weight, labels, stats, grad_loss, grad_lse, need_grad_hidden, need_grad_weight)
@@ -745,7 +748,7 @@ def gated_ffn(x, w13, w2, swiglu_limit=None, save_gate_up=False):
     ``x`` ``[M, H]``, ``w13`` ``[2*I, H]`` (gate rows first, as in :func:`fused_moe_mxfp4`), ``w2`` ``[H, I]``, all bf16 or all fp16;
     rows may lie apart.  ``swiglu_limit`` (None or 0: none) cuts gate off at the limit and up at plus and minus it, as there.
     Products are added up in fp32, and ``silu(gate) * up`` is rounded to ``x``'s dtype once, as the operand of the second product (up to
-    16 rows: held in two terms of it).
+    16 rows: held in two terms of it); beyond fp16's 65504 it is infinite.
     Returns ``out`` ``[M, H]``, or ``(out, gate_up)`` with ``save_gate_up``: ``[M, 2*I]`` before the limit, for
     :func:`gated_ffn_backward`.  The same bits in every run.  No reference counterpart.
     """
@@ -782,7 +785,8 @@ def gated_ffn_backward(grad_out, x, w13, w2, gate_up=None, swiglu_limit=None, ne
 
     ``gate_up`` is what the forward call saved; without it the first product is multiplied once more (and what the limit cuts off is
     then decided on its result rounded to ``x``'s dtype, as with the saved one).  Gradients of gate and up and ``silu(gate) * up`` are
-    rounded to ``x``'s dtype once, as operands of the next products; all sums are fp32.  The same bits in every run.
+    rounded to ``x``'s dtype once, as operands of the next products (up to 16 rows: held in two terms of it), and not scaled: in fp16 scale
+    the loss, for below 6e-5 they lose bits.  All sums are fp32.  The same bits in every run.
     """
     got = (_lib._calls or _lib.load_calls()).gated_ffn_backward(
         grad_out, x, w13, w2, gate_up, swiglu_limit, need_grad_x, need_grad_w13, need_grad_w2)
